@@ -403,6 +403,45 @@ int tannic_hip_softmax(const tannic_tensor_t* x, const tannic_tensor_t* mask, ta
  * angle of position n; dst contiguous. */
 int tannic_hip_rope(const tannic_tensor_t* x, const tannic_tensor_t* cos, const tannic_tensor_t* sin, tannic_tensor_t* dst, tannic_stream_t stream);
 
+/* ------------------------------------------------------------------ *
+ * A cache of keys and values in pages, and attention (no counterpart in
+ * the reference).  A program that serves a model keeps
+ *   keys, values [pages, kv heads, page, d]   any strides, the elements of a
+ *                                             head one after the other
+ *   table   int32 [sequences, columns]        the page with the tokens
+ *                                             column * page .. of a sequence;
+ *                                             a number outside the cache (-1)
+ *                                             where there is none
+ *   starts  int32 [sequences + 1]             sequence s has the new tokens
+ *                                             starts[s] .. starts[s + 1]
+ *   context int32 [sequences]                 its tokens before those
+ * The lengths and the table are read on the device, so that a recorded call
+ * follows them from replay to replay; whatever they hold, nothing outside the
+ * tensors is read or written.  starts ascend; rows of no sequence (those
+ * behind starts[sequences], a batch's padding) are left as they were.
+ * Sums, maxima and rotations are float (float64: double), rounded once;
+ * 16-bit weights are rounded for the matrix pipe.
+ * ------------------------------------------------------------------ */
+/* k, v [tokens, kv heads, d] into their places: token t of sequence s has the position context[s] + t - starts[s] and goes into page
+ * table[s, position / page], row position % page (nowhere if there is no such page).  With cos, sin [positions, d/2] (of k's type or
+ * float; positions beyond take their last row) the keys' pairs (2i, 2i+1) turn by the angle of their position first, and so do the
+ * rows of q [tokens, heads, d] into the contiguous `turned`; cos and sin, or q and turned, may be NULL. */
+int tannic_hip_append_pages(const tannic_tensor_t* k, const tannic_tensor_t* v, const tannic_tensor_t* table, const tannic_tensor_t* starts,
+                            const tannic_tensor_t* context, const tannic_tensor_t* cos, const tannic_tensor_t* sin, const tannic_tensor_t* q,
+                            tannic_tensor_t* keys, tannic_tensor_t* values, tannic_tensor_t* turned, tannic_stream_t stream);
+/* dst[t, h] = sum_j softmax_j(scale * q[t, h] . keys[j, h / g]) values[j, h / g] over the keys up to t's own position, g = heads / kv heads;
+ * keys of pages that do not exist are left out, a row without keys is 0.  q [tokens, heads, d], d at most 256; dst contiguous. */
+int tannic_hip_attend_pages(const tannic_tensor_t* q, const tannic_tensor_t* keys, const tannic_tensor_t* values, const tannic_tensor_t* table,
+                            const tannic_tensor_t* starts, const tannic_tensor_t* context, tannic_tensor_t* dst, tannic_stream_t stream, float scale);
+/* Copies whole pages of pool [.., pages, kv heads, page, d] (layers, keys and values in front; a page's elements lie one after the other),
+ * page sources[i] over page targets[i], one after another in the order given.  The lists are HOST memory, borrowed for the call; a
+ * recorded call keeps their numbers. */
+int tannic_hip_copy_pages(tannic_tensor_t* pool, tannic_stream_t stream, const int32_t* sources, const int32_t* targets, size_t count);
+/* The same attention over dense keys and values of another length (an encoder's states): q [batch, tokens, heads, d], k, v [batch, states,
+ * kv heads, d], every token sees the first lengths[b] states of its sequence (int32 [batch], read on the device; NULL: all of them). */
+int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const tannic_tensor_t* v, const tannic_tensor_t* lengths,
+                      tannic_tensor_t* dst, tannic_stream_t stream, float scale);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

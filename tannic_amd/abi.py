@@ -83,6 +83,7 @@ TP = C.POINTER(tensor_t)
 SP = C.POINTER(scalar_t)
 DP = C.POINTER(device_t)
 SIZE2 = C.c_size_t * 2
+I32P = C.POINTER(C.c_int32)
 
 UNARY_OPS = ["neg", "repack", "log", "exp", "sqrt", "abs", "sin", "cos", "tan", "sinh", "cosh", "tanh"]
 BINARY_OPS = ["add", "sub", "mul", "pow"]
@@ -125,6 +126,10 @@ def kernel_signatures(with_stream):
     sig["rms_norm"] = (C.c_int, [TP, TP, TP] + s + [C.c_float])
     sig["softmax"] = (C.c_int, [TP, TP, TP] + s + [C.c_float])   # the second operand (mask) may be NULL
     sig["rope"] = (C.c_int, [TP, TP, TP, TP] + s)
+    sig["append_pages"] = (C.c_int, [TP] * 11 + s)     # cos and sin, q and its destination may be NULL
+    sig["attend_pages"] = (C.c_int, [TP] * 7 + s + [C.c_float])
+    sig["copy_pages"] = (C.c_int, [TP] + s + [I32P, I32P, C.c_size_t])
+    sig["attend"] = (C.c_int, [TP] * 5 + s + [C.c_float])    # the fourth operand (lengths) may be NULL
     return sig
 
 

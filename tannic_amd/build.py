@@ -39,6 +39,8 @@ UNITS = [
     ("rows.hip", "rows.o", []),
     ("reduce.hip", "reduce.o", []),
     ("shape_ops.hip", "shape_ops.o", []),
+    ("attention.hip", "attention.o", []),
+    ("cache.hip", "cache.o", EXACT),
     ("gemm.hip", "gemm.o", []),
     ("gemm_mfma.hip", "gemm_mfma.o", []),
     ("gemm_skinny.hip", "gemm_skinny.o", []),

@@ -12,6 +12,7 @@ the reference pairs ``cpu::f`` with ``cuda::f``).
 """
 import builtins
 import ctypes as C
+import math
 import struct
 
 import numpy as np
@@ -560,3 +561,68 @@ def rope(x, cos, sin):
     """Rotary embedding of ``x [.., n, d]`` by ``cos, sin [n, d/2]`` on the pairs ``(2i, 2i+1)``; contiguous result."""
     env = _resolve(x, cos, sin)
     return _call("rope", env, [x, cos, sin], _new(x.dtype, x.shape, env))
+
+
+# ---- a cache in pages, and attention (no twin in the reference) ------------------------
+# ``keys``, ``values [pages, kv heads, page, d]`` hold every sequence's tokens in pages; ``table [sequences, columns]`` (int32) names them,
+# -1 where there is none; ``starts [sequences + 1]`` and ``context [sequences]`` (int32) say which rows of a call are a sequence's new tokens
+# and how many tokens it had before.  All of them are read on the device: a recorded call follows what is written into them.
+def _device_call(name, operands, arguments):
+    """One backend call whose operands may be missing; ``arguments(stream)`` in the order of the ABI."""
+    env = _resolve(*[t for t in operands if t is not None])
+    if env.kind != abi.DEVICE:
+        raise BackendError(f"{name}: operands are on the host and tannic_amd holds device kernels only")
+    lib = library()
+    status = lib.calls[name](*arguments(env.stream_number()))
+    if status != abi.SUCCESS:
+        detail = lib.error_message() if status == abi.ERROR else ""
+        raise TannicError(f"Unsupported dtype ({name}: {abi.STATUS_NAMES[status]}{' ' + detail if detail else ''})")
+
+
+def _packed(t):
+    return None if t is None else t.packed()
+
+
+def append_pages(k, v, keys, values, table, starts, context, cos=None, sin=None, q=None):
+    """Writes the new tokens' ``k``, ``v [tokens, kv heads, d]`` into the pages of their sequences, behind ``context``.  With ``cos, sin
+    [positions, d/2]`` the keys turn by their positions first, as ``rope`` turns them, and so does ``q [tokens, heads, d]``, which is returned."""
+    turned = None if q is None else _new(q.dtype, q.shape, _resolve(q, k))
+    operands = (k, v, table, starts, context, cos, sin, q, keys, values, turned)
+    _device_call("append_pages", operands, lambda stream: (*map(_packed, operands), stream))
+    return turned
+
+
+def attend_pages(q, keys, values, table, starts, context, scale=None):
+    """Attention of the new tokens ``q [tokens, heads, d]`` over their sequences' pages, every token over the keys up to its own position
+    (written before, see ``append_pages``); ``[tokens, heads, d]``, contiguous.  ``scale`` is ``1 / sqrt(d)`` if not given."""
+    operands = (q, keys, values, table, starts, context, _new(q.dtype, q.shape, _resolve(q, keys)))
+    scale = 1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else scale
+    _device_call("attend_pages", operands, lambda stream: (*[t.packed() for t in operands], stream, scale))
+    return operands[-1]
+
+
+def _page_numbers(pages):
+    numbers = np.asarray(pages).reshape(-1)
+    if numbers.size and (numbers.dtype.kind not in "iu" or numbers.min() < 0 or numbers.max() >= 1 << 31):
+        raise TannicError("copy_pages: the numbers of pages are whole, from 0 on and below 2^31")
+    return np.ascontiguousarray(numbers, dtype=np.int32)
+
+
+def copy_pages(pool, sources, targets):
+    """Copies page ``sources[i]`` of ``pool [.., pages, kv heads, page, d]`` over page ``targets[i]``, one after another in the order given
+    (numbers on the host); ``pool``."""
+    sources, targets = _page_numbers(sources), _page_numbers(targets)
+    if sources.size != targets.size:
+        raise TannicError("copy_pages: as many sources as targets")
+    lists = [pages.ctypes.data_as(abi.I32P) for pages in (sources, targets)]
+    _device_call("copy_pages", (pool,), lambda stream: (pool.packed(), stream, *lists, sources.size))
+    return pool
+
+
+def attend(q, k, v, lengths=None, scale=None):
+    """Attention of ``q [batch, tokens, heads, d]`` over ``k, v [batch, states, kv heads, d]`` of another length (an encoder's states), over the
+    first ``lengths[b]`` states of a sequence (int32; all of them if not given); contiguous, ``q``'s shape."""
+    operands = (q, k, v, lengths, _new(q.dtype, q.shape, _resolve(q, k)))
+    scale = 1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else scale
+    _device_call("attend", operands, lambda stream: (*map(_packed, operands), stream, scale))
+    return operands[-1]
