@@ -40,6 +40,7 @@ UNITS = [
     ("reduce.hip", "reduce.o", []),
     ("shape_ops.hip", "shape_ops.o", []),
     ("attention.hip", "attention.o", []),
+    ("attention_rows.hip", "attention_rows.o", []),
     ("cache.hip", "cache.o", EXACT),
     ("gemm.hip", "gemm.o", []),
     ("gemm_mfma.hip", "gemm_mfma.o", []),

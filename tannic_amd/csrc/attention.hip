@@ -104,6 +104,7 @@ int run_attention(const AttentionProblem& p, const void* q, const void* k, const
 }
 
 int run_attention(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    if (int status = attention_rows(dtype, p, q, k, v, out, stream); status != TANNIC_UNSUPPORTED_DTYPE) return status;
     switch (dtype) {
         case TANNIC_FLOAT16: return run_attention<f16>(p, q, k, v, out, stream);
         case TANNIC_BFLOAT16: return run_attention<bf16>(p, q, k, v, out, stream);
@@ -134,8 +135,8 @@ int tannic_hip_attend_pages(const tannic_tensor_t* q, const tannic_tensor_t* key
     AttentionProblem p{};
     p.heads = static_cast<uint32_t>(q->shape.sizes[1]);
     p.d = static_cast<uint32_t>(q->shape.sizes[2]);
-    if (q->shape.sizes[0] >= (1ull << 31) || q->shape.sizes[1] >= (1u << 16) || q->shape.sizes[0] * q->shape.sizes[1] >= (1ull << 31))
-        return refuse("attend_pages: 2^31 rows of queries or more are not supported");
+    if (q->shape.sizes[0] >= (1ull << 31) || q->shape.sizes[1] >= (1u << 16) || q->shape.sizes[0] * q->shape.sizes[1] >= (1ull << 30))
+        return refuse("attend_pages: 2^30 rows of queries or more are not supported");
     if (q->shape.sizes[2] != keys->shape.sizes[3] || q->shape.sizes[2] > kAttentionHead) return refuse("attend_pages: q and the keys have one head size, at most 256");
     if (q->shape.sizes[1] == 0 || pages.kv_heads == 0 || q->shape.sizes[1] % pages.kv_heads != 0) return refuse("attend_pages: the number of heads is a multiple of the cache's");
     if (q->shape.sizes[2] > 1 && q->strides.sizes[2] != 1) return refuse("attend_pages: the elements of a head of q lie one after the other");
@@ -169,8 +170,8 @@ int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const 
     if (k->shape.sizes[0] != batch || k->shape.sizes[3] != d) return refuse("attend: q, k and v have one batch and one head size");
     if (d > kAttentionHead) return refuse("attend: heads of more than 256 elements are not supported");
     if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0) return refuse("attend: the number of heads is a multiple of the keys'");
-    if (batch >= (1ull << 31) || n >= (1ull << 31) || heads >= (1u << 16) || states >= (1ull << 31) || batch * n >= (1ull << 31) || batch * n * heads >= (1ull << 31))
-        return refuse("attend: 2^31 rows of queries or keys or more are not supported");
+    if (batch >= (1ull << 31) || n >= (1ull << 31) || heads >= (1u << 16) || states >= (1ull << 31) || batch * n >= (1ull << 31) || batch * n * heads >= (1ull << 30))
+        return refuse("attend: 2^30 rows of queries, 2^31 keys, or more are not supported");
     if (lengths && (lengths->rank != 1 || lengths->shape.sizes[0] != batch || !rows_contiguous(lengths))) return refuse("attend: lengths [batch], contiguous");
     if (d > 1 && (q->strides.sizes[3] != 1 || (states > 0 && (k->strides.sizes[3] != 1 || v->strides.sizes[3] != 1)))) return refuse("attend: the elements of a head lie one after the other");
     if (element_count(q) == 0) return TANNIC_SUCCESS;

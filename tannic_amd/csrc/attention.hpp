@@ -89,6 +89,165 @@ __device__ inline int64_t query_offset(const AttentionProblem& p, uint32_t s, co
     return static_cast<int64_t>(s) * p.q_batch + token * p.q_token + static_cast<int64_t>(head) * p.q_head;
 }
 
+// ---- sharing the keys of all rows between blocks -------------------------------------------------------------------------------
+// A group is a tile of rows of one sequence that read the same keys (a kv head's); its keys come in units.  All groups' units, one group
+// after the other, are dealt to the blocks in equal runs, so that every block reads as many keys as the next whatever the lengths are; a
+// group that a run's end cuts is put together from its blocks' partial results afterwards.  Lengths are known on the device only: every
+// wavefront works the runs out for itself, 64 sequences at a time.
+struct Group {
+    uint32_t s, tile, head;      // of `tiles` x kv_heads in the sequence, heads innermost
+    Span span;
+    uint32_t tiles, units;       // units of each of the sequence's groups
+    uint64_t first;              // the group's first unit among all
+};
+
+template <bool PAGED, int ROWS, int UNIT>
+__device__ inline uint64_t sequence_units(const AttentionProblem& p, uint32_t s, Span& span, uint32_t& tiles, uint32_t& units) {
+    span = span_of<PAGED>(p, s);
+    if (span.count == 0) return tiles = units = 0;
+    tiles = static_cast<uint32_t>((static_cast<uint64_t>(span.count) * p.group + (ROWS - 1)) / ROWS);
+    const uint32_t keys = keys_seen(p, span, span.count - 1);
+    units = keys ? (keys + (UNIT - 1)) / UNIT : 1;      // (rows without keys are written all the same)
+    return static_cast<uint64_t>(tiles) * p.kv_heads * units;
+}
+
+__device__ inline uint64_t lanes_sum_before(uint64_t v, uint64_t& total) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint64_t upto = v;
+#pragma unroll
+    for (uint32_t step = 1; step < 64; step *= 2) {
+        const uint64_t below = __shfl_up(upto, step);
+        if (lane >= step) upto += below;
+    }
+    total = __shfl(upto, 63);
+    return upto - v;
+}
+
+// Units of all groups together.
+template <bool PAGED, int ROWS, int UNIT>
+__device__ inline uint64_t all_units(const AttentionProblem& p) {
+    uint64_t sum = 0;
+    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
+        const uint32_t s = s0 + threadIdx.x % 64;
+        Span span;
+        uint32_t tiles, units;
+        uint64_t mine = s < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, s, span, tiles, units) : 0, total;
+        lanes_sum_before(mine, total);
+        sum += total;
+    }
+    return sum;
+}
+
+// The group that holds unit `at` (there is one).
+template <bool PAGED, int ROWS, int UNIT>
+__device__ inline Group group_of(const AttentionProblem& p, uint64_t at) {
+    uint64_t base = 0;
+    Group g{};
+    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
+        const uint32_t s = s0 + threadIdx.x % 64;
+        Span span;
+        uint32_t tiles, units;
+        const uint64_t mine = s < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, s, span, tiles, units) : 0;
+        uint64_t total;
+        const uint64_t before = base + lanes_sum_before(mine, total);
+        if (at < base + total) {
+            const uint64_t here = __ballot(mine > 0 && before <= at && at < before + mine);
+            const int lane = __builtin_ctzll(here);
+            g.s = s0 + lane;
+            g.first = __shfl(before, lane);
+            break;
+        }
+        base += total;
+    }
+    g.s = __builtin_amdgcn_readfirstlane(g.s);
+    sequence_units<PAGED, ROWS, UNIT>(p, g.s, g.span, g.tiles, g.units);
+    const uint64_t number = (at - g.first) / g.units;
+    g.first += number * g.units;
+    g.tile = static_cast<uint32_t>(number / p.kv_heads);
+    g.head = static_cast<uint32_t>(number % p.kv_heads);
+    return g;
+}
+
+// The group behind g; false: g was the last.
+template <bool PAGED, int ROWS, int UNIT>
+__device__ inline bool next_group(const AttentionProblem& p, Group& g) {
+    g.first += g.units;
+    if (++g.head < p.kv_heads) return true;
+    g.head = 0;
+    if (++g.tile < g.tiles) return true;
+    g.tile = 0;
+    while (++g.s < p.sequences)
+        if (sequence_units<PAGED, ROWS, UNIT>(p, g.s, g.span, g.tiles, g.units)) return true;
+    return false;
+}
+
+__device__ inline uint64_t run_start(uint64_t block, uint64_t blocks, uint64_t units) { return block * units / blocks; }
+// the block whose run holds a unit: the last one that starts at or before it
+__device__ inline uint64_t run_of(uint64_t unit, uint64_t blocks, uint64_t units) { return ((unit + 1) * blocks - 1) / units; }
+
+// What a block leaves of a group it has a part of: ROWS x d sums, then every row's largest score (in units of log2) and sum of weights.
+// A block has at most two such parts: of the group its run starts in, and of the one it ends in.
+template <int ROWS> __host__ __device__ inline uint64_t partial_floats(uint32_t d) { return static_cast<uint64_t>(ROWS) * (d + 2); }
+
+typedef float float4a __attribute__((ext_vector_type(4)));
+typedef unsigned int uint4a __attribute__((ext_vector_type(4)));
+typedef unsigned int uint2a __attribute__((ext_vector_type(2)));
+
+// the largest / the sum over the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ inline float across_groups_max(float x) {
+    uint2a r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float across_groups_sum(float x) {
+    uint2a r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <class T> __device__ inline float4a rows_mfma(uint4a a, uint4a b, float4a c) {
+    if constexpr (std::is_same_v<T, f16>) {
+        typedef _Float16 V __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    } else if constexpr (std::is_same_v<T, bf16>) {
+        typedef __bf16 V __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    } else {
+        // four products of four: element j of both operands is the j-th
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+        return c;
+    }
+}
+
+// two weights as the matrix pipe takes them
+template <class T> __device__ inline uint32_t pack_weights(float x, float y) {
+    T v[2] = {narrow_result<T>(x), narrow_result<T>(y)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// Whether one of a register's two 16-bit values (a float) is infinite or NaN.
+template <class T> __device__ inline bool not_finite(uint32_t x) {
+    constexpr uint32_t E = std::is_same_v<T, f16> ? 0x7C00u : 0x7F80u;
+    if constexpr (sizeof(T) == 4) return (x & 0x7F800000u) == 0x7F800000u;
+    return (x & E) == E || ((x >> 16) & E) == E;
+}
+
+// The same register with those values 0.
+template <class T> __device__ inline uint32_t finite_only(uint32_t x) {
+    constexpr uint32_t E = std::is_same_v<T, f16> ? 0x7C00u : 0x7F80u;
+    if constexpr (sizeof(T) == 4) return not_finite<T>(x) ? 0u : x;
+    return ((x & E) == E ? 0u : x & 0xFFFFu) | (((x >> 16) & E) == E ? 0u : x & 0xFFFF0000u);
+}
+
+// fp16 weights are kept 2^8 times as large: those below 2^-22 of the largest lose bits first, not those below 2^-14
+template <class T> constexpr float kWeightShift = std::is_same_v<T, f16> ? 8.0f : 0.0f;
+
+// Whether the kernels of 16-byte pieces take the operands, and which of them.  SUCCESS, or UNSUPPORTED_DTYPE: they do not.
+int attention_rows(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream);
+
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 }  // namespace th

@@ -1,0 +1,439 @@
+// Attention of few rows: one token of every sequence (decoding), or a few.  16-bit types and fp32, rows in 16-byte pieces.
+// The keys and values have to be read once, and that bounds it (HBM): ROWS = 16 MT query rows that read the same kv head - a sequence's
+// tokens times the heads of a group - are one tile of the matrix pipe, and all keys of all sequences are dealt to the blocks in equal
+// runs (attention.hpp).  A block's wavefronts take 32 keys in turns (fp32: 16), each folding its own softmax; they meet in LDS at the end of a run.
+//   scores  S^T[key][row] = K Q^T: a lane of the accumulator has one row (lane % 16) and four keys (4 (lane / 16) + i), so a row's maximum and
+//           sum are one value per lane and two exchanges between lanes.
+//   values  O^T[element][row] = V^T P^T: the weights are already where the second product wants them - a lane's keys of both tiles are its
+//           eight of the product's 32 - if V's keys are taken in the same order.  16-bit V is transposed on its way out of LDS (ds_read_b64_tr_b16);
+//           fp32 V needs no LDS: an accumulator's four keys are four products.
+#include "attention.hpp"
+
+namespace th {
+
+constexpr int kRowsUnit = 64;       // keys of a unit
+
+// A lane's key: where its pieces start, or nowhere.
+struct KeyPlace {
+    int64_t k, v;
+    bool live;
+};
+
+template <class T, bool PAGED>
+__device__ inline KeyPlace key_place(const AttentionProblem& p, uint32_t s, uint32_t j, uint32_t end, uint32_t head) {
+    KeyPlace r{0, 0, false};
+    if (j >= end) return r;
+    int64_t page;
+    uint32_t in;
+    r.live = place_of<PAGED>(p, s, j, page, in);
+    if (r.live) {
+        r.k = page * p.k_page + in * p.k_token + head * p.k_head;
+        r.v = page * p.v_page + in * p.v_token + head * p.v_head;
+    }
+    return r;
+}
+
+template <class T> __device__ inline uint4a load16(const T* at) { return *reinterpret_cast<const uint4a*>(at); }
+
+template <class T, int DP> constexpr size_t rows_lds_bytes() {
+    constexpr size_t join = 4 * 16 * (DP + 4) * 4 + 4 * 16 * 2 * 4, stage = sizeof(T) == 2 ? 4 * 32 * (DP + 16) * 2 : 0;
+    return join > stage ? join : stage;
+}
+
+template <class T, int DP, int MT, bool PAGED>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial) {
+    constexpr bool HALF = sizeof(T) == 2;
+    constexpr int ROWS = 16 * MT, E = 16 / sizeof(T);       // elements of a piece
+    constexpr int KT = HALF ? 2 : 1, STEP = 16 * KT;        // tiles of 16 keys of a wavefront's step
+    constexpr int KS = DP / (4 * E);                        // steps of a score's product: four pieces each
+    constexpr int OT = DP / 16;                             // tiles of 16 elements of the result
+    constexpr int PITCH = DP + 16;                          // elements from key to key in LDS: the four rows a transposing read touches, and the 16 of a write, on different banks
+    extern __shared__ __align__(16) char lds_raw[];
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, quarter = lane / 16;
+    const uint64_t units = all_units<PAGED, ROWS, kRowsUnit>(p);
+    const uint64_t blocks = gridDim.x < units ? gridDim.x : units;      // (no run is empty)
+    if (blockIdx.x >= blocks) return;
+    const uint64_t from = run_start(blockIdx.x, blocks, units), to = run_start(blockIdx.x + 1, blocks, units);
+    Group g = group_of<PAGED, ROWS, kRowsUnit>(p, from);
+    const float factor = p.scale * 1.44269504088896340736f;      // weights are powers of two
+    uint64_t at = from;
+    while (true) {
+        const uint64_t stop = g.first + g.units < to ? g.first + g.units : to;
+        const uint32_t key_from = static_cast<uint32_t>(at - g.first) * kRowsUnit;
+        uint32_t key_to = static_cast<uint32_t>(stop - g.first) * kRowsUnit;
+        const bool whole = at == g.first && stop == g.first + g.units;
+
+        // ---- the tile's rows
+        uint4a qf[MT][KS];
+        uint32_t seen[MT], most = 0;
+        int64_t to_row[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const uint64_t row = static_cast<uint64_t>(g.tile) * ROWS + m * 16 + col;
+            const uint32_t i = p.group_div.div(static_cast<uint32_t>(row)), head = g.head * p.group + static_cast<uint32_t>(row) - i * p.group;
+            const bool live = i < g.span.count;
+            seen[m] = live ? keys_seen(p, g.span, i) : 0;
+            to_row[m] = live ? (static_cast<int64_t>(g.span.begin + i) * p.heads + head) * p.d : -1;
+            const T* const from_row = q + (live ? query_offset(p, g.s, g.span, i, head) : 0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint32_t e = (ks * 4 + quarter) * E;
+                qf[m][ks] = live && e < p.d ? load16(from_row + e) : uint4a{0, 0, 0, 0};
+            }
+            most = most > seen[m] ? most : seen[m];
+        }
+        // the last key any row of the tile sees
+        const uint32_t last_i = p.group_div.div(g.tile * ROWS + ROWS - 1);
+        most = keys_seen(p, g.span, last_i < g.span.count ? last_i : g.span.count - 1);
+        key_to = key_to < most ? key_to : most;
+        // keys up to here are seen by every live row
+        const uint32_t all_see = keys_seen(p, g.span, p.group_div.div(g.tile * ROWS));
+
+        float4a acc[MT][OT];
+        float top[MT], sum[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            top[m] = -INFINITY;
+            sum[m] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < OT; ++t) acc[m][t] = float4a{0, 0, 0, 0};
+        }
+
+        // ---- keys and values of a step: a lane has key lane % 16 of every tile, pieces lane / 16, lane / 16 + 4, ...
+        uint4a kf[KT][KS], vf[KT][KS];
+        uint32_t there[KT];
+        auto fetch = [&](uint32_t j0) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const KeyPlace at_key = key_place<T, PAGED>(p, g.s, j0 + kt * 16 + col, key_to, g.head);
+                there[kt] = static_cast<uint32_t>(__ballot(at_key.live)) & 0xFFFFu;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint32_t e = (ks * 4 + quarter) * E;
+                    kf[kt][ks] = at_key.live && e < p.d ? load16(k + at_key.k + e) : uint4a{0, 0, 0, 0};
+                    if constexpr (HALF) vf[kt][ks] = at_key.live && e < p.d ? load16(v + at_key.v + e) : uint4a{0, 0, 0, 0};
+                }
+                if constexpr (!HALF) {
+                    // fp32: piece lane % 16 (+ 16 ks') of the keys 4 (lane / 16) + i; vf[0][i * (KS / 4) + ks'] with KS / 4 = DP / 64
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int source = 4 * quarter + i;
+                        const int64_t off = __shfl(at_key.v, source);
+                        const bool live = (there[kt] >> source) & 1;
+#pragma unroll
+                        for (int c = 0; c < KS / 4; ++c) {
+                            const uint32_t e = (c * 16 + col) * E;
+                            vf[kt][i * (KS / 4) + c] = live && e < p.d ? load16(v + off + e) : uint4a{0, 0, 0, 0};
+                        }
+                    }
+                }
+            }
+        };
+        T* const mine = reinterpret_cast<T*>(lds_raw) + wave * (32 * PITCH);
+        uint32_t j0 = key_from + wave * STEP;
+        if (j0 < key_to) fetch(j0);
+        for (; j0 < key_to; j0 += 4 * STEP) {
+            if constexpr (HALF) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) *reinterpret_cast<uint4a*>(mine + (kt * 16 + col) * PITCH + (ks * 4 + quarter) * E) = vf[kt][ks];
+            }
+            uint32_t keys_here[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) keys_here[kt] = there[kt];
+            const bool full = j0 + STEP <= all_see && keys_here[0] == 0xFFFFu && keys_here[KT - 1] == 0xFFFFu;
+            // values that some rows do not see must not reach them through 0 * inf
+            bool odd_values = false;
+            if (!(j0 + STEP <= all_see) && j0 < key_to && all_see < key_to) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) odd_values = odd_values || not_finite<T>(vf[kt][ks][w]);
+                odd_values = __ballot(odd_values) != 0;
+                if (odd_values) {
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) vf[kt][ks][w] = finite_only<T>(vf[kt][ks][w]);
+                            if constexpr (HALF) *reinterpret_cast<uint4a*>(mine + (kt * 16 + col) * PITCH + (ks * 4 + quarter) * E) = vf[kt][ks];
+                        }
+                }
+            }
+            asm volatile("" ::: "memory");      // (a wavefront reads what it wrote in order)
+            float4a s[MT][KT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    s[m][kt] = float4a{0, 0, 0, 0};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) s[m][kt] = rows_mfma<T>(kf[kt][ks], qf[m][ks], s[m][kt]);
+                }
+            uint4a now[HALF ? 1 : KS];      // (fp32: this step's values stay in registers while the next ones come)
+            if constexpr (!HALF) {
+#pragma unroll
+                for (int c = 0; c < KS; ++c) now[c] = vf[0][c];
+            }
+            const uint32_t j_now = j0;
+            if (j0 + 4 * STEP < key_to) fetch(j0 + 4 * STEP);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                float high = -INFINITY;
+                bool live[KT][4];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[m][kt][i] *= factor;
+                        live[kt][i] = full || (((keys_here[kt] >> (4 * quarter + i)) & 1) && j_now + kt * 16 + 4 * quarter + i < seen[m]);
+                        high = fmaxf(high, live[kt][i] ? s[m][kt][i] : -INFINITY);
+                    }
+                high = across_groups_max(high);
+                const float above = fmaxf(top[m], high);
+                const float base = above == -INFINITY ? 0.0f : above - kWeightShift<T>;
+                const float old = __builtin_amdgcn_exp2f(top[m] - kWeightShift<T> - base);
+                top[m] = above;
+                float part = 0.0f;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[m][kt][i] = live[kt][i] ? __builtin_amdgcn_exp2f(s[m][kt][i] - base) : 0.0f;
+                        part += s[m][kt][i];
+                    }
+                sum[m] = sum[m] * old + part;
+#pragma unroll
+                for (int t = 0; t < OT; ++t) acc[m][t] *= old;
+            }
+            if constexpr (HALF) {
+                using Lds = __attribute__((address_space(3))) short;
+                typedef short short4a __attribute__((ext_vector_type(4)));
+                using Lds4 = __attribute__((address_space(3))) short4a;
+                uint4a weights[MT];
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    weights[m] = uint4a{pack_weights<T>(s[m][0][0], s[m][0][1]), pack_weights<T>(s[m][0][2], s[m][0][3]), pack_weights<T>(s[m][KT - 1][0], s[m][KT - 1][1]),
+                                        pack_weights<T>(s[m][KT - 1][2], s[m][KT - 1][3])};
+                const T* const read_from = mine + (4 * quarter + col / 4) * PITCH + 4 * (col % 4);
+#pragma unroll
+                for (int t = 0; t < OT; ++t) {
+                    const short4a low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4*)(read_from + t * 16)), high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4*)(read_from + 16 * PITCH + t * 16));
+                    uint4a values;
+                    __builtin_memcpy(&values, &low, 8);
+                    __builtin_memcpy(reinterpret_cast<char*>(&values) + 8, &high, 8);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) acc[m][t] = rows_mfma<T>(values, weights[m], acc[m][t]);
+                }
+            } else {
+                // product i has the keys 4 (lane / 16) + i; tile 4 c + w holds the elements 64 c + 4 (row of the tile) + w
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < KS / 4; ++c)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+#pragma unroll
+                            for (int m = 0; m < MT; ++m)
+                                acc[m][4 * c + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now[i * (KS / 4) + c][w]), s[m][0][i], acc[m][4 * c + w], 0, 0, 0);
+            }
+            if (odd_values) {
+                // the infinite and the NaN, key by key, where they are seen
+#pragma unroll 1
+                for (uint32_t n = 0; n < STEP; ++n) {
+                    int64_t page;
+                    uint32_t in;
+                    const uint32_t j = j_now + n;
+                    if (j >= key_to || !place_of<PAGED>(p, g.s, j, page, in)) continue;
+                    const T* const value = v + page * p.v_page + in * p.v_token + g.head * p.v_head;
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const uint32_t n16 = n % 16;
+                        float mine_w = 0.0f;
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mine_w = n == static_cast<uint32_t>(kt * 16) + 4 * (n16 / 4) + i ? s[m][kt][i] : mine_w;
+                        const float w = __shfl(mine_w, static_cast<int>(16 * (n16 / 4) + col));
+                        if (j < seen[m]) {
+#pragma unroll
+                            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t e = HALF ? t * 16 + 4 * quarter + i : 64 * (t / 4) + 4 * (4 * quarter + i) + t % 4;
+                                    const float x = e < p.d ? static_cast<float>(widen(value[e])) : 0.0f;
+                                    if (!(fabsf(x) < INFINITY)) acc[m][t][i] += w * x;
+                                }
+                        }
+                    }
+                }
+            }
+            asm volatile("" ::: "memory");
+        }
+
+        // ---- the wavefronts meet
+        const uint64_t slot = 2 * static_cast<uint64_t>(blockIdx.x) + (at == from ? 0 : 1);
+        float* const left = partial + slot * partial_floats<ROWS>(p.d);
+        float* const join = reinterpret_cast<float*>(lds_raw);
+        float* const stats = join + 4 * 16 * (DP + 4);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < OT; ++t) {
+                if constexpr (HALF) {
+                    *reinterpret_cast<float4a*>(join + (wave * 16 + col) * (DP + 4) + t * 16 + 4 * quarter) = acc[m][t];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) join[(wave * 16 + col) * (DP + 4) + 64 * (t / 4) + 4 * (4 * quarter + i) + t % 4] = acc[m][t][i];
+                }
+            }
+            const float total = across_groups_sum(sum[m]);
+            if (quarter == 0) {
+                stats[(wave * 16 + col) * 2] = top[m];
+                stats[(wave * 16 + col) * 2 + 1] = total;
+            }
+            __syncthreads();
+            const uint32_t pieces = p.d / 4;
+            for (uint32_t x = threadIdx.x; x < 16 * (DP / 4); x += 256) {
+                const uint32_t r = x / (DP / 4), piece = x % (DP / 4);
+                if (piece >= pieces) continue;
+                float above = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) above = fmaxf(above, stats[(w * 16 + r) * 2]);
+                const float base = above == -INFINITY ? 0.0f : above;
+                float total_weight = 0.0f;
+                float4a value{0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float share = __builtin_amdgcn_exp2f(stats[(w * 16 + r) * 2] - base);
+                    total_weight += stats[(w * 16 + r) * 2 + 1] * share;
+                    value += *reinterpret_cast<const float4a*>(join + (w * 16 + r) * (DP + 4) + piece * 4) * share;
+                }
+                if (whole) {
+                    const uint64_t row = static_cast<uint64_t>(g.tile) * ROWS + m * 16 + r;
+                    const uint32_t i = p.group_div.div(static_cast<uint32_t>(row)), head = g.head * p.group + static_cast<uint32_t>(row) - i * p.group;
+                    if (i < g.span.count) {
+                        T* const to = out + (static_cast<int64_t>(g.span.begin + i) * p.heads + head) * p.d + piece * 4;
+                        const float inverse = total_weight == 0.0f ? 0.0f : 1.0f / total_weight;
+                        T result[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) result[e] = narrow_result<T>(total_weight == 0.0f ? 0.0f : value[e] * inverse);
+                        __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), result, sizeof result);
+                    }
+                } else {
+                    *reinterpret_cast<float4a*>(left + (m * 16 + r) * p.d + piece * 4) = value;
+                    if (piece == 0) {
+                        left[static_cast<size_t>(ROWS) * p.d + 2 * (m * 16 + r)] = above;
+                        left[static_cast<size_t>(ROWS) * p.d + 2 * (m * 16 + r) + 1] = total_weight;
+                    }
+                }
+            }
+        }
+        if (stop == to) return;
+        at = stop;
+        if (!next_group<PAGED, ROWS, kRowsUnit>(p, g)) return;
+        __syncthreads();      // (LDS is read to the end before the next group's values are put there)
+    }
+}
+
+// Puts together the groups that runs' ends cut: the block of the first run that starts inside a group has its rows, blockIdx.y of gridDim.y parts of
+// them.  The parts are added in the order of the runs, whichever block ended first.
+template <class T, int ROWS, bool PAGED>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionProblem p, const float* partial, T* out) {
+    const uint64_t units = all_units<PAGED, ROWS, kRowsUnit>(p);
+    const uint64_t blocks = gridDim.x + 1 < units ? gridDim.x + 1 : units, here = blockIdx.x + 1;
+    if (here >= blocks) return;
+    const uint64_t at = run_start(here, blocks, units);
+    const Group g = group_of<PAGED, ROWS, kRowsUnit>(p, at);
+    if (at == g.first || run_start(here - 1, blocks, units) > g.first) return;
+    const uint64_t first = run_of(g.first, blocks, units), last = run_of(g.first + g.units - 1, blocks, units);
+    const uint32_t pieces = p.d / 4, mine = ROWS / gridDim.y;
+    for (uint32_t x = threadIdx.x; x < mine * pieces; x += 256) {
+        const uint32_t r = blockIdx.y * mine + x / pieces, piece = x % pieces;
+        const uint64_t row = static_cast<uint64_t>(g.tile) * ROWS + r;
+        const uint32_t i = p.group_div.div(static_cast<uint32_t>(row)), head = g.head * p.group + static_cast<uint32_t>(row) - i * p.group;
+        if (i >= g.span.count) continue;
+        float above = -INFINITY, total = 0.0f;
+        float4a value{0, 0, 0, 0};
+        for (uint64_t b = first; b <= last; ++b) {
+            const float* const left = partial + (2 * b + (b == first && run_start(b, blocks, units) != g.first ? 1 : 0)) * partial_floats<ROWS>(p.d);
+            const float its_top = left[static_cast<size_t>(ROWS) * p.d + 2 * r], its_sum = left[static_cast<size_t>(ROWS) * p.d + 2 * r + 1];
+            const float4a its = *reinterpret_cast<const float4a*>(left + r * p.d + piece * 4);
+            const float higher = fmaxf(above, its_top), base = higher == -INFINITY ? 0.0f : higher;
+            const float old = __builtin_amdgcn_exp2f(above - base), share = __builtin_amdgcn_exp2f(its_top - base);
+            total = total * old + its_sum * share;
+            value = value * old + its * share;
+            above = higher;
+        }
+        T* const to = out + (static_cast<int64_t>(g.span.begin + i) * p.heads + head) * p.d + piece * 4;
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        T result[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) result[e] = narrow_result<T>(total == 0.0f ? 0.0f : value[e] * inverse);
+        __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), result, sizeof result);
+    }
+}
+
+constexpr uint32_t kRowsBlocks = 512;      // two on every compute unit
+
+template <class T, int DP, int MT, bool PAGED>
+int launch_rows(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    constexpr int ROWS = 16 * MT;
+    constexpr size_t LDS = rows_lds_bytes<T, DP>();
+    static std::atomic<uint64_t> raised{0};
+    if (LDS > (64u << 10))
+        if (int status = raise_lds_limit(reinterpret_cast<const void*>(attention_rows_kernel<T, DP, MT, PAGED>), LDS, raised); status != TANNIC_SUCCESS) return status;
+    // no more blocks than units there can be
+    const uint64_t tiles = static_cast<uint64_t>(p.tokens) * p.group / ROWS + p.sequences;
+    const uint64_t most = tiles * p.kv_heads * (p.room / kRowsUnit + 1);
+    const uint32_t blocks = most < kRowsBlocks ? static_cast<uint32_t>(most) : kRowsBlocks;
+    float* partial = nullptr;
+    if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * blocks * partial_floats<ROWS>(p.d) * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+    hipLaunchKernelGGL((attention_rows_kernel<T, DP, MT, PAGED>), dim3(blocks), dim3(256), LDS, stream, p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                       static_cast<T*>(out), partial);
+    int status = launch_status("attention_rows_kernel");
+    if (status == TANNIC_SUCCESS && blocks > 1) {
+        hipLaunchKernelGGL((attention_join_kernel<T, ROWS, PAGED>), dim3(blocks - 1, 4), dim3(256), 0, stream, p, partial, static_cast<T*>(out));
+        status = launch_status("attention_join_kernel");
+    }
+    scratch_release(partial, stream);
+    return status;
+}
+
+template <class T, int DP, bool PAGED>
+int pick_rows(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    return launch_rows<T, DP, 1, PAGED>(p, q, k, v, out, stream);
+}
+
+template <class T, bool PAGED>
+int pick_head(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    if (p.d <= 64) return pick_rows<T, 64, PAGED>(p, q, k, v, out, stream);
+    if (p.d <= 128) return pick_rows<T, 128, PAGED>(p, q, k, v, out, stream);
+    return pick_rows<T, 256, PAGED>(p, q, k, v, out, stream);
+}
+
+template <class T>
+int pick_cache(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    if (p.starts) return pick_head<T, true>(p, q, k, v, out, stream);
+    return pick_head<T, false>(p, q, k, v, out, stream);
+}
+
+int attention_rows(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    if (dtype == TANNIC_FLOAT64) return TANNIC_UNSUPPORTED_DTYPE;
+    const int64_t size = static_cast<int64_t>(dtype_size(dtype));
+    // every row of every operand in 16-byte pieces
+    const int64_t grain = p.d | p.q_batch | p.q_token | p.q_head | p.k_page | p.k_head | p.k_token | p.v_page | p.v_head | p.v_token;
+    if ((grain * size) % 16 != 0 || !aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 4 * size)) return TANNIC_UNSUPPORTED_DTYPE;
+    switch (dtype) {
+        case TANNIC_FLOAT16: return pick_cache<f16>(p, q, k, v, out, stream);
+        case TANNIC_BFLOAT16: return pick_cache<bf16>(p, q, k, v, out, stream);
+        default: return pick_cache<float>(p, q, k, v, out, stream);
+    }
+}
+
+}  // namespace th
