@@ -92,98 +92,100 @@ __device__ inline int64_t query_offset(const AttentionProblem& p, uint32_t s, co
 // ---- sharing the keys of all rows between blocks -------------------------------------------------------------------------------
 // A group is a tile of rows of one sequence that read the same keys (a kv head's); its keys come in units.  All groups' units, one group
 // after the other, are dealt to the blocks in equal runs, so that every block reads as many keys as the next whatever the lengths are; a
-// group that a run's end cuts is put together from its blocks' partial results afterwards.  Lengths are known on the device only: every
-// wavefront works the runs out for itself, 64 sequences at a time.
+// group that a run's end cuts is put together from its blocks' partial results by the last of them.  Lengths are known on the device only:
+// every wavefront works the runs out for itself, 64 sequences at a time.
 struct Group {
     uint32_t s, tile, head;      // of `tiles` x kv_heads in the sequence, heads innermost
     Span span;
     uint32_t tiles, units;       // units of each of the sequence's groups
-    uint64_t first;              // the group's first unit among all
+    uint32_t first;              // the group's first unit among all
 };
 
+// Units of all of a sequence's groups.
 template <bool PAGED, int ROWS, int UNIT>
-__device__ inline uint64_t sequence_units(const AttentionProblem& p, uint32_t s, Span& span, uint32_t& tiles, uint32_t& units) {
-    span = span_of<PAGED>(p, s);
+__device__ inline uint32_t sequence_units(const AttentionProblem& p, const Span& span, uint32_t& tiles, uint32_t& units) {
     if (span.count == 0) return tiles = units = 0;
-    tiles = static_cast<uint32_t>((static_cast<uint64_t>(span.count) * p.group + (ROWS - 1)) / ROWS);
+    tiles = (span.count * p.group + (ROWS - 1)) / ROWS;
     const uint32_t keys = keys_seen(p, span, span.count - 1);
     units = keys ? (keys + (UNIT - 1)) / UNIT : 1;      // (rows without keys are written all the same)
-    return static_cast<uint64_t>(tiles) * p.kv_heads * units;
+    return tiles * p.kv_heads * units;
 }
 
-__device__ inline uint64_t lanes_sum_before(uint64_t v, uint64_t& total) {
+// The host sees to it that there are fewer units than this; sequences that overlap, against what the starts may hold, can make more of them,
+// and then nothing is done.
+constexpr uint32_t kMostUnits = (1u << 31) - 1;
+__device__ inline uint32_t sum_units(uint32_t a, uint32_t b) { return a + b < kMostUnits ? a + b : kMostUnits; }
+
+__device__ inline uint32_t lanes_sum_before(uint32_t v, uint32_t& total) {
     const uint32_t lane = threadIdx.x % 64;
-    uint64_t upto = v;
+    uint32_t upto = v;
 #pragma unroll
     for (uint32_t step = 1; step < 64; step *= 2) {
-        const uint64_t below = __shfl_up(upto, step);
-        if (lane >= step) upto += below;
+        const uint32_t below = __shfl_up(upto, step);
+        if (lane >= step) upto = sum_units(upto, below);
     }
-    total = __shfl(upto, 63);
+    total = __builtin_amdgcn_readlane(upto, 63);
     return upto - v;
 }
 
-// Units of all groups together.
-template <bool PAGED, int ROWS, int UNIT>
-__device__ inline uint64_t all_units(const AttentionProblem& p) {
-    uint64_t sum = 0;
-    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
-        const uint32_t s = s0 + threadIdx.x % 64;
-        Span span;
-        uint32_t tiles, units;
-        uint64_t mine = s < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, s, span, tiles, units) : 0, total;
-        lanes_sum_before(mine, total);
-        sum += total;
-    }
-    return sum;
-}
+// The run of this block: units from .. to, and the group that holds the first; false: there is none.
+struct Run {
+    uint32_t per, from, to;
+};
 
-// The group that holds unit `at` (there is one).
 template <bool PAGED, int ROWS, int UNIT>
-__device__ inline Group group_of(const AttentionProblem& p, uint64_t at) {
-    uint64_t base = 0;
-    Group g{};
+__device__ inline bool run_of_block(const AttentionProblem& p, uint32_t blocks, Run& run, Group& g) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint32_t all = 0, mine = 0, before = 0;
     for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
-        const uint32_t s = s0 + threadIdx.x % 64;
-        Span span;
-        uint32_t tiles, units;
-        const uint64_t mine = s < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, s, span, tiles, units) : 0;
-        uint64_t total;
-        const uint64_t before = base + lanes_sum_before(mine, total);
-        if (at < base + total) {
-            const uint64_t here = __ballot(mine > 0 && before <= at && at < before + mine);
-            const int lane = __builtin_ctzll(here);
-            g.s = s0 + lane;
-            g.first = __shfl(before, lane);
-            break;
+        uint32_t tiles, units, total;
+        mine = s0 + lane < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, span_of<PAGED>(p, s0 + lane), tiles, units) : 0;
+        before = all + lanes_sum_before(mine, total);
+        all = sum_units(all, total);
+    }
+    if (all == kMostUnits) return false;
+    run.per = (all + blocks - 1) / blocks;
+    run.from = blockIdx.x * run.per;      // (blocks * per < all + blocks)
+    if (run.from >= all) return false;
+    run.to = run.from + run.per < all ? run.from + run.per : all;
+    uint32_t s0 = 0;
+    if (p.sequences > 64) {      // (else the lanes still have what they found)
+        for (all = 0;; s0 += 64) {
+            if (s0 >= p.sequences) return false;
+            uint32_t tiles, units, total;
+            mine = s0 + lane < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, span_of<PAGED>(p, s0 + lane), tiles, units) : 0;
+            before = all + lanes_sum_before(mine, total);
+            all += total;
+            if (run.from < all) break;
         }
-        base += total;
     }
-    g.s = __builtin_amdgcn_readfirstlane(g.s);
-    sequence_units<PAGED, ROWS, UNIT>(p, g.s, g.span, g.tiles, g.units);
-    const uint64_t number = (at - g.first) / g.units;
+    const uint64_t here = __ballot(before <= run.from && run.from - before < mine);
+    if (here == 0) return false;
+    const int at = __builtin_ctzll(here);
+    g.s = s0 + at;
+    g.first = __builtin_amdgcn_readlane(before, at);
+    g.span = span_of<PAGED>(p, g.s);
+    sequence_units<PAGED, ROWS, UNIT>(p, g.span, g.tiles, g.units);
+    const uint32_t number = (run.from - g.first) / g.units;
     g.first += number * g.units;
-    g.tile = static_cast<uint32_t>(number / p.kv_heads);
-    g.head = static_cast<uint32_t>(number % p.kv_heads);
-    return g;
+    g.tile = number / p.kv_heads;
+    g.head = number % p.kv_heads;
+    return true;
 }
 
-// The group behind g; false: g was the last.
+// The group behind g (there is one).
 template <bool PAGED, int ROWS, int UNIT>
-__device__ inline bool next_group(const AttentionProblem& p, Group& g) {
+__device__ inline void next_group(const AttentionProblem& p, Group& g) {
     g.first += g.units;
-    if (++g.head < p.kv_heads) return true;
+    if (++g.head < p.kv_heads) return;
     g.head = 0;
-    if (++g.tile < g.tiles) return true;
+    if (++g.tile < g.tiles) return;
     g.tile = 0;
-    while (++g.s < p.sequences)
-        if (sequence_units<PAGED, ROWS, UNIT>(p, g.s, g.span, g.tiles, g.units)) return true;
-    return false;
+    while (++g.s < p.sequences) {
+        g.span = span_of<PAGED>(p, g.s);
+        if (sequence_units<PAGED, ROWS, UNIT>(p, g.span, g.tiles, g.units)) return;
+    }
 }
-
-__device__ inline uint64_t run_start(uint64_t block, uint64_t blocks, uint64_t units) { return block * units / blocks; }
-// the block whose run holds a unit: the last one that starts at or before it
-__device__ inline uint64_t run_of(uint64_t unit, uint64_t blocks, uint64_t units) { return ((unit + 1) * blocks - 1) / units; }
 
 // What a block leaves of a group it has a part of: ROWS x d sums, then every row's largest score (in units of log2) and sum of weights.
 // A block has at most two such parts: of the group its run starts in, and of the one it ends in.

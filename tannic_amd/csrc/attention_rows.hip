@@ -7,33 +7,36 @@
 //   values  O^T[element][row] = V^T P^T: the weights are already where the second product wants them - a lane's keys of both tiles are its
 //           eight of the product's 32 - if V's keys are taken in the same order.  16-bit V is transposed on its way out of LDS (ds_read_b64_tr_b16);
 //           fp32 V needs no LDS: an accumulator's four keys are four products.
+#include <exception>
+#include <map>
+#include <mutex>
+
 #include "attention.hpp"
 
 namespace th {
 
 constexpr int kRowsUnit = 64;       // keys of a unit
 
-// A lane's key: where its pieces start, or nowhere.
-struct KeyPlace {
-    int64_t k, v;
-    bool live;
-};
-
-template <class T, bool PAGED>
-__device__ inline KeyPlace key_place(const AttentionProblem& p, uint32_t s, uint32_t j, uint32_t end, uint32_t head) {
-    KeyPlace r{0, 0, false};
-    if (j >= end) return r;
-    int64_t page;
-    uint32_t in;
-    r.live = place_of<PAGED>(p, s, j, page, in);
-    if (r.live) {
-        r.k = page * p.k_page + in * p.k_token + head * p.k_head;
-        r.v = page * p.v_page + in * p.v_token + head * p.v_head;
-    }
-    return r;
-}
-
 template <class T> __device__ inline uint4a load16(const T* at) { return *reinterpret_cast<const uint4a*>(at); }
+
+// Partial results pass from block to block, and between the L2 caches of the dies, through the memory both see: stores and loads of device
+// scope, which no cache in between keeps.  (A store has arrived when the wavefront's count of outstanding ones says so; a release and an
+// acquire around plain accesses would write the die's whole L2 back and drop it: 10 us a call, one token behind 2048.)
+__device__ inline void store_through(float* at, float x, float y) {
+    const uint64_t bits = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(at), bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline void load_through(const float* at, float& x, float& y) {
+    const uint64_t bits = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    x = __uint_as_float(static_cast<uint32_t>(bits));
+    y = __uint_as_float(static_cast<uint32_t>(bits >> 32));
+}
+__device__ inline void load_through(const float* at, float4a& v) {
+    float x, y, z, w;
+    load_through(at, x, y);
+    load_through(at + 2, z, w);
+    v = float4a{x, y, z, w};
+}
 
 template <class T, int DP> constexpr size_t rows_lds_bytes() {
     constexpr size_t join = 4 * 16 * (DP + 4) * 4 + 4 * 16 * 2 * 4, stage = sizeof(T) == 2 ? 4 * 32 * (DP + 16) * 2 : 0;
@@ -41,7 +44,7 @@ template <class T, int DP> constexpr size_t rows_lds_bytes() {
 }
 
 template <class T, int DP, int MT, bool PAGED>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial, uint32_t* arrivals) {
     constexpr bool HALF = sizeof(T) == 2;
     constexpr int ROWS = 16 * MT, E = 16 / sizeof(T);       // elements of a piece
     constexpr int KT = HALF ? 2 : 1, STEP = 16 * KT;        // tiles of 16 keys of a wavefront's step
@@ -50,41 +53,36 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
     constexpr int PITCH = DP + 16;                          // elements from key to key in LDS: the four rows a transposing read touches, and the 16 of a write, on different banks
     extern __shared__ __align__(16) char lds_raw[];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, quarter = lane / 16;
-    const uint64_t units = all_units<PAGED, ROWS, kRowsUnit>(p);
-    const uint64_t blocks = gridDim.x < units ? gridDim.x : units;      // (no run is empty)
-    if (blockIdx.x >= blocks) return;
-    const uint64_t from = run_start(blockIdx.x, blocks, units), to = run_start(blockIdx.x + 1, blocks, units);
-    Group g = group_of<PAGED, ROWS, kRowsUnit>(p, from);
+    __shared__ uint32_t arrived;
+    Run run;
+    Group g;
+    if (!run_of_block<PAGED, ROWS, kRowsUnit>(p, gridDim.x, run, g)) return;
     const float factor = p.scale * 1.44269504088896340736f;      // weights are powers of two
-    uint64_t at = from;
+    uint32_t at = run.from;
     while (true) {
-        const uint64_t stop = g.first + g.units < to ? g.first + g.units : to;
-        const uint32_t key_from = static_cast<uint32_t>(at - g.first) * kRowsUnit;
-        uint32_t key_to = static_cast<uint32_t>(stop - g.first) * kRowsUnit;
+        const uint32_t stop = g.first + g.units < run.to ? g.first + g.units : run.to;
+        const uint32_t key_from = (at - g.first) * kRowsUnit;
+        uint32_t key_to = (stop - g.first) * kRowsUnit;
         const bool whole = at == g.first && stop == g.first + g.units;
 
         // ---- the tile's rows
         uint4a qf[MT][KS];
-        uint32_t seen[MT], most = 0;
-        int64_t to_row[MT];
+        uint32_t seen[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const uint64_t row = static_cast<uint64_t>(g.tile) * ROWS + m * 16 + col;
-            const uint32_t i = p.group_div.div(static_cast<uint32_t>(row)), head = g.head * p.group + static_cast<uint32_t>(row) - i * p.group;
+            const uint32_t row = g.tile * ROWS + m * 16 + col, i = p.group_div.div(row), head = g.head * p.group + row - i * p.group;
             const bool live = i < g.span.count;
             seen[m] = live ? keys_seen(p, g.span, i) : 0;
-            to_row[m] = live ? (static_cast<int64_t>(g.span.begin + i) * p.heads + head) * p.d : -1;
             const T* const from_row = q + (live ? query_offset(p, g.s, g.span, i, head) : 0);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const uint32_t e = (ks * 4 + quarter) * E;
                 qf[m][ks] = live && e < p.d ? load16(from_row + e) : uint4a{0, 0, 0, 0};
             }
-            most = most > seen[m] ? most : seen[m];
         }
         // the last key any row of the tile sees
         const uint32_t last_i = p.group_div.div(g.tile * ROWS + ROWS - 1);
-        most = keys_seen(p, g.span, last_i < g.span.count ? last_i : g.span.count - 1);
+        const uint32_t most = keys_seen(p, g.span, last_i < g.span.count ? last_i : g.span.count - 1);
         key_to = key_to < most ? key_to : most;
         // keys up to here are seen by every live row
         const uint32_t all_see = keys_seen(p, g.span, p.group_div.div(g.tile * ROWS));
@@ -102,23 +100,41 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
         // ---- keys and values of a step: a lane has key lane % 16 of every tile, pieces lane / 16, lane / 16 + 4, ...
         uint4a kf[KT][KS], vf[KT][KS];
         uint32_t there[KT];
-        auto fetch = [&](uint32_t j0) {
+        // which page a step's keys lie in is asked for a step before the keys themselves
+        int64_t page[KT];
+        uint32_t in_page[KT];
+        bool found[KT];
+        auto look_up = [&](uint32_t j0) {
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                const KeyPlace at_key = key_place<T, PAGED>(p, g.s, j0 + kt * 16 + col, key_to, g.head);
-                there[kt] = static_cast<uint32_t>(__ballot(at_key.live)) & 0xFFFFu;
+                const uint32_t j = j0 + kt * 16 + col;
+                found[kt] = j < key_to;
+                if (found[kt]) found[kt] = place_of<PAGED>(p, g.s, j, page[kt], in_page[kt]);
+            }
+        };
+        auto fetch = [&]() {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                there[kt] = static_cast<uint32_t>(__ballot(found[kt])) & 0xFFFFu;
+                const int64_t k_off = found[kt] ? page[kt] * p.k_page + in_page[kt] * p.k_token + g.head * p.k_head : 0;
+                const int64_t v_off = found[kt] ? page[kt] * p.v_page + in_page[kt] * p.v_token + g.head * p.v_head : 0;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t e = (ks * 4 + quarter) * E;
-                    kf[kt][ks] = at_key.live && e < p.d ? load16(k + at_key.k + e) : uint4a{0, 0, 0, 0};
-                    if constexpr (HALF) vf[kt][ks] = at_key.live && e < p.d ? load16(v + at_key.v + e) : uint4a{0, 0, 0, 0};
+                    kf[kt][ks] = found[kt] && e < p.d ? load16(k + k_off + e) : uint4a{0, 0, 0, 0};
                 }
-                if constexpr (!HALF) {
-                    // fp32: piece lane % 16 (+ 16 ks') of the keys 4 (lane / 16) + i; vf[0][i * (KS / 4) + ks'] with KS / 4 = DP / 64
+                if constexpr (HALF) {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const uint32_t e = (ks * 4 + quarter) * E;
+                        vf[kt][ks] = found[kt] && e < p.d ? load16(v + v_off + e) : uint4a{0, 0, 0, 0};
+                    }
+                } else {
+                    // fp32: piece lane % 16 (+ 16 c) of the keys 4 (lane / 16) + i; vf[0][i * (KS / 4) + c] with KS / 4 = DP / 64
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int source = 4 * quarter + i;
-                        const int64_t off = __shfl(at_key.v, source);
+                        const int64_t off = __shfl(v_off, source);
                         const bool live = (there[kt] >> source) & 1;
 #pragma unroll
                         for (int c = 0; c < KS / 4; ++c) {
@@ -131,7 +147,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
         };
         T* const mine = reinterpret_cast<T*>(lds_raw) + wave * (32 * PITCH);
         uint32_t j0 = key_from + wave * STEP;
-        if (j0 < key_to) fetch(j0);
+        if (j0 < key_to) {
+            look_up(j0);
+            fetch();
+            look_up(j0 + 4 * STEP);
+        }
         for (; j0 < key_to; j0 += 4 * STEP) {
             if constexpr (HALF) {
 #pragma unroll
@@ -180,7 +200,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 for (int c = 0; c < KS; ++c) now[c] = vf[0][c];
             }
             const uint32_t j_now = j0;
-            if (j0 + 4 * STEP < key_to) fetch(j0 + 4 * STEP);
+            if (j0 + 4 * STEP < key_to) {
+                fetch();
+                look_up(j0 + 8 * STEP);
+            }
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 float high = -INFINITY;
@@ -276,10 +299,19 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
         }
 
         // ---- the wavefronts meet
-        const uint64_t slot = 2 * static_cast<uint64_t>(blockIdx.x) + (at == from ? 0 : 1);
-        float* const left = partial + slot * partial_floats<ROWS>(p.d);
         float* const join = reinterpret_cast<float*>(lds_raw);
         float* const stats = join + 4 * 16 * (DP + 4);
+        const uint32_t pieces = p.d / 4, rows_left = g.span.count * p.group - g.tile * ROWS, rows = rows_left < ROWS ? rows_left : ROWS;
+        auto write_row = [&](uint32_t r, uint32_t piece, const float4a& value, float total) {
+            const uint32_t row = g.tile * ROWS + r, i = p.group_div.div(row), head = g.head * p.group + row - i * p.group;
+            T* const to = out + (static_cast<int64_t>(g.span.begin + i) * p.heads + head) * p.d + piece * 4;
+            const float inverse = 1.0f / total;
+            T result[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) result[e] = narrow_result<T>(total == 0.0f ? 0.0f : value[e] * inverse);
+            __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), result, sizeof result);
+        };
+        float* const left = partial + (2 * static_cast<uint64_t>(blockIdx.x) + (at == run.from ? 0 : 1)) * partial_floats<ROWS>(p.d);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             __syncthreads();
@@ -298,10 +330,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 stats[(wave * 16 + col) * 2 + 1] = total;
             }
             __syncthreads();
-            const uint32_t pieces = p.d / 4;
             for (uint32_t x = threadIdx.x; x < 16 * (DP / 4); x += 256) {
                 const uint32_t r = x / (DP / 4), piece = x % (DP / 4);
-                if (piece >= pieces) continue;
+                if (piece >= pieces || m * 16 + r >= rows) continue;
                 float above = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) above = fmaxf(above, stats[(w * 16 + r) * 2]);
@@ -315,71 +346,129 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                     value += *reinterpret_cast<const float4a*>(join + (w * 16 + r) * (DP + 4) + piece * 4) * share;
                 }
                 if (whole) {
-                    const uint64_t row = static_cast<uint64_t>(g.tile) * ROWS + m * 16 + r;
-                    const uint32_t i = p.group_div.div(static_cast<uint32_t>(row)), head = g.head * p.group + static_cast<uint32_t>(row) - i * p.group;
-                    if (i < g.span.count) {
-                        T* const to = out + (static_cast<int64_t>(g.span.begin + i) * p.heads + head) * p.d + piece * 4;
-                        const float inverse = total_weight == 0.0f ? 0.0f : 1.0f / total_weight;
-                        T result[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) result[e] = narrow_result<T>(total_weight == 0.0f ? 0.0f : value[e] * inverse);
-                        __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), result, sizeof result);
-                    }
+                    write_row(m * 16 + r, piece, value, total_weight);
                 } else {
-                    *reinterpret_cast<float4a*>(left + (m * 16 + r) * p.d + piece * 4) = value;
-                    if (piece == 0) {
-                        left[static_cast<size_t>(ROWS) * p.d + 2 * (m * 16 + r)] = above;
-                        left[static_cast<size_t>(ROWS) * p.d + 2 * (m * 16 + r) + 1] = total_weight;
+                    store_through(left + (m * 16 + r) * p.d + piece * 4, value[0], value[1]);
+                    store_through(left + (m * 16 + r) * p.d + piece * 4 + 2, value[2], value[3]);
+                    if (piece == 0) store_through(left + static_cast<size_t>(ROWS) * p.d + 2 * (m * 16 + r), above, total_weight);
+                }
+            }
+        }
+        if (!whole) {
+            // The last of the group's blocks to get here puts the parts together, in the order of the runs whichever came first; the
+            // count is 0 again behind it.  (A block's run ends in one group at most: the count of the block that has the group's first unit.)
+            const uint32_t first = g.first / run.per, last = (g.first + g.units - 1) / run.per;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const uint32_t before = __hip_atomic_fetch_add(arrivals + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (before == last - first) __hip_atomic_store(arrivals + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                arrived = before;
+            }
+            __syncthreads();
+            if (arrived == last - first) {
+                // rows * pieces results; where that leaves threads idle, several share a result's parts
+                const uint32_t results = rows * pieces;
+                uint32_t sharing = 1;
+                while (2 * sharing * results <= 256) sharing *= 2;
+                const uint32_t in_share = threadIdx.x / results;
+                for (uint32_t x = sharing == 1 ? threadIdx.x : threadIdx.x % results; x < results && (sharing == 1 || in_share < sharing); x += 256) {
+                    const uint32_t r = x / pieces, piece = x % pieces;
+                    float above = -INFINITY, total = 0.0f;
+                    float4a value{0, 0, 0, 0};
+                    // (four parts on their way at once)
+                    for (uint32_t b0 = first + (sharing == 1 ? 0 : in_share); b0 <= last; b0 += 4 * sharing) {
+                        float its_top[4], its_sum[4];
+                        float4a its_value[4];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const uint32_t b = b0 + n * sharing <= last ? b0 + n * sharing : last;
+                            const float* const its = partial + (2 * static_cast<uint64_t>(b) + (b == first && b * run.per != g.first ? 1 : 0)) * partial_floats<ROWS>(p.d);
+                            load_through(its + static_cast<size_t>(ROWS) * p.d + 2 * r, its_top[n], its_sum[n]);
+                            load_through(its + r * p.d + piece * 4, its_value[n]);
+                        }
+                        float higher = above;
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            if (b0 + n * sharing > last) its_top[n] = -INFINITY, its_sum[n] = 0.0f, its_value[n] = float4a{0, 0, 0, 0};
+                            higher = fmaxf(higher, its_top[n]);
+                        }
+                        const float base = higher == -INFINITY ? 0.0f : higher, old = __builtin_amdgcn_exp2f(above - base);
+                        total *= old;
+                        value *= old;
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const float share = __builtin_amdgcn_exp2f(its_top[n] - base);
+                            total += its_sum[n] * share;
+                            value += its_value[n] * share;
+                        }
+                        above = higher;
+                    }
+                    if (sharing == 1) {
+                        write_row(r, piece, value, total);
+                    } else {
+                        *reinterpret_cast<float4a*>(join + threadIdx.x * 4) = value;
+                        join[1024 + threadIdx.x * 2] = above;
+                        join[1024 + threadIdx.x * 2 + 1] = total;
+                    }
+                }
+                if (sharing > 1) {
+                    __syncthreads();
+                    if (threadIdx.x < results) {
+                        float above = -INFINITY, total = 0.0f;
+                        float4a value{0, 0, 0, 0};
+                        for (uint32_t n = 0; n < sharing; ++n) above = fmaxf(above, join[1024 + (n * results + threadIdx.x) * 2]);
+                        const float base = above == -INFINITY ? 0.0f : above;
+                        for (uint32_t n = 0; n < sharing; ++n) {
+                            const uint32_t from = n * results + threadIdx.x;
+                            const float share = __builtin_amdgcn_exp2f(join[1024 + from * 2] - base);
+                            total += join[1024 + from * 2 + 1] * share;
+                            value += *reinterpret_cast<const float4a*>(join + from * 4) * share;
+                        }
+                        write_row(threadIdx.x / pieces, threadIdx.x % pieces, value, total);
                     }
                 }
             }
         }
-        if (stop == to) return;
+        if (stop == run.to) return;
         at = stop;
-        if (!next_group<PAGED, ROWS, kRowsUnit>(p, g)) return;
+        next_group<PAGED, ROWS, kRowsUnit>(p, g);
         __syncthreads();      // (LDS is read to the end before the next group's values are put there)
     }
 }
 
-// Puts together the groups that runs' ends cut: the block of the first run that starts inside a group has its rows, blockIdx.y of gridDim.y parts of
-// them.  The parts are added in the order of the runs, whichever block ended first.
-template <class T, int ROWS, bool PAGED>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionProblem p, const float* partial, T* out) {
-    const uint64_t units = all_units<PAGED, ROWS, kRowsUnit>(p);
-    const uint64_t blocks = gridDim.x + 1 < units ? gridDim.x + 1 : units, here = blockIdx.x + 1;
-    if (here >= blocks) return;
-    const uint64_t at = run_start(here, blocks, units);
-    const Group g = group_of<PAGED, ROWS, kRowsUnit>(p, at);
-    if (at == g.first || run_start(here - 1, blocks, units) > g.first) return;
-    const uint64_t first = run_of(g.first, blocks, units), last = run_of(g.first + g.units - 1, blocks, units);
-    const uint32_t pieces = p.d / 4, mine = ROWS / gridDim.y;
-    for (uint32_t x = threadIdx.x; x < mine * pieces; x += 256) {
-        const uint32_t r = blockIdx.y * mine + x / pieces, piece = x % pieces;
-        const uint64_t row = static_cast<uint64_t>(g.tile) * ROWS + r;
-        const uint32_t i = p.group_div.div(static_cast<uint32_t>(row)), head = g.head * p.group + static_cast<uint32_t>(row) - i * p.group;
-        if (i >= g.span.count) continue;
-        float above = -INFINITY, total = 0.0f;
-        float4a value{0, 0, 0, 0};
-        for (uint64_t b = first; b <= last; ++b) {
-            const float* const left = partial + (2 * b + (b == first && run_start(b, blocks, units) != g.first ? 1 : 0)) * partial_floats<ROWS>(p.d);
-            const float its_top = left[static_cast<size_t>(ROWS) * p.d + 2 * r], its_sum = left[static_cast<size_t>(ROWS) * p.d + 2 * r + 1];
-            const float4a its = *reinterpret_cast<const float4a*>(left + r * p.d + piece * 4);
-            const float higher = fmaxf(above, its_top), base = higher == -INFINITY ? 0.0f : higher;
-            const float old = __builtin_amdgcn_exp2f(above - base), share = __builtin_amdgcn_exp2f(its_top - base);
-            total = total * old + its_sum * share;
-            value = value * old + its * share;
-            above = higher;
-        }
-        T* const to = out + (static_cast<int64_t>(g.span.begin + i) * p.heads + head) * p.d + piece * 4;
-        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-        T result[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) result[e] = narrow_result<T>(total == 0.0f ? 0.0f : value[e] * inverse);
-        __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), result, sizeof result);
-    }
-}
-
 constexpr uint32_t kRowsBlocks = 512;      // two on every compute unit
+
+// The counts of blocks that have left their part of a group: one array per stream, 0 between calls.  It is cleared once, on a stream of its
+// own, so that a first call that is being recorded does not leave the clearing to the replay; kept until the process ends.
+int arrivals_of(hipStream_t stream, uint32_t*& arrivals) try {
+    static std::mutex mutex;
+    static std::map<std::pair<int, hipStream_t>, uint32_t*> known;
+    int device = 0;
+    TH_TRY(hipGetDevice(&device));
+    std::lock_guard<std::mutex> lock(mutex);
+    const auto at = known.try_emplace({device, stream}, nullptr).first;
+    if (at->second == nullptr) {
+        void* counts = nullptr;
+        hipStream_t own = nullptr;
+        hipError_t err = hipMalloc(&counts, kRowsBlocks * sizeof(uint32_t));
+        if (err == hipSuccess) err = hipStreamCreateWithFlags(&own, hipStreamNonBlocking);
+        if (err == hipSuccess) err = hipMemsetAsync(counts, 0, kRowsBlocks * sizeof(uint32_t), own);
+        if (err == hipSuccess) err = hipStreamSynchronize(own);
+        if (own) (void)hipStreamDestroy(own);
+        if (err != hipSuccess) {
+            if (counts) (void)hipFree(counts);
+            set_error("attention: counts of arrivals", __FILE__, __LINE__, err);
+            return TANNIC_ERROR;
+        }
+        at->second = static_cast<uint32_t*>(counts);
+    }
+    arrivals = at->second;
+    return TANNIC_SUCCESS;
+} catch (const std::exception& e) {
+    set_error_text(e.what());
+    return TANNIC_ERROR;
+}
 
 template <class T, int DP, int MT, bool PAGED>
 int launch_rows(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
@@ -391,16 +480,15 @@ int launch_rows(const AttentionProblem& p, const void* q, const void* k, const v
     // no more blocks than units there can be
     const uint64_t tiles = static_cast<uint64_t>(p.tokens) * p.group / ROWS + p.sequences;
     const uint64_t most = tiles * p.kv_heads * (p.room / kRowsUnit + 1);
+    if (most >= kMostUnits) return TANNIC_UNSUPPORTED_DTYPE;
     const uint32_t blocks = most < kRowsBlocks ? static_cast<uint32_t>(most) : kRowsBlocks;
+    uint32_t* arrivals = nullptr;
+    if (int status = arrivals_of(stream, arrivals); status != TANNIC_SUCCESS) return status;
     float* partial = nullptr;
     if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * blocks * partial_floats<ROWS>(p.d) * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
     hipLaunchKernelGGL((attention_rows_kernel<T, DP, MT, PAGED>), dim3(blocks), dim3(256), LDS, stream, p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                       static_cast<T*>(out), partial);
-    int status = launch_status("attention_rows_kernel");
-    if (status == TANNIC_SUCCESS && blocks > 1) {
-        hipLaunchKernelGGL((attention_join_kernel<T, ROWS, PAGED>), dim3(blocks - 1, 4), dim3(256), 0, stream, p, partial, static_cast<T*>(out));
-        status = launch_status("attention_join_kernel");
-    }
+                       static_cast<T*>(out), partial, arrivals);
+    const int status = launch_status("attention_rows_kernel");
     scratch_release(partial, stream);
     return status;
 }
