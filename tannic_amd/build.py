@@ -41,6 +41,7 @@ UNITS = [
     ("shape_ops.hip", "shape_ops.o", []),
     ("attention.hip", "attention.o", []),
     ("attention_rows.hip", "attention_rows.o", []),
+    ("attention_tile.hip", "attention_tile.o", []),
     ("cache.hip", "cache.o", EXACT),
     ("gemm.hip", "gemm.o", []),
     ("gemm_mfma.hip", "gemm_mfma.o", []),

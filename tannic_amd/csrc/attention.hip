@@ -3,6 +3,10 @@
 // A Tannic program writes it as products, a scale, a mask and a softmax, which need keys and values in one dense tensor and move the
 // scores through memory four times; here a row's scores live in registers, and its softmax is folded key by key:
 //   top' = max(top, s),  sum' = sum * exp(top - top') + exp(s - top'),  acc' = acc * exp(top - top') + exp(s - top') * V
+#include <exception>
+#include <map>
+#include <mutex>
+
 #include "attention.hpp"
 #include "lanes.hpp"
 
@@ -94,6 +98,37 @@ __global__ __launch_bounds__(256) void attention_any_kernel(AttentionProblem p, 
     }
 }
 
+// The counts of blocks that have left their part of a group: one array per stream, 0 between calls.  It is cleared once, on a stream of its
+// own, so that a first call that is being recorded does not leave the clearing to the replay; kept until the process ends.
+int attention_arrivals(hipStream_t stream, uint32_t*& arrivals) try {
+    static std::mutex mutex;
+    static std::map<std::pair<int, hipStream_t>, uint32_t*> known;
+    int device = 0;
+    TH_TRY(hipGetDevice(&device));
+    std::lock_guard<std::mutex> lock(mutex);
+    const auto at = known.try_emplace({device, stream}, nullptr).first;
+    if (at->second == nullptr) {
+        void* counts = nullptr;
+        hipStream_t own = nullptr;
+        hipError_t err = hipMalloc(&counts, kAttentionArrivals * sizeof(uint32_t));
+        if (err == hipSuccess) err = hipStreamCreateWithFlags(&own, hipStreamNonBlocking);
+        if (err == hipSuccess) err = hipMemsetAsync(counts, 0, kAttentionArrivals * sizeof(uint32_t), own);
+        if (err == hipSuccess) err = hipStreamSynchronize(own);
+        if (own) (void)hipStreamDestroy(own);
+        if (err != hipSuccess) {
+            if (counts) (void)hipFree(counts);
+            set_error("attention: counts of arrivals", __FILE__, __LINE__, err);
+            return TANNIC_ERROR;
+        }
+        at->second = static_cast<uint32_t*>(counts);
+    }
+    arrivals = at->second;
+    return TANNIC_SUCCESS;
+} catch (const std::exception& e) {
+    set_error_text(e.what());
+    return TANNIC_ERROR;
+}
+
 template <class T>
 int run_attention(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
     const dim3 grid(p.tokens * p.heads);
@@ -103,8 +138,19 @@ int run_attention(const AttentionProblem& p, const void* q, const void* k, const
     return launch_status("attention_any_kernel");
 }
 
+// The kernels that take every row of every operand in 16-byte pieces: tiles of 128 rows of the matrix pipe where the sequences have that many on average, else few rows at a time.
+int attention_pieces(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    const int64_t size = static_cast<int64_t>(dtype_size(dtype));
+    const int64_t grain = p.d | p.q_batch | p.q_token | p.q_head | p.k_page | p.k_head | p.k_token | p.v_page | p.v_head | p.v_token;
+    if ((grain * size) % 16 != 0 || !aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 4 * size)) return TANNIC_UNSUPPORTED_DTYPE;
+    if (static_cast<uint64_t>(p.tokens) * p.group >= 64ull * p.sequences) {
+        if (int status = attention_tile(dtype, p, q, k, v, out, stream); status != TANNIC_UNSUPPORTED_DTYPE) return status;
+    }
+    return attention_rows(dtype, p, q, k, v, out, stream);
+}
+
 int run_attention(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
-    if (int status = attention_rows(dtype, p, q, k, v, out, stream); status != TANNIC_UNSUPPORTED_DTYPE) return status;
+    if (int status = attention_pieces(dtype, p, q, k, v, out, stream); status != TANNIC_UNSUPPORTED_DTYPE) return status;
     switch (dtype) {
         case TANNIC_FLOAT16: return run_attention<f16>(p, q, k, v, out, stream);
         case TANNIC_BFLOAT16: return run_attention<bf16>(p, q, k, v, out, stream);

@@ -247,8 +247,32 @@ template <class T> __device__ inline uint32_t finite_only(uint32_t x) {
 // fp16 weights are kept 2^8 times as large: those below 2^-22 of the largest lose bits first, not those below 2^-14
 template <class T> constexpr float kWeightShift = std::is_same_v<T, f16> ? 8.0f : 0.0f;
 
-// Whether the kernels of 16-byte pieces take the operands, and which of them.  SUCCESS, or UNSUPPORTED_DTYPE: they do not.
+// Partial results pass from block to block, and between the L2 caches of the dies, through the memory both see: stores and loads of device
+// scope, which no cache in between keeps.  (A store has arrived when the wavefront's count of outstanding ones says so; a release and an
+// acquire around plain accesses would write the die's whole L2 back and drop it: 10 us a call, one token behind 2048.)
+__device__ inline void store_through(float* at, float x, float y) {
+    const uint64_t bits = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(at), bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline void load_through(const float* at, float& x, float& y) {
+    const uint64_t bits = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    x = __uint_as_float(static_cast<uint32_t>(bits));
+    y = __uint_as_float(static_cast<uint32_t>(bits >> 32));
+}
+__device__ inline void load_through(const float* at, float4a& v) {
+    float x, y, z, w;
+    load_through(at, x, y);
+    load_through(at + 2, z, w);
+    v = float4a{x, y, z, w};
+}
+
+// How many blocks of a group have left their part: counts on a stream, 0 between calls.
+constexpr uint32_t kAttentionArrivals = 1024;
+int attention_arrivals(hipStream_t stream, uint32_t*& arrivals);
+
+// The kernels of 16-byte pieces.  UNSUPPORTED_DTYPE: nothing was done, another kernel has to take the operands.
 int attention_rows(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream);
+int attention_tile(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream);
 
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 

@@ -7,10 +7,6 @@
 //   values  O^T[element][row] = V^T P^T: the weights are already where the second product wants them - a lane's keys of both tiles are its
 //           eight of the product's 32 - if V's keys are taken in the same order.  16-bit V is transposed on its way out of LDS (ds_read_b64_tr_b16);
 //           fp32 V needs no LDS: an accumulator's four keys are four products.
-#include <exception>
-#include <map>
-#include <mutex>
-
 #include "attention.hpp"
 
 namespace th {
@@ -18,25 +14,6 @@ namespace th {
 constexpr int kRowsUnit = 64;       // keys of a unit
 
 template <class T> __device__ inline uint4a load16(const T* at) { return *reinterpret_cast<const uint4a*>(at); }
-
-// Partial results pass from block to block, and between the L2 caches of the dies, through the memory both see: stores and loads of device
-// scope, which no cache in between keeps.  (A store has arrived when the wavefront's count of outstanding ones says so; a release and an
-// acquire around plain accesses would write the die's whole L2 back and drop it: 10 us a call, one token behind 2048.)
-__device__ inline void store_through(float* at, float x, float y) {
-    const uint64_t bits = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(at), bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ inline void load_through(const float* at, float& x, float& y) {
-    const uint64_t bits = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    x = __uint_as_float(static_cast<uint32_t>(bits));
-    y = __uint_as_float(static_cast<uint32_t>(bits >> 32));
-}
-__device__ inline void load_through(const float* at, float4a& v) {
-    float x, y, z, w;
-    load_through(at, x, y);
-    load_through(at + 2, z, w);
-    v = float4a{x, y, z, w};
-}
 
 template <class T, int DP> constexpr size_t rows_lds_bytes() {
     constexpr size_t join = 4 * 16 * (DP + 4) * 4 + 4 * 16 * 2 * 4, stage = sizeof(T) == 2 ? 4 * 32 * (DP + 16) * 2 : 0;
@@ -439,36 +416,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
 
 constexpr uint32_t kRowsBlocks = 512;      // two on every compute unit
 
-// The counts of blocks that have left their part of a group: one array per stream, 0 between calls.  It is cleared once, on a stream of its
-// own, so that a first call that is being recorded does not leave the clearing to the replay; kept until the process ends.
-int arrivals_of(hipStream_t stream, uint32_t*& arrivals) try {
-    static std::mutex mutex;
-    static std::map<std::pair<int, hipStream_t>, uint32_t*> known;
-    int device = 0;
-    TH_TRY(hipGetDevice(&device));
-    std::lock_guard<std::mutex> lock(mutex);
-    const auto at = known.try_emplace({device, stream}, nullptr).first;
-    if (at->second == nullptr) {
-        void* counts = nullptr;
-        hipStream_t own = nullptr;
-        hipError_t err = hipMalloc(&counts, kRowsBlocks * sizeof(uint32_t));
-        if (err == hipSuccess) err = hipStreamCreateWithFlags(&own, hipStreamNonBlocking);
-        if (err == hipSuccess) err = hipMemsetAsync(counts, 0, kRowsBlocks * sizeof(uint32_t), own);
-        if (err == hipSuccess) err = hipStreamSynchronize(own);
-        if (own) (void)hipStreamDestroy(own);
-        if (err != hipSuccess) {
-            if (counts) (void)hipFree(counts);
-            set_error("attention: counts of arrivals", __FILE__, __LINE__, err);
-            return TANNIC_ERROR;
-        }
-        at->second = static_cast<uint32_t*>(counts);
-    }
-    arrivals = at->second;
-    return TANNIC_SUCCESS;
-} catch (const std::exception& e) {
-    set_error_text(e.what());
-    return TANNIC_ERROR;
-}
+static_assert(kRowsBlocks <= kAttentionArrivals);
 
 template <class T, int DP, int MT, bool PAGED>
 int launch_rows(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
@@ -483,7 +431,7 @@ int launch_rows(const AttentionProblem& p, const void* q, const void* k, const v
     if (most >= kMostUnits) return TANNIC_UNSUPPORTED_DTYPE;
     const uint32_t blocks = most < kRowsBlocks ? static_cast<uint32_t>(most) : kRowsBlocks;
     uint32_t* arrivals = nullptr;
-    if (int status = arrivals_of(stream, arrivals); status != TANNIC_SUCCESS) return status;
+    if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
     float* partial = nullptr;
     if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * blocks * partial_floats<ROWS>(p.d) * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
     hipLaunchKernelGGL((attention_rows_kernel<T, DP, MT, PAGED>), dim3(blocks), dim3(256), LDS, stream, p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
@@ -512,15 +460,11 @@ int pick_cache(const AttentionProblem& p, const void* q, const void* k, const vo
 }
 
 int attention_rows(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
-    if (dtype == TANNIC_FLOAT64) return TANNIC_UNSUPPORTED_DTYPE;
-    const int64_t size = static_cast<int64_t>(dtype_size(dtype));
-    // every row of every operand in 16-byte pieces
-    const int64_t grain = p.d | p.q_batch | p.q_token | p.q_head | p.k_page | p.k_head | p.k_token | p.v_page | p.v_head | p.v_token;
-    if ((grain * size) % 16 != 0 || !aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 4 * size)) return TANNIC_UNSUPPORTED_DTYPE;
     switch (dtype) {
         case TANNIC_FLOAT16: return pick_cache<f16>(p, q, k, v, out, stream);
         case TANNIC_BFLOAT16: return pick_cache<bf16>(p, q, k, v, out, stream);
-        default: return pick_cache<float>(p, q, k, v, out, stream);
+        case TANNIC_FLOAT32: return pick_cache<float>(p, q, k, v, out, stream);
+        default: return TANNIC_UNSUPPORTED_DTYPE;
     }
 }
 

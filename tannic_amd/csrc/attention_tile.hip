@@ -1,0 +1,540 @@
+// Attention of many rows (chunks of a prompt, a decoder's inputs over an encoder's states), 16-bit types: bound by the matrix pipe.
+// A block's four wavefronts have 32 rows each of one tile (a sequence's tokens times the heads of a group) and walk through the keys in steps of KT:
+// keys and values of the next step go from memory straight to LDS while this step's are multiplied, all wavefronts reading the same ones.
+//   scores  S^T[key][row] = K Q^T on v_mfma_f32_32x32x16: a lane has one row (lane % 32) and 16 of the tile's 32 keys, so that a row's
+//           maximum and sum are one value per lane, and one exchange with the lane 32 further;
+//   values  O^T[element][row] = V^T P^T: the lane's weights are the second product's operand as they are, if V's keys are taken in the
+//           accumulator's order; V is transposed on its way out of LDS (ds_read_b64_tr_b16).
+// The running maximum follows the scores only when one exceeds it by 2^8 (in the weights' power of two): sums in fp32 have the room, and the
+// 64 to 128 sums of a lane are rescaled a few times in a row's life instead of every step.
+#include "attention.hpp"
+
+namespace th {
+
+// ---- items: a tile's rows of one kv head over a chunk of its keys -----------------------------------------------------------------
+// Every sequence has tiles x kv heads groups of `chunks` items, those of the last tile (which see the most keys) first.  With fewer groups than blocks that run
+// at a time the keys are shared in chunks; the last of a group's blocks puts its parts together.
+struct Item {
+    uint32_t s, tile, head, chunk, chunk_units;      // units of a chunk
+    uint32_t number;                                 // among all
+    Span span;
+};
+
+template <bool PAGED, int ROWS, int UNIT>
+__device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_shared, uint32_t least_units, Item& item) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint32_t all = 0, groups = 0;
+    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
+        uint32_t tiles = 0, units = 0, total;
+        const uint32_t mine = s0 + lane < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, span_of<PAGED>(p, s0 + lane), tiles, units) : 0;
+        lanes_sum_before(mine, total);
+        all = sum_units(all, total);
+        lanes_sum_before(tiles * p.kv_heads, total);
+        groups = sum_units(groups, total);
+    }
+    if (all == kMostUnits) return false;
+    uint32_t per = kMostUnits;
+    if (groups < most_shared) {
+        per = (all + most_shared - 1) / most_shared;
+        per = per > least_units ? per : least_units;
+    }
+    uint32_t before_all = 0;
+    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
+        uint32_t tiles = 0, units = 0, total;
+        if (s0 + lane < p.sequences) sequence_units<PAGED, ROWS, UNIT>(p, span_of<PAGED>(p, s0 + lane), tiles, units);
+        const uint32_t chunks = units > per ? (units + per - 1) / per : 1, mine = tiles * p.kv_heads * chunks;
+        const uint32_t before = before_all + lanes_sum_before(mine, total);
+        const uint64_t here = __ballot(before <= blockIdx.x && blockIdx.x - before < mine);
+        if (here) {
+            const int at = __builtin_ctzll(here);
+            item.s = s0 + at;
+            item.span = span_of<PAGED>(p, item.s);
+            sequence_units<PAGED, ROWS, UNIT>(p, item.span, tiles, units);
+            const uint32_t its_chunks = units > per ? (units + per - 1) / per : 1;
+            uint32_t rest = blockIdx.x - __builtin_amdgcn_readlane(before, at);
+            item.chunk = rest % its_chunks;
+            rest /= its_chunks;
+            item.head = rest % p.kv_heads;
+            item.tile = tiles - 1 - rest / p.kv_heads;
+            item.chunk_units = per;
+            item.number = blockIdx.x;
+            return true;
+        }
+        before_all = sum_units(before_all, total);
+    }
+    return false;
+}
+
+typedef float float16a __attribute__((ext_vector_type(16)));
+
+template <class T> __device__ inline float16a tile_mfma(uint4a a, uint4a b, float16a c) {
+    if constexpr (std::is_same_v<T, f16>) {
+        typedef _Float16 V __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    } else {
+        typedef __bf16 V __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    }
+}
+
+// the other half's value (lane ^ 32) beside this lane's
+__device__ inline float halves_max(float x) {
+    const uint2a r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float halves_sum(float x) {
+    const uint2a r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+using LdsVoid = __attribute__((address_space(3))) void*;
+using GlobalVoid = __attribute__((address_space(1))) void*;
+
+// Eight transposing reads of 16 keys of V (the four tiles of 32 elements, two of the keys' four rows each) and the wait for them in one statement:
+// as builtins they would be made to wait for the loads to LDS that are on their way for the next step.
+__device__ inline void read_values(uint32_t at0, uint32_t at1, uint32_t at2, uint32_t at3, uint32_t next, uint4a v[4]) {
+    uint2a a0, a1, b0, b1, c0, c1, d0, d1;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\t"
+        "ds_read_b64_tr_b16 %1, %12\n\t"
+        "ds_read_b64_tr_b16 %2, %9\n\t"
+        "ds_read_b64_tr_b16 %3, %13\n\t"
+        "ds_read_b64_tr_b16 %4, %10\n\t"
+        "ds_read_b64_tr_b16 %5, %14\n\t"
+        "ds_read_b64_tr_b16 %6, %11\n\t"
+        "ds_read_b64_tr_b16 %7, %15\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(a0), "=&v"(a1), "=&v"(b0), "=&v"(b1), "=&v"(c0), "=&v"(c1), "=&v"(d0), "=&v"(d1)
+        : "v"(at0), "v"(at1), "v"(at2), "v"(at3), "v"(at0 + next), "v"(at1 + next), "v"(at2 + next), "v"(at3 + next)
+        : "memory");
+    v[0] = uint4a{a0[0], a0[1], a1[0], a1[1]};
+    v[1] = uint4a{b0[0], b0[1], b1[0], b1[1]};
+    v[2] = uint4a{c0[0], c0[1], c1[0], c1[1]};
+    v[3] = uint4a{d0[0], d0[1], d1[0], d1[1]};
+}
+__device__ inline void read_values(uint32_t at0, uint32_t at1, uint32_t next, uint4a v[2]) {
+    uint2a a0, a1, b0, b1;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4\n\t"
+        "ds_read_b64_tr_b16 %1, %6\n\t"
+        "ds_read_b64_tr_b16 %2, %5\n\t"
+        "ds_read_b64_tr_b16 %3, %7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(a0), "=&v"(a1), "=&v"(b0), "=&v"(b1)
+        : "v"(at0), "v"(at1), "v"(at0 + next), "v"(at1 + next)
+        : "memory");
+    v[0] = uint4a{a0[0], a0[1], a1[0], a1[1]};
+    v[1] = uint4a{b0[0], b0[1], b1[0], b1[1]};
+}
+
+constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
+template <int DP> constexpr int kTileKeys = DP > 128 ? 32 : 64;
+template <int DP> constexpr size_t tile_lds_bytes() { return 4 * kTileKeys<DP> * DP * 2 + 2 * kTileKeys<DP> + 16; }
+
+template <class T, int DP, bool PAGED>
+__global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_tile_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial, uint32_t* arrivals,
+                                                                                          uint32_t most_shared, uint32_t least_units) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int KT = kTileKeys<DP>, NT = KT / 32;         // keys of a step, tiles of 32 of them
+    constexpr int KS = DP / 16, OT = DP / 32;               // products of a tile's scores; tiles of 32 elements
+    constexpr int LPR = DP / 8, RPI = 64 / LPR;             // 16-byte pieces of a row; rows of a load
+    constexpr int KPW = KT / kTileWaves, LOADS = KPW / RPI; // keys a wavefront brings, in so many loads each for K and V
+    constexpr uint32_t TILE = KT * DP * 2;                  // bytes
+    extern __shared__ __align__(16) char lds_raw[];         // K, V of step 0; K, V of step 1; which keys of either are there
+    uint8_t* const there = reinterpret_cast<uint8_t*>(lds_raw + 4 * TILE);
+    volatile uint32_t* const arrived = reinterpret_cast<volatile uint32_t*>(lds_raw + 4 * TILE + 2 * KT);
+    volatile uint32_t* const odd_step = arrived + 1;     // the step in which a value was not finite
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
+    Item item;
+    if (!item_of_block<PAGED, kTileRows, KT>(p, most_shared, least_units, item)) return;
+    const Span span = item.span;
+    const uint32_t rows_all = span.count * p.group;
+    const uint32_t first_i = p.group_div.div(item.tile * kTileRows);
+    uint32_t last_i = p.group_div.div(item.tile * kTileRows + kTileRows - 1);
+    last_i = last_i < span.count ? last_i : span.count - 1;
+    const uint32_t all_see = keys_seen(p, span, first_i), most = keys_seen(p, span, last_i);     // by every row of the tile, by the last
+    const uint32_t units = most ? (most + KT - 1) / KT : 1, chunks = units > item.chunk_units ? (units + item.chunk_units - 1) / item.chunk_units : 1;
+    if (item.chunk >= chunks) return;      // (the tile sees fewer keys than the sequence's last)
+    const uint32_t key_from = chunks > 1 ? item.chunk * item.chunk_units * KT : 0;
+    const uint32_t key_end = chunks > 1 ? key_from + item.chunk_units * KT : most;
+    const uint32_t key_to = key_end < most ? key_end : most;
+
+    // ---- this lane's row
+    const uint32_t row = item.tile * kTileRows + wave * 32 + col, i_row = p.group_div.div(row), q_head = item.head * p.group + row - i_row * p.group;
+    const bool row_lives = i_row < span.count;
+    const uint32_t seen = row_lives ? keys_seen(p, span, i_row) : 0;
+    // a negative scale turns the queries round, so that the largest score is that of the largest product; without a scale they are 0
+    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u, keep = p.scale == 0.0f ? 0u : ~0u;
+    const float factor = (p.scale == 0.0f ? 1.0f : fabsf(p.scale)) * 1.44269504088896340736f;
+    uint4a qf[KS];
+    {
+        const T* const from = q + (row_lives ? query_offset(p, item.s, span, i_row, q_head) : 0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const uint32_t e = ks * 16 + half * 8;
+            uint4a x = row_lives && e < p.d ? *reinterpret_cast<const uint4a*>(from + e) : uint4a{0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x[w] = (x[w] ^ flip) & keep;
+            qf[ks] = x;
+        }
+    }
+
+    // ---- bringing a step's keys and values to LDS
+    // A row's pieces lie in an order of their own, so that the 16 rows a score's operand takes the same piece of, and the four rows of a transposing read, fall
+    // on different banks.
+    auto k_place = [](uint32_t r) -> uint32_t { return DP == 64 ? (r >> 1) & 7u : r & 15u; };
+    auto v_place = [](uint32_t r) -> uint32_t { return DP == 64 ? ((r >> 1) & 1u) * 4 : (r & 3u) * 4; };
+    uint32_t k_lane[LOADS], v_lane[LOADS];      // bytes from the wavefront's first key
+    uint32_t k_pieces = 0, v_pieces = 0;        // bit i: the lane's piece of load i is one of the head's (d may be below DP)
+    const uint32_t piece = lane % LPR, row_in = lane / LPR;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const uint32_t r = i * RPI + row_in, in_tile = wave * KPW + r, k_piece = piece ^ k_place(in_tile), v_piece = piece ^ v_place(in_tile);
+        k_lane[i] = r * static_cast<uint32_t>(p.k_token) * 2 + k_piece * 16;
+        v_lane[i] = r * static_cast<uint32_t>(p.v_token) * 2 + v_piece * 16;
+        k_pieces |= (k_piece * 8 < p.d ? 1u : 0u) << i;
+        v_pieces |= (v_piece * 8 < p.d ? 1u : 0u) << i;
+    }
+    // (places beyond the head's pieces are never written: 0 all the time)
+    if (p.d < DP) {
+        for (uint32_t x = threadIdx.x; x < 4 * TILE / 16; x += 64 * kTileWaves) reinterpret_cast<uint4a*>(lds_raw)[x] = uint4a{0, 0, 0, 0};
+        __syncthreads();
+    }
+    // A wavefront's keys of a step mostly lie in one page, whose number is asked for a step before; key by key otherwise.
+    const bool together = !PAGED || p.page % KPW == 0;
+    uint32_t next_page = ~0u, next_in = 0;
+    auto look_up = [&](uint32_t j0) {
+        const uint32_t j = j0 + wave * KPW;
+        int64_t page = -1;
+        next_page = ~0u;
+        if (together && j + KPW <= key_to && place_of<PAGED>(p, item.s, j, page, next_in)) next_page = static_cast<uint32_t>(page);
+    };
+    auto bring = [&](uint32_t j0, uint32_t buffer) {
+        char* const k_to = lds_raw + buffer * (2 * TILE) + wave * (LOADS * 1024);
+        char* const v_to = k_to + TILE;
+        const uint32_t page = __builtin_amdgcn_readfirstlane(next_page), in_page = __builtin_amdgcn_readfirstlane(next_in);
+        if (page != ~0u) {
+            const char* const k_from = reinterpret_cast<const char*>(k + (page * p.k_page + in_page * p.k_token + item.head * p.k_head));
+            const char* const v_from = reinterpret_cast<const char*>(v + (page * p.v_page + in_page * p.v_token + item.head * p.v_head));
+            if (p.d == DP) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) __builtin_amdgcn_global_load_lds((GlobalVoid)(k_from + k_lane[i]), (LdsVoid)(k_to + i * 1024), 16, 0, 0);
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) __builtin_amdgcn_global_load_lds((GlobalVoid)(v_from + v_lane[i]), (LdsVoid)(v_to + i * 1024), 16, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    if (k_pieces & (1u << i)) __builtin_amdgcn_global_load_lds((GlobalVoid)(k_from + k_lane[i]), (LdsVoid)(k_to + i * 1024), 16, 0, 0);
+                    if (v_pieces & (1u << i)) __builtin_amdgcn_global_load_lds((GlobalVoid)(v_from + v_lane[i]), (LdsVoid)(v_to + i * 1024), 16, 0, 0);
+                }
+            }
+            if (lane < KPW) there[buffer * KT + wave * KPW + lane] = 1;
+        } else {
+#pragma unroll 1
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                const uint32_t r = i * RPI + row_in, in_tile = wave * KPW + r, j = j0 + in_tile;
+                int64_t its_page = 0;
+                uint32_t in = 0;
+                const bool lives = j < key_to && place_of<PAGED>(p, item.s, j, its_page, in);
+                const uint32_t k_piece = piece ^ k_place(in_tile), v_piece = piece ^ v_place(in_tile);
+                if (lives && (k_pieces & (1u << i)))
+                    __builtin_amdgcn_global_load_lds((GlobalVoid)(k + (its_page * p.k_page + in * p.k_token + item.head * p.k_head + k_piece * 8)), (LdsVoid)(k_to + i * 1024), 16, 0, 0);
+                if (lives && (v_pieces & (1u << i)))
+                    __builtin_amdgcn_global_load_lds((GlobalVoid)(v + (its_page * p.v_page + in * p.v_token + item.head * p.v_head + v_piece * 8)), (LdsVoid)(v_to + i * 1024), 16, 0, 0);
+                if (!lives) *reinterpret_cast<uint4a*>(v_to + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};      // (what was there may be infinite; its weight is 0)
+                if (piece == 0) there[buffer * KT + in_tile] = lives;
+            }
+        }
+    };
+    auto arrive = [] {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    float16a acc[OT];
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    float top = -INFINITY, sum = 0.0f;      // of the products before the scale; the lane's own keys
+
+    // where this lane reads: K's row col (+ 32 per tile), V's rows 4 half + lane / 4 % 4 (+ 8 per read), elements 16 (lane / 16 % 2) + 4 (lane % 4)
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsVoid)lds_raw));
+    const uint32_t v_row = 4 * half + (lane % 16) / 4;
+    uint32_t v_at[OT];
+#pragma unroll
+    for (int t = 0; t < OT; ++t) {
+        const uint32_t v_piece = t * 4 + ((lane / 16) % 2) * 2 + (lane % 4) / 2;
+        v_at[t] = lds_at + TILE + v_row * (DP * 2) + (v_piece ^ v_place(v_row)) * 16 + (lane % 2) * 8;
+    }
+
+    if (threadIdx.x == 0) *odd_step = 0;
+    if (key_from < key_to) {
+        look_up(key_from);
+        bring(key_from, 0);
+        look_up(key_from + KT);
+    }
+    arrive();
+    uint32_t buffer = 0, odd_from = ~0u;
+    for (uint32_t j0 = key_from; j0 < key_to; j0 += KT, buffer ^= 1) {
+        const uint64_t keys = __ballot(there[buffer * KT + lane % KT] != 0);      // (32 keys: twice the same)
+        if (j0 + KT < key_to) {
+            bring(j0 + KT, buffer ^ 1);
+            look_up(j0 + 2 * KT);
+        }
+        const char* const k_tile = lds_raw + buffer * (2 * TILE);
+        const bool full = keys == ~0ull && j0 + KT <= all_see;
+        // Values that some of the tile's rows do not see must not reach those through 0 * inf: where there are such keys, the infinite and the NaN
+        // among the values are 0 for the product, and are added in the end where they are seen.
+        if (j0 + KT > all_see && all_see < most) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                uint4a* const at = reinterpret_cast<uint4a*>(lds_raw + buffer * (2 * TILE) + TILE + wave * (LOADS * 1024) + i * 1024 + lane * 16);
+                uint4a x = *at;
+                bool odd = false;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) odd = odd || not_finite<T>(x[w]);
+                if (odd) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) x[w] = finite_only<T>(x[w]);
+                    *at = x;
+                    *odd_step = j0 + 1;
+                }
+            }
+            __syncthreads();
+            if (*odd_step == j0 + 1 && odd_from == ~0u) odd_from = j0;
+        }
+        // (a few keys' pieces at a time: all of them at once would take the registers of the sums)
+        float16a s[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+        uint4a kf[2][2 * NT];
+        auto read_keys = [&](int ks, uint4a to[2 * NT]) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint32_t r = n * 32 + col;
+                    to[u * NT + n] = *reinterpret_cast<const uint4a*>(k_tile + r * (DP * 2) + (((ks + u) * 2 + half) ^ k_place(r)) * 16);
+                }
+        };
+        read_keys(0, kf[0]);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks += 2) {
+            if (ks + 2 < KS) read_keys(ks + 2, kf[(ks / 2 + 1) % 2]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[n] = tile_mfma<T>(kf[(ks / 2) % 2][u * NT + n], qf[ks + u], s[n]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // a lane's keys are 32 n + 8 (i / 4) + 4 half + i % 4
+        if (!full) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t from = j0 + n * 32, left = seen > from ? seen - from : 0;
+                const uint32_t mine = (static_cast<uint32_t>(keys >> (32 * n)) & (left < 32 ? (1u << left) - 1 : ~0u)) >> (4 * half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(mine & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
+            }
+        }
+        float high = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) high = fmaxf(high, s[n][i]);
+        high = halves_max(high);
+        if (__ballot(high * factor > top * factor + 8.0f || (top == -INFINITY && high > -INFINITY))) {
+            const float above = fmaxf(top, high);
+            const float old = top == above ? 1.0f : __builtin_amdgcn_exp2f((top - above) * factor);
+            top = above;
+            sum *= old;
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][i] *= old;
+        }
+        const float base = top == -INFINITY ? 0.0f : top * factor - kWeightShift<T> / 2;
+        uint32_t weights[NT][8];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], factor, -base)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], factor, -base));
+                sum += x;
+                sum += y;
+                weights[n][i / 2] = pack_weights<T>(x, y);
+            }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const uint4a w{weights[n][kk * 4], weights[n][kk * 4 + 1], weights[n][kk * 4 + 2], weights[n][kk * 4 + 3]};
+                const uint32_t from = buffer * (2 * TILE) + (n * 32 + kk * 16) * (DP * 2);
+#pragma unroll
+                for (int t = 0; t < OT; t += 4) {
+                    uint4a values[4];
+                    if constexpr (OT >= 4) read_values(v_at[t] + from, v_at[t + 1] + from, v_at[t + 2] + from, v_at[t + 3] + from, 8 * (DP * 2), values);
+                    else read_values(v_at[0] + from, v_at[1] + from, 8 * (DP * 2), values);
+#pragma unroll
+                    for (int u = 0; u < (OT < 4 ? OT : 4); ++u) acc[t + u] = tile_mfma<T>(values[u], w, acc[t + u]);
+                }
+            }
+        arrive();
+    }
+    sum = halves_sum(sum);
+    if (odd_from < key_to) {
+#pragma unroll 1
+        for (uint32_t j = odd_from; j < key_to; ++j) {
+            int64_t page;
+            uint32_t in;
+            if (!place_of<PAGED>(p, item.s, j, page, in) || j >= seen) continue;
+            const T* const value = v + page * p.v_page + static_cast<int64_t>(in) * p.v_token + item.head * p.v_head;
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t e = t * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                    const float x = e < p.d ? static_cast<float>(widen(value[e])) : 0.0f;
+                    if (!(fabsf(x) < INFINITY)) acc[t][i] += x;      // (any weight above 0 says the same)
+                    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+    }
+
+    // ---- a lane has its row's elements 32 t + 8 (i / 4) + 4 half + i % 4
+    T* const to = out + (static_cast<int64_t>(span.begin + i_row) * p.heads + q_head) * p.d;
+    if (chunks == 1) {
+        if (row_lives) {
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const uint32_t e = t * 32 + 2 * i + 4 * half;
+                    if (e < p.d) {
+                        T result[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) result[u] = narrow_result<T>(sum == 0.0f ? 0.0f : acc[t][i + u] * inverse);
+                        __builtin_memcpy(__builtin_assume_aligned(to + e, 8), result, 8);
+                    }
+                }
+        }
+        return;
+    }
+    // ---- or a part of it, put together by the group's last block (attention.hpp: through the memory that all dies see)
+    const uint32_t rows = rows_all - item.tile * kTileRows < kTileRows ? rows_all - item.tile * kTileRows : kTileRows, my_row = wave * 32 + col;
+    const uint64_t slot = partial_floats<kTileRows>(p.d);
+    {
+        float* const left = partial + item.number * slot;
+        if (row_lives) {
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const uint32_t e = t * 32 + 2 * i + 4 * half;
+                    if (e < p.d) {
+                        store_through(left + my_row * p.d + e, acc[t][i], acc[t][i + 1]);
+                        store_through(left + my_row * p.d + e + 2, acc[t][i + 2], acc[t][i + 3]);
+                    }
+                }
+            if (half == 0) store_through(left + static_cast<size_t>(kTileRows) * p.d + 2 * my_row, top == -INFINITY ? -INFINITY : top * factor, sum);
+        }
+    }
+    const uint32_t first = item.number - item.chunk;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(arrivals + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == chunks - 1) __hip_atomic_store(arrivals + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *arrived = before;
+    }
+    __syncthreads();
+    if (*arrived != chunks - 1) return;
+    const uint32_t pieces = p.d / 4;
+    const float* const parts = partial + first * slot;
+    for (uint32_t x = threadIdx.x; x < rows * pieces; x += 64 * kTileWaves) {
+        const uint32_t r = x / pieces, e = x % pieces * 4;
+        float above = -INFINITY, total = 0.0f;
+        float4a value{0, 0, 0, 0};
+        for (uint32_t c0 = 0; c0 < chunks; c0 += 4) {
+            float its_top[4], its_sum[4];
+            float4a its_value[4];
+#pragma unroll
+            for (uint32_t n = 0; n < 4; ++n) {
+                const float* const its = parts + (c0 + n < chunks ? c0 + n : chunks - 1) * slot;
+                load_through(its + static_cast<size_t>(kTileRows) * p.d + 2 * r, its_top[n], its_sum[n]);
+                load_through(its + r * p.d + e, its_value[n]);
+            }
+            float higher = above;
+#pragma unroll
+            for (uint32_t n = 0; n < 4; ++n) {
+                if (c0 + n >= chunks) its_top[n] = -INFINITY, its_sum[n] = 0.0f, its_value[n] = float4a{0, 0, 0, 0};
+                higher = fmaxf(higher, its_top[n]);
+            }
+            const float base = higher == -INFINITY ? 0.0f : higher, old = __builtin_amdgcn_exp2f(above - base);
+            total *= old;
+            value *= old;
+#pragma unroll
+            for (uint32_t n = 0; n < 4; ++n) {
+                const float share = __builtin_amdgcn_exp2f(its_top[n] - base);
+                total += its_sum[n] * share;
+                value += its_value[n] * share;
+            }
+            above = higher;
+        }
+        const uint32_t its_row = item.tile * kTileRows + r, i = p.group_div.div(its_row), head = item.head * p.group + its_row - i * p.group;
+        T result[4];
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) result[u] = narrow_result<T>(total == 0.0f ? 0.0f : value[u] * inverse);
+        __builtin_memcpy(__builtin_assume_aligned(out + (static_cast<int64_t>(span.begin + i) * p.heads + head) * p.d + e, 8), result, 8);
+    }
+#endif
+}
+
+constexpr uint32_t kTileShared = 512;       // groups from which on keys are not shared: two blocks on every compute unit
+constexpr uint32_t kTileLeast = 4;          // units of a chunk, at least
+
+template <class T, int DP, bool PAGED>
+int launch_tile(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    constexpr size_t LDS = tile_lds_bytes<DP>();
+    static std::atomic<uint64_t> raised{0};
+    if (LDS > (64u << 10))
+        if (int status = raise_lds_limit(reinterpret_cast<const void*>(attention_tile_kernel<T, DP, PAGED>), LDS, raised); status != TANNIC_SUCCESS) return status;
+    // as many blocks as there can be items: shared groups have at most kTileShared items more than there are groups
+    const uint64_t groups = (static_cast<uint64_t>(p.tokens) * p.group / kTileRows + p.sequences) * p.kv_heads;
+    if (groups * (p.room / kTileKeys<DP> + 1) >= kMostUnits || groups + kTileShared >= kMostUnits) return TANNIC_UNSUPPORTED_DTYPE;
+    uint32_t* arrivals = nullptr;
+    if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
+    static_assert(2 * kTileShared <= kAttentionArrivals);
+    float* partial = nullptr;
+    if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * kTileShared * partial_floats<kTileRows>(p.d) * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+    hipLaunchKernelGGL((attention_tile_kernel<T, DP, PAGED>), dim3(static_cast<uint32_t>(groups + kTileShared)), dim3(64 * kTileWaves), LDS, stream, p, static_cast<const T*>(q),
+                       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(out), partial, arrivals, kTileShared, kTileLeast);
+    const int status = launch_status("attention_tile_kernel");
+    scratch_release(partial, stream);
+    return status;
+}
+
+template <class T, bool PAGED>
+int pick_tile(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    if (p.d <= 64) return launch_tile<T, 64, PAGED>(p, q, k, v, out, stream);
+    if (p.d <= 128) return launch_tile<T, 128, PAGED>(p, q, k, v, out, stream);
+    return launch_tile<T, 256, PAGED>(p, q, k, v, out, stream);
+}
+
+int attention_tile(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    // (a lane's offsets from its wavefront's first key fit 32 bits)
+    const int64_t far = int64_t(1) << 25;
+    if (p.k_token < 0 || p.v_token < 0 || p.k_token >= far || p.v_token >= far) return TANNIC_UNSUPPORTED_DTYPE;
+    if (dtype == TANNIC_FLOAT16) return p.starts ? pick_tile<f16, true>(p, q, k, v, out, stream) : pick_tile<f16, false>(p, q, k, v, out, stream);
+    if (dtype == TANNIC_BFLOAT16) return p.starts ? pick_tile<bf16, true>(p, q, k, v, out, stream) : pick_tile<bf16, false>(p, q, k, v, out, stream);
+    return TANNIC_UNSUPPORTED_DTYPE;
+}
+
+}  // namespace th
