@@ -36,7 +36,7 @@ class DeviceLibrary:
             fn.restype, fn.argtypes = res, args
             self.kernels[name] = fn
             call = self.cdll["tannic_hip_" + name]
-            call.restype, call.argtypes = res, [C.c_char_p if a is abi.TP else C.c_size_t if a is abi.stream_t else a for a in args]
+            call.restype, call.argtypes = res, [C.c_char_p if a is abi.TP else C.c_size_t if a is abi.stream_t else C.c_void_p if a is abi.I32P else a for a in args]
             self.calls[name] = call
         for name, (res, args) in abi.runtime_signatures().items():
             fn = getattr(self.cdll, "tannic_hip_" + name)

@@ -13,8 +13,8 @@ namespace th {
 struct AppendProblem {
     PageTable pages;
     uint32_t tokens, heads, d;              // heads: of q, 0 without it
-    uint32_t d_vectors, row_vectors;        // vectors of a head, of a token's rows of q, k and v
-    FastDiv d_vectors_div;
+    uint32_t rows, side;                    // a token's rows of q, k and v; how many of them a block holds side by side
+    FastDiv d_vectors_div;                  // vectors of a row
     int64_t q_token, q_head, k_token, k_head, v_token, v_head;
     int64_t kc_page, kc_head, kc_token, vc_page, vc_head, vc_token;
     uint32_t positions;                     // rows of the tables of angles, 0: nothing is rotated
@@ -27,88 +27,98 @@ struct alignas(WHOLE ? 16 : sizeof(T)) Few {
     T v[N];
 };
 
-template <class T>
-__device__ inline float angle_at(const void* table, size_t at, bool wide) {
-    return wide ? static_cast<const float*>(table)[at] : static_cast<float>(widen(static_cast<const T*>(table)[at]));
-}
-
-// A block per token; VEC elements of a row per thread.  The pairs (2i, 2i + 1) turn in fp32 (float64: in double) and are rounded once, as tannic_hip_rope does.
-template <class T, int VEC, bool WHOLE>
+// blockIdx.x: a token, blockIdx.y: ROUNDS times as many of its rows as 256 threads hold side by side.  A thread has the same elements of all its rows, so that the angles
+// are loaded once (before: with every vector, 49.5 us for 8500 tokens of 32 + 2 * 8 heads of 128), and asks for the rows before the lengths and the table
+// have said where they go.  The pairs (2i, 2i + 1) turn in fp32 (float64: in double) and are rounded once, as tannic_hip_rope does.
+template <class T, int VEC, bool WHOLE, int ROUNDS>
 __global__ __launch_bounds__(256) void append_pages_kernel(AppendProblem p, const T* q, const T* k, const T* v, const void* cs, const void* sn, T* keys, T* values, T* turned) {
     using A = std::conditional_t<std::is_same_v<T, double>, double, float>;
     using Vector = Few<T, VEC, WHOLE>;
+    constexpr int PAIRS = VEC > 1 ? VEC / 2 : 1;
     const uint32_t token = blockIdx.x;
+    uint32_t beside, e;
+    p.d_vectors_div.divmod(threadIdx.x, beside, e);
+    e *= VEC;
+    if (beside >= p.side) beside = p.rows;      // (threads over: no row)
+    const uint32_t first = blockIdx.y * (p.side * ROUNDS) + beside;
+    Vector x[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const uint32_t head = first + r * p.side < p.rows ? first + r * p.side : p.rows - 1;
+        const T* const row = head < p.heads ? q + token * p.q_token + head * p.q_head
+                             : head < p.heads + p.pages.kv_heads ? k + token * p.k_token + (head - p.heads) * p.k_head
+                                                                 : v + token * p.v_token + (head - p.heads - p.pages.kv_heads) * p.v_head;
+        x[r] = *reinterpret_cast<const Vector*>(row + e);
+    }
     const uint32_t s = sequence_of(p.pages.starts, p.pages.sequences, token);
     const int32_t from = p.pages.starts[s], to = p.pages.starts[s + 1], before = p.pages.context[s];
     if (static_cast<int32_t>(token) < from || static_cast<int32_t>(token) >= to) return;      // no sequence's token
     // (from is at most the token's number; a negative one is taken as 0)
     const uint64_t position = static_cast<uint64_t>(before < 0 ? 0 : before) + (token - static_cast<uint32_t>(from < 0 ? 0 : from));
     bool held = position < p.pages.room;
-    uint32_t column = 0, row = 0;
+    uint32_t column = 0, in_page = 0;
     int32_t page = -1;
     if (held) {
-        p.pages.page_div.divmod(static_cast<uint32_t>(position), column, row);
+        p.pages.page_div.divmod(static_cast<uint32_t>(position), column, in_page);
         page = p.pages.table[static_cast<int64_t>(s) * p.pages.table_row + column];
         held = static_cast<uint32_t>(page) < p.pages.pages;
     }
-    const size_t angles = static_cast<size_t>(position < p.positions ? position : p.positions ? p.positions - 1 : 0) * (p.d / 2);
-    for (uint32_t i = threadIdx.x; i < p.row_vectors; i += 256) {
-        uint32_t head, e;
-        p.d_vectors_div.divmod(i, head, e);
-        e *= VEC;
-        const T* from_row;
-        T* to_row;
-        bool turn = p.positions > 0;
-        if (head < p.heads) {
-            from_row = q + token * p.q_token + head * p.q_head;
-            to_row = turned + (static_cast<size_t>(token) * p.heads + head) * p.d;
-        } else {
-            if (!held) return;      // (the rows of q come first)
-            head -= p.heads;
-            if (head < p.pages.kv_heads) {
-                from_row = k + token * p.k_token + head * p.k_head;
-                to_row = keys + page * p.kc_page + head * p.kc_head + row * p.kc_token;
-            } else {
-                head -= p.pages.kv_heads;
-                from_row = v + token * p.v_token + head * p.v_head;
-                to_row = values + page * p.vc_page + head * p.vc_head + row * p.vc_token;
-                turn = false;
-            }
-        }
-        Vector x = *reinterpret_cast<const Vector*>(from_row + e);
-        if constexpr (VEC > 1) {
-            if (turn) {
+    A c[PAIRS], n[PAIRS];
+    const bool turns = VEC > 1 && p.positions > 0;
+    if (turns) {
+        const size_t at = static_cast<size_t>(position < p.positions ? position : p.positions - 1) * (p.d / 2) + e / 2;
+        if (p.wide_angles) {
+            const auto cv = *reinterpret_cast<const Few<float, PAIRS, false>*>(static_cast<const float*>(cs) + at), nv = *reinterpret_cast<const Few<float, PAIRS, false>*>(static_cast<const float*>(sn) + at);
 #pragma unroll
-                for (int u = 0; u < VEC; u += 2) {
-                    A c, n;
-                    if constexpr (std::is_same_v<T, double>) {
-                        c = p.wide_angles ? static_cast<const float*>(cs)[angles + (e + u) / 2] : static_cast<const double*>(cs)[angles + (e + u) / 2];
-                        n = p.wide_angles ? static_cast<const float*>(sn)[angles + (e + u) / 2] : static_cast<const double*>(sn)[angles + (e + u) / 2];
-                    } else {
-                        c = angle_at<T>(cs, angles + (e + u) / 2, p.wide_angles);
-                        n = angle_at<T>(sn, angles + (e + u) / 2, p.wide_angles);
-                    }
-                    const A even = static_cast<A>(widen(x.v[u])), odd = static_cast<A>(widen(x.v[u + 1]));
-                    x.v[u] = narrow<T>(even * c - odd * n);
-                    x.v[u + 1] = narrow<T>(even * n + odd * c);
-                }
+            for (int u = 0; u < PAIRS; ++u) c[u] = cv.v[u], n[u] = nv.v[u];
+        } else {
+            const auto cv = *reinterpret_cast<const Few<T, PAIRS, false>*>(static_cast<const T*>(cs) + at), nv = *reinterpret_cast<const Few<T, PAIRS, false>*>(static_cast<const T*>(sn) + at);
+#pragma unroll
+            for (int u = 0; u < PAIRS; ++u) c[u] = static_cast<A>(widen(cv.v[u])), n[u] = static_cast<A>(widen(nv.v[u]));
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        uint32_t head = first + r * p.side;
+        if (head >= p.rows) return;
+        if (turns && head < p.heads + p.pages.kv_heads) {
+#pragma unroll
+            for (int u = 0; u + 1 < VEC; u += 2) {
+                const A even = static_cast<A>(widen(x[r].v[u])), odd = static_cast<A>(widen(x[r].v[u + 1]));
+                x[r].v[u] = narrow<T>(even * c[u / 2] - odd * n[u / 2]);
+                x[r].v[u + 1] = narrow<T>(even * n[u / 2] + odd * c[u / 2]);
             }
         }
-        *reinterpret_cast<Vector*>(to_row + e) = x;
+        T* row;
+        if (head < p.heads) row = turned + (static_cast<size_t>(token) * p.heads + head) * p.d;
+        else if (!held) return;      // (the rows of q come first)
+        else if (head < p.heads + p.pages.kv_heads) row = keys + page * p.kc_page + (head - p.heads) * p.kc_head + in_page * p.kc_token;
+        else row = values + page * p.vc_page + (head - p.heads - p.pages.kv_heads) * p.vc_head + in_page * p.vc_token;
+        *reinterpret_cast<Vector*>(row + e) = x[r];
     }
 }
 
 template <class T, int VEC, bool WHOLE>
 int launch_append(AppendProblem& p, const void* q, const void* k, const void* v, const void* cs, const void* sn, void* keys, void* values, void* turned, hipStream_t stream) {
-    p.d_vectors = p.d / VEC;
-    p.row_vectors = p.d_vectors * (p.heads + 2 * p.pages.kv_heads);
-    p.d_vectors_div = FastDiv(p.d_vectors);
-    hipLaunchKernelGGL((append_pages_kernel<T, VEC, WHOLE>), dim3(p.tokens), dim3(256), 0, stream, p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), cs, sn,
-                       static_cast<T*>(keys), static_cast<T*>(values), static_cast<T*>(turned));
-    return launch_status("append_pages_kernel");
+    const uint32_t vectors = p.d / VEC;
+    p.rows = p.heads + 2 * p.pages.kv_heads;
+    p.side = 256 / vectors;
+    p.d_vectors_div = FastDiv(vectors);
+    auto launch = [&](auto rounds) {
+        constexpr int ROUNDS = decltype(rounds)::value;
+        const dim3 grid(p.tokens, (p.rows + p.side * ROUNDS - 1) / (p.side * ROUNDS));
+        if (grid.y > 65535) return refuse("append_pages: so many heads of this size are not supported");
+        hipLaunchKernelGGL((append_pages_kernel<T, VEC, WHOLE, ROUNDS>), grid, dim3(256), 0, stream, p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), cs, sn,
+                           static_cast<T*>(keys), static_cast<T*>(values), static_cast<T*>(turned));
+        return launch_status("append_pages_kernel");
+    };
+    // few tokens: a row per thread, on more blocks
+    if (p.tokens * static_cast<uint64_t>(p.rows) * vectors < 256 * 1024) return launch(std::integral_constant<int, 1>{});
+    return launch(std::integral_constant<int, 3>{});
 }
 
 // ---- pages to pages -----------------------------------------------------------------------------------------------------------
+typedef uint32_t uint4c __attribute__((ext_vector_type(4)));
 constexpr int kCopyDims = 4;      // dims in front of the pages, at most
 struct CopyPlace {
     uint32_t lead[kCopyDims];     // extents in front of the pages
@@ -121,8 +131,8 @@ struct CopyPairs {
     int32_t source[N], target[N];
 };
 
-// One page (of one layer, keys or values) per blockIdx.y and z; a block moves 256 * UNROLL vectors.
-template <class V, int N, int UNROLL>
+// One page (of one layer, keys or values) per blockIdx.y and z, a vector per thread (512 MB of pages past the caches, us with one / two / four: 195 / 199 / 201).
+template <class V, int N, bool PAST>
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyPlace p, CopyPairs<N> pairs, char* pool) {
     uint32_t rest = blockIdx.z;
     int64_t off = 0;
@@ -133,25 +143,24 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyPlace p, CopyPairs<
     }
     const V* const from = reinterpret_cast<const V*>(pool + off + pairs.source[blockIdx.y] * p.page_stride);
     V* const to = reinterpret_cast<V*>(pool + off + pairs.target[blockIdx.y] * p.page_stride);
-    const uint32_t first = blockIdx.x * (256 * UNROLL) + threadIdx.x;
-    V x[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-        if (first + u * 256 < p.units) x[u] = from[first + u * 256];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-        if (first + u * 256 < p.units) to[first + u * 256] = x[u];
+    const uint32_t at = blockIdx.x * 256 + threadIdx.x;
+    if (at >= p.units) return;
+    if constexpr (PAST) __builtin_nontemporal_store(__builtin_nontemporal_load(from + at), to + at);
+    else to[at] = from[at];
 }
+
+constexpr uint64_t kCopyPast = uint64_t(64) << 20;      // bytes of a launch
 
 template <class V, int N>
 int launch_copy(CopyPlace p, uint64_t page_bytes, uint32_t leads, const int32_t* sources, const int32_t* targets, uint32_t count, char* pool, hipStream_t stream) {
-    constexpr int UNROLL = 4;
     CopyPairs<N> pairs;
     std::memcpy(pairs.source, sources, count * sizeof(int32_t));
     std::memcpy(pairs.target, targets, count * sizeof(int32_t));
     p.units = static_cast<uint32_t>(page_bytes / sizeof(V));
-    const dim3 grid((p.units + 256 * UNROLL - 1) / (256 * UNROLL), count, leads);
-    hipLaunchKernelGGL((copy_pages_kernel<V, N, UNROLL>), grid, dim3(256), 0, stream, p, pairs, pool);
+    const dim3 grid((p.units + 255) / 256, count, leads);
+    // A compaction goes past the caches (512 MB of pages 210 us through them, 195 past them); what a fork copies is read soon after (4.7 both ways).
+    if (page_bytes * leads * count >= kCopyPast) hipLaunchKernelGGL((copy_pages_kernel<V, N, true>), grid, dim3(256), 0, stream, p, pairs, pool);
+    else hipLaunchKernelGGL((copy_pages_kernel<V, N, false>), grid, dim3(256), 0, stream, p, pairs, pool);
     return launch_status("copy_pages_kernel");
 }
 
@@ -175,7 +184,7 @@ int run_copies(const CopyPlace& p, uint64_t page_bytes, uint32_t leads, uint32_t
         if (from.empty()) return TANNIC_SUCCESS;
         const uint32_t n = static_cast<uint32_t>(from.size());
         int status;
-        if (grain % 16 == 0) status = launch_copy<uint4>(p, page_bytes, leads, from.data(), to.data(), n, pool, stream);
+        if (grain % 16 == 0) status = launch_copy<uint4c>(p, page_bytes, leads, from.data(), to.data(), n, pool, stream);
         else if (grain % 4 == 0) status = launch_copy<uint32_t>(p, page_bytes, leads, from.data(), to.data(), n, pool, stream);
         else status = launch_copy<uint8_t>(p, page_bytes, leads, from.data(), to.data(), n, pool, stream);
         for (uint32_t i = 0; marks && i < n; ++i) touched[from[i]] = touched[to[i]] = 0;
@@ -228,7 +237,7 @@ int tannic_hip_append_pages(const tannic_tensor_t* k, const tannic_tensor_t* v, 
             !rows_contiguous(cos) || !rows_contiguous(sin))
             return refuse("append_pages: cos and sin [positions, d/2], contiguous, for an even d");
     }
-    if (tokens >= (1ull << 31) || heads >= (1u << 16) || d >= (1u << 12)) return refuse("append_pages: 2^31 tokens, 2^16 heads or heads of 4096 elements or more are not supported");
+    if (tokens >= (1ull << 31) || heads >= (1u << 16) || d > 256) return refuse("append_pages: 2^31 tokens, 2^16 heads or heads of more than 256 elements are not supported");
     if (tokens == 0 || d == 0 || heads + k->shape.sizes[1] == 0 || p.pages.sequences == 0) return TANNIC_SUCCESS;
     if (int status = on_device_of("append_pages: the operands live on a device", keys, values, k, v, table, starts, context, cos, sin, q, turned); status != TANNIC_SUCCESS) return status;
     p.tokens = static_cast<uint32_t>(tokens);

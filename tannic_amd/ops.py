@@ -10,6 +10,7 @@ this package: they raise unless a host function table was registered with
 ``set_host_functions`` (the test-suite registers its CPU checker there, the way
 the reference pairs ``cpu::f`` with ``cuda::f``).
 """
+import array
 import builtins
 import ctypes as C
 import math
@@ -567,62 +568,76 @@ def rope(x, cos, sin):
 # ``keys``, ``values [pages, kv heads, page, d]`` hold every sequence's tokens in pages; ``table [sequences, columns]`` (int32) names them,
 # -1 where there is none; ``starts [sequences + 1]`` and ``context [sequences]`` (int32) say which rows of a call are a sequence's new tokens
 # and how many tokens it had before.  All of them are read on the device: a recorded call follows what is written into them.
-def _device_call(name, operands, arguments):
-    """One backend call whose operands may be missing; ``arguments(stream)`` in the order of the ABI."""
-    env = _resolve(*[t for t in operands if t is not None])
+def _device_of(name, *tensors):
+    env = _resolve(*tensors)
     if env.kind != abi.DEVICE:
         raise BackendError(f"{name}: operands are on the host and tannic_amd holds device kernels only")
-    lib = library()
-    status = lib.calls[name](*arguments(env.stream_number()))
+    return env
+
+
+def _checked(name, status):
     if status != abi.SUCCESS:
-        detail = lib.error_message() if status == abi.ERROR else ""
+        detail = library().error_message() if status == abi.ERROR else ""
         raise TannicError(f"Unsupported dtype ({name}: {abi.STATUS_NAMES[status]}{' ' + detail if detail else ''})")
-
-
-def _packed(t):
-    return None if t is None else t.packed()
 
 
 def append_pages(k, v, keys, values, table, starts, context, cos=None, sin=None, q=None):
     """Writes the new tokens' ``k``, ``v [tokens, kv heads, d]`` into the pages of their sequences, behind ``context``.  With ``cos, sin
     [positions, d/2]`` the keys turn by their positions first, as ``rope`` turns them, and so does ``q [tokens, heads, d]``, which is returned."""
-    turned = None if q is None else _new(q.dtype, q.shape, _resolve(q, k))
-    operands = (k, v, table, starts, context, cos, sin, q, keys, values, turned)
-    _device_call("append_pages", operands, lambda stream: (*map(_packed, operands), stream))
+    given = [t for t in (cos, sin, q) if t is not None]
+    env = _device_of("append_pages", k, v, keys, values, table, starts, context, *given)
+    turned = None if q is None else Tensor.fresh(q.dtype, q.shape, env)
+    _checked("append_pages", library().calls["append_pages"](
+        k.packed(), v.packed(), table.packed(), starts.packed(), context.packed(), None if cos is None else cos.packed(), None if sin is None else sin.packed(),
+        None if q is None else q.packed(), keys.packed(), values.packed(), None if q is None else turned.packed(), env.stream_number()))
     return turned
 
 
 def attend_pages(q, keys, values, table, starts, context, scale=None):
     """Attention of the new tokens ``q [tokens, heads, d]`` over their sequences' pages, every token over the keys up to its own position
     (written before, see ``append_pages``); ``[tokens, heads, d]``, contiguous.  ``scale`` is ``1 / sqrt(d)`` if not given."""
-    operands = (q, keys, values, table, starts, context, _new(q.dtype, q.shape, _resolve(q, keys)))
+    env = _device_of("attend_pages", q, keys, values, table, starts, context)
+    dst = Tensor.fresh(q.dtype, q.shape, env)
     scale = 1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else scale
-    _device_call("attend_pages", operands, lambda stream: (*[t.packed() for t in operands], stream, scale))
-    return operands[-1]
+    _checked("attend_pages", library().calls["attend_pages"](q.packed(), keys.packed(), values.packed(), table.packed(), starts.packed(), context.packed(), dst.packed(),
+                                                             env.stream_number(), scale))
+    return dst
 
 
 def _page_numbers(pages):
+    """The numbers as int32, and their address."""
+    if type(pages) is list or type(pages) is tuple:
+        try:
+            numbers = array.array("i", pages)
+            if builtins.min(numbers, default=0) < 0:
+                raise TannicError("copy_pages: the numbers of pages are whole, from 0 on and below 2^31")
+            return numbers, numbers.buffer_info()[0], len(numbers)
+        except (TypeError, OverflowError):
+            pass      # (no Python integers, or beyond int32: looked at below)
     numbers = np.asarray(pages).reshape(-1)
     if numbers.size and (numbers.dtype.kind not in "iu" or numbers.min() < 0 or numbers.max() >= 1 << 31):
         raise TannicError("copy_pages: the numbers of pages are whole, from 0 on and below 2^31")
-    return np.ascontiguousarray(numbers, dtype=np.int32)
+    numbers = np.ascontiguousarray(numbers, dtype=np.int32)
+    return numbers, numbers.ctypes.data, numbers.size
 
 
 def copy_pages(pool, sources, targets):
     """Copies page ``sources[i]`` of ``pool [.., pages, kv heads, page, d]`` over page ``targets[i]``, one after another in the order given
     (numbers on the host); ``pool``."""
-    sources, targets = _page_numbers(sources), _page_numbers(targets)
-    if sources.size != targets.size:
+    _from, sources, count = _page_numbers(sources)
+    _to, targets, same = _page_numbers(targets)
+    if count != same:
         raise TannicError("copy_pages: as many sources as targets")
-    lists = [pages.ctypes.data_as(abi.I32P) for pages in (sources, targets)]
-    _device_call("copy_pages", (pool,), lambda stream: (pool.packed(), stream, *lists, sources.size))
+    env = _device_of("copy_pages", pool)
+    _checked("copy_pages", library().calls["copy_pages"](pool.packed(), env.stream_number(), sources, targets, count))
     return pool
 
 
 def attend(q, k, v, lengths=None, scale=None):
     """Attention of ``q [batch, tokens, heads, d]`` over ``k, v [batch, states, kv heads, d]`` of another length (an encoder's states), over the
     first ``lengths[b]`` states of a sequence (int32; all of them if not given); contiguous, ``q``'s shape."""
-    operands = (q, k, v, lengths, _new(q.dtype, q.shape, _resolve(q, k)))
+    env = _device_of("attend", q, k, v) if lengths is None else _device_of("attend", q, k, v, lengths)
+    dst = Tensor.fresh(q.dtype, q.shape, env)
     scale = 1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else scale
-    _device_call("attend", operands, lambda stream: (*map(_packed, operands), stream, scale))
-    return operands[-1]
+    _checked("attend", library().calls["attend"](q.packed(), k.packed(), v.packed(), None if lengths is None else lengths.packed(), dst.packed(), env.stream_number(), scale))
+    return dst
