@@ -226,8 +226,14 @@ template <class T> __device__ inline float4a rows_mfma(uint4a a, uint4a b, float
 
 // two weights as the matrix pipe takes them
 template <class T> __device__ inline uint32_t pack_weights(float x, float y) {
-    T v[2] = {narrow_result<T>(x), narrow_result<T>(y)};
-    return __builtin_bit_cast(uint32_t, v);
+    typedef float float2a __attribute__((ext_vector_type(2)));
+    if constexpr (std::is_same_v<T, bf16>) {
+        typedef __bf16 V __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2a{x, y}), V));
+    } else {
+        typedef _Float16 V __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2a{x, y}), V));
+    }
 }
 
 // Whether one of a register's two 16-bit values (a float) is infinite or NaN.

@@ -8,6 +8,7 @@
 // The running maximum follows the scores only when one exceeds it by 2^8 (in the weights' power of two): sums in fp32 have the room, and the
 // 64 to 128 sums of a lane are rescaled a few times in a row's life instead of every step.
 #include "attention.hpp"
+#include "gemm_tiles.hpp"
 
 namespace th {
 
@@ -23,10 +24,15 @@ struct Item {
 template <bool PAGED, int ROWS, int UNIT>
 __device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_shared, uint32_t least_units, Item& item) {
     const uint32_t lane = threadIdx.x % 64;
-    uint32_t all = 0, groups = 0;
+    uint32_t all = 0, groups = 0, tiles = 0, units = 0;
+    Span span{};
     for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
-        uint32_t tiles = 0, units = 0, total;
-        const uint32_t mine = s0 + lane < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, span_of<PAGED>(p, s0 + lane), tiles, units) : 0;
+        uint32_t total, mine = 0;
+        tiles = 0;
+        if (s0 + lane < p.sequences) {
+            span = span_of<PAGED>(p, s0 + lane);
+            mine = sequence_units<PAGED, ROWS, UNIT>(p, span, tiles, units);
+        }
         lanes_sum_before(mine, total);
         all = sum_units(all, total);
         lanes_sum_before(tiles * p.kv_heads, total);
@@ -40,22 +46,30 @@ __device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_sh
     }
     uint32_t before_all = 0;
     for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
-        uint32_t tiles = 0, units = 0, total;
-        if (s0 + lane < p.sequences) sequence_units<PAGED, ROWS, UNIT>(p, span_of<PAGED>(p, s0 + lane), tiles, units);
+        if (p.sequences > 64) {      // (else the lanes still have what they found)
+            tiles = 0;
+            if (s0 + lane < p.sequences) {
+                span = span_of<PAGED>(p, s0 + lane);
+                sequence_units<PAGED, ROWS, UNIT>(p, span, tiles, units);
+            }
+        }
         const uint32_t chunks = units > per ? (units + per - 1) / per : 1, mine = tiles * p.kv_heads * chunks;
+        uint32_t total;
         const uint32_t before = before_all + lanes_sum_before(mine, total);
         const uint64_t here = __ballot(before <= blockIdx.x && blockIdx.x - before < mine);
         if (here) {
             const int at = __builtin_ctzll(here);
             item.s = s0 + at;
-            item.span = span_of<PAGED>(p, item.s);
-            sequence_units<PAGED, ROWS, UNIT>(p, item.span, tiles, units);
-            const uint32_t its_chunks = units > per ? (units + per - 1) / per : 1;
+            item.span.begin = __builtin_amdgcn_readlane(span.begin, at);
+            item.span.count = __builtin_amdgcn_readlane(span.count, at);
+            item.span.keys = __builtin_amdgcn_readlane(span.keys, at);
+            item.span.step = PAGED ? 1 : 0;
+            const uint32_t its_chunks = __builtin_amdgcn_readlane(chunks, at);
             uint32_t rest = blockIdx.x - __builtin_amdgcn_readlane(before, at);
             item.chunk = rest % its_chunks;
             rest /= its_chunks;
             item.head = rest % p.kv_heads;
-            item.tile = tiles - 1 - rest / p.kv_heads;
+            item.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - rest / p.kv_heads;
             item.chunk_units = per;
             item.number = blockIdx.x;
             return true;
@@ -90,38 +104,38 @@ __device__ inline float halves_sum(float x) {
 using LdsVoid = __attribute__((address_space(3))) void*;
 using GlobalVoid = __attribute__((address_space(1))) void*;
 
-// Eight transposing reads of 16 keys of V (the four tiles of 32 elements, two of the keys' four rows each) and the wait for them in one statement:
-// as builtins they would be made to wait for the loads to LDS that are on their way for the next step.
-__device__ inline void read_values(uint32_t at0, uint32_t at1, uint32_t at2, uint32_t at3, uint32_t next, uint4a v[4]) {
+// The transposing reads of 16 keys of V (four or two tiles of 32 elements, two of the keys' four rows each, FROM and NEXT bytes on) and the wait for them in one
+// statement: as builtins they would be made to wait for the loads to LDS that are on their way for the steps after.
+template <int FROM, int NEXT> __device__ inline void read_values(const uint32_t at[4], uint4a v[4]) {
     uint2a a0, a1, b0, b1, c0, c1, d0, d1;
     asm volatile(
-        "ds_read_b64_tr_b16 %0, %8\n\t"
-        "ds_read_b64_tr_b16 %1, %12\n\t"
-        "ds_read_b64_tr_b16 %2, %9\n\t"
-        "ds_read_b64_tr_b16 %3, %13\n\t"
-        "ds_read_b64_tr_b16 %4, %10\n\t"
-        "ds_read_b64_tr_b16 %5, %14\n\t"
-        "ds_read_b64_tr_b16 %6, %11\n\t"
-        "ds_read_b64_tr_b16 %7, %15\n\t"
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(a0), "=&v"(a1), "=&v"(b0), "=&v"(b1), "=&v"(c0), "=&v"(c1), "=&v"(d0), "=&v"(d1)
-        : "v"(at0), "v"(at1), "v"(at2), "v"(at3), "v"(at0 + next), "v"(at1 + next), "v"(at2 + next), "v"(at3 + next)
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(FROM), "n"(FROM + NEXT)
         : "memory");
     v[0] = uint4a{a0[0], a0[1], a1[0], a1[1]};
     v[1] = uint4a{b0[0], b0[1], b1[0], b1[1]};
     v[2] = uint4a{c0[0], c0[1], c1[0], c1[1]};
     v[3] = uint4a{d0[0], d0[1], d1[0], d1[1]};
 }
-__device__ inline void read_values(uint32_t at0, uint32_t at1, uint32_t next, uint4a v[2]) {
+template <int FROM, int NEXT> __device__ inline void read_values2(const uint32_t at[2], uint4a v[2]) {
     uint2a a0, a1, b0, b1;
     asm volatile(
-        "ds_read_b64_tr_b16 %0, %4\n\t"
-        "ds_read_b64_tr_b16 %1, %6\n\t"
-        "ds_read_b64_tr_b16 %2, %5\n\t"
-        "ds_read_b64_tr_b16 %3, %7\n\t"
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(a0), "=&v"(a1), "=&v"(b0), "=&v"(b1)
-        : "v"(at0), "v"(at1), "v"(at0 + next), "v"(at1 + next)
+        : "v"(at[0]), "v"(at[1]), "n"(FROM), "n"(FROM + NEXT)
         : "memory");
     v[0] = uint4a{a0[0], a0[1], a1[0], a1[1]};
     v[1] = uint4a{b0[0], b0[1], b1[0], b1[1]};
@@ -129,6 +143,8 @@ __device__ inline void read_values(uint32_t at0, uint32_t at1, uint32_t next, ui
 
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 template <int DP> constexpr int kTileKeys = DP > 128 ? 32 : 64;
+template <int DP> __host__ __device__ constexpr uint64_t tile_partial_floats() { return static_cast<uint64_t>(kTileRows) * (DP + 2); }
+template <int V> using Index = std::integral_constant<int, V>;
 template <int DP> constexpr size_t tile_lds_bytes() { return 4 * kTileKeys<DP> * DP * 2 + 2 * kTileKeys<DP> + 16; }
 
 template <class T, int DP, bool PAGED>
@@ -140,7 +156,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     constexpr int LPR = DP / 8, RPI = 64 / LPR;             // 16-byte pieces of a row; rows of a load
     constexpr int KPW = KT / kTileWaves, LOADS = KPW / RPI; // keys a wavefront brings, in so many loads each for K and V
     constexpr uint32_t TILE = KT * DP * 2;                  // bytes
-    extern __shared__ __align__(16) char lds_raw[];         // K, V of step 0; K, V of step 1; which keys of either are there
+    extern __shared__ __align__(16) char lds_raw[];         // keys of two steps, values of two; which keys of either are there
     uint8_t* const there = reinterpret_cast<uint8_t*>(lds_raw + 4 * TILE);
     volatile uint32_t* const arrived = reinterpret_cast<volatile uint32_t*>(lds_raw + 4 * TILE + 2 * KT);
     volatile uint32_t* const odd_step = arrived + 1;     // the step in which a value was not finite
@@ -148,7 +164,6 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     Item item;
     if (!item_of_block<PAGED, kTileRows, KT>(p, most_shared, least_units, item)) return;
     const Span span = item.span;
-    const uint32_t rows_all = span.count * p.group;
     const uint32_t first_i = p.group_div.div(item.tile * kTileRows);
     uint32_t last_i = p.group_div.div(item.tile * kTileRows + kTileRows - 1);
     last_i = last_i < span.count ? last_i : span.count - 1;
@@ -195,40 +210,40 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         k_pieces |= (k_piece * 8 < p.d ? 1u : 0u) << i;
         v_pieces |= (v_piece * 8 < p.d ? 1u : 0u) << i;
     }
-    // (places beyond the head's pieces are never written: 0 all the time)
-    if (p.d < DP) {
-        for (uint32_t x = threadIdx.x; x < 4 * TILE / 16; x += 64 * kTileWaves) reinterpret_cast<uint4a*>(lds_raw)[x] = uint4a{0, 0, 0, 0};
-        __syncthreads();
-    }
-    // A wavefront's keys of a step mostly lie in one page, whose number is asked for a step before; key by key otherwise.
+    // The second buffer of values starts as 0 (see below); places beyond the head's pieces are never written, 0 all the time.
+    for (uint32_t x = (p.d < DP ? 0 : 3 * TILE / 16) + threadIdx.x; x < 4 * TILE / 16; x += 64 * kTileWaves) reinterpret_cast<uint4a*>(lds_raw)[x] = uint4a{0, 0, 0, 0};
+    if (p.d < DP) __syncthreads();
+    // A wavefront's keys of a step mostly lie in one page, whose number is asked for a step before; key by key otherwise.  The values follow a step behind the keys.
     const bool together = !PAGED || p.page % KPW == 0;
-    uint32_t next_page = ~0u, next_in = 0;
+    uint32_t next_page = ~0u, next_in = 0, last_page = ~0u, last_in = 0, page_before = ~0u, in_before = 0;      // of the keys that come next, came last, came before those
     auto look_up = [&](uint32_t j0) {
         const uint32_t j = j0 + wave * KPW;
         int64_t page = -1;
         next_page = ~0u;
         if (together && j + KPW <= key_to && place_of<PAGED>(p, item.s, j, page, next_in)) next_page = static_cast<uint32_t>(page);
     };
-    auto bring = [&](uint32_t j0, uint32_t buffer) {
-        char* const k_to = lds_raw + buffer * (2 * TILE) + wave * (LOADS * 1024);
-        char* const v_to = k_to + TILE;
-        const uint32_t page = __builtin_amdgcn_readfirstlane(next_page), in_page = __builtin_amdgcn_readfirstlane(next_in);
+    auto bring = [&](auto of_keys, uint32_t j0, uint32_t buffer, bool before = false) {
+        constexpr bool KEYS = decltype(of_keys)::value;
+        const T* const base = (KEYS ? k + static_cast<int64_t>(item.head) * p.k_head : v + static_cast<int64_t>(item.head) * p.v_head);
+        const int64_t page_stride = KEYS ? p.k_page : p.v_page, token_stride = KEYS ? p.k_token : p.v_token;
+        const uint32_t pieces = KEYS ? k_pieces : v_pieces;
+        char* const to = lds_raw + (KEYS ? buffer : 2 + buffer) * TILE + wave * (LOADS * 1024);
+        if constexpr (KEYS) {
+            page_before = last_page, in_before = last_in;
+            last_page = __builtin_amdgcn_readfirstlane(next_page), last_in = __builtin_amdgcn_readfirstlane(next_in);
+        }
+        const uint32_t page = before ? page_before : last_page, in_page = before ? in_before : last_in;
         if (page != ~0u) {
-            const char* const k_from = reinterpret_cast<const char*>(k + (page * p.k_page + in_page * p.k_token + item.head * p.k_head));
-            const char* const v_from = reinterpret_cast<const char*>(v + (page * p.v_page + in_page * p.v_token + item.head * p.v_head));
+            const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + (page * page_stride + in_page * token_stride)), 0, 0x7FFFFFFF, 0x00020000);
             if (p.d == DP) {
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i) __builtin_amdgcn_global_load_lds((GlobalVoid)(k_from + k_lane[i]), (LdsVoid)(k_to + i * 1024), 16, 0, 0);
-#pragma unroll
-                for (int i = 0; i < LOADS; ++i) __builtin_amdgcn_global_load_lds((GlobalVoid)(v_from + v_lane[i]), (LdsVoid)(v_to + i * 1024), 16, 0, 0);
+                for (int i = 0; i < LOADS; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsVoid)(to + i * 1024), 16, KEYS ? k_lane[i] : v_lane[i], 0, 0, 0);
             } else {
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i) {
-                    if (k_pieces & (1u << i)) __builtin_amdgcn_global_load_lds((GlobalVoid)(k_from + k_lane[i]), (LdsVoid)(k_to + i * 1024), 16, 0, 0);
-                    if (v_pieces & (1u << i)) __builtin_amdgcn_global_load_lds((GlobalVoid)(v_from + v_lane[i]), (LdsVoid)(v_to + i * 1024), 16, 0, 0);
-                }
+                for (int i = 0; i < LOADS; ++i)
+                    if (pieces & (1u << i)) __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsVoid)(to + i * 1024), 16, KEYS ? k_lane[i] : v_lane[i], 0, 0, 0);
             }
-            if (lane < KPW) there[buffer * KT + wave * KPW + lane] = 1;
+            if (KEYS && lane < KPW) there[buffer * KT + wave * KPW + lane] = 1;
         } else {
 #pragma unroll 1
             for (uint32_t i = 0; i < LOADS; ++i) {
@@ -236,13 +251,11 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
                 int64_t its_page = 0;
                 uint32_t in = 0;
                 const bool lives = j < key_to && place_of<PAGED>(p, item.s, j, its_page, in);
-                const uint32_t k_piece = piece ^ k_place(in_tile), v_piece = piece ^ v_place(in_tile);
-                if (lives && (k_pieces & (1u << i)))
-                    __builtin_amdgcn_global_load_lds((GlobalVoid)(k + (its_page * p.k_page + in * p.k_token + item.head * p.k_head + k_piece * 8)), (LdsVoid)(k_to + i * 1024), 16, 0, 0);
-                if (lives && (v_pieces & (1u << i)))
-                    __builtin_amdgcn_global_load_lds((GlobalVoid)(v + (its_page * p.v_page + in * p.v_token + item.head * p.v_head + v_piece * 8)), (LdsVoid)(v_to + i * 1024), 16, 0, 0);
-                if (!lives) *reinterpret_cast<uint4a*>(v_to + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};      // (what was there may be infinite; its weight is 0)
-                if (piece == 0) there[buffer * KT + in_tile] = lives;
+                const uint32_t its_piece = piece ^ (KEYS ? k_place(in_tile) : v_place(in_tile));
+                if (lives && (pieces & (1u << i)))
+                    __builtin_amdgcn_global_load_lds((GlobalVoid)(base + (its_page * page_stride + in * token_stride + its_piece * 8)), (LdsVoid)(to + i * 1024), 16, 0, 0);
+                if (!KEYS && !lives) *reinterpret_cast<uint4a*>(to + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};      // (what was there may be infinite; its weight is 0)
+                if (KEYS && piece == 0) there[buffer * KT + in_tile] = lives;
             }
         }
     };
@@ -259,132 +272,177 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
     float top = -INFINITY, sum = 0.0f;      // of the products before the scale; the lane's own keys
 
-    // where this lane reads: K's row col (+ 32 per tile), V's rows 4 half + lane / 4 % 4 (+ 8 per read), elements 16 (lane / 16 % 2) + 4 (lane % 4)
+    // where this lane reads: K's row col (+ 32 per tile); V's rows 4 half + lane / 4 % 4 (+ 8 per read), elements 16 (lane / 16 % 2) + 4 (lane % 4)
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsVoid)lds_raw));
+    const uint32_t k_at = col * (DP * 2) + (half ^ k_place(col)) * 16;      // (piece 2 ks + half: ks changes other bits of the place)
     const uint32_t v_row = 4 * half + (lane % 16) / 4;
     uint32_t v_at[OT];
 #pragma unroll
     for (int t = 0; t < OT; ++t) {
         const uint32_t v_piece = t * 4 + ((lane / 16) % 2) * 2 + (lane % 4) / 2;
-        v_at[t] = lds_at + TILE + v_row * (DP * 2) + (v_piece ^ v_place(v_row)) * 16 + (lane % 2) * 8;
+        v_at[t] = lds_at + 2 * TILE + v_row * (DP * 2) + (v_piece ^ v_place(v_row)) * 16 + (lane % 2) * 8;
     }
 
-    if (threadIdx.x == 0) *odd_step = 0;
-    if (key_from < key_to) {
-        look_up(key_from);
-        bring(key_from, 0);
-        look_up(key_from + KT);
-    }
-    arrive();
-    uint32_t buffer = 0, odd_from = ~0u;
-    for (uint32_t j0 = key_from; j0 < key_to; j0 += KT, buffer ^= 1) {
-        const uint64_t keys = __ballot(there[buffer * KT + lane % KT] != 0);      // (32 keys: twice the same)
-        if (j0 + KT < key_to) {
-            bring(j0 + KT, buffer ^ 1);
-            look_up(j0 + 2 * KT);
+    // The work on a tile of 32 keys is spread over three turns, so that the matrix pipe has the tiles before and after to work on while a tile's weights are
+    // computed: in turn n the scores of tile n + 1 (from K), the weights of tile n, the sums of tile n - 1 (from V).  Between the turns of a step's last but one
+    // and last tile the wavefronts meet: the next step's keys and this one's values have come, and the buffers before them are free for the ones after.
+    float16a s;                      // scores of the tile whose turn it is
+    uint32_t weights[8];             // of the tile before
+    uint32_t odd_from = ~0u, buffer = 0;
+    const uint32_t steps = key_from < key_to ? (key_to - key_from + KT - 1) / KT : 0;
+    auto scores_of = [&](uint32_t from_buffer, uint32_t tile, int ks) -> uint4a {
+        return *reinterpret_cast<const uint4a*>(lds_raw + from_buffer * TILE + tile * (32 * DP * 2) + (k_at ^ (ks * 32)));
+    };
+    // (The first tile has none before it: its weights are 0, and so is that buffer of values.  What the last one's turn makes of the keys behind it is not used.)
+    auto turn = [&](auto value_tile_tag, uint32_t keys, uint32_t j, uint32_t k_buffer, uint32_t k_tile, uint32_t v_buffer) {
+        constexpr int V_FROM = decltype(value_tile_tag)::value * (32 * DP * 2);
+        uint4a kf[2][2];
+        kf[0][0] = scores_of(k_buffer, k_tile, 0), kf[0][1] = scores_of(k_buffer, k_tile, 1);
+        // a lane's keys are 8 (i / 4) + 4 half + i % 4
+        if (keys != ~0u || j + 32 > all_see) {
+            const uint32_t left = seen > j ? seen - j : 0;
+            const uint32_t mine = (keys & (left < 32 ? (1u << left) - 1 : ~0u)) >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!(mine & (1u << (8 * (i / 4) + i % 4)))) s[i] = -INFINITY;
         }
-        const char* const k_tile = lds_raw + buffer * (2 * TILE);
-        const bool full = keys == ~0ull && j0 + KT <= all_see;
-        // Values that some of the tile's rows do not see must not reach those through 0 * inf: where there are such keys, the infinite and the NaN
-        // among the values are 0 for the product, and are added in the end where they are seen.
-        if (j0 + KT > all_see && all_see < most) {
+        float high = s[0];
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                uint4a* const at = reinterpret_cast<uint4a*>(lds_raw + buffer * (2 * TILE) + TILE + wave * (LOADS * 1024) + i * 1024 + lane * 16);
-                uint4a x = *at;
-                bool odd = false;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) odd = odd || not_finite<T>(x[w]);
-                if (odd) {
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) x[w] = finite_only<T>(x[w]);
-                    *at = x;
-                    *odd_step = j0 + 1;
-                }
-            }
-            __syncthreads();
-            if (*odd_step == j0 + 1 && odd_from == ~0u) odd_from = j0;
-        }
-        // (a few keys' pieces at a time: all of them at once would take the registers of the sums)
-        float16a s[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
-        uint4a kf[2][2 * NT];
-        auto read_keys = [&](int ks, uint4a to[2 * NT]) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint32_t r = n * 32 + col;
-                    to[u * NT + n] = *reinterpret_cast<const uint4a*>(k_tile + r * (DP * 2) + (((ks + u) * 2 + half) ^ k_place(r)) * 16);
-                }
-        };
-        read_keys(0, kf[0]);
-#pragma unroll
-        for (int ks = 0; ks < KS; ks += 2) {
-            if (ks + 2 < KS) read_keys(ks + 2, kf[(ks / 2 + 1) % 2]);
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) s[n] = tile_mfma<T>(kf[(ks / 2) % 2][u * NT + n], qf[ks + u], s[n]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // a lane's keys are 32 n + 8 (i / 4) + 4 half + i % 4
-        if (!full) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint32_t from = j0 + n * 32, left = seen > from ? seen - from : 0;
-                const uint32_t mine = (static_cast<uint32_t>(keys >> (32 * n)) & (left < 32 ? (1u << left) - 1 : ~0u)) >> (4 * half);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!(mine & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
-            }
-        }
-        float high = s[0][0];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) high = fmaxf(high, s[n][i]);
+        for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
         high = halves_max(high);
-        if (__ballot(high * factor > top * factor + 8.0f || (top == -INFINITY && high > -INFINITY))) {
+        float old = 1.0f;
+        const bool higher = __ballot(high * factor > top * factor + 8.0f || (top == -INFINITY && high > -INFINITY)) != 0;
+        if (higher) {
             const float above = fmaxf(top, high);
-            const float old = top == above ? 1.0f : __builtin_amdgcn_exp2f((top - above) * factor);
+            old = top == above ? 1.0f : __builtin_amdgcn_exp2f((top - above) * factor);
             top = above;
             sum *= old;
+        }
+        const float base = top == -INFINITY ? 0.0f : top * factor - kWeightShift<T> / 2;
+        float16a next;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next[i] = 0.0f;
+        uint32_t fresh[8];
+        uint4a values[4], w{};
+        uint32_t at[OT];
+#pragma unroll
+        for (int t = 0; t < OT; ++t) at[t] = v_at[t] + v_buffer * TILE;
+        float first_of_pair = 0.0f;
+        static_for<KS>([&](auto c_tag) {
+            constexpr int c = decltype(c_tag)::value;
+            if constexpr (c % 2 == 0 && c + 2 < KS) kf[(c / 2 + 1) % 2][0] = scores_of(k_buffer, k_tile, c + 2), kf[(c / 2 + 1) % 2][1] = scores_of(k_buffer, k_tile, c + 3);
+            constexpr int kk = c / OT, t = c % OT, GROUP = OT < 4 ? OT : 4;
+            if constexpr (t == 0) w = uint4a{weights[kk * 4], weights[kk * 4 + 1], weights[kk * 4 + 2], weights[kk * 4 + 3]};
+            if constexpr (t % GROUP == 0) {
+                constexpr int FROM = V_FROM + kk * (16 * DP * 2);
+                if constexpr (GROUP == 4) read_values<FROM, 8 * DP * 2>(at + t, values);
+                else read_values2<FROM, 8 * DP * 2>(at + t, values);
+            }
+            acc[t] = tile_mfma<T>(values[t % GROUP], w, acc[t]);
+            next = tile_mfma<T>(kf[(c / 2) % 2][c % 2], qf[c], next);
+            // 16 / KS weights of this tile
+#pragma unroll
+            for (int i = c * 16 / KS; i < (c + 1) * 16 / KS; ++i) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, -base));
+                sum += x;
+                if (i % 2 == 0) first_of_pair = x;
+                else fresh[i / 2] = pack_weights<T>(first_of_pair, x);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if (higher) {
 #pragma unroll
             for (int t = 0; t < OT; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[t][i] *= old;
         }
-        const float base = top == -INFINITY ? 0.0f : top * factor - kWeightShift<T> / 2;
-        uint32_t weights[NT][8];
+        s = next;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < 8; ++i) weights[i] = fresh[i];
+    };
+    // Values that some of the tile's rows do not see must not reach those through 0 * inf: where there are such keys, the infinite and the NaN
+    // among the values are 0 for the product, and are added in the end where they are seen.
+    auto sort_values = [&](uint32_t j0, uint32_t v_buffer) {
+        if (j0 + KT <= all_see || all_see >= most) return;
+#pragma unroll 1
+        for (int i = 0; i < LOADS; ++i) {
+            uint4a* const at = reinterpret_cast<uint4a*>(lds_raw + (2 + v_buffer) * TILE + wave * (LOADS * 1024) + i * 1024 + lane * 16);
+            uint4a x = *at;
+            bool odd = false;
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], factor, -base)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], factor, -base));
-                sum += x;
-                sum += y;
-                weights[n][i / 2] = pack_weights<T>(x, y);
+            for (int w = 0; w < 4; ++w) odd = odd || not_finite<T>(x[w]);
+            if (odd) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) x[w] = finite_only<T>(x[w]);
+                *at = x;
+                *odd_step = j0 + 1;
             }
+        }
+        __syncthreads();
+        if (*odd_step == j0 + 1 && odd_from == ~0u) odd_from = j0;
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (threadIdx.x == 0) *odd_step = 0;
+    if (steps > 0) {
+        look_up(key_from);
+        bring(Yes{}, key_from, 0);
+        if constexpr (NT == 2) bring(No{}, key_from, 0);
+        look_up(key_from + KT);
+        if (steps > 1) bring(Yes{}, key_from + KT, 1);
+        look_up(key_from + 2 * KT);
+    }
+    arrive();
+    if (steps > 0) {
+        // the first tile's scores
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < 8; ++i) weights[i] = 0;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                const uint4a w{weights[n][kk * 4], weights[n][kk * 4 + 1], weights[n][kk * 4 + 2], weights[n][kk * 4 + 3]};
-                const uint32_t from = buffer * (2 * TILE) + (n * 32 + kk * 16) * (DP * 2);
+        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-                for (int t = 0; t < OT; t += 4) {
-                    uint4a values[4];
-                    if constexpr (OT >= 4) read_values(v_at[t] + from, v_at[t + 1] + from, v_at[t + 2] + from, v_at[t + 3] + from, 8 * (DP * 2), values);
-                    else read_values(v_at[0] + from, v_at[1] + from, 8 * (DP * 2), values);
-#pragma unroll
-                    for (int u = 0; u < (OT < 4 ? OT : 4); ++u) acc[t + u] = tile_mfma<T>(values[u], w, acc[t + u]);
-                }
+        for (int ks = 0; ks < KS; ++ks) s = tile_mfma<T>(scores_of(0, 0, ks), qf[ks], s);
+        uint64_t keys = __ballot(there[lane % KT] != 0), keys_next = 0;      // (32 keys: twice the same)
+        for (uint32_t step = 0; step < steps; ++step, buffer ^= 1) {
+            const uint32_t j0 = key_from + step * KT;
+            if constexpr (NT == 2) turn(Index<1>{}, static_cast<uint32_t>(keys), j0, buffer, 1, buffer ^ 1);
+            // Here the keys of the next step and the values of this one (one tile a step: of the one before) are there, and what is before them has been read.
+            arrive();
+            if (step + 1 < steps) keys_next = __ballot(there[(buffer ^ 1) * KT + lane % KT] != 0);
+            if constexpr (NT == 2) {
+                if (step + 1 < steps) bring(No{}, j0 + KT, buffer ^ 1);
+            } else {
+                bring(No{}, j0, buffer, step + 1 < steps);
             }
-        arrive();
+            if (step + 2 < steps) {
+                bring(Yes{}, j0 + 2 * KT, buffer);
+                look_up(j0 + 3 * KT);
+            }
+            if (NT == 2) sort_values(j0, buffer);
+            else if (step > 0) sort_values(j0 - KT, buffer ^ 1);
+            if constexpr (NT == 2) turn(Index<0>{}, static_cast<uint32_t>(keys >> 32), j0 + 32, buffer ^ 1, 0, buffer);
+            else turn(Index<0>{}, static_cast<uint32_t>(keys), j0, buffer ^ 1, 0, buffer ^ 1);
+            keys = keys_next;
+        }
+        // the last tile's sums
+        if constexpr (NT == 1) {
+            arrive();
+            sort_values(key_from + (steps - 1) * KT, buffer ^ 1);
+        }
+        uint32_t at[OT];
+#pragma unroll
+        for (int t = 0; t < OT; ++t) at[t] = v_at[t] + (buffer ^ 1) * TILE;
+        static_for<2>([&](auto kk_tag) {
+            constexpr int kk = decltype(kk_tag)::value, GROUP = OT < 4 ? OT : 4, FROM = (NT - 1) * (32 * DP * 2) + kk * (16 * DP * 2);
+            const uint4a w{weights[kk * 4], weights[kk * 4 + 1], weights[kk * 4 + 2], weights[kk * 4 + 3]};
+#pragma unroll
+            for (int t = 0; t < OT; t += GROUP) {
+                uint4a values[4];
+                if constexpr (GROUP == 4) read_values<FROM, 8 * DP * 2>(at + t, values);
+                else read_values2<FROM, 8 * DP * 2>(at + t, values);
+#pragma unroll
+                for (int u = 0; u < GROUP; ++u) acc[t + u] = tile_mfma<T>(values[u], w, acc[t + u]);
+            }
+        });
     }
     sum = halves_sum(sum);
     if (odd_from < key_to) {
@@ -407,45 +465,38 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     }
 
     // ---- a lane has its row's elements 32 t + 8 (i / 4) + 4 half + i % 4
-    T* const to = out + (static_cast<int64_t>(span.begin + i_row) * p.heads + q_head) * p.d;
-    if (chunks == 1) {
-        if (row_lives) {
-            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    auto write_row = [&](const float16a* of, float total) {
+        if (!row_lives) return;
+        T* const to = out + (static_cast<int64_t>(span.begin + i_row) * p.heads + q_head) * p.d;
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-            for (int t = 0; t < OT; ++t)
+        for (int t = 0; t < OT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const uint32_t e = t * 32 + 2 * i + 4 * half;
-                    if (e < p.d) {
-                        T result[4];
+            for (int i = 0; i < 16; i += 4) {
+                const uint32_t e = t * 32 + 2 * i + 4 * half;
+                if (e < p.d) {
+                    T result[4];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) result[u] = narrow_result<T>(sum == 0.0f ? 0.0f : acc[t][i + u] * inverse);
-                        __builtin_memcpy(__builtin_assume_aligned(to + e, 8), result, 8);
-                    }
+                    for (int u = 0; u < 4; ++u) result[u] = narrow_result<T>(total == 0.0f ? 0.0f : of[t][i + u] * inverse);
+                    __builtin_memcpy(__builtin_assume_aligned(to + e, 8), result, 8);
                 }
-        }
+            }
+    };
+    if (chunks == 1) {
+        write_row(acc, sum);
         return;
     }
-    // ---- or a part of it, put together by the group's last block (attention.hpp: through the memory that all dies see)
-    const uint32_t rows = rows_all - item.tile * kTileRows < kTileRows ? rows_all - item.tile * kTileRows : kTileRows, my_row = wave * 32 + col;
-    const uint64_t slot = partial_floats<kTileRows>(p.d);
-    {
-        float* const left = partial + item.number * slot;
-        if (row_lives) {
+    // ---- or a part of it, as the lanes have it, put together by the group's last block (attention.hpp: through the memory that all dies see)
+    constexpr uint64_t SLOT = tile_partial_floats<DP>(), STATS = static_cast<uint64_t>(kTileRows) * DP;
+    const uint32_t my_row = wave * 32 + col, first = item.number - item.chunk;
+    if (row_lives) {
+        float* const left = partial + item.number * SLOT;
 #pragma unroll
-            for (int t = 0; t < OT; ++t)
+        for (int t = 0; t < OT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const uint32_t e = t * 32 + 2 * i + 4 * half;
-                    if (e < p.d) {
-                        store_through(left + my_row * p.d + e, acc[t][i], acc[t][i + 1]);
-                        store_through(left + my_row * p.d + e + 2, acc[t][i + 2], acc[t][i + 3]);
-                    }
-                }
-            if (half == 0) store_through(left + static_cast<size_t>(kTileRows) * p.d + 2 * my_row, top == -INFINITY ? -INFINITY : top * factor, sum);
-        }
+            for (int i = 0; i < 16; i += 2) store_through(left + ((t * 8 + i / 2) * (64 * kTileWaves) + threadIdx.x) * 2, acc[t][i], acc[t][i + 1]);
+        if (half == 0) store_through(left + STATS + 2 * my_row, top == -INFINITY ? -INFINITY : top * factor, sum);
     }
-    const uint32_t first = item.number - item.chunk;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -454,46 +505,45 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         *arrived = before;
     }
     __syncthreads();
-    if (*arrived != chunks - 1) return;
-    const uint32_t pieces = p.d / 4;
-    const float* const parts = partial + first * slot;
-    for (uint32_t x = threadIdx.x; x < rows * pieces; x += 64 * kTileWaves) {
-        const uint32_t r = x / pieces, e = x % pieces * 4;
-        float above = -INFINITY, total = 0.0f;
-        float4a value{0, 0, 0, 0};
-        for (uint32_t c0 = 0; c0 < chunks; c0 += 4) {
-            float its_top[4], its_sum[4];
-            float4a its_value[4];
-#pragma unroll
-            for (uint32_t n = 0; n < 4; ++n) {
-                const float* const its = parts + (c0 + n < chunks ? c0 + n : chunks - 1) * slot;
-                load_through(its + static_cast<size_t>(kTileRows) * p.d + 2 * r, its_top[n], its_sum[n]);
-                load_through(its + r * p.d + e, its_value[n]);
-            }
-            float higher = above;
-#pragma unroll
-            for (uint32_t n = 0; n < 4; ++n) {
-                if (c0 + n >= chunks) its_top[n] = -INFINITY, its_sum[n] = 0.0f, its_value[n] = float4a{0, 0, 0, 0};
-                higher = fmaxf(higher, its_top[n]);
-            }
-            const float base = higher == -INFINITY ? 0.0f : higher, old = __builtin_amdgcn_exp2f(above - base);
-            total *= old;
-            value *= old;
-#pragma unroll
-            for (uint32_t n = 0; n < 4; ++n) {
-                const float share = __builtin_amdgcn_exp2f(its_top[n] - base);
-                total += its_sum[n] * share;
-                value += its_value[n] * share;
-            }
-            above = higher;
-        }
-        const uint32_t its_row = item.tile * kTileRows + r, i = p.group_div.div(its_row), head = item.head * p.group + its_row - i * p.group;
-        T result[4];
-        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) result[u] = narrow_result<T>(total == 0.0f ? 0.0f : value[u] * inverse);
-        __builtin_memcpy(__builtin_assume_aligned(out + (static_cast<int64_t>(span.begin + i) * p.heads + head) * p.d + e, 8), result, 8);
+    if (*arrived != chunks - 1 || !row_lives) return;
+    const float* const parts = partial + first * SLOT;
+    float above = -INFINITY, total = 0.0f;
+    for (uint32_t c = 0; c < chunks; ++c) {
+        float its_top, its_sum;
+        load_through(parts + c * SLOT + STATS + 2 * my_row, its_top, its_sum);
+        above = fmaxf(above, its_top);
     }
+    const float base = above == -INFINITY ? 0.0f : above;
+    float16a whole[OT];
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) whole[t][i] = 0.0f;
+    for (uint32_t c = 0; c < chunks; ++c) {      // (in the order of the chunks, whichever block is the last)
+        const float* const its = parts + c * SLOT;
+        float its_top, its_sum;
+        load_through(its + STATS + 2 * my_row, its_top, its_sum);
+        const float share = __builtin_amdgcn_exp2f(its_top - base);
+        total += its_sum * share;
+        if (c == item.chunk) {
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) whole[t][i] += acc[t][i] * share;
+        } else {
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    float x, y;
+                    load_through(its + ((t * 8 + i / 2) * (64 * kTileWaves) + threadIdx.x) * 2, x, y);
+                    whole[t][i] += x * share;
+                    whole[t][i + 1] += y * share;
+                    if (i == 14) __builtin_amdgcn_sched_barrier(0);      // (a few loads at a time)
+                }
+        }
+    }
+    write_row(whole, total);
 #endif
 }
 
@@ -513,7 +563,7 @@ int launch_tile(const AttentionProblem& p, const void* q, const void* k, const v
     if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
     static_assert(2 * kTileShared <= kAttentionArrivals);
     float* partial = nullptr;
-    if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * kTileShared * partial_floats<kTileRows>(p.d) * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+    if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * kTileShared * tile_partial_floats<DP>() * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
     hipLaunchKernelGGL((attention_tile_kernel<T, DP, PAGED>), dim3(static_cast<uint32_t>(groups + kTileShared)), dim3(64 * kTileWaves), LDS, stream, p, static_cast<const T*>(q),
                        static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(out), partial, arrivals, kTileShared, kTileLeast);
     const int status = launch_status("attention_tile_kernel");
