@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     for (int t = 0; t < OT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
-    float top = -INFINITY, sum = 0.0f;      // of the products before the scale; the lane's own keys
+    float top = -INFINITY, base = 0.0f, sum = 0.0f;      // of the products before the scale, and what it takes off a score; the sum over the lane's own keys
 
     // where this lane reads: K's row col (+ 32 per tile); V's rows 4 half + lane / 4 % 4 (+ 8 per read), elements 16 (lane / 16 % 2) + 4 (lane % 4)
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsVoid)lds_raw));
@@ -306,19 +306,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
             for (int i = 0; i < 16; ++i)
                 if (!(mine & (1u << (8 * (i / 4) + i % 4)))) s[i] = -INFINITY;
         }
-        float high = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
-        high = halves_max(high);
-        float old = 1.0f;
-        const bool higher = __ballot(high * factor > top * factor + 8.0f || (top == -INFINITY && high > -INFINITY)) != 0;
-        if (higher) {
-            const float above = fmaxf(top, high);
-            old = top == above ? 1.0f : __builtin_amdgcn_exp2f((top - above) * factor);
-            top = above;
-            sum *= old;
-        }
-        const float base = top == -INFINITY ? 0.0f : top * factor - kWeightShift<T> / 2;
+        // The weights are computed against the largest score so far while this tile's is still being found; if it turns out to be too much larger they are computed again.
+        float high = -INFINITY, part = 0.0f;
         float16a next;
 #pragma unroll
         for (int i = 0; i < 16; ++i) next[i] = 0.0f;
@@ -344,18 +333,37 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
 #pragma unroll
             for (int i = c * 16 / KS; i < (c + 1) * 16 / KS; ++i) {
                 const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, -base));
-                sum += x;
-                if (i % 2 == 0) first_of_pair = x;
-                else fresh[i / 2] = pack_weights<T>(first_of_pair, x);
+                part += x;
+                if (i % 2 == 0) {
+                    first_of_pair = x;
+                } else {
+                    fresh[i / 2] = pack_weights<T>(first_of_pair, x);
+                    high = fmaxf(fmaxf(high, s[i - 1]), s[i]);
+                    asm volatile("" : "+v"(fresh[i / 2]), "+v"(part), "+v"(high));      // (here, and not where they are used)
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         });
-        if (higher) {
+        high = halves_max(high);
+        if (__ballot(high * factor > top * factor + 8.0f || (top == -INFINITY && high > -INFINITY)) != 0) {
+            const float above = fmaxf(top, high), old = top == above ? 1.0f : __builtin_amdgcn_exp2f((top - above) * factor);
+            top = above;
+            base = above == -INFINITY ? 0.0f : above * factor - kWeightShift<T> / 2;
+            sum *= old;
+            part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, -base)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], factor, -base));
+                part += x;
+                part += y;
+                fresh[i / 2] = pack_weights<T>(x, y);
+            }
 #pragma unroll
             for (int t = 0; t < OT; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[t][i] *= old;
         }
+        sum += part;
         s = next;
 #pragma unroll
         for (int i = 0; i < 8; ++i) weights[i] = fresh[i];
@@ -513,7 +521,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         load_through(parts + c * SLOT + STATS + 2 * my_row, its_top, its_sum);
         above = fmaxf(above, its_top);
     }
-    const float base = above == -INFINITY ? 0.0f : above;
+    base = above == -INFINITY ? 0.0f : above;
     float16a whole[OT];
 #pragma unroll
     for (int t = 0; t < OT; ++t)
