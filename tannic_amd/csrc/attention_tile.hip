@@ -102,43 +102,27 @@ __device__ inline float halves_sum(float x) {
 }
 
 using LdsVoid = __attribute__((address_space(3))) void*;
-using GlobalVoid = __attribute__((address_space(1))) void*;
 
-// The transposing reads of 16 keys of V (four or two tiles of 32 elements, two of the keys' four rows each, FROM and NEXT bytes on) and the wait for them in one
-// statement: as builtins they would be made to wait for the loads to LDS that are on their way for the steps after.
-template <int FROM, int NEXT> __device__ inline void read_values(const uint32_t at[4], uint4a v[4]) {
-    uint2a a0, a1, b0, b1, c0, c1, d0, d1;
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(a0), "=&v"(a1), "=&v"(b0), "=&v"(b1), "=&v"(c0), "=&v"(c1), "=&v"(d0), "=&v"(d1)
-        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(FROM), "n"(FROM + NEXT)
-        : "memory");
-    v[0] = uint4a{a0[0], a0[1], a1[0], a1[1]};
-    v[1] = uint4a{b0[0], b0[1], b1[0], b1[1]};
-    v[2] = uint4a{c0[0], c0[1], c1[0], c1[1]};
-    v[3] = uint4a{d0[0], d0[1], d1[0], d1[1]};
+// Loads from memory straight to LDS: the wavefront's 64 lanes' 16 bytes each, one after the other from `to` on.  They are written as assembly because a builtin makes the
+// compiler put a wait for all of them before every transposing read that follows (the two might touch the same bytes, for all it knows), which would leave nothing of a
+// step's head start.  They have no register that anything could read too early; arrive() waits for them.
+typedef int int4a __attribute__((ext_vector_type(4)));
+__device__ inline void load_to_lds(int4a from, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory", "m0");
 }
-template <int FROM, int NEXT> __device__ inline void read_values2(const uint32_t at[2], uint4a v[2]) {
-    uint2a a0, a1, b0, b1;
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
-        "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
-        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
-        "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(a0), "=&v"(a1), "=&v"(b0), "=&v"(b1)
-        : "v"(at[0]), "v"(at[1]), "n"(FROM), "n"(FROM + NEXT)
-        : "memory");
-    v[0] = uint4a{a0[0], a0[1], a1[0], a1[1]};
-    v[1] = uint4a{b0[0], b0[1], b1[0], b1[1]};
+__device__ inline void load_to_lds(const void* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+}
+
+typedef short short4a __attribute__((ext_vector_type(4)));
+using LdsShort4 = __attribute__((address_space(3))) short4a;
+// the lane's element of a tile's 16 keys: two of its four rows each, `next` bytes apart
+template <int NEXT> __device__ inline uint4a read_values(const char* at) {
+    const short4a low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4*)at), high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4*)(at + NEXT));
+    uint4a v;
+    __builtin_memcpy(&v, &low, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&v) + 8, &high, 8);
+    return v;
 }
 
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
@@ -195,6 +179,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     }
 
     // ---- bringing a step's keys and values to LDS
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsVoid)lds_raw));
     // A row's pieces lie in an order of their own, so that the 16 rows a score's operand takes the same piece of, and the four rows of a transposing read, fall
     // on different banks.
     auto k_place = [](uint32_t r) -> uint32_t { return DP == 64 ? (r >> 1) & 7u : r & 15u; };
@@ -227,21 +212,22 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         const T* const base = (KEYS ? k + static_cast<int64_t>(item.head) * p.k_head : v + static_cast<int64_t>(item.head) * p.v_head);
         const int64_t page_stride = KEYS ? p.k_page : p.v_page, token_stride = KEYS ? p.k_token : p.v_token;
         const uint32_t pieces = KEYS ? k_pieces : v_pieces;
-        char* const to = lds_raw + (KEYS ? buffer : 2 + buffer) * TILE + wave * (LOADS * 1024);
+        const uint32_t place = (KEYS ? buffer : 2 + buffer) * TILE + wave * (LOADS * 1024), to = __builtin_amdgcn_readfirstlane(lds_at + place);
         if constexpr (KEYS) {
             page_before = last_page, in_before = last_in;
             last_page = __builtin_amdgcn_readfirstlane(next_page), last_in = __builtin_amdgcn_readfirstlane(next_in);
         }
         const uint32_t page = before ? page_before : last_page, in_page = before ? in_before : last_in;
         if (page != ~0u) {
-            const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + (page * page_stride + in_page * token_stride)), 0, 0x7FFFFFFF, 0x00020000);
+            const uint64_t start = reinterpret_cast<uint64_t>(base + (page * page_stride + in_page * token_stride));
+            const int4a from{__builtin_amdgcn_readfirstlane(static_cast<int>(start)), __builtin_amdgcn_readfirstlane(static_cast<int>(start >> 32) & 0xFFFF), 0x7FFFFFFF, 0x00020000};
             if (p.d == DP) {
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsVoid)(to + i * 1024), 16, KEYS ? k_lane[i] : v_lane[i], 0, 0, 0);
+                for (int i = 0; i < LOADS; ++i) load_to_lds(from, KEYS ? k_lane[i] : v_lane[i], to + i * 1024);
             } else {
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i)
-                    if (pieces & (1u << i)) __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsVoid)(to + i * 1024), 16, KEYS ? k_lane[i] : v_lane[i], 0, 0, 0);
+                    if (pieces & (1u << i)) load_to_lds(from, KEYS ? k_lane[i] : v_lane[i], to + i * 1024);
             }
             if (KEYS && lane < KPW) there[buffer * KT + wave * KPW + lane] = 1;
         } else {
@@ -253,8 +239,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
                 const bool lives = j < key_to && place_of<PAGED>(p, item.s, j, its_page, in);
                 const uint32_t its_piece = piece ^ (KEYS ? k_place(in_tile) : v_place(in_tile));
                 if (lives && (pieces & (1u << i)))
-                    __builtin_amdgcn_global_load_lds((GlobalVoid)(base + (its_page * page_stride + in * token_stride + its_piece * 8)), (LdsVoid)(to + i * 1024), 16, 0, 0);
-                if (!KEYS && !lives) *reinterpret_cast<uint4a*>(to + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};      // (what was there may be infinite; its weight is 0)
+                    load_to_lds(base + (its_page * page_stride + in * token_stride + its_piece * 8), to + i * 1024);
+                if (!KEYS && !lives) *reinterpret_cast<uint4a*>(lds_raw + place + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};      // (what was there may be infinite; its weight is 0)
                 if (KEYS && piece == 0) there[buffer * KT + in_tile] = lives;
             }
         }
@@ -273,14 +259,13 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     float top = -INFINITY, base = 0.0f, sum = 0.0f;      // of the products before the scale, and what it takes off a score; the sum over the lane's own keys
 
     // where this lane reads: K's row col (+ 32 per tile); V's rows 4 half + lane / 4 % 4 (+ 8 per read), elements 16 (lane / 16 % 2) + 4 (lane % 4)
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsVoid)lds_raw));
     const uint32_t k_at = col * (DP * 2) + (half ^ k_place(col)) * 16;      // (piece 2 ks + half: ks changes other bits of the place)
     const uint32_t v_row = 4 * half + (lane % 16) / 4;
     uint32_t v_at[OT];
 #pragma unroll
     for (int t = 0; t < OT; ++t) {
         const uint32_t v_piece = t * 4 + ((lane / 16) % 2) * 2 + (lane % 4) / 2;
-        v_at[t] = lds_at + 2 * TILE + v_row * (DP * 2) + (v_piece ^ v_place(v_row)) * 16 + (lane % 2) * 8;
+        v_at[t] = 2 * TILE + v_row * (DP * 2) + (v_piece ^ v_place(v_row)) * 16 + (lane % 2) * 8;
     }
 
     // The work on a tile of 32 keys is spread over three turns, so that the matrix pipe has the tiles before and after to work on while a tile's weights are
@@ -298,6 +283,12 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         constexpr int V_FROM = decltype(value_tile_tag)::value * (32 * DP * 2);
         uint4a kf[2][2];
         kf[0][0] = scores_of(k_buffer, k_tile, 0), kf[0][1] = scores_of(k_buffer, k_tile, 1);
+        uint4a values[3];
+        auto value_of = [&](const char* tile, int n) -> uint4a { return read_values<8 * DP * 2>(tile + v_at[n % OT] + (n / OT) * (16 * DP * 2)); };
+        {
+            const char* const tile = lds_raw + v_buffer * TILE + V_FROM;
+            values[0] = value_of(tile, 0), values[1] = value_of(tile, 1);
+        }
         // a lane's keys are 8 (i / 4) + 4 half + i % 4
         if (keys != ~0u || j + 32 > all_see) {
             const uint32_t left = seen > j ? seen - j : 0;
@@ -312,22 +303,16 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
 #pragma unroll
         for (int i = 0; i < 16; ++i) next[i] = 0.0f;
         uint32_t fresh[8];
-        uint4a values[4], w{};
-        uint32_t at[OT];
-#pragma unroll
-        for (int t = 0; t < OT; ++t) at[t] = v_at[t] + v_buffer * TILE;
+        uint4a w{};
+        const char* const v_tile = lds_raw + v_buffer * TILE + V_FROM;
         float first_of_pair = 0.0f;
         static_for<KS>([&](auto c_tag) {
             constexpr int c = decltype(c_tag)::value;
             if constexpr (c % 2 == 0 && c + 2 < KS) kf[(c / 2 + 1) % 2][0] = scores_of(k_buffer, k_tile, c + 2), kf[(c / 2 + 1) % 2][1] = scores_of(k_buffer, k_tile, c + 3);
-            constexpr int kk = c / OT, t = c % OT, GROUP = OT < 4 ? OT : 4;
+            constexpr int kk = c / OT, t = c % OT;
             if constexpr (t == 0) w = uint4a{weights[kk * 4], weights[kk * 4 + 1], weights[kk * 4 + 2], weights[kk * 4 + 3]};
-            if constexpr (t % GROUP == 0) {
-                constexpr int FROM = V_FROM + kk * (16 * DP * 2);
-                if constexpr (GROUP == 4) read_values<FROM, 8 * DP * 2>(at + t, values);
-                else read_values2<FROM, 8 * DP * 2>(at + t, values);
-            }
-            acc[t] = tile_mfma<T>(values[t % GROUP], w, acc[t]);
+            if constexpr (c + 2 < KS) values[(c + 2) % 3] = value_of(v_tile, c + 2);
+            acc[t] = tile_mfma<T>(values[c % 3], w, acc[t]);
             next = tile_mfma<T>(kf[(c / 2) % 2][c % 2], qf[c], next);
             // 16 / KS weights of this tile
 #pragma unroll
@@ -436,21 +421,12 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
             arrive();
             sort_values(key_from + (steps - 1) * KT, buffer ^ 1);
         }
-        uint32_t at[OT];
 #pragma unroll
-        for (int t = 0; t < OT; ++t) at[t] = v_at[t] + (buffer ^ 1) * TILE;
-        static_for<2>([&](auto kk_tag) {
-            constexpr int kk = decltype(kk_tag)::value, GROUP = OT < 4 ? OT : 4, FROM = (NT - 1) * (32 * DP * 2) + kk * (16 * DP * 2);
+        for (int kk = 0; kk < 2; ++kk) {
             const uint4a w{weights[kk * 4], weights[kk * 4 + 1], weights[kk * 4 + 2], weights[kk * 4 + 3]};
 #pragma unroll
-            for (int t = 0; t < OT; t += GROUP) {
-                uint4a values[4];
-                if constexpr (GROUP == 4) read_values<FROM, 8 * DP * 2>(at + t, values);
-                else read_values2<FROM, 8 * DP * 2>(at + t, values);
-#pragma unroll
-                for (int u = 0; u < GROUP; ++u) acc[t + u] = tile_mfma<T>(values[u], w, acc[t + u]);
-            }
-        });
+            for (int t = 0; t < OT; ++t) acc[t] = tile_mfma<T>(read_values<8 * DP * 2>(lds_raw + v_at[t] + (buffer ^ 1) * TILE + ((NT - 1) * 32 + kk * 16) * (DP * 2)), w, acc[t]);
+        }
     }
     sum = halves_sum(sum);
     if (odd_from < key_to) {
