@@ -129,7 +129,7 @@ constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 template <int DP> constexpr int kTileKeys = DP > 128 ? 32 : 64;
 template <int DP> __host__ __device__ constexpr uint64_t tile_partial_floats() { return static_cast<uint64_t>(kTileRows) * (DP + 2); }
 template <int V> using Index = std::integral_constant<int, V>;
-template <int DP> constexpr size_t tile_lds_bytes() { return 4 * kTileKeys<DP> * DP * 2 + 2 * kTileKeys<DP> + 16; }
+template <int DP> constexpr size_t tile_lds_bytes() { return 4 * kTileKeys<DP> * DP * 2 + 2 * kTileKeys<DP> + 16 + 4 * 1024; }
 
 template <class T, int DP, bool PAGED>
 __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_tile_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial, uint32_t* arrivals,
@@ -184,20 +184,18 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     // on different banks.
     auto k_place = [](uint32_t r) -> uint32_t { return DP == 64 ? (r >> 1) & 7u : r & 15u; };
     auto v_place = [](uint32_t r) -> uint32_t { return DP == 64 ? ((r >> 1) & 1u) * 4 : (r & 3u) * 4; };
+    // Rows that are not there, and the pieces behind a head of less than DP elements, are beyond what the loads may reach: 0 is put in their place.
+    constexpr uint32_t BEYOND = 0x80000000u;
     uint32_t k_lane[LOADS], v_lane[LOADS];      // bytes from the wavefront's first key
-    uint32_t k_pieces = 0, v_pieces = 0;        // bit i: the lane's piece of load i is one of the head's (d may be below DP)
     const uint32_t piece = lane % LPR, row_in = lane / LPR;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
         const uint32_t r = i * RPI + row_in, in_tile = wave * KPW + r, k_piece = piece ^ k_place(in_tile), v_piece = piece ^ v_place(in_tile);
-        k_lane[i] = r * static_cast<uint32_t>(p.k_token) * 2 + k_piece * 16;
-        v_lane[i] = r * static_cast<uint32_t>(p.v_token) * 2 + v_piece * 16;
-        k_pieces |= (k_piece * 8 < p.d ? 1u : 0u) << i;
-        v_pieces |= (v_piece * 8 < p.d ? 1u : 0u) << i;
+        k_lane[i] = k_piece * 8 < p.d ? r * static_cast<uint32_t>(p.k_token) * 2 + k_piece * 16 : BEYOND;
+        v_lane[i] = v_piece * 8 < p.d ? r * static_cast<uint32_t>(p.v_token) * 2 + v_piece * 16 : BEYOND;
     }
-    // The second buffer of values starts as 0 (see below); places beyond the head's pieces are never written, 0 all the time.
-    for (uint32_t x = (p.d < DP ? 0 : 3 * TILE / 16) + threadIdx.x; x < 4 * TILE / 16; x += 64 * kTileWaves) reinterpret_cast<uint4a*>(lds_raw)[x] = uint4a{0, 0, 0, 0};
-    if (p.d < DP) __syncthreads();
+    // The second buffer of values starts as 0 (see below).
+    for (uint32_t x = threadIdx.x; x < TILE / 16; x += 64 * kTileWaves) reinterpret_cast<uint4a*>(lds_raw + 3 * TILE)[x] = uint4a{0, 0, 0, 0};
     // A wavefront's keys of a step mostly lie in one page, whose number is asked for a step before; key by key otherwise.  The values follow a step behind the keys.
     const bool together = !PAGED || p.page % KPW == 0;
     uint32_t next_page = ~0u, next_in = 0, last_page = ~0u, last_in = 0, page_before = ~0u, in_before = 0;      // of the keys that come next, came last, came before those
@@ -205,45 +203,48 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         const uint32_t j = j0 + wave * KPW;
         int64_t page = -1;
         next_page = ~0u;
-        if (together && j + KPW <= key_to && place_of<PAGED>(p, item.s, j, page, next_in)) next_page = static_cast<uint32_t>(page);
+        if (together && j < key_to && place_of<PAGED>(p, item.s, j, page, next_in)) next_page = static_cast<uint32_t>(page);
     };
-    auto bring = [&](auto of_keys, uint32_t j0, uint32_t buffer, bool before = false) {
+    struct Fetch {      // loads that are to be issued: from where, and to where in LDS
+        int4a from;
+        uint32_t to;
+    };
+    const Fetch nothing{{0, 0, 0, 0x00020000}, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(lds_at + 4 * TILE + 2 * KT + 16))};      // (a place that nobody reads)
+    auto bring = [&](auto of_keys, uint32_t j0, uint32_t buffer, bool before = false) -> Fetch {
         constexpr bool KEYS = decltype(of_keys)::value;
         const T* const base = (KEYS ? k + static_cast<int64_t>(item.head) * p.k_head : v + static_cast<int64_t>(item.head) * p.v_head);
         const int64_t page_stride = KEYS ? p.k_page : p.v_page, token_stride = KEYS ? p.k_token : p.v_token;
-        const uint32_t pieces = KEYS ? k_pieces : v_pieces;
         const uint32_t place = (KEYS ? buffer : 2 + buffer) * TILE + wave * (LOADS * 1024), to = __builtin_amdgcn_readfirstlane(lds_at + place);
         if constexpr (KEYS) {
             page_before = last_page, in_before = last_in;
             last_page = __builtin_amdgcn_readfirstlane(next_page), last_in = __builtin_amdgcn_readfirstlane(next_in);
         }
-        const uint32_t page = before ? page_before : last_page, in_page = before ? in_before : last_in;
-        if (page != ~0u) {
-            const uint64_t start = reinterpret_cast<uint64_t>(base + (page * page_stride + in_page * token_stride));
-            const int4a from{__builtin_amdgcn_readfirstlane(static_cast<int>(start)), __builtin_amdgcn_readfirstlane(static_cast<int>(start >> 32) & 0xFFFF), 0x7FFFFFFF, 0x00020000};
-            if (p.d == DP) {
-#pragma unroll
-                for (int i = 0; i < LOADS; ++i) load_to_lds(from, KEYS ? k_lane[i] : v_lane[i], to + i * 1024);
-            } else {
-#pragma unroll
-                for (int i = 0; i < LOADS; ++i)
-                    if (pieces & (1u << i)) load_to_lds(from, KEYS ? k_lane[i] : v_lane[i], to + i * 1024);
-            }
-            if (KEYS && lane < KPW) there[buffer * KT + wave * KPW + lane] = 1;
-        } else {
-#pragma unroll 1
-            for (uint32_t i = 0; i < LOADS; ++i) {
-                const uint32_t r = i * RPI + row_in, in_tile = wave * KPW + r, j = j0 + in_tile;
-                int64_t its_page = 0;
-                uint32_t in = 0;
-                const bool lives = j < key_to && place_of<PAGED>(p, item.s, j, its_page, in);
-                const uint32_t its_piece = piece ^ (KEYS ? k_place(in_tile) : v_place(in_tile));
-                if (lives && (pieces & (1u << i)))
-                    load_to_lds(base + (its_page * page_stride + in * token_stride + its_piece * 8), to + i * 1024);
-                if (!KEYS && !lives) *reinterpret_cast<uint4a*>(lds_raw + place + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};      // (what was there may be infinite; its weight is 0)
-                if (KEYS && piece == 0) there[buffer * KT + in_tile] = lives;
-            }
+        if (together) {
+            const uint32_t page = before ? page_before : last_page, in_page = before ? in_before : last_in, left = key_to - (j0 + wave * KPW);
+            const uint32_t here = page == ~0u ? 0 : left < KPW ? left : KPW;
+            const uint64_t start = reinterpret_cast<uint64_t>(base) + (here ? (page * page_stride + in_page * token_stride) * 2 : 0);
+            const uint32_t bytes = here ? (here - 1) * static_cast<uint32_t>(token_stride) * 2 + p.d * 2 : 0;
+            if (KEYS && lane < KPW) there[buffer * KT + wave * KPW + lane] = lane < here;
+            return Fetch{{__builtin_amdgcn_readfirstlane(static_cast<int>(start)), __builtin_amdgcn_readfirstlane(static_cast<int>(start >> 32) & 0xFFFF), __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), 0x00020000}, to};
         }
+#pragma unroll 1
+        for (uint32_t i = 0; i < LOADS; ++i) {
+            const uint32_t r = i * RPI + row_in, in_tile = wave * KPW + r, j = j0 + in_tile;
+            int64_t its_page = 0;
+            uint32_t in = 0;
+            const bool lives = j < key_to && place_of<PAGED>(p, item.s, j, its_page, in);
+            const uint32_t its_piece = piece ^ (KEYS ? k_place(in_tile) : v_place(in_tile));
+            if (lives && its_piece * 8 < p.d) load_to_lds(base + (its_page * page_stride + in * token_stride + its_piece * 8), to + i * 1024);
+            else *reinterpret_cast<uint4a*>(lds_raw + place + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};
+            if (KEYS && piece == 0) there[buffer * KT + in_tile] = lives;
+        }
+        return nothing;
+    };
+    auto fetch_keys = [&](const Fetch& f, int i) { load_to_lds(f.from, k_lane[i], f.to + i * 1024); };
+    auto fetch_values = [&](const Fetch& f, int i) { load_to_lds(f.from, v_lane[i], f.to + i * 1024); };
+    auto fetch_all = [&](const Fetch& f, auto&& fetch) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) fetch(f, i);
     };
     auto arrive = [] {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -279,7 +280,10 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         return *reinterpret_cast<const uint4a*>(lds_raw + from_buffer * TILE + tile * (32 * DP * 2) + (k_at ^ (ks * 32)));
     };
     // (The first tile has none before it: its weights are 0, and so is that buffer of values.  What the last one's turn makes of the keys behind it is not used.)
-    auto turn = [&](auto value_tile_tag, uint32_t keys, uint32_t j, uint32_t k_buffer, uint32_t k_tile, uint32_t v_buffer) {
+    // FETCH: the loads of the next step's values and of the keys behind those go out one by one between the products (all at once they keep the wavefront waiting for the
+    // memory pipe's queue: 1700 of a step's 4600 clocks).
+    auto turn = [&](auto fetch_tag, const Fetch& next_values, const Fetch& next_keys, auto value_tile_tag, uint32_t keys, uint32_t j, uint32_t k_buffer, uint32_t k_tile, uint32_t v_buffer) {
+        constexpr bool FETCH = decltype(fetch_tag)::value;
         constexpr int V_FROM = decltype(value_tile_tag)::value * (32 * DP * 2);
         uint4a kf[2][2];
         kf[0][0] = scores_of(k_buffer, k_tile, 0), kf[0][1] = scores_of(k_buffer, k_tile, 1);
@@ -314,6 +318,10 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
             if constexpr (c + 2 < KS) values[(c + 2) % 3] = value_of(v_tile, c + 2);
             acc[t] = tile_mfma<T>(values[c % 3], w, acc[t]);
             next = tile_mfma<T>(kf[(c / 2) % 2][c % 2], qf[c], next);
+            if constexpr (FETCH && c < 2 * LOADS) {
+                if constexpr (c % 2 == 0) fetch_values(next_values, c / 2);
+                else fetch_keys(next_keys, c / 2);
+            }
             // 16 / KS weights of this tile
 #pragma unroll
             for (int i = c * 16 / KS; i < (c + 1) * 16 / KS; ++i) {
@@ -379,10 +387,10 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     if (threadIdx.x == 0) *odd_step = 0;
     if (steps > 0) {
         look_up(key_from);
-        bring(Yes{}, key_from, 0);
-        if constexpr (NT == 2) bring(No{}, key_from, 0);
+        fetch_all(bring(Yes{}, key_from, 0), fetch_keys);
+        if constexpr (NT == 2) fetch_all(bring(No{}, key_from, 0), fetch_values);
         look_up(key_from + KT);
-        if (steps > 1) bring(Yes{}, key_from + KT, 1);
+        if (steps > 1) fetch_all(bring(Yes{}, key_from + KT, 1), fetch_keys);
         look_up(key_from + 2 * KT);
     }
     arrive();
@@ -397,23 +405,24 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         uint64_t keys = __ballot(there[lane % KT] != 0), keys_next = 0;      // (32 keys: twice the same)
         for (uint32_t step = 0; step < steps; ++step, buffer ^= 1) {
             const uint32_t j0 = key_from + step * KT;
-            if constexpr (NT == 2) turn(Index<1>{}, static_cast<uint32_t>(keys), j0, buffer, 1, buffer ^ 1);
+            Fetch next_values = nothing, next_keys = nothing;
+            if constexpr (NT == 2) turn(No{}, nothing, nothing, Index<1>{}, static_cast<uint32_t>(keys), j0, buffer, 1, buffer ^ 1);
             // Here the keys of the next step and the values of this one (one tile a step: of the one before) are there, and what is before them has been read.
             arrive();
             if (step + 1 < steps) keys_next = __ballot(there[(buffer ^ 1) * KT + lane % KT] != 0);
             if constexpr (NT == 2) {
-                if (step + 1 < steps) bring(No{}, j0 + KT, buffer ^ 1);
+                if (step + 1 < steps) next_values = bring(No{}, j0 + KT, buffer ^ 1);
             } else {
-                bring(No{}, j0, buffer, step + 1 < steps);
+                next_values = bring(No{}, j0, buffer, step + 1 < steps);
             }
             if (step + 2 < steps) {
-                bring(Yes{}, j0 + 2 * KT, buffer);
+                next_keys = bring(Yes{}, j0 + 2 * KT, buffer);
                 look_up(j0 + 3 * KT);
             }
             if (NT == 2) sort_values(j0, buffer);
             else if (step > 0) sort_values(j0 - KT, buffer ^ 1);
-            if constexpr (NT == 2) turn(Index<0>{}, static_cast<uint32_t>(keys >> 32), j0 + 32, buffer ^ 1, 0, buffer);
-            else turn(Index<0>{}, static_cast<uint32_t>(keys), j0, buffer ^ 1, 0, buffer ^ 1);
+            if constexpr (NT == 2) turn(Yes{}, next_values, next_keys, Index<0>{}, static_cast<uint32_t>(keys >> 32), j0 + 32, buffer ^ 1, 0, buffer);
+            else turn(Yes{}, next_values, next_keys, Index<0>{}, static_cast<uint32_t>(keys), j0, buffer ^ 1, 0, buffer ^ 1);
             keys = keys_next;
         }
         // the last tile's sums
@@ -563,9 +572,9 @@ int pick_tile(const AttentionProblem& p, const void* q, const void* k, const voi
 }
 
 int attention_tile(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
-    // (a lane's offsets from its wavefront's first key fit 32 bits)
+    // (a lane's offsets from its wavefront's first key fit 32 bits, and rows ascend)
     const int64_t far = int64_t(1) << 25;
-    if (p.k_token < 0 || p.v_token < 0 || p.k_token >= far || p.v_token >= far) return TANNIC_UNSUPPORTED_DTYPE;
+    if ((p.page > 1 && (p.k_token < p.d || p.v_token < p.d)) || p.k_token >= far || p.v_token >= far) return TANNIC_UNSUPPORTED_DTYPE;
     if (dtype == TANNIC_FLOAT16) return p.starts ? pick_tile<f16, true>(p, q, k, v, out, stream) : pick_tile<f16, false>(p, q, k, v, out, stream);
     if (dtype == TANNIC_BFLOAT16) return p.starts ? pick_tile<bf16, true>(p, q, k, v, out, stream) : pick_tile<bf16, false>(p, q, k, v, out, stream);
     return TANNIC_UNSUPPORTED_DTYPE;
