@@ -67,20 +67,27 @@ __device__ inline uint32_t keys_seen(const AttentionProblem& p, const Span& s, u
     return n < p.room ? n : p.room;
 }
 
-// Where key j of sequence s lies: the page (or, dense, the sequence) and the row in it; false: nowhere.
+// Where key j of sequence s is said to lie: the number of its page (dense: of the sequence) and its row there.  Nothing here waits for the number: whether there is such
+// a page is asked (page_exists) when the key is.
 template <bool PAGED>
-__device__ inline bool place_of(const AttentionProblem& p, uint32_t s, uint32_t j, int64_t& page, uint32_t& row) {
+__device__ inline uint32_t page_of(const AttentionProblem& p, uint32_t s, uint32_t j, uint32_t& row) {
     if constexpr (PAGED) {
         uint32_t column;
         p.page_div.divmod(j, column, row);
-        const int32_t id = p.table[static_cast<int64_t>(s) * p.table_row + column];
-        page = id;
-        return static_cast<uint32_t>(id) < p.pages;
+        return static_cast<uint32_t>(p.table[static_cast<int64_t>(s) * p.table_row + column]);
     } else {
-        page = s;
         row = j;
-        return true;
+        return s;
     }
+}
+__device__ inline bool page_exists(const AttentionProblem& p, uint32_t page) { return page < p.pages; }
+
+// Both at once.
+template <bool PAGED>
+__device__ inline bool place_of(const AttentionProblem& p, uint32_t s, uint32_t j, int64_t& page, uint32_t& row) {
+    const uint32_t id = page_of<PAGED>(p, s, j, row);
+    page = id;
+    return page_exists(p, id);
 }
 
 __device__ inline int64_t query_offset(const AttentionProblem& p, uint32_t s, const Span& span, uint32_t i, uint32_t head) {

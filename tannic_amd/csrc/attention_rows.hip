@@ -78,20 +78,20 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
         uint4a kf[KT][KS], vf[KT][KS];
         uint32_t there[KT];
         // which page a step's keys lie in is asked for a step before the keys themselves
-        int64_t page[KT];
-        uint32_t in_page[KT];
-        bool found[KT];
+        uint32_t page[KT], in_page[KT];
         auto look_up = [&](uint32_t j0) {
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
                 const uint32_t j = j0 + kt * 16 + col;
-                found[kt] = j < key_to;
-                if (found[kt]) found[kt] = place_of<PAGED>(p, g.s, j, page[kt], in_page[kt]);
+                page[kt] = ~0u, in_page[kt] = 0;
+                if (j < key_to) page[kt] = page_of<PAGED>(p, g.s, j, in_page[kt]);
             }
         };
         auto fetch = [&]() {
+            bool found[KT];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
+                found[kt] = page_exists(p, page[kt]);
                 there[kt] = static_cast<uint32_t>(__ballot(found[kt])) & 0xFFFFu;
                 const int64_t k_off = found[kt] ? page[kt] * p.k_page + in_page[kt] * p.k_token + g.head * p.k_head : 0;
                 const int64_t v_off = found[kt] ? page[kt] * p.v_page + in_page[kt] * p.v_token + g.head * p.v_head : 0;

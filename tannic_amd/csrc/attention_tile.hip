@@ -201,9 +201,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     uint32_t next_page = ~0u, next_in = 0, last_page = ~0u, last_in = 0, page_before = ~0u, in_before = 0;      // of the keys that come next, came last, came before those
     auto look_up = [&](uint32_t j0) {
         const uint32_t j = j0 + wave * KPW;
-        int64_t page = -1;
         next_page = ~0u;
-        if (together && j < key_to && place_of<PAGED>(p, item.s, j, page, next_in)) next_page = static_cast<uint32_t>(page);
+        if (together && j < key_to) next_page = page_of<PAGED>(p, item.s, j, next_in);
     };
     struct Fetch {      // loads that are to be issued: from where, and to where in LDS
         int4a from;
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         }
         if (together) {
             const uint32_t page = before ? page_before : last_page, in_page = before ? in_before : last_in, left = key_to - (j0 + wave * KPW);
-            const uint32_t here = page == ~0u ? 0 : left < KPW ? left : KPW;
+            const uint32_t here = !page_exists(p, page) ? 0 : left < KPW ? left : KPW;
             const uint64_t start = reinterpret_cast<uint64_t>(base) + (here ? (page * page_stride + in_page * token_stride) * 2 : 0);
             const uint32_t bytes = here ? (here - 1) * static_cast<uint32_t>(token_stride) * 2 + p.d * 2 : 0;
             if (KEYS && lane < KPW) there[buffer * KT + wave * KPW + lane] = lane < here;
