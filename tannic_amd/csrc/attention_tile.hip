@@ -196,48 +196,78 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     }
     // The second buffer of values starts as 0 (see below).
     for (uint32_t x = threadIdx.x; x < TILE / 16; x += 64 * kTileWaves) reinterpret_cast<uint4a*>(lds_raw + 3 * TILE)[x] = uint4a{0, 0, 0, 0};
-    // A wavefront's keys of a step mostly lie in one page, whose number is asked for a step before; key by key otherwise.  The values follow a step behind the keys.
-    const bool together = !PAGED || p.page % KPW == 0;
-    uint32_t next_page = ~0u, next_in = 0, last_page = ~0u, last_in = 0, page_before = ~0u, in_before = 0;      // of the keys that come next, came last, came before those
-    auto look_up = [&](uint32_t j0) {
-        const uint32_t j = j0 + wave * KPW;
-        next_page = ~0u;
-        if (together && j < key_to) next_page = page_of<PAGED>(p, item.s, j, next_in);
-    };
     struct Fetch {      // loads that are to be issued: from where, and to where in LDS
         int4a from;
         uint32_t to;
     };
     const Fetch nothing{{0, 0, 0, 0x00020000}, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(lds_at + 4 * TILE + 2 * KT + 16))};      // (a place that nobody reads)
-    auto bring = [&](auto of_keys, uint32_t j0, uint32_t buffer, bool before = false) -> Fetch {
+    auto fetch_from = [&](const T* base, int64_t offset, uint32_t token_stride, uint32_t here, uint32_t to) -> Fetch {
+        const uint64_t start = reinterpret_cast<uint64_t>(base + offset);
+        return Fetch{{__builtin_amdgcn_readfirstlane(static_cast<int>(start)), __builtin_amdgcn_readfirstlane(static_cast<int>(start >> 32) & 0xFFFF),
+                      __builtin_amdgcn_readfirstlane(static_cast<int>(here ? (here - 1) * token_stride * 2 + p.d * 2 : 0)), 0x00020000},
+                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(lds_at + to + wave * (LOADS * 1024)))};
+    };
+    // A wavefront's keys of a step mostly lie in one page: lane w holds the number of wavefront w's, asked for a step before it is needed, and which keys of the step are there
+    // follows from the four.  Where pages end inside a wavefront's keys they are looked up one by one, and `there` says which of them are.
+    const bool together = !PAGED || p.page % KPW == 0;
+    const T* const k_head = k + static_cast<int64_t>(item.head) * p.k_head;
+    const T* const v_head = v + static_cast<int64_t>(item.head) * p.v_head;
+    const bool alike = p.k_page == p.v_page && p.k_token == p.v_token;
+    uint32_t next_page = ~0u, next_in = 0;
+    auto look_up = [&](uint32_t j0) {
+        const uint32_t j = j0 + (lane % kTileWaves) * KPW;
+        next_page = ~0u;
+        if (together && j < key_to) next_page = page_of<PAGED>(p, item.s, j, next_in);
+    };
+    // the values of a step's keys are brought one (one tile a step: two) steps after them
+    struct Pending {
+        int64_t offset;
+        uint32_t here;
+    };
+    Pending values_next{0, 0}, values_after{0, 0};
+    constexpr uint64_t ALL = ~0ull >> (64 - KT);
+    auto one_by_one = [&](auto of_keys, uint32_t j0, uint32_t buffer) {
         constexpr bool KEYS = decltype(of_keys)::value;
-        const T* const base = (KEYS ? k + static_cast<int64_t>(item.head) * p.k_head : v + static_cast<int64_t>(item.head) * p.v_head);
-        const int64_t page_stride = KEYS ? p.k_page : p.v_page, token_stride = KEYS ? p.k_token : p.v_token;
         const uint32_t place = (KEYS ? buffer : 2 + buffer) * TILE + wave * (LOADS * 1024), to = __builtin_amdgcn_readfirstlane(lds_at + place);
-        if constexpr (KEYS) {
-            page_before = last_page, in_before = last_in;
-            last_page = __builtin_amdgcn_readfirstlane(next_page), last_in = __builtin_amdgcn_readfirstlane(next_in);
-        }
-        if (together) {
-            const uint32_t page = before ? page_before : last_page, in_page = before ? in_before : last_in, left = key_to - (j0 + wave * KPW);
-            const uint32_t here = !page_exists(p, page) ? 0 : left < KPW ? left : KPW;
-            const uint64_t start = reinterpret_cast<uint64_t>(base) + (here ? (page * page_stride + in_page * token_stride) * 2 : 0);
-            const uint32_t bytes = here ? (here - 1) * static_cast<uint32_t>(token_stride) * 2 + p.d * 2 : 0;
-            if (KEYS && lane < KPW) there[buffer * KT + wave * KPW + lane] = lane < here;
-            return Fetch{{__builtin_amdgcn_readfirstlane(static_cast<int>(start)), __builtin_amdgcn_readfirstlane(static_cast<int>(start >> 32) & 0xFFFF), __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), 0x00020000}, to};
-        }
 #pragma unroll 1
         for (uint32_t i = 0; i < LOADS; ++i) {
             const uint32_t r = i * RPI + row_in, in_tile = wave * KPW + r, j = j0 + in_tile;
-            int64_t its_page = 0;
+            int64_t page = 0;
             uint32_t in = 0;
-            const bool lives = j < key_to && place_of<PAGED>(p, item.s, j, its_page, in);
+            const bool lives = j < key_to && place_of<PAGED>(p, item.s, j, page, in);
             const uint32_t its_piece = piece ^ (KEYS ? k_place(in_tile) : v_place(in_tile));
-            if (lives && its_piece * 8 < p.d) load_to_lds(base + (its_page * page_stride + in * token_stride + its_piece * 8), to + i * 1024);
+            if (lives && its_piece * 8 < p.d) load_to_lds((KEYS ? k_head + page * p.k_page + in * p.k_token : v_head + page * p.v_page + in * p.v_token) + its_piece * 8, to + i * 1024);
             else *reinterpret_cast<uint4a*>(lds_raw + place + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};
             if (KEYS && piece == 0) there[buffer * KT + in_tile] = lives;
         }
-        return nothing;
+    };
+    auto bring_keys = [&](uint32_t j0, uint32_t buffer, uint64_t& keys) -> Fetch {
+        if (!together) {
+            one_by_one(std::true_type{}, j0, buffer);
+            return nothing;
+        }
+        const uint32_t live = static_cast<uint32_t>(__ballot(page_exists(p, next_page))) & ((1u << kTileWaves) - 1);
+        const uint32_t page = __builtin_amdgcn_readlane(next_page, wave), in = __builtin_amdgcn_readlane(next_in, wave), j = j0 + wave * KPW;
+        const uint32_t here = !((live >> wave) & 1) ? 0 : key_to - j < KPW ? key_to - j : KPW;
+        const int64_t k_off = here ? page * p.k_page + in * p.k_token : 0, v_off = alike ? k_off : here ? page * p.v_page + in * p.v_token : 0;
+        values_after = values_next;
+        values_next = Pending{v_off, here};
+        keys = ALL;
+        if (live != (1u << kTileWaves) - 1 || j0 + KT > key_to) {
+            keys = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < kTileWaves; ++w) keys |= static_cast<uint64_t>((live >> w) & 1 ? (1u << KPW) - 1 : 0u) << (w * KPW);
+            const uint32_t left = key_to > j0 ? key_to - j0 : 0;
+            if (left < KT) keys &= (1ull << left) - 1;
+        }
+        return fetch_from(k_head, k_off, static_cast<uint32_t>(p.k_token), here, buffer * TILE);
+    };
+    auto bring_values = [&](const Pending& of, uint32_t j0, uint32_t buffer) -> Fetch {
+        if (!together) {
+            one_by_one(std::false_type{}, j0, buffer);
+            return nothing;
+        }
+        return fetch_from(v_head, of.offset, static_cast<uint32_t>(p.v_token), of.here, (2 + buffer) * TILE);
     };
     auto fetch_keys = [&](const Fetch& f, int i) { load_to_lds(f.from, k_lane[i], f.to + i * 1024); };
     auto fetch_values = [&](const Fetch& f, int i) { load_to_lds(f.from, v_lane[i], f.to + i * 1024); };
@@ -384,12 +414,13 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     using Yes = std::true_type;
     using No = std::false_type;
     if (threadIdx.x == 0) *odd_step = 0;
+    uint64_t keys = 0, keys_next = 0, keys_after = 0;      // which keys of this step, the next and the one behind it are there
     if (steps > 0) {
         look_up(key_from);
-        fetch_all(bring(Yes{}, key_from, 0), fetch_keys);
-        if constexpr (NT == 2) fetch_all(bring(No{}, key_from, 0), fetch_values);
+        fetch_all(bring_keys(key_from, 0, keys), fetch_keys);
+        if constexpr (NT == 2) fetch_all(bring_values(values_next, key_from, 0), fetch_values);
         look_up(key_from + KT);
-        if (steps > 1) fetch_all(bring(Yes{}, key_from + KT, 1), fetch_keys);
+        fetch_all(bring_keys(key_from + KT, 1, keys_next), fetch_keys);
         look_up(key_from + 2 * KT);
     }
     arrive();
@@ -401,28 +432,23 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s = tile_mfma<T>(scores_of(0, 0, ks), qf[ks], s);
-        uint64_t keys = __ballot(there[lane % KT] != 0), keys_next = 0;      // (32 keys: twice the same)
+        if (!together) keys = __ballot(there[lane % KT] != 0) & ALL;
         for (uint32_t step = 0; step < steps; ++step, buffer ^= 1) {
             const uint32_t j0 = key_from + step * KT;
-            Fetch next_values = nothing, next_keys = nothing;
             if constexpr (NT == 2) turn(No{}, nothing, nothing, Index<1>{}, static_cast<uint32_t>(keys), j0, buffer, 1, buffer ^ 1);
             // Here the keys of the next step and the values of this one (one tile a step: of the one before) are there, and what is before them has been read.
             arrive();
-            if (step + 1 < steps) keys_next = __ballot(there[(buffer ^ 1) * KT + lane % KT] != 0);
-            if constexpr (NT == 2) {
-                if (step + 1 < steps) next_values = bring(No{}, j0 + KT, buffer ^ 1);
-            } else {
-                next_values = bring(No{}, j0, buffer, step + 1 < steps);
-            }
-            if (step + 2 < steps) {
-                next_keys = bring(Yes{}, j0 + 2 * KT, buffer);
-                look_up(j0 + 3 * KT);
-            }
+            if (!together) keys_next = __ballot(there[(buffer ^ 1) * KT + lane % KT] != 0) & ALL;
+            // (behind the last step's keys there are none: nothing comes)
+            const Fetch next_values = NT == 2 ? bring_values(values_next, j0 + KT, buffer ^ 1) : bring_values(values_after, j0, buffer);
+            const Fetch next_keys = bring_keys(j0 + 2 * KT, buffer, keys_after);
+            look_up(j0 + 3 * KT);
             if (NT == 2) sort_values(j0, buffer);
             else if (step > 0) sort_values(j0 - KT, buffer ^ 1);
             if constexpr (NT == 2) turn(Yes{}, next_values, next_keys, Index<0>{}, static_cast<uint32_t>(keys >> 32), j0 + 32, buffer ^ 1, 0, buffer);
             else turn(Yes{}, next_values, next_keys, Index<0>{}, static_cast<uint32_t>(keys), j0, buffer ^ 1, 0, buffer ^ 1);
             keys = keys_next;
+            keys_next = keys_after;
         }
         // the last tile's sums
         if constexpr (NT == 1) {
