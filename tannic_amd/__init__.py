@@ -13,3 +13,4 @@ from .tensor import Tensor, Host, Device, tensor
 from . import ops
 from .ops import TannicError
 from .graph import Graph
+from .paged_cache import PagedCache

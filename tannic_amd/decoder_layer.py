@@ -135,6 +135,57 @@ def forward_fused(s, w, x, cos, sin, mask, trace=None):
     return out
 
 
+def _feed_forward(s, w, h):
+    hn = ops.rms_norm(h, w["g2"], s.eps)
+    if "w13" in w:
+        both = ops.matmul(hn, w["w13"].transpose())
+        gate, up = both[..., 0:s.ffn], both[..., s.ffn:2 * s.ffn]
+    else:
+        gate, up = ops.matmul(hn, w["w1"].transpose()), ops.matmul(hn, w["w3"].transpose())
+    return ops.add(h, ops.matmul(ops.swiglu(gate, up), w["w2"].transpose()))
+
+
+def forward_paged(s, w, x, cos, sin, cache, layer, step, trace=None):
+    """The layer over the new tokens of several sequences, whose earlier keys and values lie in the pages of a cache (``paged_cache``).
+
+    x: [1, tokens, hidden], the rows of ``step``'s sequences one after the other; cos, sin: [positions, head_dim/2] for every position a
+    sequence can come to, in x's dtype or float32.  The new keys and values are written into layer ``layer`` of the cache; no scores go through memory."""
+    _, tokens, _ = x.shape
+    xn = ops.rms_norm(x, w["g1"], s.eps)
+    if "wqkv" in w:
+        qkv = ops.matmul(xn, w["wqkv"].transpose()).view(tokens, s.heads + 2 * s.kv_heads, s.head_dim)
+        q, k, v = qkv[:, 0:s.heads], qkv[:, s.heads:s.heads + s.kv_heads], qkv[:, s.heads + s.kv_heads:]
+    else:
+        q, k, v = (ops.matmul(xn, w[name].transpose()).view(tokens, heads, s.head_dim) for name, heads in (("wq", s.heads), ("wk", s.kv_heads), ("wv", s.kv_heads)))
+    keys, values = cache.keys(layer), cache.values(layer)
+    q_rot = ops.append_pages(k, v, keys, values, step.table, step.starts, step.context, cos, sin, q)
+    o = ops.attend_pages(q_rot, keys, values, step.table, step.starts, step.context)
+    h = ops.add(x, ops.matmul(o.view(1, tokens, s.heads * s.head_dim), w["wo"].transpose()))
+    out = _feed_forward(s, w, h)
+    _keep(trace, xn=xn, q=q, k=k, v=v, q_rot=q_rot, o=o, h=h, out=out)
+    return out
+
+
+def cross_weight_shapes(s):
+    """name -> shape of the parameters of a layer's attention to an encoder's states (of the same width as the layer)."""
+    return {"cq": (s.heads * s.head_dim, s.hidden), "ck": (s.kv_heads * s.head_dim, s.hidden), "cv": (s.kv_heads * s.head_dim, s.hidden),
+            "co": (s.hidden, s.heads * s.head_dim), "g3": (s.hidden,)}
+
+
+def encoder_keys(s, w, states):
+    """Keys and values of an encoder's states [batch, states, hidden], once for all tokens that attend to them: [batch, states, kv heads, head_dim] each."""
+    batch, n, _ = states.shape
+    return tuple(ops.matmul(states, w[name].transpose()).view(batch, n, s.kv_heads, s.head_dim) for name in ("ck", "cv"))
+
+
+def cross_attention(s, w, x, k, v, lengths=None):
+    """x [batch, tokens, hidden] plus its attention to an encoder's states (``encoder_keys``), the first ``lengths[b]`` of sequence b."""
+    batch, n, _ = x.shape
+    q = ops.matmul(ops.rms_norm(x, w["g3"], s.eps), w["cq"].transpose()).view(batch, n, s.heads, s.head_dim)
+    o = ops.attend(q, k, v, lengths).view(batch, n, s.heads * s.head_dim)
+    return ops.add(x, ops.matmul(o, w["co"].transpose()))
+
+
 def forward(s, w, x, cos, sin, mask, one, trace=None):
     """x: [1, seq, hidden].  Returns the layer's output, same shape and dtype.  ``trace``: a dictionary that receives
     the intermediate tensors."""
