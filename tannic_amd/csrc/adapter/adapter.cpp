@@ -134,6 +134,20 @@ status softmax(const tensor_t* x, const tensor_t* mask, tensor_t* d, stream_t q,
     return code(tannic_hip_softmax(in(x), mask ? in(mask) : nullptr, out(d), st(q), scale));
 }
 status rope(const tensor_t* x, const tensor_t* c, const tensor_t* s, tensor_t* d, stream_t q) { return code(tannic_hip_rope(in(x), in(c), in(s), out(d), st(q))); }
+status append_pages(const tensor_t* k, const tensor_t* v, const tensor_t* table, const tensor_t* starts, const tensor_t* context, const tensor_t* cos, const tensor_t* sin,
+                    const tensor_t* q, tensor_t* keys, tensor_t* values, tensor_t* turned, stream_t s) {
+    return code(tannic_hip_append_pages(in(k), in(v), in(table), in(starts), in(context), in(cos), in(sin), in(q), out(keys), out(values), out(turned), st(s)));
+}
+status attend_pages(const tensor_t* q, const tensor_t* keys, const tensor_t* values, const tensor_t* table, const tensor_t* starts, const tensor_t* context, tensor_t* d, stream_t s,
+                    float scale) {
+    return code(tannic_hip_attend_pages(in(q), in(keys), in(values), in(table), in(starts), in(context), out(d), st(s), scale));
+}
+status copy_pages(tensor_t* pool, stream_t s, const int32_t* sources, const int32_t* targets, size_t count) {
+    return code(tannic_hip_copy_pages(out(pool), st(s), sources, targets, count));
+}
+status attend(const tensor_t* q, const tensor_t* k, const tensor_t* v, const tensor_t* lengths, tensor_t* d, stream_t s, float scale) {
+    return code(tannic_hip_attend(in(q), in(k), in(v), in(lengths), out(d), st(s), scale));
+}
 
 Recording::Recording(int device) {
     tannic_device_t dvc{};

@@ -131,6 +131,13 @@ status cast(const tensor_t*, tensor_t*, stream_t);
 status rms_norm(const tensor_t* x, const tensor_t* gain, tensor_t*, stream_t, float eps);
 status softmax(const tensor_t* x, const tensor_t* mask_or_null, tensor_t*, stream_t, float scale);
 status rope(const tensor_t* x, const tensor_t* cos, const tensor_t* sin, tensor_t*, stream_t);
+// a cache in pages, and attention (tannic_hip_append_pages, ...): what may be missing is a null pointer
+status append_pages(const tensor_t* k, const tensor_t* v, const tensor_t* table, const tensor_t* starts, const tensor_t* context, const tensor_t* cos_or_null,
+                    const tensor_t* sin_or_null, const tensor_t* q_or_null, tensor_t* keys, tensor_t* values, tensor_t* turned_or_null, stream_t);
+status attend_pages(const tensor_t* q, const tensor_t* keys, const tensor_t* values, const tensor_t* table, const tensor_t* starts, const tensor_t* context, tensor_t*, stream_t,
+                    float scale);
+status copy_pages(tensor_t* pool, stream_t, const int32_t* sources, const int32_t* targets, size_t count);
+status attend(const tensor_t* q, const tensor_t* k, const tensor_t* v, const tensor_t* lengths_or_null, tensor_t*, stream_t, float scale);
 
 // A sequence of the front end's evaluations on one device recorded once and replayed as one HIP graph
 // (tannic_hip_graph_begin / end / launch / destroy):

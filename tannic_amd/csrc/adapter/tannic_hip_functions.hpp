@@ -1,5 +1,5 @@
 // Expression nodes for the operators this backend adds to Tannic's surface: division, dtype conversion, value max / min
-// over an axis, and the one-pass row operators (softmax, rms_norm, swiglu, rope).  Include it after the front end's headers in
+// over an axis, the one-pass row operators (softmax, rms_norm, swiglu, rope), and attention over a cache in pages.  Include it after the front end's headers in
 // a program that links the `cuda::` adapter; the nodes compose with every other expression:
 //
 //     Tensor y = rms_norm(x, gain, 1e-5f) * 2.0f;
@@ -13,8 +13,10 @@
 // these operators, so the nodes evaluate on a Device only; on Host they throw.
 #pragma once
 
+#include <cstdint>
 #include <initializer_list>
 #include <variant>
+#include <vector>
 
 #include "callback.hpp"
 #include "concepts.hpp"
@@ -149,6 +151,32 @@ struct RotaryEmbedding {
     }
 };
 
+struct Attention {      // over keys and values of another length
+    float scale;
+    constexpr type result(type dtype) const { return dtype; }
+    void forward(Tensor const& queries, Tensor const& keys, Tensor const& values, Tensor& target) const {
+        on_device({&queries, &keys, &values}, target, "attend", [&](stream_t s) {
+            return tannic_hip::attend(get_tensor(queries.id()), get_tensor(keys.id()), get_tensor(values.id()), nullptr, get_tensor(target.id()), s, scale);
+        });
+    }
+    void forward(Tensor const& queries, Tensor const& keys, Tensor const& values, Tensor const& lengths, Tensor& target) const {
+        on_device({&queries, &keys, &values, &lengths}, target, "attend", [&](stream_t s) {
+            return tannic_hip::attend(get_tensor(queries.id()), get_tensor(keys.id()), get_tensor(values.id()), get_tensor(lengths.id()), get_tensor(target.id()), s, scale);
+        });
+    }
+};
+
+struct PagedAttention {      // over the pages of a cache
+    float scale;
+    constexpr type result(type dtype) const { return dtype; }
+    void forward(Tensor const& queries, Tensor const& keys, Tensor const& values, Tensor const& table, Tensor const& starts, Tensor const& context, Tensor& target) const {
+        on_device({&queries, &keys, &values, &table, &starts, &context}, target, "attend_pages", [&](stream_t s) {
+            return tannic_hip::attend_pages(get_tensor(queries.id()), get_tensor(keys.id()), get_tensor(values.id()), get_tensor(table.id()), get_tensor(starts.id()),
+                                            get_tensor(context.id()), get_tensor(target.id()), s, scale);
+        });
+    }
+};
+
 }  // namespace tannic::hip
 
 namespace tannic {
@@ -201,6 +229,50 @@ constexpr auto softmax(Source&& source, Mask&& mask, float scale = 1.0f) {
 template <Composable Source, Composable Cosines, Composable Sines>
 constexpr auto rope(Source&& source, Cosines&& cosines, Sines&& sines) {
     return hip::Rowwise<hip::RotaryEmbedding, Source, Cosines, Sines>{{}, std::forward<Source>(source), std::forward<Cosines>(cosines), std::forward<Sines>(sines)};
+}
+
+// attention of q [batch, tokens, heads, d] over k, v [batch, states, kv heads, d] (the first lengths[b] states of a sequence), scores times `scale`
+template <Composable Queries, Composable Keys, Composable Values>
+constexpr auto attend(Queries&& queries, Keys&& keys, Values&& values, float scale) {
+    return hip::Rowwise<hip::Attention, Queries, Keys, Values>{{scale}, std::forward<Queries>(queries), std::forward<Keys>(keys), std::forward<Values>(values)};
+}
+template <Composable Queries, Composable Keys, Composable Values, Composable Lengths>
+constexpr auto attend(Queries&& queries, Keys&& keys, Values&& values, Lengths&& lengths, float scale) {
+    return hip::Rowwise<hip::Attention, Queries, Keys, Values, Lengths>{
+        {scale}, std::forward<Queries>(queries), std::forward<Keys>(keys), std::forward<Values>(values), std::forward<Lengths>(lengths)};
+}
+
+// A cache keys, values [pages, kv heads, page, d] in pages; table [sequences, columns], starts [sequences + 1] and context [sequences] (int32, on the
+// device) as include/tannic_hip.h describes them.
+// attention of the new tokens q [tokens, heads, d] over the pages of their sequences
+template <Composable Queries, Composable Keys, Composable Values, Composable Table, Composable Starts, Composable Lengths>
+constexpr auto attend_pages(Queries&& queries, Keys&& keys, Values&& values, Table&& table, Starts&& starts, Lengths&& context, float scale) {
+    return hip::Rowwise<hip::PagedAttention, Queries, Keys, Values, Table, Starts, Lengths>{
+        {scale}, std::forward<Queries>(queries), std::forward<Keys>(keys), std::forward<Values>(values), std::forward<Table>(table), std::forward<Starts>(starts), std::forward<Lengths>(context)};
+}
+
+// The writing side is evaluated where it is called: k, v [tokens, kv heads, d] into their places, and with angles [positions, d/2] the keys and q turned by
+// their positions first; the turned q comes back.
+inline void append_pages(Tensor const& k, Tensor const& v, Tensor& keys, Tensor& values, Tensor const& table, Tensor const& starts, Tensor const& context) {
+    hip::on_device({&k, &v, &values, &table, &starts, &context}, keys, "append_pages", [&](stream_t s) {
+        return tannic_hip::append_pages(get_tensor(k.id()), get_tensor(v.id()), get_tensor(table.id()), get_tensor(starts.id()), get_tensor(context.id()), nullptr, nullptr, nullptr,
+                                        get_tensor(keys.id()), get_tensor(values.id()), nullptr, s);
+    });
+}
+inline Tensor append_pages(Tensor const& k, Tensor const& v, Tensor& keys, Tensor& values, Tensor const& table, Tensor const& starts, Tensor const& context, Tensor const& cosines,
+                           Tensor const& sines, Tensor const& q) {
+    Tensor turned(q.dtype(), q.shape());
+    hip::on_device({&k, &v, &keys, &values, &table, &starts, &context, &cosines, &sines, &q}, turned, "append_pages", [&](stream_t s) {
+        return tannic_hip::append_pages(get_tensor(k.id()), get_tensor(v.id()), get_tensor(table.id()), get_tensor(starts.id()), get_tensor(context.id()), get_tensor(cosines.id()),
+                                        get_tensor(sines.id()), get_tensor(q.id()), get_tensor(keys.id()), get_tensor(values.id()), get_tensor(turned.id()), s);
+    });
+    return turned;
+}
+
+// page sources[i] of pool [.., pages, kv heads, page, d] over page targets[i], one after another
+inline void copy_pages(Tensor& pool, std::vector<int32_t> const& sources, std::vector<int32_t> const& targets) {
+    if (sources.size() != targets.size()) throw Exception("copy_pages: as many sources as targets");
+    hip::on_device({&pool}, pool, "copy_pages", [&](stream_t s) { return tannic_hip::copy_pages(get_tensor(pool.id()), s, sources.data(), targets.data(), sources.size()); });
 }
 
 }  // namespace tannic
