@@ -31,8 +31,7 @@ __global__ __launch_bounds__(256) void attention_any_kernel(AttentionProblem p, 
     using A = std::conditional_t<std::is_same_v<T, double>, double, float>;
     __shared__ A query[kAttentionHead], weight[4][64], part[4][kAttentionHead], tops[4], sums[4];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    uint32_t token, head;
-    p.heads_div.divmod(blockIdx.x, token, head);
+    const uint32_t token = blockIdx.x, head = blockIdx.y;
     const uint32_t s = PAGED ? sequence_of(p.starts, p.sequences, token) : token / p.per_sequence;
     const Span span = span_of<PAGED>(p, s);
     if (token < span.begin || token - span.begin >= span.count) return;   // no sequence's row: left as it is
@@ -94,7 +93,7 @@ __global__ __launch_bounds__(256) void attention_any_kernel(AttentionProblem p, 
     if (threadIdx.x < p.d) {
         A value = 0;
         for (int w = 0; w < 4; ++w) value += part[w][threadIdx.x] * share[w];
-        out[static_cast<size_t>(blockIdx.x) * p.d + threadIdx.x] = narrow<T>(total == A(0) ? A(0) : value / total);
+        out[(static_cast<size_t>(token) * p.heads + head) * p.d + threadIdx.x] = narrow<T>(total == A(0) ? A(0) : value / total);
     }
 }
 
@@ -131,19 +130,21 @@ int attention_arrivals(hipStream_t stream, uint32_t*& arrivals) try {
 
 template <class T>
 int run_attention(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
-    const dim3 grid(p.tokens * p.heads);
+    const dim3 grid(p.tokens, p.heads);
     const T *pq = static_cast<const T*>(q), *pk = static_cast<const T*>(k), *pv = static_cast<const T*>(v);
     if (p.starts) hipLaunchKernelGGL((attention_any_kernel<T, true>), grid, dim3(256), 0, stream, p, pq, pk, pv, static_cast<T*>(out));
     else hipLaunchKernelGGL((attention_any_kernel<T, false>), grid, dim3(256), 0, stream, p, pq, pk, pv, static_cast<T*>(out));
     return launch_status("attention_any_kernel");
 }
 
-// The kernels that take every row of every operand in 16-byte pieces: tiles of 128 rows of the matrix pipe where the sequences have that many on average, else few rows at a time.
+// The kernels that take every row of every operand in 16-byte pieces: tiles of 128 rows of the matrix pipe where the rows of a sequence and kv head are more than the 16 of a
+// tile of the other's on average (that one would read the keys twice: 8 tokens of 32 / 8 heads of 128 of 16 sequences behind 8192 173 us instead of 109, 12 tokens 287 instead
+// of 111; 4 tokens, one tile for both, 111 and 107, and of 8 sequences' 16 heads of 64 over 2000 states 15 and 20).
 int attention_pieces(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
     const int64_t size = static_cast<int64_t>(dtype_size(dtype));
     const int64_t grain = p.d | p.q_batch | p.q_token | p.q_head | p.k_page | p.k_head | p.k_token | p.v_page | p.v_head | p.v_token;
     if ((grain * size) % 16 != 0 || !aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 4 * size)) return TANNIC_UNSUPPORTED_DTYPE;
-    if (static_cast<uint64_t>(p.tokens) * p.group >= 64ull * p.sequences) {
+    if (static_cast<uint64_t>(p.tokens) * p.group > 16ull * p.sequences) {
         if (int status = attention_tile(dtype, p, q, k, v, out, stream); status != TANNIC_UNSUPPORTED_DTYPE) return status;
     }
     return attention_rows(dtype, p, q, k, v, out, stream);
@@ -181,8 +182,8 @@ int tannic_hip_attend_pages(const tannic_tensor_t* q, const tannic_tensor_t* key
     AttentionProblem p{};
     p.heads = static_cast<uint32_t>(q->shape.sizes[1]);
     p.d = static_cast<uint32_t>(q->shape.sizes[2]);
-    if (q->shape.sizes[0] >= (1ull << 31) || q->shape.sizes[1] >= (1u << 16) || q->shape.sizes[0] * q->shape.sizes[1] >= (1ull << 30))
-        return refuse("attend_pages: 2^30 rows of queries or more are not supported");
+    if (q->shape.sizes[0] >= kMostBlocks || q->shape.sizes[1] >= (1u << 16) || q->shape.sizes[0] * q->shape.sizes[1] >= (1ull << 30))
+        return refuse("attend_pages: 2^24 tokens, 2^16 heads or 2^30 rows of queries or more are not supported");
     if (q->shape.sizes[2] != keys->shape.sizes[3] || q->shape.sizes[2] > kAttentionHead) return refuse("attend_pages: q and the keys have one head size, at most 256");
     if (q->shape.sizes[1] == 0 || pages.kv_heads == 0 || q->shape.sizes[1] % pages.kv_heads != 0) return refuse("attend_pages: the number of heads is a multiple of the cache's");
     if (q->shape.sizes[2] > 1 && q->strides.sizes[2] != 1) return refuse("attend_pages: the elements of a head of q lie one after the other");
@@ -198,7 +199,6 @@ int tannic_hip_attend_pages(const tannic_tensor_t* q, const tannic_tensor_t* key
     p.starts = pages.starts, p.context = pages.context, p.table = pages.table, p.table_row = pages.table_row;
     p.columns = pages.columns, p.pages = pages.pages, p.page = pages.page, p.page_div = pages.page_div, p.room = pages.room;
     p.group = p.heads / p.kv_heads;
-    p.heads_div = FastDiv(p.heads);
     p.group_div = FastDiv(p.group);
     p.scale = scale;
     return run_attention(q->dtype, p, q->address, keys->address, values->address, dst->address, as_stream(stream));
@@ -216,8 +216,8 @@ int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const 
     if (k->shape.sizes[0] != batch || k->shape.sizes[3] != d) return refuse("attend: q, k and v have one batch and one head size");
     if (d > kAttentionHead) return refuse("attend: heads of more than 256 elements are not supported");
     if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0) return refuse("attend: the number of heads is a multiple of the keys'");
-    if (batch >= (1ull << 31) || n >= (1ull << 31) || heads >= (1u << 16) || states >= (1ull << 31) || batch * n >= (1ull << 31) || batch * n * heads >= (1ull << 30))
-        return refuse("attend: 2^30 rows of queries, 2^31 keys, or more are not supported");
+    if (batch >= kMostBlocks || n >= kMostBlocks || heads >= (1u << 16) || states >= (1ull << 31) || batch * n >= kMostBlocks || batch * n * heads >= (1ull << 30))
+        return refuse("attend: 2^24 tokens, 2^16 heads, 2^30 rows of queries, 2^31 keys or more are not supported");
     if (lengths && (lengths->rank != 1 || lengths->shape.sizes[0] != batch || !rows_contiguous(lengths))) return refuse("attend: lengths [batch], contiguous");
     if (d > 1 && (q->strides.sizes[3] != 1 || (states > 0 && (k->strides.sizes[3] != 1 || v->strides.sizes[3] != 1)))) return refuse("attend: the elements of a head lie one after the other");
     if (element_count(q) == 0) return TANNIC_SUCCESS;
@@ -237,7 +237,6 @@ int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const 
     p.pages = p.sequences;
     p.page = p.room;
     p.group = p.heads / p.kv_heads;
-    p.heads_div = FastDiv(p.heads);
     p.group_div = FastDiv(p.group);
     p.scale = scale;
     return run_attention(q->dtype, p, q->address, k->address, v->address, dst->address, as_stream(stream));

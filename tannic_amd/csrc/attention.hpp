@@ -16,7 +16,7 @@ namespace th {
 struct AttentionProblem {
     uint32_t sequences, per_sequence, tokens;   // tokens: rows of q and of the result over all sequences
     uint32_t heads, kv_heads, group, d;
-    FastDiv heads_div, group_div;
+    FastDiv group_div;
     int64_t q_batch, q_token, q_head;
     int64_t k_page, k_head, k_token;
     int64_t v_page, v_head, v_token;

@@ -1,5 +1,5 @@
 // Attention of few rows: one token of every sequence (decoding), or a few.  16-bit types and fp32, rows in 16-byte pieces.
-// The keys and values have to be read once, and that bounds it (HBM): ROWS = 16 MT query rows that read the same kv head - a sequence's
+// The keys and values have to be read once, and that bounds it (HBM): ROWS = 16 query rows that read the same kv head - a sequence's
 // tokens times the heads of a group - are one tile of the matrix pipe, and all keys of all sequences are dealt to the blocks in equal
 // runs (attention.hpp).  A block's wavefronts take 32 keys in turns (fp32: 16), each folding its own softmax; they meet in LDS at the end of a run.
 //   scores  S^T[key][row] = K Q^T: a lane of the accumulator has one row (lane % 16) and four keys (4 (lane / 16) + i), so a row's maximum and
@@ -20,10 +20,10 @@ template <class T, int DP> constexpr size_t rows_lds_bytes() {
     return join > stage ? join : stage;
 }
 
-template <class T, int DP, int MT, bool PAGED>
+template <class T, int DP, bool PAGED>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial, uint32_t* arrivals) {
     constexpr bool HALF = sizeof(T) == 2;
-    constexpr int ROWS = 16 * MT, E = 16 / sizeof(T);       // elements of a piece
+    constexpr int ROWS = 16, E = 16 / sizeof(T);       // elements of a piece
     constexpr int KT = HALF ? 2 : 1, STEP = 16 * KT;        // tiles of 16 keys of a wavefront's step
     constexpr int KS = DP / (4 * E);                        // steps of a score's product: four pieces each
     constexpr int OT = DP / 16;                             // tiles of 16 elements of the result
@@ -43,19 +43,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
         const bool whole = at == g.first && stop == g.first + g.units;
 
         // ---- the tile's rows
-        uint4a qf[MT][KS];
-        uint32_t seen[MT];
+        uint4a qf[KS];
+        const uint32_t row = g.tile * ROWS + col, i = p.group_div.div(row), head = g.head * p.group + row - i * p.group;
+        const bool row_lives = i < g.span.count;
+        const uint32_t seen = row_lives ? keys_seen(p, g.span, i) : 0;
+        const T* const from_row = q + (row_lives ? query_offset(p, g.s, g.span, i, head) : 0);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const uint32_t row = g.tile * ROWS + m * 16 + col, i = p.group_div.div(row), head = g.head * p.group + row - i * p.group;
-            const bool live = i < g.span.count;
-            seen[m] = live ? keys_seen(p, g.span, i) : 0;
-            const T* const from_row = q + (live ? query_offset(p, g.s, g.span, i, head) : 0);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint32_t e = (ks * 4 + quarter) * E;
-                qf[m][ks] = live && e < p.d ? load16(from_row + e) : uint4a{0, 0, 0, 0};
-            }
+        for (int ks = 0; ks < KS; ++ks) {
+            const uint32_t e = (ks * 4 + quarter) * E;
+            qf[ks] = row_lives && e < p.d ? load16(from_row + e) : uint4a{0, 0, 0, 0};
         }
         // the last key any row of the tile sees
         const uint32_t last_i = p.group_div.div(g.tile * ROWS + ROWS - 1);
@@ -64,15 +60,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
         // keys up to here are seen by every live row
         const uint32_t all_see = keys_seen(p, g.span, p.group_div.div(g.tile * ROWS));
 
-        float4a acc[MT][OT];
-        float top[MT], sum[MT];
+        float4a acc[OT];
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            top[m] = -INFINITY;
-            sum[m] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < OT; ++t) acc[m][t] = float4a{0, 0, 0, 0};
-        }
+        for (int t = 0; t < OT; ++t) acc[t] = float4a{0, 0, 0, 0};
 
         // ---- keys and values of a step: a lane has key lane % 16 of every tile, pieces lane / 16, lane / 16 + 4, ...
         uint4a kf[KT][KS], vf[KT][KS];
@@ -162,15 +153,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 }
             }
             asm volatile("" ::: "memory");      // (a wavefront reads what it wrote in order)
-            float4a s[MT][KT];
+            float4a s[KT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int kt = 0; kt < KT; ++kt) {
+                s[kt] = float4a{0, 0, 0, 0};
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    s[m][kt] = float4a{0, 0, 0, 0};
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) s[m][kt] = rows_mfma<T>(kf[kt][ks], qf[m][ks], s[m][kt]);
-                }
+                for (int ks = 0; ks < KS; ++ks) s[kt] = rows_mfma<T>(kf[kt][ks], qf[ks], s[kt]);
+            }
             uint4a now[HALF ? 1 : KS];      // (fp32: this step's values stay in registers while the next ones come)
             if constexpr (!HALF) {
 #pragma unroll
@@ -181,44 +170,37 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 fetch();
                 look_up(j0 + 8 * STEP);
             }
+            float high = -INFINITY;
+            bool live[KT][4];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                float high = -INFINITY;
-                bool live[KT][4];
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                for (int i = 0; i < 4; ++i) {
+                    s[kt][i] *= factor;
+                    live[kt][i] = full || (((keys_here[kt] >> (4 * quarter + i)) & 1) && j_now + kt * 16 + 4 * quarter + i < seen);
+                    high = fmaxf(high, live[kt][i] ? s[kt][i] : -INFINITY);
+                }
+            high = across_groups_max(high);
+            const float above = fmaxf(top, high);
+            const float base = above == -INFINITY ? 0.0f : above - kWeightShift<T>;
+            const float old = __builtin_amdgcn_exp2f(top - kWeightShift<T> - base);
+            top = above;
+            float part = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[m][kt][i] *= factor;
-                        live[kt][i] = full || (((keys_here[kt] >> (4 * quarter + i)) & 1) && j_now + kt * 16 + 4 * quarter + i < seen[m]);
-                        high = fmaxf(high, live[kt][i] ? s[m][kt][i] : -INFINITY);
-                    }
-                high = across_groups_max(high);
-                const float above = fmaxf(top[m], high);
-                const float base = above == -INFINITY ? 0.0f : above - kWeightShift<T>;
-                const float old = __builtin_amdgcn_exp2f(top[m] - kWeightShift<T> - base);
-                top[m] = above;
-                float part = 0.0f;
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                for (int i = 0; i < 4; ++i) {
+                    s[kt][i] = live[kt][i] ? __builtin_amdgcn_exp2f(s[kt][i] - base) : 0.0f;
+                    part += s[kt][i];
+                }
+            sum = sum * old + part;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[m][kt][i] = live[kt][i] ? __builtin_amdgcn_exp2f(s[m][kt][i] - base) : 0.0f;
-                        part += s[m][kt][i];
-                    }
-                sum[m] = sum[m] * old + part;
-#pragma unroll
-                for (int t = 0; t < OT; ++t) acc[m][t] *= old;
-            }
+            for (int t = 0; t < OT; ++t) acc[t] *= old;
             if constexpr (HALF) {
                 using Lds = __attribute__((address_space(3))) short;
                 typedef short short4a __attribute__((ext_vector_type(4)));
                 using Lds4 = __attribute__((address_space(3))) short4a;
-                uint4a weights[MT];
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    weights[m] = uint4a{pack_weights<T>(s[m][0][0], s[m][0][1]), pack_weights<T>(s[m][0][2], s[m][0][3]), pack_weights<T>(s[m][KT - 1][0], s[m][KT - 1][1]),
-                                        pack_weights<T>(s[m][KT - 1][2], s[m][KT - 1][3])};
+                const uint4a weights{pack_weights<T>(s[0][0], s[0][1]), pack_weights<T>(s[0][2], s[0][3]), pack_weights<T>(s[KT - 1][0], s[KT - 1][1]), pack_weights<T>(s[KT - 1][2], s[KT - 1][3])};
                 const T* const read_from = mine + (4 * quarter + col / 4) * PITCH + 4 * (col % 4);
 #pragma unroll
                 for (int t = 0; t < OT; ++t) {
@@ -226,8 +208,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                     uint4a values;
                     __builtin_memcpy(&values, &low, 8);
                     __builtin_memcpy(reinterpret_cast<char*>(&values) + 8, &high, 8);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) acc[m][t] = rows_mfma<T>(values, weights[m], acc[m][t]);
+                    acc[t] = rows_mfma<T>(values, weights, acc[t]);
                 }
             } else {
                 // product i has the keys 4 (lane / 16) + i; tile 4 c + w holds the elements 64 c + 4 (row of the tile) + w
@@ -237,9 +218,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                     for (int c = 0; c < KS / 4; ++c)
 #pragma unroll
                         for (int w = 0; w < 4; ++w)
-#pragma unroll
-                            for (int m = 0; m < MT; ++m)
-                                acc[m][4 * c + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now[i * (KS / 4) + c][w]), s[m][0][i], acc[m][4 * c + w], 0, 0, 0);
+                            acc[4 * c + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now[i * (KS / 4) + c][w]), s[0][i], acc[4 * c + w], 0, 0, 0);
             }
             if (odd_values) {
                 // the infinite and the NaN, key by key, where they are seen
@@ -250,25 +229,22 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                     const uint32_t j = j_now + n;
                     if (j >= key_to || !place_of<PAGED>(p, g.s, j, page, in)) continue;
                     const T* const value = v + page * p.v_page + in * p.v_token + g.head * p.v_head;
+                    const uint32_t n16 = n % 16;
+                    float mine_w = 0.0f;
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const uint32_t n16 = n % 16;
-                        float mine_w = 0.0f;
+                    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                        for (int kt = 0; kt < KT; ++kt)
+                        for (int i = 0; i < 4; ++i) mine_w = n == static_cast<uint32_t>(kt * 16) + 4 * (n16 / 4) + i ? s[kt][i] : mine_w;
+                    const float w = __shfl(mine_w, static_cast<int>(16 * (n16 / 4) + col));
+                    if (j < seen) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) mine_w = n == static_cast<uint32_t>(kt * 16) + 4 * (n16 / 4) + i ? s[m][kt][i] : mine_w;
-                        const float w = __shfl(mine_w, static_cast<int>(16 * (n16 / 4) + col));
-                        if (j < seen[m]) {
+                        for (int t = 0; t < OT; ++t)
 #pragma unroll
-                            for (int t = 0; t < OT; ++t)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const uint32_t e = HALF ? t * 16 + 4 * quarter + i : 64 * (t / 4) + 4 * (4 * quarter + i) + t % 4;
-                                    const float x = e < p.d ? static_cast<float>(widen(value[e])) : 0.0f;
-                                    if (!(fabsf(x) < INFINITY)) acc[m][t][i] += w * x;
-                                }
-                        }
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t e = HALF ? t * 16 + 4 * quarter + i : 64 * (t / 4) + 4 * (4 * quarter + i) + t % 4;
+                                const float x = e < p.d ? static_cast<float>(widen(value[e])) : 0.0f;
+                                if (!(fabsf(x) < INFINITY)) acc[t][i] += w * x;
+                            }
                     }
                 }
             }
@@ -289,46 +265,43 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
             __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), result, sizeof result);
         };
         float* const left = partial + (2 * static_cast<uint64_t>(blockIdx.x) + (at == run.from ? 0 : 1)) * partial_floats<ROWS>(p.d);
+        __syncthreads();
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            __syncthreads();
+        for (int t = 0; t < OT; ++t) {
+            if constexpr (HALF) {
+                *reinterpret_cast<float4a*>(join + (wave * 16 + col) * (DP + 4) + t * 16 + 4 * quarter) = acc[t];
+            } else {
 #pragma unroll
-            for (int t = 0; t < OT; ++t) {
-                if constexpr (HALF) {
-                    *reinterpret_cast<float4a*>(join + (wave * 16 + col) * (DP + 4) + t * 16 + 4 * quarter) = acc[m][t];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) join[(wave * 16 + col) * (DP + 4) + 64 * (t / 4) + 4 * (4 * quarter + i) + t % 4] = acc[m][t][i];
-                }
+                for (int i = 0; i < 4; ++i) join[(wave * 16 + col) * (DP + 4) + 64 * (t / 4) + 4 * (4 * quarter + i) + t % 4] = acc[t][i];
             }
-            const float total = across_groups_sum(sum[m]);
-            if (quarter == 0) {
-                stats[(wave * 16 + col) * 2] = top[m];
-                stats[(wave * 16 + col) * 2 + 1] = total;
+        }
+        const float total = across_groups_sum(sum);
+        if (quarter == 0) {
+            stats[(wave * 16 + col) * 2] = top;
+            stats[(wave * 16 + col) * 2 + 1] = total;
+        }
+        __syncthreads();
+        for (uint32_t x = threadIdx.x; x < 16 * (DP / 4); x += 256) {
+            const uint32_t r = x / (DP / 4), piece = x % (DP / 4);
+            if (piece >= pieces || r >= rows) continue;
+            float above = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) above = fmaxf(above, stats[(w * 16 + r) * 2]);
+            const float base = above == -INFINITY ? 0.0f : above;
+            float total_weight = 0.0f;
+            float4a value{0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float share = __builtin_amdgcn_exp2f(stats[(w * 16 + r) * 2] - base);
+                total_weight += stats[(w * 16 + r) * 2 + 1] * share;
+                value += *reinterpret_cast<const float4a*>(join + (w * 16 + r) * (DP + 4) + piece * 4) * share;
             }
-            __syncthreads();
-            for (uint32_t x = threadIdx.x; x < 16 * (DP / 4); x += 256) {
-                const uint32_t r = x / (DP / 4), piece = x % (DP / 4);
-                if (piece >= pieces || m * 16 + r >= rows) continue;
-                float above = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) above = fmaxf(above, stats[(w * 16 + r) * 2]);
-                const float base = above == -INFINITY ? 0.0f : above;
-                float total_weight = 0.0f;
-                float4a value{0, 0, 0, 0};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float share = __builtin_amdgcn_exp2f(stats[(w * 16 + r) * 2] - base);
-                    total_weight += stats[(w * 16 + r) * 2 + 1] * share;
-                    value += *reinterpret_cast<const float4a*>(join + (w * 16 + r) * (DP + 4) + piece * 4) * share;
-                }
-                if (whole) {
-                    write_row(m * 16 + r, piece, value, total_weight);
-                } else {
-                    store_through(left + (m * 16 + r) * p.d + piece * 4, value[0], value[1]);
-                    store_through(left + (m * 16 + r) * p.d + piece * 4 + 2, value[2], value[3]);
-                    if (piece == 0) store_through(left + static_cast<size_t>(ROWS) * p.d + 2 * (m * 16 + r), above, total_weight);
-                }
+            if (whole) {
+                write_row(r, piece, value, total_weight);
+            } else {
+                store_through(left + r * p.d + piece * 4, value[0], value[1]);
+                store_through(left + r * p.d + piece * 4 + 2, value[2], value[3]);
+                if (piece == 0) store_through(left + static_cast<size_t>(ROWS) * p.d + 2 * r, above, total_weight);
             }
         }
         if (!whole) {
@@ -414,43 +387,38 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
     }
 }
 
-constexpr uint32_t kRowsBlocks = 512;      // two on every compute unit
+// as many as run at a time: two on every compute unit, of the largest heads one (512 of those: 51 us instead of 40 for a token of 16 sequences behind 4096, 12 heads of 256)
+template <int DP> constexpr uint32_t kRowsBlocks = DP > 128 ? 256 : 512;
+static_assert(kRowsBlocks<64> <= kAttentionArrivals);
 
-static_assert(kRowsBlocks <= kAttentionArrivals);
-
-template <class T, int DP, int MT, bool PAGED>
+template <class T, int DP, bool PAGED>
 int launch_rows(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
-    constexpr int ROWS = 16 * MT;
+    constexpr int ROWS = 16;
     constexpr size_t LDS = rows_lds_bytes<T, DP>();
     static std::atomic<uint64_t> raised{0};
     if (LDS > (64u << 10))
-        if (int status = raise_lds_limit(reinterpret_cast<const void*>(attention_rows_kernel<T, DP, MT, PAGED>), LDS, raised); status != TANNIC_SUCCESS) return status;
+        if (int status = raise_lds_limit(reinterpret_cast<const void*>(attention_rows_kernel<T, DP, PAGED>), LDS, raised); status != TANNIC_SUCCESS) return status;
     // no more blocks than units there can be
     const uint64_t tiles = static_cast<uint64_t>(p.tokens) * p.group / ROWS + p.sequences;
     const uint64_t most = tiles * p.kv_heads * (p.room / kRowsUnit + 1);
     if (most >= kMostUnits) return TANNIC_UNSUPPORTED_DTYPE;
-    const uint32_t blocks = most < kRowsBlocks ? static_cast<uint32_t>(most) : kRowsBlocks;
+    const uint32_t blocks = most < kRowsBlocks<DP> ? static_cast<uint32_t>(most) : kRowsBlocks<DP>;
     uint32_t* arrivals = nullptr;
     if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
     float* partial = nullptr;
     if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * blocks * partial_floats<ROWS>(p.d) * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
-    hipLaunchKernelGGL((attention_rows_kernel<T, DP, MT, PAGED>), dim3(blocks), dim3(256), LDS, stream, p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+    hipLaunchKernelGGL((attention_rows_kernel<T, DP, PAGED>), dim3(blocks), dim3(256), LDS, stream, p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
                        static_cast<T*>(out), partial, arrivals);
     const int status = launch_status("attention_rows_kernel");
     scratch_release(partial, stream);
     return status;
 }
 
-template <class T, int DP, bool PAGED>
-int pick_rows(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
-    return launch_rows<T, DP, 1, PAGED>(p, q, k, v, out, stream);
-}
-
 template <class T, bool PAGED>
 int pick_head(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
-    if (p.d <= 64) return pick_rows<T, 64, PAGED>(p, q, k, v, out, stream);
-    if (p.d <= 128) return pick_rows<T, 128, PAGED>(p, q, k, v, out, stream);
-    return pick_rows<T, 256, PAGED>(p, q, k, v, out, stream);
+    if (p.d <= 64) return launch_rows<T, 64, PAGED>(p, q, k, v, out, stream);
+    if (p.d <= 128) return launch_rows<T, 128, PAGED>(p, q, k, v, out, stream);
+    return launch_rows<T, 256, PAGED>(p, q, k, v, out, stream);
 }
 
 template <class T>

@@ -7,6 +7,8 @@
 //           accumulator's order; V is transposed on its way out of LDS (ds_read_b64_tr_b16).
 // The running maximum follows the scores only when one exceeds it by 2^8 (in the weights' power of two): sums in fp32 have the room, and the
 // 64 to 128 sums of a lane are rescaled a few times in a row's life instead of every step.
+#include <algorithm>
+
 #include "attention.hpp"
 #include "gemm_tiles.hpp"
 
@@ -22,7 +24,7 @@ struct Item {
 };
 
 template <bool PAGED, int ROWS, int UNIT>
-__device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_shared, uint32_t least_units, Item& item) {
+__device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_groups, uint32_t most_shared, uint32_t least_units, Item& item) {
     const uint32_t lane = threadIdx.x % 64;
     uint32_t all = 0, groups = 0, tiles = 0, units = 0;
     Span span{};
@@ -38,7 +40,8 @@ __device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_sh
         lanes_sum_before(tiles * p.kv_heads, total);
         groups = sum_units(groups, total);
     }
-    if (all == kMostUnits) return false;
+    // (more groups than the rows of q make: sequences that overlap, against what the starts may hold; there are not the blocks for them)
+    if (all == kMostUnits || groups > most_groups) return false;
     uint32_t per = kMostUnits;
     if (groups < most_shared) {
         per = (all + most_shared - 1) / most_shared;
@@ -125,6 +128,7 @@ template <int NEXT> __device__ inline uint4a read_values(const char* at) {
     return v;
 }
 
+constexpr uint32_t kTileJoin = 8;            // parts put together at a time (4 / 8 / 16, us: 16 tokens behind 32768 56 / 60 / 66, 128 rows of 8 * 16 heads over 2000 states 27 / 25 / 26)
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 template <int DP> constexpr int kTileKeys = DP > 128 ? 32 : 64;
 template <int DP> __host__ __device__ constexpr uint64_t tile_partial_floats() { return static_cast<uint64_t>(kTileRows) * (DP + 2); }
@@ -132,8 +136,8 @@ template <int V> using Index = std::integral_constant<int, V>;
 template <int DP> constexpr size_t tile_lds_bytes() { return 4 * kTileKeys<DP> * DP * 2 + 2 * kTileKeys<DP> + 16 + 4 * 1024; }
 
 template <class T, int DP, bool PAGED>
-__global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_tile_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial, uint32_t* arrivals,
-                                                                                          uint32_t most_shared, uint32_t least_units) {
+__global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attention_tile_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial, uint32_t* arrivals,
+                                                                                          uint32_t most_groups, uint32_t most_shared, uint32_t least_units) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int KT = kTileKeys<DP>, NT = KT / 32;         // keys of a step, tiles of 32 of them
     constexpr int KS = DP / 16, OT = DP / 32;               // products of a tile's scores; tiles of 32 elements
@@ -146,7 +150,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
     volatile uint32_t* const odd_step = arrived + 1;     // the step in which a value was not finite
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
     Item item;
-    if (!item_of_block<PAGED, kTileRows, KT>(p, most_shared, least_units, item)) return;
+    if (!item_of_block<PAGED, kTileRows, KT>(p, most_groups, most_shared, least_units, item)) return;
     const Span span = item.span;
     const uint32_t first_i = p.group_div.div(item.tile * kTileRows);
     uint32_t last_i = p.group_div.div(item.tile * kTileRows + kTileRows - 1);
@@ -504,69 +508,89 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : 2) void attention_t
         write_row(acc, sum);
         return;
     }
-    // ---- or a part of it, as the lanes have it, put together by the group's last block (attention.hpp: through the memory that all dies see)
+    // ---- or a part of it, as the lanes have it.  kTileJoin parts that lie beside each other are put together by the last of their blocks to get here, what comes of
+    // them by the last of those that have kTileJoin of these, and so on: always the same ones in the same order, whichever block is last.  (One block that reads all 64
+    // parts of a group: 166 us for 16 tokens of 32 heads behind 32768; so: 60.)
     constexpr uint64_t SLOT = tile_partial_floats<DP>(), STATS = static_cast<uint64_t>(kTileRows) * DP;
-    const uint32_t my_row = wave * 32 + col, first = item.number - item.chunk;
-    if (row_lives) {
-        float* const left = partial + item.number * SLOT;
-#pragma unroll
-        for (int t = 0; t < OT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) store_through(left + ((t * 8 + i / 2) * (64 * kTileWaves) + threadIdx.x) * 2, acc[t][i], acc[t][i + 1]);
-        if (half == 0) store_through(left + STATS + 2 * my_row, top == -INFINITY ? -INFINITY : top * factor, sum);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const uint32_t before = __hip_atomic_fetch_add(arrivals + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (before == chunks - 1) __hip_atomic_store(arrivals + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *arrived = before;
-    }
-    __syncthreads();
-    if (*arrived != chunks - 1 || !row_lives) return;
-    const float* const parts = partial + first * SLOT;
-    float above = -INFINITY, total = 0.0f;
-    for (uint32_t c = 0; c < chunks; ++c) {
-        float its_top, its_sum;
-        load_through(parts + c * SLOT + STATS + 2 * my_row, its_top, its_sum);
-        above = fmaxf(above, its_top);
-    }
-    base = above == -INFINITY ? 0.0f : above;
-    float16a whole[OT];
-#pragma unroll
-    for (int t = 0; t < OT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) whole[t][i] = 0.0f;
-    for (uint32_t c = 0; c < chunks; ++c) {      // (in the order of the chunks, whichever block is the last)
-        const float* const its = parts + c * SLOT;
-        float its_top, its_sum;
-        load_through(its + STATS + 2 * my_row, its_top, its_sum);
-        const float share = __builtin_amdgcn_exp2f(its_top - base);
-        total += its_sum * share;
-        if (c == item.chunk) {
+    constexpr uint32_t AT_ONCE = DP > 64 ? 4 : 2;      // parts whose loads are on their way, 8 of each (4 of the small heads: registers of the loop above spill)
+    const uint32_t my_row = wave * 32 + col;
+    float* const group_parts = partial + static_cast<uint64_t>(item.number - item.chunk) * SLOT;
+    uint32_t* const group_arrivals = arrivals + (item.number - item.chunk);
+    top = top == -INFINITY ? -INFINITY : top * factor;
+    uint32_t parts = chunks, mine = item.chunk, apart = 1;      // a part's place is `apart` from the next one's
+#pragma unroll 1
+    for (uint32_t level = 0; parts > 1; ++level, parts = (parts + kTileJoin - 1) / kTileJoin, mine /= kTileJoin, apart *= kTileJoin) {
+        const uint32_t first = mine - mine % kTileJoin, together_here = parts - first < kTileJoin ? parts - first : kTileJoin;
+        if (together_here == 1) continue;
+        float* const its = group_parts + static_cast<uint64_t>(first * apart) * SLOT;
+        if (row_lives) {
+            float* const left = its + static_cast<uint64_t>((mine - first) * apart) * SLOT;
 #pragma unroll
             for (int t = 0; t < OT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) whole[t][i] += acc[t][i] * share;
-        } else {
+                for (int i = 0; i < 16; i += 2) store_through(left + ((t * 8 + i / 2) * (64 * kTileWaves) + threadIdx.x) * 2, acc[t][i], acc[t][i + 1]);
+            if (half == 0) store_through(left + STATS + 2 * my_row, top, sum);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            // (two parts or more here: a count for each level)
+            uint32_t* const count = group_arrivals + first * apart + level;
+            const uint32_t before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (before == together_here - 1) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *arrived = before;
+        }
+        __syncthreads();
+        if (*arrived != together_here - 1) return;
+        if (row_lives) {
+            float its_top[kTileJoin], its_sum[kTileJoin];
 #pragma unroll
-            for (int t = 0; t < OT; ++t)
+            for (uint32_t c = 0; c < kTileJoin; ++c) {
+                its_top[c] = -INFINITY, its_sum[c] = 0.0f;
+                if (c < together_here) load_through(its + static_cast<uint64_t>(c * apart) * SLOT + STATS + 2 * my_row, its_top[c], its_sum[c]);
+            }
+            top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    float x, y;
-                    load_through(its + ((t * 8 + i / 2) * (64 * kTileWaves) + threadIdx.x) * 2, x, y);
-                    whole[t][i] += x * share;
-                    whole[t][i + 1] += y * share;
-                    if (i == 14) __builtin_amdgcn_sched_barrier(0);      // (a few loads at a time)
+            for (uint32_t c = 0; c < kTileJoin; ++c) top = fmaxf(top, its_top[c]);
+            sum = 0.0f;
+#pragma unroll
+            for (uint32_t c = 0; c < kTileJoin; ++c) {
+                its_top[c] = __builtin_amdgcn_exp2f(its_top[c] - (top == -INFINITY ? 0.0f : top));      // its share
+                sum += its_sum[c] * its_top[c];
+            }
+#pragma unroll
+            for (int t = 0; t < OT; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+#pragma unroll
+                for (uint32_t c0 = 0; c0 < kTileJoin; c0 += AT_ONCE) {
+                    float x[AT_ONCE][16];
+#pragma unroll
+                    for (uint32_t c = 0; c < AT_ONCE; ++c)
+                        if (c0 + c < together_here) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2)
+                                load_through(its + static_cast<uint64_t>((c0 + c) * apart) * SLOT + ((t * 8 + i / 2) * (64 * kTileWaves) + threadIdx.x) * 2, x[c][i], x[c][i + 1]);
+                        }
+#pragma unroll
+                    for (uint32_t c = 0; c < AT_ONCE; ++c)
+                        if (c0 + c < together_here) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[t][i] += x[c][i] * its_top[c0 + c];
+                        }
                 }
+            }
         }
     }
-    write_row(whole, total);
+    write_row(acc, sum);
 #endif
 }
 
-constexpr uint32_t kTileShared = 512;       // groups from which on keys are not shared: two blocks on every compute unit
-constexpr uint32_t kTileLeast = 4;          // units of a chunk, at least
+// groups from which on keys are not shared: as many as run at a time, two on every compute unit, of the largest heads one (8 tokens of 16 sequences behind 4096, us with
+// 512 / 256: 32 heads of 128 behind 8192 109 / 121, 12 heads of 256 105 / 67)
+template <int DP> constexpr uint32_t kTileShared = DP > 128 ? 256 : 512;
+// units of a chunk, at least (2 / 4 / 8, us: 8 tokens behind 1000 21 / 19 / 22, 16 tokens behind 4096 35 / 33 / 36)
+constexpr uint32_t kTileLeast = 4;
 
 template <class T, int DP, bool PAGED>
 int launch_tile(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
@@ -574,16 +598,17 @@ int launch_tile(const AttentionProblem& p, const void* q, const void* k, const v
     static std::atomic<uint64_t> raised{0};
     if (LDS > (64u << 10))
         if (int status = raise_lds_limit(reinterpret_cast<const void*>(attention_tile_kernel<T, DP, PAGED>), LDS, raised); status != TANNIC_SUCCESS) return status;
-    // as many blocks as there can be items: shared groups have at most kTileShared items more than there are groups
-    const uint64_t groups = (static_cast<uint64_t>(p.tokens) * p.group / kTileRows + p.sequences) * p.kv_heads;
-    if (groups * (p.room / kTileKeys<DP> + 1) >= kMostUnits || groups + kTileShared >= kMostUnits) return TANNIC_UNSUPPORTED_DTYPE;
+    // as many blocks as there can be items: shared groups have at most kTileShared<DP> items more than there are groups, and none of fewer than kTileLeast units but its last
+    const uint64_t groups = (static_cast<uint64_t>(p.tokens) * p.group / kTileRows + p.sequences) * p.kv_heads, units = p.room / kTileKeys<DP> + 1;
+    if (groups * units >= kMostUnits || groups + kTileShared<DP> >= kMostBlocks) return TANNIC_UNSUPPORTED_DTYPE;
+    const uint64_t items = std::min<uint64_t>(groups + kTileShared<DP>, groups * ((units + kTileLeast - 1) / kTileLeast)), parts = std::min<uint64_t>(items, 2 * kTileShared<DP>);
     uint32_t* arrivals = nullptr;
     if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
-    static_assert(2 * kTileShared <= kAttentionArrivals);
+    static_assert(2 * kTileShared<DP> <= kAttentionArrivals);
     float* partial = nullptr;
-    if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * kTileShared * tile_partial_floats<DP>() * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
-    hipLaunchKernelGGL((attention_tile_kernel<T, DP, PAGED>), dim3(static_cast<uint32_t>(groups + kTileShared)), dim3(64 * kTileWaves), LDS, stream, p, static_cast<const T*>(q),
-                       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(out), partial, arrivals, kTileShared, kTileLeast);
+    if (scratch_acquire(reinterpret_cast<void**>(&partial), parts * tile_partial_floats<DP>() * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+    hipLaunchKernelGGL((attention_tile_kernel<T, DP, PAGED>), dim3(static_cast<uint32_t>(items)), dim3(64 * kTileWaves), LDS, stream, p, static_cast<const T*>(q),
+                       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(out), partial, arrivals, static_cast<uint32_t>(groups), kTileShared<DP>, kTileLeast);
     const int status = launch_status("attention_tile_kernel");
     scratch_release(partial, stream);
     return status;
@@ -596,10 +621,12 @@ int pick_tile(const AttentionProblem& p, const void* q, const void* k, const voi
     return launch_tile<T, 256, PAGED>(p, q, k, v, out, stream);
 }
 
-int attention_tile(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+int attention_tile(int dtype, const AttentionProblem& described, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
+    AttentionProblem p = described;
+    if (p.page == 1) p.k_token = p.v_token = p.d;      // (of one row there is no next: what the loads take for it is behind the last byte that they may reach)
     // (a lane's offsets from its wavefront's first key fit 32 bits, and rows ascend)
     const int64_t far = int64_t(1) << 25;
-    if ((p.page > 1 && (p.k_token < p.d || p.v_token < p.d)) || p.k_token >= far || p.v_token >= far) return TANNIC_UNSUPPORTED_DTYPE;
+    if (p.k_token < p.d || p.v_token < p.d || p.k_token >= far || p.v_token >= far) return TANNIC_UNSUPPORTED_DTYPE;
     if (dtype == TANNIC_FLOAT16) return p.starts ? pick_tile<f16, true>(p, q, k, v, out, stream) : pick_tile<f16, false>(p, q, k, v, out, stream);
     if (dtype == TANNIC_BFLOAT16) return p.starts ? pick_tile<bf16, true>(p, q, k, v, out, stream) : pick_tile<bf16, false>(p, q, k, v, out, stream);
     return TANNIC_UNSUPPORTED_DTYPE;

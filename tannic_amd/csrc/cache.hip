@@ -237,7 +237,7 @@ int tannic_hip_append_pages(const tannic_tensor_t* k, const tannic_tensor_t* v, 
             !rows_contiguous(cos) || !rows_contiguous(sin))
             return refuse("append_pages: cos and sin [positions, d/2], contiguous, for an even d");
     }
-    if (tokens >= (1ull << 31) || heads >= (1u << 16) || d > 256) return refuse("append_pages: 2^31 tokens, 2^16 heads or heads of more than 256 elements are not supported");
+    if (tokens >= kMostBlocks || heads >= (1u << 16) || d > 256) return refuse("append_pages: 2^24 tokens, 2^16 heads or heads of more than 256 elements are not supported");
     if (tokens == 0 || d == 0 || heads + k->shape.sizes[1] == 0 || p.pages.sequences == 0) return TANNIC_SUCCESS;
     if (int status = on_device_of("append_pages: the operands live on a device", keys, values, k, v, table, starts, context, cos, sin, q, turned); status != TANNIC_SUCCESS) return status;
     p.tokens = static_cast<uint32_t>(tokens);

@@ -43,6 +43,8 @@ inline int on_device_of(const char* text, const tannic_tensor_t* first, const Ts
     return TANNIC_SUCCESS;
 }
 
+constexpr uint64_t kMostBlocks = 1u << 24;      // of 256 threads: a launch has fewer than 2^32 of those
+
 struct PageTable {
     uint32_t sequences, columns, pages, page, kv_heads, room;
     const int32_t *starts, *context, *table;

@@ -139,3 +139,11 @@ def test_copy_pages_lists():
     lib = ta.library()
     assert lib.kernels["copy_pages"](C.byref(zeros((4, 2, 4, 8), ta.boolean).descriptor()), abi.stream_t(0), numbers(0), numbers(1), 1) == abi.UNSUPPORTED_DTYPE
     assert lib.kernels["copy_pages"](C.byref(pool.descriptor()), abi.stream_t(0), None, None, 1) == abi.ERROR
+
+
+def test_more_tokens_than_a_launch_has_blocks():
+    many, one = zeros((1 << 24, 1, 1), ta.float16), zeros((1, 1, 1, 1), ta.float16)
+    table, starts, context = zeros((1, 1), ta.int32), zeros((2,), ta.int32), zeros((1,), ta.int32)
+    for status, message in (call("attend_pages", [many, one, one, table, starts, context, many], 1.0), call("append_pages", [many, many, table, starts, context, None, None, None, one, one, None]),
+                            call("attend", [zeros((1, 1 << 24, 1, 1), ta.float16), one, one, None, zeros((1, 1 << 24, 1, 1), ta.float16)], 1.0)):
+        assert status == abi.ERROR and "2^24" in message, message

@@ -247,3 +247,38 @@ def test_offsets_past_32_bits(device):
         for h in (0, 15):
             want, slack, size = head_attention(q[:, h], k[:, h // 2], v[:, h // 2], float(np.float32(1 / np.sqrt(d))), 1001 - n + np.arange(n))
             assert_within(got[:, h], want, slack, size, ta.float16, np.abs(v[:, h // 2]).sum(0))
+
+
+@pytest.mark.parametrize("dtype", [ta.float16, ta.bfloat16, ta.float32], ids=str)
+@pytest.mark.parametrize("new,context,heads", [([8], [2200], (4, 1, 64)), ([5], [5000], (4, 1, 128)), ([9], [33500], (4, 1, 64)), ([4, 30], [3000, 1500], (6, 1, 256))], ids=str)
+def test_few_rows_over_many_parts(new, context, heads, dtype, device):
+    """A few rows of one group over keys that many blocks share, so that parts are put together more than once."""
+    rng = np.random.default_rng(hash((tuple(new), heads)) & 0xFFFF)
+    check(Cache(rng, dtype, device, *heads, 16, new, context), device)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens", [1, 40, 200])
+def test_one_state_that_is_not_finite(tokens, dtype, device):
+    """Nothing stands behind a single key: its value is the result, the infinite one too."""
+    rng = np.random.default_rng(tokens)
+    k, v = rounded(rng.standard_normal((2, 2, 1, 3, 64)), dtype)
+    q = rounded(rng.standard_normal((2, tokens, 6, 64)), dtype)
+    v[0, 0, 1, 5], v[1, 0, 2, 60], v[1, 0, 0, 8] = np.inf, -np.inf, np.nan
+    got = ops.attend(*(ta.tensor(x, dtype, device) for x in (q, k, v)), None, 0.125).numpy()
+    want = np.broadcast_to(np.repeat(v, 2, axis=2), q.shape)
+    assert np.array_equal(np.asarray(got, np.float64), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [ta.bfloat16, ta.float32], ids=str)
+def test_sequences_that_overlap_leave_nothing_behind(dtype, device):
+    """Starts that descend are against what they may hold: no row outside q is written, and the next call's results are right."""
+    rng = np.random.default_rng(17)
+    c = Cache(rng, dtype, device, 4, 1, 64, 16, [1300], [700])
+    n = 16
+    table = ta.tensor(np.repeat(c.host_table, n, axis=0), ta.int32, device)
+    starts = ta.tensor(np.array([0, 1300] * (n // 2) + [0]), ta.int32, device)
+    q = ta.tensor(c.q, dtype, device)
+    ops.attend_pages(q, c.keys, c.values, table, starts, ta.tensor(np.full(n, 700), ta.int32, device), 0.125)
+    check(c, device)
+    check(Cache(rng, dtype, device, 4, 1, 64, 16, [30], [2500]), device)
