@@ -137,14 +137,15 @@ int run_attention(const AttentionProblem& p, const void* q, const void* k, const
     return launch_status("attention_any_kernel");
 }
 
-// The kernels that take every row of every operand in 16-byte pieces: tiles of 128 rows of the matrix pipe where the rows of a sequence and kv head are more than the 16 of a
-// tile of the other's on average (that one would read the keys twice: 8 tokens of 32 / 8 heads of 128 of 16 sequences behind 8192 173 us instead of 109, 12 tokens 287 instead
-// of 111; 4 tokens, one tile for both, 111 and 107, and of 8 sequences' 16 heads of 64 over 2000 states 15 and 20).
+// The kernels that take every row of every operand in 16-byte pieces: tiles of 128 rows of the matrix pipe where the rows of a sequence and kv head are more on average than the
+// 16 of the other's tiles, which reads the keys for each (8 tokens of 32 / 8 heads of 128 of 16 sequences behind 8192 173 us there and 109 here, 12 tokens 287 and 111; 4 tokens,
+// one tile for both, 111 and 107, and of 8 sequences' 16 heads of 64 over 2000 states 15 and 20); more than 32 for heads above 128 (12 / 2 heads of 256: 5 tokens of 2 sequences
+// behind 4096 37 and 52, of 16 66 and 66, 8 tokens of 16 83 and 67).
 int attention_pieces(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
     const int64_t size = static_cast<int64_t>(dtype_size(dtype));
     const int64_t grain = p.d | p.q_batch | p.q_token | p.q_head | p.k_page | p.k_head | p.k_token | p.v_page | p.v_head | p.v_token;
     if ((grain * size) % 16 != 0 || !aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 4 * size)) return TANNIC_UNSUPPORTED_DTYPE;
-    if (static_cast<uint64_t>(p.tokens) * p.group > 16ull * p.sequences) {
+    if (static_cast<uint64_t>(p.tokens) * p.group > (p.d > 128 ? 32ull : 16ull) * p.sequences) {
         if (int status = attention_tile(dtype, p, q, k, v, out, stream); status != TANNIC_UNSUPPORTED_DTYPE) return status;
     }
     return attention_rows(dtype, p, q, k, v, out, stream);

@@ -264,7 +264,16 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
             for (int e = 0; e < 4; ++e) result[e] = narrow_result<T>(total == 0.0f ? 0.0f : value[e] * inverse);
             __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), result, sizeof result);
         };
-        float* const left = partial + (2 * static_cast<uint64_t>(blockIdx.x) + (at == run.from ? 0 : 1)) * partial_floats<ROWS>(p.d);
+        const uint32_t slot = static_cast<uint32_t>(partial_floats<ROWS>(p.d)), level_floats = 2 * gridDim.x * slot;      // (9 million floats at most)
+        // (a block has two parts at most: of the group its run starts in, and of one that starts behind that)
+        auto part_of = [&](uint32_t level, uint32_t block) -> float* {
+            return partial + (level % 2) * level_floats + (2 * block + (block * run.per < g.first ? 1 : 0)) * slot;
+        };
+        auto leave = [&](float* left, uint32_t r, uint32_t piece, const float4a& value, float above, float total) {
+            store_through(left + r * p.d + piece * 4, value[0], value[1]);
+            store_through(left + r * p.d + piece * 4 + 2, value[2], value[3]);
+            if (piece == 0) store_through(left + static_cast<size_t>(ROWS) * p.d + 2 * r, above, total);
+        };
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < OT; ++t) {
@@ -296,86 +305,99 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 total_weight += stats[(w * 16 + r) * 2 + 1] * share;
                 value += *reinterpret_cast<const float4a*>(join + (w * 16 + r) * (DP + 4) + piece * 4) * share;
             }
-            if (whole) {
-                write_row(r, piece, value, total_weight);
-            } else {
-                store_through(left + r * p.d + piece * 4, value[0], value[1]);
-                store_through(left + r * p.d + piece * 4 + 2, value[2], value[3]);
-                if (piece == 0) store_through(left + static_cast<size_t>(ROWS) * p.d + 2 * r, above, total_weight);
-            }
+            if (whole) write_row(r, piece, value, total_weight);
+            else leave(part_of(0, blockIdx.x), r, piece, value, above, total_weight);
         }
         if (!whole) {
-            // The last of the group's blocks to get here puts the parts together, in the order of the runs whichever came first; the
-            // count is 0 again behind it.  (A block's run ends in one group at most: the count of the block that has the group's first unit.)
-            const uint32_t first = g.first / run.per, last = (g.first + g.units - 1) / run.per;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                const uint32_t before = __hip_atomic_fetch_add(arrivals + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (before == last - first) __hip_atomic_store(arrivals + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                arrived = before;
-            }
-            __syncthreads();
-            if (arrived == last - first) {
-                // rows * pieces results; where that leaves threads idle, several share a result's parts
-                const uint32_t results = rows * pieces;
-                uint32_t sharing = 1;
-                while (2 * sharing * results <= 256) sharing *= 2;
-                const uint32_t in_share = threadIdx.x / results;
-                for (uint32_t x = sharing == 1 ? threadIdx.x : threadIdx.x % results; x < results && (sharing == 1 || in_share < sharing); x += 256) {
-                    const uint32_t r = x / pieces, piece = x % pieces;
+            // So many parts that lie beside each other are put together by the last of their blocks to get here, what comes of them by the last of those that have so many of
+            // these, and so on: always the same ones in the same order, whichever block is last.  A count is 0 again behind its last block; there is one for each level: of
+            // two parts or more, the first's block is not the group's last (which may have counts of the next group).
+            // (All parts by one block: 3 tokens of 16 / 4 heads of 128 behind 117 and 12655, fp32, 53 us; so: 29.)
+            const uint32_t first = g.first / run.per, last = (g.first + g.units - 1) / run.per;      // the blocks that have its parts
+            const uint32_t results = rows * pieces;
+            const uint32_t log_most = results <= 128 ? 6 : results <= 256 ? 5 : 4;      // (as many as 256 threads read in eight turns, or sixteen)
+            // where that leaves threads idle, several share a result's parts
+            uint32_t sharing = 1;
+            while (2 * sharing * results <= 256) sharing *= 2;
+            const uint32_t in_share = sharing == 1 ? 0 : threadIdx.x / results;
+            uint32_t parts = last - first + 1, mine_at = blockIdx.x - first;
+#pragma unroll 1
+            for (uint32_t level = 0, apart = 0; parts > 1; ++level, apart += log_most) {
+                const uint32_t from = mine_at >> log_most << log_most, here = parts - from < 1u << log_most ? parts - from : 1u << log_most, leader = first + (from << apart);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (here > 1) {
+                    if (threadIdx.x == 0) {
+                        uint32_t* const count = arrivals + leader + level;
+                        const uint32_t before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        if (before == here - 1) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        arrived = before;
+                    }
+                    __syncthreads();
+                    if (arrived != here - 1) break;
+                }
+                parts = (parts + (1u << log_most) - 1) >> log_most;
+                mine_at >>= log_most;
+                float* const left = part_of(level + 1, leader);
+                const float* const its_first = part_of(level, leader);
+                const float* const its_others = partial + (level % 2) * level_floats + 2 * leader * slot;
+                const uint32_t its_step = 2 * slot << apart;
+                for (uint32_t x0 = 0; x0 < results; x0 += 256) {
+                    uint32_t x = sharing == 1 ? x0 + threadIdx.x : threadIdx.x % results;
                     float above = -INFINITY, total = 0.0f;
                     float4a value{0, 0, 0, 0};
-                    // (four parts on their way at once)
-                    for (uint32_t b0 = first + (sharing == 1 ? 0 : in_share); b0 <= last; b0 += 4 * sharing) {
-                        float its_top[4], its_sum[4];
-                        float4a its_value[4];
+                    if (x < results && in_share < sharing) {
+                        const uint32_t r = x / pieces, piece = x % pieces;
+                        constexpr int N = 4;      // parts on their way at once
+                        for (uint32_t n0 = in_share; n0 < here; n0 += N * sharing) {
+                            float its_top[N], its_sum[N];
+                            float4a its_value[N];
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const uint32_t b = b0 + n * sharing <= last ? b0 + n * sharing : last;
-                            const float* const its = partial + (2 * static_cast<uint64_t>(b) + (b == first && b * run.per != g.first ? 1 : 0)) * partial_floats<ROWS>(p.d);
-                            load_through(its + static_cast<size_t>(ROWS) * p.d + 2 * r, its_top[n], its_sum[n]);
-                            load_through(its + r * p.d + piece * 4, its_value[n]);
-                        }
-                        float higher = above;
+                            for (int n = 0; n < N; ++n) {
+                                const uint32_t at_part = n0 + n * sharing < here ? n0 + n * sharing : here - 1;
+                                const float* const its = (at_part == 0 ? its_first : its_others) + at_part * its_step;
+                                load_through(its + ROWS * p.d + 2 * r, its_top[n], its_sum[n]);
+                                load_through(its + r * p.d + piece * 4, its_value[n]);
+                            }
+                            float higher = above;
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            if (b0 + n * sharing > last) its_top[n] = -INFINITY, its_sum[n] = 0.0f, its_value[n] = float4a{0, 0, 0, 0};
-                            higher = fmaxf(higher, its_top[n]);
-                        }
-                        const float base = higher == -INFINITY ? 0.0f : higher, old = __builtin_amdgcn_exp2f(above - base);
-                        total *= old;
-                        value *= old;
+                            for (int n = 0; n < N; ++n) {
+                                if (n0 + n * sharing >= here) its_top[n] = -INFINITY, its_sum[n] = 0.0f, its_value[n] = float4a{0, 0, 0, 0};
+                                higher = fmaxf(higher, its_top[n]);
+                            }
+                            const float base = higher == -INFINITY ? 0.0f : higher, old = __builtin_amdgcn_exp2f(above - base);
+                            total *= old;
+                            value *= old;
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const float share = __builtin_amdgcn_exp2f(its_top[n] - base);
-                            total += its_sum[n] * share;
-                            value += its_value[n] * share;
+                            for (int n = 0; n < N; ++n) {
+                                const float share = __builtin_amdgcn_exp2f(its_top[n] - base);
+                                total += its_sum[n] * share;
+                                value += its_value[n] * share;
+                            }
+                            above = higher;
                         }
-                        above = higher;
                     }
-                    if (sharing == 1) {
-                        write_row(r, piece, value, total);
-                    } else {
+                    if (sharing > 1) {      // (then there is one turn)
                         *reinterpret_cast<float4a*>(join + threadIdx.x * 4) = value;
                         join[1024 + threadIdx.x * 2] = above;
                         join[1024 + threadIdx.x * 2 + 1] = total;
-                    }
-                }
-                if (sharing > 1) {
-                    __syncthreads();
-                    if (threadIdx.x < results) {
-                        float above = -INFINITY, total = 0.0f;
-                        float4a value{0, 0, 0, 0};
-                        for (uint32_t n = 0; n < sharing; ++n) above = fmaxf(above, join[1024 + (n * results + threadIdx.x) * 2]);
-                        const float base = above == -INFINITY ? 0.0f : above;
-                        for (uint32_t n = 0; n < sharing; ++n) {
-                            const uint32_t from = n * results + threadIdx.x;
-                            const float share = __builtin_amdgcn_exp2f(join[1024 + from * 2] - base);
-                            total += join[1024 + from * 2 + 1] * share;
-                            value += *reinterpret_cast<const float4a*>(join + from * 4) * share;
+                        __syncthreads();
+                        x = threadIdx.x;
+                        if (x < results) {
+                            above = -INFINITY, total = 0.0f, value = float4a{0, 0, 0, 0};
+                            for (uint32_t n = 0; n < sharing; ++n) above = fmaxf(above, join[1024 + (n * results + x) * 2]);
+                            const float base = above == -INFINITY ? 0.0f : above;
+                            for (uint32_t n = 0; n < sharing; ++n) {
+                                const uint32_t its = n * results + x;
+                                const float share = __builtin_amdgcn_exp2f(join[1024 + its * 2] - base);
+                                total += join[1024 + its * 2 + 1] * share;
+                                value += *reinterpret_cast<const float4a*>(join + its * 4) * share;
+                            }
                         }
-                        write_row(threadIdx.x / pieces, threadIdx.x % pieces, value, total);
+                    }
+                    if (x < results) {
+                        if (__builtin_expect(parts == 1, 1)) write_row(x / pieces, x % pieces, value, total);
+                        else leave(left, x / pieces, x % pieces, value, above, total);
                     }
                 }
             }
@@ -406,7 +428,7 @@ int launch_rows(const AttentionProblem& p, const void* q, const void* k, const v
     uint32_t* arrivals = nullptr;
     if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
     float* partial = nullptr;
-    if (scratch_acquire(reinterpret_cast<void**>(&partial), 2 * blocks * partial_floats<ROWS>(p.d) * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+    if (scratch_acquire(reinterpret_cast<void**>(&partial), 4 * blocks * partial_floats<ROWS>(p.d) * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
     hipLaunchKernelGGL((attention_rows_kernel<T, DP, PAGED>), dim3(blocks), dim3(256), LDS, stream, p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
                        static_cast<T*>(out), partial, arrivals);
     const int status = launch_status("attention_rows_kernel");

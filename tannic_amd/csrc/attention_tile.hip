@@ -589,8 +589,9 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
 // groups from which on keys are not shared: as many as run at a time, two on every compute unit, of the largest heads one (8 tokens of 16 sequences behind 4096, us with
 // 512 / 256: 32 heads of 128 behind 8192 109 / 121, 12 heads of 256 105 / 67)
 template <int DP> constexpr uint32_t kTileShared = DP > 128 ? 256 : 512;
-// units of a chunk, at least (2 / 4 / 8, us: 8 tokens behind 1000 21 / 19 / 22, 16 tokens behind 4096 35 / 33 / 36)
-constexpr uint32_t kTileLeast = 4;
+// units of a chunk, at least: 256 keys (128 / 256 / 512, us: 8 tokens of 32 heads of 128 behind 1000 21 / 19 / 22, 16 behind 4096 35 / 33 / 36; 198 tokens of 12 heads of 256
+// over 1422 states 55 / 46 / 42, 91 tokens of 25 sequences 70 / 63 / 63, 3 tokens over 4069 states 47 / 51 / 52)
+template <int DP> constexpr uint32_t kTileLeast = 256 / kTileKeys<DP>;
 
 template <class T, int DP, bool PAGED>
 int launch_tile(const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
@@ -598,17 +599,17 @@ int launch_tile(const AttentionProblem& p, const void* q, const void* k, const v
     static std::atomic<uint64_t> raised{0};
     if (LDS > (64u << 10))
         if (int status = raise_lds_limit(reinterpret_cast<const void*>(attention_tile_kernel<T, DP, PAGED>), LDS, raised); status != TANNIC_SUCCESS) return status;
-    // as many blocks as there can be items: shared groups have at most kTileShared<DP> items more than there are groups, and none of fewer than kTileLeast units but its last
+    // as many blocks as there can be items: shared groups have at most kTileShared<DP> items more than there are groups, and none of fewer than kTileLeast<DP> units but its last
     const uint64_t groups = (static_cast<uint64_t>(p.tokens) * p.group / kTileRows + p.sequences) * p.kv_heads, units = p.room / kTileKeys<DP> + 1;
     if (groups * units >= kMostUnits || groups + kTileShared<DP> >= kMostBlocks) return TANNIC_UNSUPPORTED_DTYPE;
-    const uint64_t items = std::min<uint64_t>(groups + kTileShared<DP>, groups * ((units + kTileLeast - 1) / kTileLeast)), parts = std::min<uint64_t>(items, 2 * kTileShared<DP>);
+    const uint64_t items = std::min<uint64_t>(groups + kTileShared<DP>, groups * ((units + kTileLeast<DP> - 1) / kTileLeast<DP>)), parts = std::min<uint64_t>(items, 2 * kTileShared<DP>);
     uint32_t* arrivals = nullptr;
     if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
     static_assert(2 * kTileShared<DP> <= kAttentionArrivals);
     float* partial = nullptr;
     if (scratch_acquire(reinterpret_cast<void**>(&partial), parts * tile_partial_floats<DP>() * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
     hipLaunchKernelGGL((attention_tile_kernel<T, DP, PAGED>), dim3(static_cast<uint32_t>(items)), dim3(64 * kTileWaves), LDS, stream, p, static_cast<const T*>(q),
-                       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(out), partial, arrivals, static_cast<uint32_t>(groups), kTileShared<DP>, kTileLeast);
+                       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(out), partial, arrivals, static_cast<uint32_t>(groups), kTileShared<DP>, kTileLeast<DP>);
     const int status = launch_status("attention_tile_kernel");
     scratch_release(partial, stream);
     return status;
