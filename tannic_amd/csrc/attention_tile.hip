@@ -133,7 +133,7 @@ constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 template <int DP> constexpr int kTileKeys = DP > 128 ? 32 : 64;
 template <int DP> __host__ __device__ constexpr uint64_t tile_partial_floats() { return static_cast<uint64_t>(kTileRows) * (DP + 2); }
 template <int V> using Index = std::integral_constant<int, V>;
-template <int DP> constexpr size_t tile_lds_bytes() { return 4 * kTileKeys<DP> * DP * 2 + 2 * kTileKeys<DP> + 16 + 4 * 1024; }
+template <int DP> constexpr size_t tile_lds_bytes() { return 4 * kTileKeys<DP> * DP * 2 + 16 + 4 * 1024; }
 
 template <class T, int DP, bool PAGED>
 __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attention_tile_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial, uint32_t* arrivals,
@@ -144,9 +144,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
     constexpr int LPR = DP / 8, RPI = 64 / LPR;             // 16-byte pieces of a row; rows of a load
     constexpr int KPW = KT / kTileWaves, LOADS = KPW / RPI; // keys a wavefront brings, in so many loads each for K and V
     constexpr uint32_t TILE = KT * DP * 2;                  // bytes
-    extern __shared__ __align__(16) char lds_raw[];         // keys of two steps, values of two; which keys of either are there
-    uint8_t* const there = reinterpret_cast<uint8_t*>(lds_raw + 4 * TILE);
-    volatile uint32_t* const arrived = reinterpret_cast<volatile uint32_t*>(lds_raw + 4 * TILE + 2 * KT);
+    extern __shared__ __align__(16) char lds_raw[];         // keys of two steps, values of two
+    volatile uint32_t* const arrived = reinterpret_cast<volatile uint32_t*>(lds_raw + 4 * TILE);
     volatile uint32_t* const odd_step = arrived + 1;     // the step in which a value was not finite
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
     Item item;
@@ -204,7 +203,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
         int4a from;
         uint32_t to;
     };
-    const Fetch nothing{{0, 0, 0, 0x00020000}, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(lds_at + 4 * TILE + 2 * KT + 16))};      // (a place that nobody reads)
+    const Fetch nothing{{0, 0, 0, 0x00020000}, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(lds_at + 4 * TILE + 16))};      // (a place that nobody reads)
     auto fetch_from = [&](const T* base, int64_t offset, uint32_t token_stride, uint32_t here, uint32_t to) -> Fetch {
         const uint64_t start = reinterpret_cast<uint64_t>(base + offset);
         return Fetch{{__builtin_amdgcn_readfirstlane(static_cast<int>(start)), __builtin_amdgcn_readfirstlane(static_cast<int>(start >> 32) & 0xFFFF),
@@ -212,16 +211,16 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
                      static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(lds_at + to + wave * (LOADS * 1024)))};
     };
     // A wavefront's keys of a step mostly lie in one page: lane w holds the number of wavefront w's, asked for a step before it is needed, and which keys of the step are there
-    // follows from the four.  Where pages end inside a wavefront's keys they are looked up one by one, and `there` says which of them are.
+    // follows from the four.  Where pages end inside a wavefront's keys lane n holds the number of key n's.
     const bool together = !PAGED || p.page % KPW == 0;
     const T* const k_head = k + static_cast<int64_t>(item.head) * p.k_head;
     const T* const v_head = v + static_cast<int64_t>(item.head) * p.v_head;
     const bool alike = p.k_page == p.v_page && p.k_token == p.v_token;
     uint32_t next_page = ~0u, next_in = 0;
     auto look_up = [&](uint32_t j0) {
-        const uint32_t j = j0 + (lane % kTileWaves) * KPW;
+        const uint32_t j = j0 + (together ? (lane % kTileWaves) * KPW : lane % KT);
         next_page = ~0u;
-        if (together && j < key_to) next_page = page_of<PAGED>(p, item.s, j, next_in);
+        if (j < key_to) next_page = page_of<PAGED>(p, item.s, j, next_in);
     };
     // the values of a step's keys are brought one (one tile a step: two) steps after them
     struct Pending {
@@ -229,25 +228,26 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
         uint32_t here;
     };
     Pending values_next{0, 0}, values_after{0, 0};
+    uint32_t v_next_page = ~0u, v_next_in = 0, v_after_page = ~0u, v_after_in = 0;      // (key by key)
     constexpr uint64_t ALL = ~0ull >> (64 - KT);
-    auto one_by_one = [&](auto of_keys, uint32_t j0, uint32_t buffer) {
+    auto one_by_one = [&](auto of_keys, uint32_t key_page, uint32_t key_in, uint32_t buffer) {
         constexpr bool KEYS = decltype(of_keys)::value;
         const uint32_t place = (KEYS ? buffer : 2 + buffer) * TILE + wave * (LOADS * 1024), to = __builtin_amdgcn_readfirstlane(lds_at + place);
 #pragma unroll 1
         for (uint32_t i = 0; i < LOADS; ++i) {
-            const uint32_t r = i * RPI + row_in, in_tile = wave * KPW + r, j = j0 + in_tile;
-            int64_t page = 0;
-            uint32_t in = 0;
-            const bool lives = j < key_to && place_of<PAGED>(p, item.s, j, page, in);
-            const uint32_t its_piece = piece ^ (KEYS ? k_place(in_tile) : v_place(in_tile));
-            if (lives && its_piece * 8 < p.d) load_to_lds((KEYS ? k_head + page * p.k_page + in * p.k_token : v_head + page * p.v_page + in * p.v_token) + its_piece * 8, to + i * 1024);
+            const uint32_t in_tile = wave * KPW + i * RPI + row_in, its_piece = piece ^ (KEYS ? k_place(in_tile) : v_place(in_tile));
+            const uint32_t page = __shfl(key_page, in_tile), in = __shfl(key_in, in_tile);
+            if (page_exists(p, page) && its_piece * 8 < p.d)
+                load_to_lds((KEYS ? k_head + page * p.k_page + in * p.k_token : v_head + page * p.v_page + in * p.v_token) + its_piece * 8, to + i * 1024);
             else *reinterpret_cast<uint4a*>(lds_raw + place + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};
-            if (KEYS && piece == 0) there[buffer * KT + in_tile] = lives;
         }
     };
     auto bring_keys = [&](uint32_t j0, uint32_t buffer, uint64_t& keys) -> Fetch {
         if (!together) {
-            one_by_one(std::true_type{}, j0, buffer);
+            v_after_page = v_next_page, v_after_in = v_next_in;
+            v_next_page = next_page, v_next_in = next_in;
+            keys = __ballot(page_exists(p, next_page)) & ALL;
+            one_by_one(std::true_type{}, next_page, next_in, buffer);
             return nothing;
         }
         const uint32_t live = static_cast<uint32_t>(__ballot(page_exists(p, next_page))) & ((1u << kTileWaves) - 1);
@@ -266,9 +266,9 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
         }
         return fetch_from(k_head, k_off, static_cast<uint32_t>(p.k_token), here, buffer * TILE);
     };
-    auto bring_values = [&](const Pending& of, uint32_t j0, uint32_t buffer) -> Fetch {
+    auto bring_values = [&](const Pending& of, uint32_t key_page, uint32_t key_in, uint32_t buffer) -> Fetch {
         if (!together) {
-            one_by_one(std::false_type{}, j0, buffer);
+            one_by_one(std::false_type{}, key_page, key_in, buffer);
             return nothing;
         }
         return fetch_from(v_head, of.offset, static_cast<uint32_t>(p.v_token), of.here, (2 + buffer) * TILE);
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
     if (steps > 0) {
         look_up(key_from);
         fetch_all(bring_keys(key_from, 0, keys), fetch_keys);
-        if constexpr (NT == 2) fetch_all(bring_values(values_next, key_from, 0), fetch_values);
+        if constexpr (NT == 2) fetch_all(bring_values(values_next, v_next_page, v_next_in, 0), fetch_values);
         look_up(key_from + KT);
         fetch_all(bring_keys(key_from + KT, 1, keys_next), fetch_keys);
         look_up(key_from + 2 * KT);
@@ -436,15 +436,13 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
         for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s = tile_mfma<T>(scores_of(0, 0, ks), qf[ks], s);
-        if (!together) keys = __ballot(there[lane % KT] != 0) & ALL;
         for (uint32_t step = 0; step < steps; ++step, buffer ^= 1) {
             const uint32_t j0 = key_from + step * KT;
             if constexpr (NT == 2) turn(No{}, nothing, nothing, Index<1>{}, static_cast<uint32_t>(keys), j0, buffer, 1, buffer ^ 1);
             // Here the keys of the next step and the values of this one (one tile a step: of the one before) are there, and what is before them has been read.
             arrive();
-            if (!together) keys_next = __ballot(there[(buffer ^ 1) * KT + lane % KT] != 0) & ALL;
             // (behind the last step's keys there are none: nothing comes)
-            const Fetch next_values = NT == 2 ? bring_values(values_next, j0 + KT, buffer ^ 1) : bring_values(values_after, j0, buffer);
+            const Fetch next_values = NT == 2 ? bring_values(values_next, v_next_page, v_next_in, buffer ^ 1) : bring_values(values_after, v_after_page, v_after_in, buffer);
             const Fetch next_keys = bring_keys(j0 + 2 * KT, buffer, keys_after);
             look_up(j0 + 3 * KT);
             if (NT == 2) sort_values(j0, buffer);
