@@ -233,10 +233,13 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
     auto one_by_one = [&](auto of_keys, uint32_t key_page, uint32_t key_in, uint32_t buffer) {
         constexpr bool KEYS = decltype(of_keys)::value;
         const uint32_t place = (KEYS ? buffer : 2 + buffer) * TILE + wave * (LOADS * 1024), to = __builtin_amdgcn_readfirstlane(lds_at + place);
-#pragma unroll 1
+        uint32_t pages_of[LOADS], ins_of[LOADS];
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) pages_of[i] = __shfl(key_page, wave * KPW + i * RPI + row_in), ins_of[i] = __shfl(key_in, wave * KPW + i * RPI + row_in);
+#pragma unroll
         for (uint32_t i = 0; i < LOADS; ++i) {
             const uint32_t in_tile = wave * KPW + i * RPI + row_in, its_piece = piece ^ (KEYS ? k_place(in_tile) : v_place(in_tile));
-            const uint32_t page = __shfl(key_page, in_tile), in = __shfl(key_in, in_tile);
+            const uint32_t page = pages_of[i], in = ins_of[i];
             if (page_exists(p, page) && its_piece * 8 < p.d)
                 load_to_lds((KEYS ? k_head + page * p.k_page + in * p.k_token : v_head + page * p.v_page + in * p.v_token) + its_piece * 8, to + i * 1024);
             else *reinterpret_cast<uint4a*>(lds_raw + place + i * 1024 + lane * 16) = uint4a{0, 0, 0, 0};
