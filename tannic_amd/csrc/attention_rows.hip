@@ -11,7 +11,9 @@
 
 namespace th {
 
-constexpr int kRowsUnit = 64;       // keys of a unit
+// keys of a unit: a step of each of the four wavefronts (half of that, 16-bit: a token behind 2048 13.2 us instead of 11.5, of 8 sequences' 16 heads of 64 over 1024 states 13.3 and
+// 12.6; twice that 13.1 and 11.8)
+template <class T> constexpr int kRowsUnit = sizeof(T) == 2 ? 128 : 64;
 
 template <class T> __device__ inline uint4a load16(const T* at) { return *reinterpret_cast<const uint4a*>(at); }
 
@@ -33,13 +35,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
     __shared__ uint32_t arrived;
     Run run;
     Group g;
-    if (!run_of_block<PAGED, ROWS, kRowsUnit>(p, gridDim.x, run, g)) return;
+    if (!run_of_block<PAGED, ROWS, kRowsUnit<T>>(p, gridDim.x, run, g)) return;
     const float factor = p.scale * 1.44269504088896340736f;      // weights are powers of two
     uint32_t at = run.from;
     while (true) {
         const uint32_t stop = g.first + g.units < run.to ? g.first + g.units : run.to;
-        const uint32_t key_from = (at - g.first) * kRowsUnit;
-        uint32_t key_to = (stop - g.first) * kRowsUnit;
+        const uint32_t key_from = (at - g.first) * kRowsUnit<T>;
+        uint32_t key_to = (stop - g.first) * kRowsUnit<T>;
         const bool whole = at == g.first && stop == g.first + g.units;
 
         // ---- the tile's rows
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                     float4a value{0, 0, 0, 0};
                     if (x < results && in_share < sharing) {
                         const uint32_t r = x / pieces, piece = x % pieces;
-                        constexpr int N = 4;      // parts on their way at once
+                        constexpr int N = HALF ? 4 : 8;      // parts on their way at once (fp32, 8 instead of 4: 41 us instead of 43 for 36 tokens of 2 sequences behind 53 and 2516)
                         for (uint32_t n0 = in_share; n0 < here; n0 += N * sharing) {
                             float its_top[N], its_sum[N];
                             float4a its_value[N];
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
         }
         if (stop == run.to) return;
         at = stop;
-        next_group<PAGED, ROWS, kRowsUnit>(p, g);
+        next_group<PAGED, ROWS, kRowsUnit<T>>(p, g);
         __syncthreads();      // (LDS is read to the end before the next group's values are put there)
     }
 }
@@ -422,7 +424,7 @@ int launch_rows(const AttentionProblem& p, const void* q, const void* k, const v
         if (int status = raise_lds_limit(reinterpret_cast<const void*>(attention_rows_kernel<T, DP, PAGED>), LDS, raised); status != TANNIC_SUCCESS) return status;
     // no more blocks than units there can be
     const uint64_t tiles = static_cast<uint64_t>(p.tokens) * p.group / ROWS + p.sequences;
-    const uint64_t most = tiles * p.kv_heads * (p.room / kRowsUnit + 1);
+    const uint64_t most = tiles * p.kv_heads * (p.room / kRowsUnit<T> + 1);
     if (most >= kMostUnits) return TANNIC_UNSUPPORTED_DTYPE;
     const uint32_t blocks = most < kRowsBlocks<DP> ? static_cast<uint32_t>(most) : kRowsBlocks<DP>;
     uint32_t* arrivals = nullptr;
