@@ -128,7 +128,9 @@ template <int NEXT> __device__ inline uint4a read_values(const char* at) {
     return v;
 }
 
-constexpr uint32_t kTileJoin = 8;            // parts put together at a time (4 / 8 / 16, us: 16 tokens behind 32768 56 / 60 / 66, 128 rows of 8 * 16 heads over 2000 states 27 / 25 / 26)
+// parts put together at a time: a block reads them at no more than a compute unit's rate, so few and often of the larger heads (4 / 8, us: 16 tokens of 32 heads of 128 behind 32768
+// 56 / 59, 20 tokens of 12 heads of 256 behind 28185 72 / 85, 198 over 1422 states 44 / 43; 128 tokens of 8 * 16 heads of 64 over 2000 states 27 / 24)
+template <int DP> constexpr uint32_t kTileJoin = DP > 64 ? 4 : 8;
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 template <int DP> constexpr int kTileKeys = DP > 128 ? 32 : 64;
 template <int DP> __host__ __device__ constexpr uint64_t tile_partial_floats() { return static_cast<uint64_t>(kTileRows) * (DP + 2); }
@@ -509,8 +511,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
         write_row(acc, sum);
         return;
     }
-    // ---- or a part of it, as the lanes have it.  kTileJoin parts that lie beside each other are put together by the last of their blocks to get here, what comes of
-    // them by the last of those that have kTileJoin of these, and so on: always the same ones in the same order, whichever block is last.  (One block that reads all 64
+    // ---- or a part of it, as the lanes have it.  kTileJoin<DP> parts that lie beside each other are put together by the last of their blocks to get here, what comes of
+    // them by the last of those that have kTileJoin<DP> of these, and so on: always the same ones in the same order, whichever block is last.  (One block that reads all 64
     // parts of a group: 166 us for 16 tokens of 32 heads behind 32768; so: 60.)
     constexpr uint64_t SLOT = tile_partial_floats<DP>(), STATS = static_cast<uint64_t>(kTileRows) * DP;
     constexpr uint32_t AT_ONCE = DP > 64 ? 4 : 2;      // parts whose loads are on their way, 8 of each (4 of the small heads: registers of the loop above spill)
@@ -520,8 +522,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
     top = top == -INFINITY ? -INFINITY : top * factor;
     uint32_t parts = chunks, mine = item.chunk, apart = 1;      // a part's place is `apart` from the next one's
 #pragma unroll 1
-    for (uint32_t level = 0; parts > 1; ++level, parts = (parts + kTileJoin - 1) / kTileJoin, mine /= kTileJoin, apart *= kTileJoin) {
-        const uint32_t first = mine - mine % kTileJoin, together_here = parts - first < kTileJoin ? parts - first : kTileJoin;
+    for (uint32_t level = 0; parts > 1; ++level, parts = (parts + kTileJoin<DP> - 1) / kTileJoin<DP>, mine /= kTileJoin<DP>, apart *= kTileJoin<DP>) {
+        const uint32_t first = mine - mine % kTileJoin<DP>, together_here = parts - first < kTileJoin<DP> ? parts - first : kTileJoin<DP>;
         if (together_here == 1) continue;
         float* const its = group_parts + static_cast<uint64_t>(first * apart) * SLOT;
         if (row_lives) {
@@ -544,18 +546,18 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
         __syncthreads();
         if (*arrived != together_here - 1) return;
         if (row_lives) {
-            float its_top[kTileJoin], its_sum[kTileJoin];
+            float its_top[kTileJoin<DP>], its_sum[kTileJoin<DP>];
 #pragma unroll
-            for (uint32_t c = 0; c < kTileJoin; ++c) {
+            for (uint32_t c = 0; c < kTileJoin<DP>; ++c) {
                 its_top[c] = -INFINITY, its_sum[c] = 0.0f;
                 if (c < together_here) load_through(its + static_cast<uint64_t>(c * apart) * SLOT + STATS + 2 * my_row, its_top[c], its_sum[c]);
             }
             top = -INFINITY;
 #pragma unroll
-            for (uint32_t c = 0; c < kTileJoin; ++c) top = fmaxf(top, its_top[c]);
+            for (uint32_t c = 0; c < kTileJoin<DP>; ++c) top = fmaxf(top, its_top[c]);
             sum = 0.0f;
 #pragma unroll
-            for (uint32_t c = 0; c < kTileJoin; ++c) {
+            for (uint32_t c = 0; c < kTileJoin<DP>; ++c) {
                 its_top[c] = __builtin_amdgcn_exp2f(its_top[c] - (top == -INFINITY ? 0.0f : top));      // its share
                 sum += its_sum[c] * its_top[c];
             }
@@ -564,7 +566,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
 #pragma unroll
-                for (uint32_t c0 = 0; c0 < kTileJoin; c0 += AT_ONCE) {
+                for (uint32_t c0 = 0; c0 < kTileJoin<DP>; c0 += AT_ONCE) {
                     float x[AT_ONCE][16];
 #pragma unroll
                     for (uint32_t c = 0; c < AT_ONCE; ++c)
