@@ -420,7 +420,8 @@ int tannic_hip_rope(const tannic_tensor_t* x, const tannic_tensor_t* cos, const 
  * tensors is read or written.  starts ascend; rows of no sequence (those
  * behind starts[sequences], a batch's padding) are left as they were.
  * Sums, maxima and rotations are float (float64: double), rounded once;
- * 16-bit weights are rounded for the matrix pipe.
+ * 16-bit weights are rounded for the matrix pipe.  A call has fewer than 2^24
+ * tokens, a sequence fewer than 2^31 keys.
  * ------------------------------------------------------------------ */
 /* k, v [tokens, kv heads, d] into their places: token t of sequence s has the position context[s] + t - starts[s] and goes into page
  * table[s, position / page], row position % page (nowhere if there is no such page).  With cos, sin [positions, d/2] (of k's type or

@@ -583,7 +583,8 @@ def _checked(name, status):
 
 def append_pages(k, v, keys, values, table, starts, context, cos=None, sin=None, q=None):
     """Writes the new tokens' ``k``, ``v [tokens, kv heads, d]`` into the pages of their sequences, behind ``context``.  With ``cos, sin
-    [positions, d/2]`` the keys turn by their positions first, as ``rope`` turns them, and so does ``q [tokens, heads, d]``, which is returned."""
+    [positions, d/2]`` the keys turn by their positions first, as ``rope`` turns them, and so does ``q [tokens, heads, d]``, which is returned (rows of no sequence, a
+    batch's padding, are not written, there or in the cache)."""
     given = [t for t in (cos, sin, q) if t is not None]
     env = _device_of("append_pages", k, v, keys, values, table, starts, context, *given)
     turned = None if q is None else Tensor.fresh(q.dtype, q.shape, env)
@@ -595,7 +596,8 @@ def append_pages(k, v, keys, values, table, starts, context, cos=None, sin=None,
 
 def attend_pages(q, keys, values, table, starts, context, scale=None):
     """Attention of the new tokens ``q [tokens, heads, d]`` over their sequences' pages, every token over the keys up to its own position
-    (written before, see ``append_pages``); ``[tokens, heads, d]``, contiguous.  ``scale`` is ``1 / sqrt(d)`` if not given."""
+    (written before, see ``append_pages``); ``[tokens, heads, d]``, contiguous (rows of no sequence, a batch's
+    padding, are not written: whatever the memory held).  ``scale`` is ``1 / sqrt(d)`` if not given."""
     env = _device_of("attend_pages", q, keys, values, table, starts, context)
     dst = Tensor.fresh(q.dtype, q.shape, env)
     scale = 1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else scale
