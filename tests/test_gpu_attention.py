@@ -1,5 +1,6 @@
 """Attention over a paged cache and over dense states of another length, against the definition in 64 bits."""
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -282,3 +283,62 @@ def test_sequences_that_overlap_leave_nothing_behind(dtype, device):
     ops.attend_pages(q, c.keys, c.values, table, starts, ta.tensor(np.full(n, 700), ta.int32, device), 0.125)
     check(c, device)
     check(Cache(rng, dtype, device, 4, 1, 64, 16, [30], [2500]), device)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_no_states_at_all(tokens, dtype, device):
+    q = ta.tensor(np.ones((2, tokens, 4, 64)), dtype, device)
+    empty = ta.Tensor(dtype, (2, 0, 2, 64)).initialize(device)
+    assert (ops.attend(q, empty, empty).numpy() == 0).all()
+
+
+def test_calls_of_two_threads(device):
+    """Each thread's calls share keys between blocks, on whatever streams they get: no counts and no partial results are mixed up."""
+    rng = np.random.default_rng(18)
+    shapes = [((8, 2, 128), [1, 1], [3000, 1700]), ((4, 1, 64), [30], [4000])]
+    caches = [Cache(rng, ta.bfloat16, device, *heads, 16, new, context) for heads, new, context in shapes]
+    q = [ta.tensor(c.q, ta.bfloat16, device) for c in caches]
+    want = [ops.attend_pages(x, c.keys, c.values, c.table, c.starts, c.lengths, 0.1).storage() for x, c in zip(q, caches)]
+    results = [[], []]
+
+    def work(i):
+        c = caches[i]
+        for _ in range(40):
+            results[i].append(ops.attend_pages(q[i], c.keys, c.values, c.table, c.starts, c.lengths, 0.1))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    ta.library().device_synchronize()
+    for w, got in zip(want, results):
+        assert len(got) == 40
+        for g in got:
+            np.testing.assert_array_equal(g.storage(), w)
+
+
+@pytest.mark.parametrize("dtype", [ta.float16, ta.bfloat16], ids=str)
+@pytest.mark.parametrize("page,d", [(7, 64), (20, 128), (33, 256), (24, 64)])
+def test_chunks_over_pages_that_end_inside_a_step(page, d, dtype, device):
+    """What later tokens hold is infinite or NaN, pages are missing in the middle, and one of them ends with the last key."""
+    rng = np.random.default_rng(page)
+    context, n = 2 * page + 150, 3 * page - 2 * page % 5 + 40
+    c = Cache(rng, dtype, device, 6, 1, d, page, [n], [context])
+    keys, values = c.keys.numpy(), c.values.numpy()
+    for j, bad in ((context + n - 1, np.inf), (context + n - 2, np.nan), (context + n // 2, -np.inf)):
+        values[c.host_table[0, j // page], 0, j % page, 3] = bad
+        c.v[0][j, 0, 3] = bad
+    c.table = ta.tensor(np.where(np.arange(c.host_table.shape[1]) == 1, -1, c.host_table), ta.int32, device)
+    got = ops.attend_pages(ta.tensor(c.q, dtype, device), ta.tensor(keys, dtype, device), ta.tensor(values, dtype, device), c.table, c.starts, c.lengths, 0.125).numpy()
+    with np.errstate(all="ignore"):
+        want, slack, size, total = c.expected(0.125, missing=[(0, 1)])
+    first = n // 2      # the first row that sees one of them; column 3 is no number, or infinite, from there on
+    assert np.isneginf(got[first:n - 2, :, 3]).all() and np.isnan(got[n - 2:, :, 3]).all()
+    total[...] = np.abs(np.where(np.isfinite(c.v[0]), c.v[0], 0)).sum(0)
+    keep = np.ones(got.shape, bool)
+    keep[first:, :, 3] = False
+    for x in (got, want, slack, size):
+        x[~keep] = 0
+    assert_within(got, want, slack, size, dtype, total)
