@@ -25,7 +25,8 @@ __device__ inline double exponential(double x) { return exp(x); }
 constexpr uint32_t kAttentionHead = 256;   // elements of a head, at most
 
 // Any type, alignment and head size: a block per query row, its four wavefronts taking 64 keys in turns; a lane has one key's score,
-// then every lane adds the 64 values' elements lane, lane + 64, ...
+// then every lane adds the 64 values' elements lane, lane + 64, ...  Bound by its loads of the keys, a lane's own row each (a token of 32 heads of 128 behind 2048, bf16:
+// 453 us, where the others take 11.6).
 template <class T, bool PAGED>
 __global__ __launch_bounds__(256) void attention_any_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out) {
     using A = std::conditional_t<std::is_same_v<T, double>, double, float>;
