@@ -18,16 +18,19 @@
 namespace th {
 
 // ---- items: a tile's rows of one kv head over a chunk of its keys -----------------------------------------------------------------
-// Every sequence has tiles x kv heads groups of `chunks` items, those of the last tile (which see the most keys) first.  With fewer groups than blocks that run
-// at a time the keys are shared in chunks; the last of a group's blocks puts its parts together.
+// Every sequence has tiles x kv heads groups of items, those of the last tile (which see the most keys) first.  With `places` blocks that run at a time, a place's share of all
+// keys is as many as a group should have: one that has a quarter more is cut into equal chunks, and the last of its blocks puts the parts together.  (Cut only where there are fewer groups than places: 64 sequences behind 64 to 32768, 16 tokens of
+// 32 / 8 heads of 128 each, 751 us; so: 302.)
 struct Item {
-    uint32_t s, tile, head, chunk, chunk_units;      // units of a chunk
-    uint32_t number;                                 // among all
+    uint32_t s, tile, head, chunk, share;            // share: units of a place
+    uint32_t part;                                   // of the parts of all groups that are cut, its group's first
     Span span;
 };
 
+__device__ inline uint32_t chunks_of(uint32_t units, uint32_t share) { return units > share + share / 4 ? (units + share - 1) / share : 1; }
+
 template <bool PAGED, int ROWS, int UNIT>
-__device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_groups, uint32_t most_shared, uint32_t least_units, Item& item) {
+__device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_groups, uint32_t places, uint32_t least_units, Item& item) {
     const uint32_t lane = threadIdx.x % 64;
     uint32_t all = 0, groups = 0, tiles = 0, units = 0;
     Span span{};
@@ -45,12 +48,9 @@ __device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_gr
     }
     // (more groups than the rows of q make: sequences that overlap, against what the starts may hold; there are not the blocks for them)
     if (all == kMostUnits || groups > most_groups) return false;
-    uint32_t per = kMostUnits;
-    if (groups < most_shared) {
-        per = (all + most_shared - 1) / most_shared;
-        per = per > least_units ? per : least_units;
-    }
-    uint32_t before_all = 0;
+    uint32_t share = (all + places - 1) / places;
+    share = share > least_units ? share : least_units;
+    uint32_t before_all = 0, parts_all = 0;
     for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
         if (p.sequences > 64) {      // (else the lanes still have what they found)
             tiles = 0;
@@ -59,9 +59,9 @@ __device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_gr
                 sequence_units<PAGED, ROWS, UNIT>(p, span, tiles, units);
             }
         }
-        const uint32_t chunks = units > per ? (units + per - 1) / per : 1, mine = tiles * p.kv_heads * chunks;
-        uint32_t total;
-        const uint32_t before = before_all + lanes_sum_before(mine, total);
+        const uint32_t chunks = chunks_of(units, share), mine = tiles * p.kv_heads * chunks;
+        uint32_t total, parts;
+        const uint32_t before = before_all + lanes_sum_before(mine, total), parts_before = parts_all + lanes_sum_before(chunks > 1 ? mine : 0, parts);
         const uint64_t here = __ballot(before <= blockIdx.x && blockIdx.x - before < mine);
         if (here) {
             const int at = __builtin_ctzll(here);
@@ -70,17 +70,17 @@ __device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_gr
             item.span.count = __builtin_amdgcn_readlane(span.count, at);
             item.span.keys = __builtin_amdgcn_readlane(span.keys, at);
             item.span.step = PAGED ? 1 : 0;
-            const uint32_t its_chunks = __builtin_amdgcn_readlane(chunks, at);
-            uint32_t rest = blockIdx.x - __builtin_amdgcn_readlane(before, at);
-            item.chunk = rest % its_chunks;
-            rest /= its_chunks;
+            const uint32_t its_chunks = __builtin_amdgcn_readlane(chunks, at), in_sequence = blockIdx.x - __builtin_amdgcn_readlane(before, at);
+            uint32_t rest = in_sequence / its_chunks;
+            item.chunk = in_sequence - rest * its_chunks;
+            item.part = __builtin_amdgcn_readlane(parts_before, at) + rest * its_chunks;
             item.head = rest % p.kv_heads;
             item.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - rest / p.kv_heads;
-            item.chunk_units = per;
-            item.number = blockIdx.x;
+            item.share = share;
             return true;
         }
         before_all = sum_units(before_all, total);
+        parts_all += parts;
     }
     return false;
 }
@@ -142,7 +142,7 @@ template <int DP> constexpr size_t tile_lds_bytes() { return 4 * kTileKeys<DP> *
 
 template <class T, int DP, bool PAGED>
 __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) void attention_tile_kernel(AttentionProblem p, const T* q, const T* k, const T* v, T* out, float* partial, uint32_t* arrivals,
-                                                                                          uint32_t most_groups, uint32_t most_shared, uint32_t least_units) {
+                                                                                          uint32_t most_groups, uint32_t places, uint32_t least_units) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int KT = kTileKeys<DP>, NT = KT / 32;         // keys of a step, tiles of 32 of them
     constexpr int KS = DP / 16, OT = DP / 32;               // products of a tile's scores; tiles of 32 elements
@@ -154,17 +154,15 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
     volatile uint32_t* const odd_step = arrived + 1;     // the step in which a value was not finite
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
     Item item;
-    if (!item_of_block<PAGED, kTileRows, KT>(p, most_groups, most_shared, least_units, item)) return;
+    if (!item_of_block<PAGED, kTileRows, KT>(p, most_groups, places, least_units, item)) return;
     const Span span = item.span;
     const uint32_t first_i = p.group_div.div(item.tile * kTileRows);
     uint32_t last_i = p.group_div.div(item.tile * kTileRows + kTileRows - 1);
     last_i = last_i < span.count ? last_i : span.count - 1;
     const uint32_t all_see = keys_seen(p, span, first_i), most = keys_seen(p, span, last_i);     // by every row of the tile, by the last
-    const uint32_t units = most ? (most + KT - 1) / KT : 1, chunks = units > item.chunk_units ? (units + item.chunk_units - 1) / item.chunk_units : 1;
+    const uint32_t units = most ? (most + KT - 1) / KT : 1, chunks = chunks_of(units, item.share), chunk_units = (units + chunks - 1) / chunks;
     if (item.chunk >= chunks) return;      // (the tile sees fewer keys than the sequence's last)
-    const uint32_t key_from = chunks > 1 ? item.chunk * item.chunk_units * KT : 0;
-    const uint32_t key_end = chunks > 1 ? key_from + item.chunk_units * KT : most;
-    const uint32_t key_to = key_end < most ? key_end : most;
+    const uint32_t key_from = item.chunk * chunk_units * KT, key_end = key_from + chunk_units * KT, key_to = key_end < most ? key_end : most;
 
     // ---- this lane's row
     const uint32_t row = item.tile * kTileRows + wave * 32 + col, i_row = p.group_div.div(row), q_head = item.head * p.group + row - i_row * p.group;
@@ -520,8 +518,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
     constexpr uint64_t SLOT = tile_partial_floats<DP>(), STATS = static_cast<uint64_t>(kTileRows) * DP;
     constexpr uint32_t AT_ONCE = DP > 64 ? 4 : 2;      // parts whose loads are on their way, 8 of each (4 of the small heads: registers of the loop above spill)
     const uint32_t my_row = wave * 32 + col;
-    float* const group_parts = partial + static_cast<uint64_t>(item.number - item.chunk) * SLOT;
-    uint32_t* const group_arrivals = arrivals + (item.number - item.chunk);
+    float* const group_parts = partial + static_cast<uint64_t>(item.part) * SLOT;
+    uint32_t* const group_arrivals = arrivals + item.part;
     top = top == -INFINITY ? -INFINITY : top * factor;
     uint32_t parts = chunks, mine = item.chunk, apart = 1;      // a part's place is `apart` from the next one's
 #pragma unroll 1
@@ -592,9 +590,9 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
 #endif
 }
 
-// groups from which on keys are not shared: as many as run at a time, two on every compute unit, of the largest heads one (8 tokens of 16 sequences behind 4096, us with
-// 512 / 256: 32 heads of 128 behind 8192 109 / 121, 12 heads of 256 105 / 67)
-template <int DP> constexpr uint32_t kTileShared = DP > 128 ? 256 : 512;
+// blocks that run at a time: two on every compute unit, of the largest heads one (8 tokens of 16 sequences, us with 512 / 256: 32 heads of 128 behind 8192 109 / 121, 12 heads of
+// 256 behind 4096 105 / 67); of heads up to 64 there are three, but with 768 places 128 tokens of 8 * 16 heads over 2000 states take 28 us instead of 24
+template <int DP> constexpr uint32_t kTilePlaces = DP > 128 ? 256 : 512;
 // units of a chunk, at least: 256 keys (128 / 256 / 512, us: 8 tokens of 32 heads of 128 behind 1000 21 / 19 / 22, 16 behind 4096 35 / 33 / 36; 198 tokens of 12 heads of 256
 // over 1422 states 55 / 46 / 42, 91 tokens of 25 sequences 70 / 63 / 63, 3 tokens over 4069 states 47 / 51 / 52)
 template <int DP> constexpr uint32_t kTileLeast = 256 / kTileKeys<DP>;
@@ -605,17 +603,18 @@ int launch_tile(const AttentionProblem& p, const void* q, const void* k, const v
     static std::atomic<uint64_t> raised{0};
     if (LDS > (64u << 10))
         if (int status = raise_lds_limit(reinterpret_cast<const void*>(attention_tile_kernel<T, DP, PAGED>), LDS, raised); status != TANNIC_SUCCESS) return status;
-    // as many blocks as there can be items: shared groups have at most kTileShared<DP> items more than there are groups, and none of fewer than kTileLeast<DP> units but its last
+    // As many blocks as there can be items: what is cut has no more items than places and groups together, none of fewer units than kTileLeast but a group's last.  Groups are
+    // cut if they have more than 5 / 4 of a place's share: there are fewer than 4 / 5 of the places of those, and fewer than 9 / 5 parts of them.
     const uint64_t groups = (static_cast<uint64_t>(p.tokens) * p.group / kTileRows + p.sequences) * p.kv_heads, units = p.room / kTileKeys<DP> + 1;
-    if (groups * units >= kMostUnits || groups + kTileShared<DP> >= kMostBlocks) return TANNIC_UNSUPPORTED_DTYPE;
-    const uint64_t items = std::min<uint64_t>(groups + kTileShared<DP>, groups * ((units + kTileLeast<DP> - 1) / kTileLeast<DP>)), parts = std::min<uint64_t>(items, 2 * kTileShared<DP>);
+    if (groups * units >= kMostUnits || groups + kTilePlaces<DP> >= kMostBlocks) return TANNIC_UNSUPPORTED_DTYPE;
+    const uint64_t items = std::min<uint64_t>(groups + kTilePlaces<DP>, groups * ((units + kTileLeast<DP> - 1) / kTileLeast<DP>)), parts = std::min<uint64_t>(items, 2 * kTilePlaces<DP>);
     uint32_t* arrivals = nullptr;
     if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
-    static_assert(2 * kTileShared<DP> <= kAttentionArrivals);
+    static_assert(2 * kTilePlaces<DP> <= kAttentionArrivals);
     float* partial = nullptr;
     if (scratch_acquire(reinterpret_cast<void**>(&partial), parts * tile_partial_floats<DP>() * sizeof(float), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
     hipLaunchKernelGGL((attention_tile_kernel<T, DP, PAGED>), dim3(static_cast<uint32_t>(items)), dim3(64 * kTileWaves), LDS, stream, p, static_cast<const T*>(q),
-                       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(out), partial, arrivals, static_cast<uint32_t>(groups), kTileShared<DP>, kTileLeast<DP>);
+                       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(out), partial, arrivals, static_cast<uint32_t>(groups), kTilePlaces<DP>, kTileLeast<DP>);
     const int status = launch_status("attention_tile_kernel");
     scratch_release(partial, stream);
     return status;

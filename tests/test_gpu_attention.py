@@ -342,3 +342,14 @@ def test_chunks_over_pages_that_end_inside_a_step(page, d, dtype, device):
     for x in (got, want, slack, size):
         x[~keep] = 0
     assert_within(got, want, slack, size, dtype, total)
+
+
+@pytest.mark.parametrize("dtype", [ta.float16, ta.bfloat16], ids=str)
+@pytest.mark.parametrize("heads", [(48, 8, 64), (34, 2, 256)], ids=str)
+def test_a_long_sequence_among_many(heads, dtype, device):
+    """More groups than blocks run at a time, and one sequence that is much longer than a block's share of all keys."""
+    rng = np.random.default_rng(19)
+    n = 600 // heads[1] if heads[1] == 8 else 140
+    context = rng.integers(0, 40, n)
+    context[n // 3], context[n - 1] = 4000, 1500
+    check(Cache(rng, dtype, device, *heads, 16, [3] * n, context.tolist()), device)
