@@ -140,37 +140,67 @@ struct Run {
     uint32_t per, from, to;
 };
 
+// Lane l looks after the sequences l * each .. + each (one of up to 64): f(span) is what a sequence counts for; how much the lane's count for, together.  (64 at a time, twice, one
+// after the other: 82 us for a token of 512 sequences behind 128, 32 / 8 heads of 128; so: 76.)
+template <bool PAGED, class F>
+__device__ inline uint32_t lanes_share(const AttentionProblem& p, uint32_t each, F&& f) {
+    const uint32_t from = threadIdx.x % 64 * each;
+    uint32_t mine = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < each; ++i) {
+        const bool there = from + i < p.sequences;
+        Span span = span_of<PAGED>(p, there ? from + i : p.sequences - 1);
+        span.count = there ? span.count : 0;
+        mine = sum_units(mine, f(span));
+    }
+    return mine;
+}
+
+// The sequence that counts for place `at` of all, and how much those before it count for, from what a lane's sequences count for and those of the lanes before; false: there is none.
+template <bool PAGED, class F>
+__device__ inline bool sequence_at(const AttentionProblem& p, uint32_t each, uint32_t mine, uint32_t before, uint32_t at, F&& f, uint32_t& s, uint32_t& first) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint64_t here = __ballot(before <= at && at - before < mine);
+    if (here == 0) return false;
+    int l = __builtin_ctzll(here);
+    s = l * each;
+    first = __builtin_amdgcn_readlane(before, l);
+    if (each == 1) return true;
+    const uint32_t end = s + each < p.sequences ? s + each : p.sequences;
+    for (; s < end; s += 64) {
+        Span span = span_of<PAGED>(p, s + lane < end ? s + lane : end - 1);
+        span.count = s + lane < end ? span.count : 0;
+        mine = f(span);
+        uint32_t total;
+        before = first + lanes_sum_before(mine, total);
+        here = __ballot(before <= at && at - before < mine);
+        if (here) {
+            l = __builtin_ctzll(here);
+            s += l;
+            first = __builtin_amdgcn_readlane(before, l);
+            return true;
+        }
+        first += total;
+    }
+    return false;
+}
+
 template <bool PAGED, int ROWS, int UNIT>
 __device__ inline bool run_of_block(const AttentionProblem& p, uint32_t blocks, Run& run, Group& g) {
-    const uint32_t lane = threadIdx.x % 64;
-    uint32_t all = 0, mine = 0, before = 0;
-    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
-        uint32_t tiles, units, total;
-        mine = s0 + lane < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, span_of<PAGED>(p, s0 + lane), tiles, units) : 0;
-        before = all + lanes_sum_before(mine, total);
-        all = sum_units(all, total);
-    }
+    const uint32_t each = (p.sequences + 63) / 64;
+    const auto units_of = [&](const Span& span) -> uint32_t {
+        uint32_t tiles, units;
+        return sequence_units<PAGED, ROWS, UNIT>(p, span, tiles, units);
+    };
+    const uint32_t mine = lanes_share<PAGED>(p, each, units_of);
+    uint32_t all;
+    const uint32_t before = lanes_sum_before(mine, all);
     if (all == kMostUnits) return false;
     run.per = (all + blocks - 1) / blocks;
     run.from = blockIdx.x * run.per;      // (blocks * per < all + blocks)
     if (run.from >= all) return false;
     run.to = run.from + run.per < all ? run.from + run.per : all;
-    uint32_t s0 = 0;
-    if (p.sequences > 64) {      // (else the lanes still have what they found)
-        for (all = 0;; s0 += 64) {
-            if (s0 >= p.sequences) return false;
-            uint32_t tiles, units, total;
-            mine = s0 + lane < p.sequences ? sequence_units<PAGED, ROWS, UNIT>(p, span_of<PAGED>(p, s0 + lane), tiles, units) : 0;
-            before = all + lanes_sum_before(mine, total);
-            all += total;
-            if (run.from < all) break;
-        }
-    }
-    const uint64_t here = __ballot(before <= run.from && run.from - before < mine);
-    if (here == 0) return false;
-    const int at = __builtin_ctzll(here);
-    g.s = s0 + at;
-    g.first = __builtin_amdgcn_readlane(before, at);
+    if (!sequence_at<PAGED>(p, each, mine, before, run.from, units_of, g.s, g.first)) return false;
     g.span = span_of<PAGED>(p, g.s);
     sequence_units<PAGED, ROWS, UNIT>(p, g.span, g.tiles, g.units);
     const uint32_t number = (run.from - g.first) / g.units;

@@ -31,58 +31,74 @@ __device__ inline uint32_t chunks_of(uint32_t units, uint32_t share) { return un
 
 template <bool PAGED, int ROWS, int UNIT>
 __device__ inline bool item_of_block(const AttentionProblem& p, uint32_t most_groups, uint32_t places, uint32_t least_units, Item& item) {
-    const uint32_t lane = threadIdx.x % 64;
-    uint32_t all = 0, groups = 0, tiles = 0, units = 0;
+    const uint32_t each = (p.sequences + 63) / 64;
+    uint32_t all, groups, units = 0, tiles = 0, share = 0;
     Span span{};
-    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
-        uint32_t total, mine = 0;
-        tiles = 0;
-        if (s0 + lane < p.sequences) {
-            span = span_of<PAGED>(p, s0 + lane);
-            mine = sequence_units<PAGED, ROWS, UNIT>(p, span, tiles, units);
-        }
-        lanes_sum_before(mine, total);
-        all = sum_units(all, total);
-        lanes_sum_before(tiles * p.kv_heads, total);
-        groups = sum_units(groups, total);
-    }
+    uint32_t my_groups = 0, my_parts = 0;
+    const uint32_t my_units = lanes_share<PAGED>(p, each, [&](const Span& its) -> uint32_t {
+        span = its;
+        const uint32_t n = sequence_units<PAGED, ROWS, UNIT>(p, span, tiles, units);
+        my_groups = sum_units(my_groups, tiles * p.kv_heads);
+        return n;
+    });
+    lanes_sum_before(my_units, all);
+    lanes_sum_before(my_groups, groups);
     // (more groups than the rows of q make: sequences that overlap, against what the starts may hold; there are not the blocks for them)
     if (all == kMostUnits || groups > most_groups) return false;
-    uint32_t share = (all + places - 1) / places;
+    share = (all + places - 1) / places;
     share = share > least_units ? share : least_units;
-    uint32_t before_all = 0, parts_all = 0;
-    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 64) {
-        if (p.sequences > 64) {      // (else the lanes still have what they found)
-            tiles = 0;
-            if (s0 + lane < p.sequences) {
-                span = span_of<PAGED>(p, s0 + lane);
-                sequence_units<PAGED, ROWS, UNIT>(p, span, tiles, units);
-            }
-        }
+    const auto items_of = [&](const Span& its) -> uint32_t {
+        sequence_units<PAGED, ROWS, UNIT>(p, its, tiles, units);
         const uint32_t chunks = chunks_of(units, share), mine = tiles * p.kv_heads * chunks;
-        uint32_t total, parts;
-        const uint32_t before = before_all + lanes_sum_before(mine, total), parts_before = parts_all + lanes_sum_before(chunks > 1 ? mine : 0, parts);
-        const uint64_t here = __ballot(before <= blockIdx.x && blockIdx.x - before < mine);
-        if (here) {
-            const int at = __builtin_ctzll(here);
-            item.s = s0 + at;
-            item.span.begin = __builtin_amdgcn_readlane(span.begin, at);
-            item.span.count = __builtin_amdgcn_readlane(span.count, at);
-            item.span.keys = __builtin_amdgcn_readlane(span.keys, at);
-            item.span.step = PAGED ? 1 : 0;
-            const uint32_t its_chunks = __builtin_amdgcn_readlane(chunks, at), in_sequence = blockIdx.x - __builtin_amdgcn_readlane(before, at);
-            uint32_t rest = in_sequence / its_chunks;
-            item.chunk = in_sequence - rest * its_chunks;
-            item.part = __builtin_amdgcn_readlane(parts_before, at) + rest * its_chunks;
-            item.head = rest % p.kv_heads;
-            item.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - rest / p.kv_heads;
-            item.share = share;
-            return true;
-        }
-        before_all = sum_units(before_all, total);
-        parts_all += parts;
+        my_parts += chunks > 1 ? mine : 0;
+        return mine;
+    };
+    uint32_t mine;
+    if (each == 1) {      // (the lanes still have what they found)
+        const uint32_t chunks = chunks_of(units, share);
+        mine = tiles * p.kv_heads * chunks;
+        my_parts = chunks > 1 ? mine : 0;
+    } else {
+        mine = lanes_share<PAGED>(p, each, items_of);
     }
-    return false;
+    uint32_t total, parts;
+    uint32_t before = lanes_sum_before(mine, total), parts_before = lanes_sum_before(my_parts, parts);
+    const auto holds_block = [&]() -> uint64_t { return __ballot(before <= blockIdx.x && blockIdx.x - before < mine); };
+    uint64_t here = holds_block();
+    if (here == 0) return false;
+    int at = __builtin_ctzll(here);
+    item.s = at * each;
+    if (each > 1) {
+        const uint32_t lane = threadIdx.x % 64, end = item.s + each < p.sequences ? item.s + each : p.sequences;
+        uint32_t first = __builtin_amdgcn_readlane(before, at), first_part = __builtin_amdgcn_readlane(parts_before, at);
+        for (;; item.s += 64) {
+            if (item.s >= end) return false;
+            const bool there = item.s + lane < end;
+            span = span_of<PAGED>(p, there ? item.s + lane : end - 1);
+            span.count = there ? span.count : 0;
+            my_parts = 0;
+            mine = items_of(span);
+            before = first + lanes_sum_before(mine, total);
+            parts_before = first_part + lanes_sum_before(my_parts, parts);
+            if ((here = holds_block()) != 0) break;
+            first += total;
+            first_part += parts;
+        }
+        at = __builtin_ctzll(here);
+        item.s += at;
+    }
+    item.span.begin = __builtin_amdgcn_readlane(span.begin, at);
+    item.span.count = __builtin_amdgcn_readlane(span.count, at);
+    item.span.keys = __builtin_amdgcn_readlane(span.keys, at);
+    item.span.step = PAGED ? 1 : 0;
+    const uint32_t its_chunks = chunks_of(__builtin_amdgcn_readlane(units, at), share), in_sequence = blockIdx.x - __builtin_amdgcn_readlane(before, at);
+    uint32_t rest = in_sequence / its_chunks;
+    item.chunk = in_sequence - rest * its_chunks;
+    item.part = __builtin_amdgcn_readlane(parts_before, at) + rest * its_chunks;
+    item.head = rest % p.kv_heads;
+    item.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - rest / p.kv_heads;
+    item.share = share;
+    return true;
 }
 
 typedef float float16a __attribute__((ext_vector_type(16)));

@@ -353,3 +353,21 @@ def test_a_long_sequence_among_many(heads, dtype, device):
     context = rng.integers(0, 40, n)
     context[n // 3], context[n - 1] = 4000, 1500
     check(Cache(rng, dtype, device, *heads, 16, [3] * n, context.tolist()), device)
+
+
+@pytest.mark.parametrize("dtype", [ta.float16, ta.float32, ta.float64], ids=str)
+@pytest.mark.parametrize("most", [1, 40])
+@pytest.mark.parametrize("n", [64, 65, 130, 300])
+def test_many_sequences(n, most, dtype, device):
+    """More sequences than a wavefront has lanes, some without new tokens."""
+    rng = np.random.default_rng(n)
+    new = rng.integers(0, most + 1, n) if most == 1 else np.where(rng.random(n) < 0.1, rng.integers(20, most, n), rng.integers(0, 3, n))
+    check(Cache(rng, dtype, device, 8, 1, 16, 16, new.tolist(), rng.integers(0, 70, n).tolist()), device)
+
+
+def test_more_sequences_than_lanes_squared(device):
+    """Each lane looks after more than 64 sequences."""
+    rng = np.random.default_rng(20)
+    n = 64 * 65 + 3
+    for new in (rng.integers(0, 2, n), np.where(np.arange(n) % 50 == 7, 30, 0)):
+        check(Cache(rng, ta.bfloat16, device, 32, 1, 16, 16, new.tolist(), rng.integers(0, 5, n).tolist()), device)
