@@ -83,24 +83,24 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 if (j < key_to) page[kt] = page_of<PAGED>(p, g.s, j, in_page[kt]);
             }
         };
-        auto fetch = [&]() {
-            bool found[KT];
+        // (mostly every key of the step is there and heads have DP elements: then nothing is asked of the loads one by one)
+        auto fetch_step = [&](auto every_tag) {
+            constexpr bool EVERY = decltype(every_tag)::value;
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                found[kt] = page_exists(p, page[kt]);
-                there[kt] = static_cast<uint32_t>(__ballot(found[kt])) & 0xFFFFu;
-                const int64_t k_off = found[kt] ? page[kt] * p.k_page + in_page[kt] * p.k_token + g.head * p.k_head : 0;
-                const int64_t v_off = found[kt] ? page[kt] * p.v_page + in_page[kt] * p.v_token + g.head * p.v_head : 0;
+                const bool found = EVERY || page_exists(p, page[kt]);
+                const int64_t k_off = found ? page[kt] * p.k_page + in_page[kt] * p.k_token + g.head * p.k_head : 0;
+                const int64_t v_off = found ? page[kt] * p.v_page + in_page[kt] * p.v_token + g.head * p.v_head : 0;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t e = (ks * 4 + quarter) * E;
-                    kf[kt][ks] = found[kt] && e < p.d ? load16(k + k_off + e) : uint4a{0, 0, 0, 0};
+                    kf[kt][ks] = EVERY || (found && e < p.d) ? load16(k + k_off + e) : uint4a{0, 0, 0, 0};
                 }
                 if constexpr (HALF) {
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
                         const uint32_t e = (ks * 4 + quarter) * E;
-                        vf[kt][ks] = found[kt] && e < p.d ? load16(v + v_off + e) : uint4a{0, 0, 0, 0};
+                        vf[kt][ks] = EVERY || (found && e < p.d) ? load16(v + v_off + e) : uint4a{0, 0, 0, 0};
                     }
                 } else {
                     // fp32: piece lane % 16 (+ 16 c) of the keys 4 (lane / 16) + i; vf[0][i * (KS / 4) + c] with KS / 4 = DP / 64
@@ -108,15 +108,25 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                     for (int i = 0; i < 4; ++i) {
                         const int source = 4 * quarter + i;
                         const int64_t off = __shfl(v_off, source);
-                        const bool live = (there[kt] >> source) & 1;
+                        const bool live = EVERY || ((there[kt] >> source) & 1);
 #pragma unroll
                         for (int c = 0; c < KS / 4; ++c) {
                             const uint32_t e = (c * 16 + col) * E;
-                            vf[kt][i * (KS / 4) + c] = live && e < p.d ? load16(v + off + e) : uint4a{0, 0, 0, 0};
+                            vf[kt][i * (KS / 4) + c] = EVERY || (live && e < p.d) ? load16(v + off + e) : uint4a{0, 0, 0, 0};
                         }
                     }
                 }
             }
+        };
+        auto fetch = [&]() {
+            bool every = p.d == DP;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                there[kt] = static_cast<uint32_t>(__ballot(page_exists(p, page[kt]))) & 0xFFFFu;
+                every = every && there[kt] == 0xFFFFu;
+            }
+            if (every) fetch_step(std::true_type{});
+            else fetch_step(std::false_type{});
         };
         T* const mine = reinterpret_cast<T*>(lds_raw) + wave * (32 * PITCH);
         uint32_t j0 = key_from + wave * STEP;
@@ -176,31 +186,35 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 look_up(j0 + 8 * STEP);
             }
             float high = -INFINITY;
-            bool live[KT][4];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[kt] *= factor;
+            if (!full) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(((keys_here[kt] >> (4 * quarter + i)) & 1) && j_now + kt * 16 + 4 * quarter + i < seen)) s[kt][i] = -INFINITY;
+            }
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[kt][i] *= factor;
-                    live[kt][i] = full || (((keys_here[kt] >> (4 * quarter + i)) & 1) && j_now + kt * 16 + 4 * quarter + i < seen);
-                    high = fmaxf(high, live[kt][i] ? s[kt][i] : -INFINITY);
-                }
+                for (int i = 0; i < 4; ++i) high = fmaxf(high, s[kt][i]);
             high = across_groups_max(high);
-            const float above = fmaxf(top, high);
-            const float base = above == -INFINITY ? 0.0f : above - kWeightShift<T>;
-            const float old = __builtin_amdgcn_exp2f(top - kWeightShift<T> - base);
+            const float above = fmaxf(top, high), base = above == -INFINITY ? 0.0f : above - kWeightShift<T>;
+            if (__ballot(above > top) != 0) {
+                const float old = __builtin_amdgcn_exp2f(top - kWeightShift<T> - base);
+                sum *= old;
+#pragma unroll
+                for (int t = 0; t < OT; ++t) acc[t] *= old;
+            }
             top = above;
-            float part = 0.0f;
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[kt][i] = live[kt][i] ? __builtin_amdgcn_exp2f(s[kt][i] - base) : 0.0f;
-                    part += s[kt][i];
+                    s[kt][i] = __builtin_amdgcn_exp2f(s[kt][i] - base);
+                    sum += s[kt][i];
                 }
-            sum = sum * old + part;
-#pragma unroll
-            for (int t = 0; t < OT; ++t) acc[t] *= old;
             if constexpr (HALF) {
                 using Lds = __attribute__((address_space(3))) short;
                 typedef short short4a __attribute__((ext_vector_type(4)));
