@@ -102,7 +102,7 @@ __device__ inline int64_t query_offset(const AttentionProblem& p, uint32_t s, co
 // group that a run's end cuts is put together from its blocks' partial results by the last of them.  Lengths are known on the device only:
 // every wavefront works the runs out for itself, 64 sequences at a time.
 struct Group {
-    uint32_t s, tile, head;      // of `tiles` x kv_heads in the sequence, heads innermost
+    uint32_t s, tile, head;      // of kv_heads x `tiles` in the sequence, tiles innermost
     Span span;
     uint32_t tiles, units;       // units of each of the sequence's groups
     uint32_t first;              // the group's first unit among all
@@ -137,7 +137,7 @@ __device__ inline uint32_t lanes_sum_before(uint32_t v, uint32_t& total) {
 
 // The run of this block: units from .. to, and the group that holds the first; false: there is none.
 struct Run {
-    uint32_t per, from, to;
+    uint32_t block, per, from, to;      // the number among the runs
 };
 
 // Lane l looks after the sequences l * each .. + each (one of up to 64): f(span) is what a sequence counts for; how much the lane's count for, together.  (64 at a time, twice, one
@@ -197,7 +197,16 @@ __device__ inline bool run_of_block(const AttentionProblem& p, uint32_t blocks, 
     const uint32_t before = lanes_sum_before(mine, all);
     if (all == kMostUnits) return false;
     run.per = (all + blocks - 1) / blocks;
-    run.from = blockIdx.x * run.per;      // (blocks * per < all + blocks)
+    // Blocks go round the eight dies (blocks is a multiple of eight).  Neighbouring runs belong on one die where its L2 can serve several tiles with the same keys (fp32, 700 tokens
+    // of 8 sequences' 16 heads of 64 over 500 to 2000 states 455 us apart and 396 together, 16 tokens of 8 sequences behind 4096 172 and 138), but not short runs (prompts of 17 to
+    // 100 tokens 10.9 and 12.4) or single tiles (a token over 1024 states 12.7 and 15.0, 4 tokens of 16 sequences behind 8192, bf16, 111 and 114).
+    run.block = blockIdx.x;
+    if (run.per >= 8 && p.tokens * p.group > ROWS * p.sequences) {
+        const uint32_t of_die = ((all + run.per - 1) / run.per + 7) / 8;
+        if (blockIdx.x / 8 >= of_die) return false;
+        run.block = blockIdx.x % 8 * of_die + blockIdx.x / 8;
+    }
+    run.from = run.block * run.per;      // (blocks * per < all + blocks)
     if (run.from >= all) return false;
     run.to = run.from + run.per < all ? run.from + run.per : all;
     if (!sequence_at<PAGED>(p, each, mine, before, run.from, units_of, g.s, g.first)) return false;
@@ -205,8 +214,8 @@ __device__ inline bool run_of_block(const AttentionProblem& p, uint32_t blocks, 
     sequence_units<PAGED, ROWS, UNIT>(p, g.span, g.tiles, g.units);
     const uint32_t number = (run.from - g.first) / g.units;
     g.first += number * g.units;
-    g.tile = number / p.kv_heads;
-    g.head = number % p.kv_heads;
+    g.head = number / g.tiles;
+    g.tile = number % g.tiles;
     return true;
 }
 
@@ -214,10 +223,10 @@ __device__ inline bool run_of_block(const AttentionProblem& p, uint32_t blocks, 
 template <bool PAGED, int ROWS, int UNIT>
 __device__ inline void next_group(const AttentionProblem& p, Group& g) {
     g.first += g.units;
-    if (++g.head < p.kv_heads) return;
-    g.head = 0;
     if (++g.tile < g.tiles) return;
     g.tile = 0;
+    if (++g.head < p.kv_heads) return;
+    g.head = 0;
     while (++g.s < p.sequences) {
         g.span = span_of<PAGED>(p, g.s);
         if (sequence_units<PAGED, ROWS, UNIT>(p, g.span, g.tiles, g.units)) return;

@@ -8,8 +8,8 @@
 //           eight of the product's 32 - if V's keys are taken in the same order.  16-bit V is transposed on its way out of LDS (ds_read_b64_tr_b16);
 //           fp32 V needs no LDS: an accumulator's four keys are four products.
 // Measured, a token of every sequence, 32 / 8 heads of 128: 4 sequences behind 32768 to 131072 (1.22 GB, bf16) 219 us, 5.6 TB/s, in the middle 6.1 as large reads alone; 32
-// behind 64 to 4096 (133 MB, fp16) 38.8; one behind 2048 11.6, all of it one access after the other: lengths, table, keys, parts, their join.  fp32 chunks come here too, 0.4 of
-// the fp32 pipe's rate (512 tokens behind 1024: 196 us).
+// behind 64 to 4096 (133 MB, fp16) 38.8; one behind 2048 11.2, all of it one access after the other: lengths, table, keys, parts, their join.  fp32 chunks come here too, half
+// of the fp32 pipe's rate (512 tokens behind 1024: 158 us).
 #include "attention.hpp"
 
 namespace th {
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 value += *reinterpret_cast<const float4a*>(join + (w * 16 + r) * (DP + 4) + piece * 4) * share;
             }
             if (whole) write_row(r, piece, value, total_weight);
-            else leave(part_of(0, blockIdx.x), r, piece, value, above, total_weight);
+            else leave(part_of(0, run.block), r, piece, value, above, total_weight);
         }
         if (!whole) {
             // So many parts that lie beside each other are put together by the last of their blocks to get here, what comes of them by the last of those that have so many of
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
             uint32_t sharing = 1;
             while (2 * sharing * results <= 256) sharing *= 2;
             const uint32_t in_share = sharing == 1 ? 0 : threadIdx.x / results;
-            uint32_t parts = last - first + 1, mine_at = blockIdx.x - first;
+            uint32_t parts = last - first + 1, mine_at = run.block - first;
 #pragma unroll 1
             for (uint32_t level = 0, apart = 0; parts > 1; ++level, apart += log_most) {
                 const uint32_t from = mine_at >> log_most << log_most, here = parts - from < 1u << log_most ? parts - from : 1u << log_most, leader = first + (from << apart);
@@ -443,7 +443,7 @@ int launch_rows(const AttentionProblem& p, const void* q, const void* k, const v
     const uint64_t tiles = static_cast<uint64_t>(p.tokens) * p.group / ROWS + p.sequences;
     const uint64_t most = tiles * p.kv_heads * (p.room / kRowsUnit<T> + 1);
     if (most >= kMostUnits) return TANNIC_UNSUPPORTED_DTYPE;
-    const uint32_t blocks = most < kRowsBlocks<DP> ? static_cast<uint32_t>(most) : kRowsBlocks<DP>;
+    const uint32_t blocks = most < kRowsBlocks<DP> ? (static_cast<uint32_t>(most) + 7) / 8 * 8 : kRowsBlocks<DP>;      // (as many on each die)
     uint32_t* arrivals = nullptr;
     if (int status = attention_arrivals(stream, arrivals); status != TANNIC_SUCCESS) return status;
     float* partial = nullptr;
