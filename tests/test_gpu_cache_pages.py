@@ -167,3 +167,26 @@ def test_copies_past_32_bits(device):
     ops.copy_into(pool[8999:9000], ta.tensor(x, ta.float16, device))
     ops.copy_pages(pool, [8999], [8300])
     np.testing.assert_array_equal(ops.repack(pool[8300:8301]).numpy(), x)
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 300, 4163])
+def test_append_to_many_sequences(n, device):
+    """More sequences than a wavefront has lanes, empty ones in front, behind and in between, tokens of no sequence at both ends."""
+    rng = np.random.default_rng(n)
+    new = rng.integers(0, 3, n)
+    new[[0, 1, n - 1]] = 0
+    total, first = int(new.sum()), 2
+    context = rng.integers(0, 4, n)
+    table = rng.permutation(2 * n).reshape(n, 2)                  # pages of 4, at most 5 tokens
+    k = rounded(rng.standard_normal((total + 5, 1, 8)), ta.bfloat16)
+    keys, values = (ta.tensor(np.zeros((2 * n, 1, 4, 8)), ta.bfloat16, device) for _ in range(2))
+    starts = first + np.concatenate([[0], np.cumsum(new)])
+    dk = ta.tensor(k, ta.bfloat16, device)
+    ops.append_pages(dk, dk, keys, values, *(ta.tensor(x, ta.int32, device) for x in (table, starts, context)))
+    want = np.zeros((2 * n, 1, 4, 8))
+    for s in range(n):
+        for i in range(new[s]):
+            at = context[s] + i
+            want[table[s, at // 4], 0, at % 4] = k[starts[s] + i, 0]
+    np.testing.assert_array_equal(keys.numpy(), want)
+    np.testing.assert_array_equal(values.numpy(), want)
