@@ -8,7 +8,7 @@
 //           eight of the product's 32 - if V's keys are taken in the same order.  16-bit V is transposed on its way out of LDS (ds_read_b64_tr_b16);
 //           fp32 V needs no LDS: an accumulator's four keys are four products.
 // Measured, a token of every sequence, 32 / 8 heads of 128: 4 sequences behind 32768 to 131072 (1.22 GB, bf16) 219 us, 5.6 TB/s, in the middle 6.1 as large reads alone; 32
-// behind 64 to 4096 (133 MB, fp16) 38.8; one behind 2048 11.2, all of it one access after the other: lengths, table, keys, parts, their join.  fp32 chunks come here too, half
+// behind 64 to 4096 (133 MB, fp16) 37.9; one behind 2048 11.2, all of it one access after the other: lengths, table, keys, parts, their join.  fp32 chunks come here too, half
 // of the fp32 pipe's rate (512 tokens behind 1024: 158 us).
 #include "attention.hpp"
 
@@ -83,7 +83,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 if (j < key_to) page[kt] = page_of<PAGED>(p, g.s, j, in_page[kt]);
             }
         };
-        // (mostly every key of the step is there and heads have DP elements: then nothing is asked of the loads one by one)
+        // (fp32, whose chunks are bound by the instructions between their products: mostly every key of the step is there and heads have DP elements, and then nothing is asked of the
+        // loads one by one, 159 us instead of 195 for 512 tokens behind 1024; the 16-bit types wait for the memory: 39.1 us with and 37.9 without for 32 sequences behind 64 to 4096)
         auto fetch_step = [&](auto every_tag) {
             constexpr bool EVERY = decltype(every_tag)::value;
 #pragma unroll
@@ -119,13 +120,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
             }
         };
         auto fetch = [&]() {
-            bool every = p.d == DP;
+            bool every = !HALF && p.d == DP;
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
                 there[kt] = static_cast<uint32_t>(__ballot(page_exists(p, page[kt]))) & 0xFFFFu;
                 every = every && there[kt] == 0xFFFFu;
             }
-            if (every) fetch_step(std::true_type{});
+            if constexpr (HALF) fetch_step(std::false_type{});
+            else if (every) fetch_step(std::true_type{});
             else fetch_step(std::false_type{});
         };
         T* const mine = reinterpret_cast<T*>(lds_raw) + wave * (32 * PITCH);
