@@ -3,6 +3,7 @@
 #pragma once
 
 #include "cache.hpp"
+#include "meeting.hpp"
 
 namespace th {
 

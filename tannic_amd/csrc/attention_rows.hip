@@ -331,8 +331,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
         }
         if (!whole) {
             // So many parts that lie beside each other are put together by the last of their blocks to get here, what comes of them by the last of those that have so many of
-            // these, and so on: always the same ones in the same order, whichever block is last.  A count is 0 again behind its last block; there is one for each level: of
-            // two parts or more, the first's block is not the group's last (which may have counts of the next group).
+            // these, and so on: always the same ones in the same order, whichever block is last.  A count is 0 again behind its last block; a group's lie behind its first block
+            // and up to its last, where the next group's may begin.
             // (All parts by one block: 3 tokens of 16 / 4 heads of 128 behind 117 and 12655, fp32, 53 us; so: 29.)
             const uint32_t first = g.first / run.per, last = (g.first + g.units - 1) / run.per;      // the blocks that have its parts
             const uint32_t results = rows * pieces;
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attention_rows_kernel(A
                 __syncthreads();
                 if (here > 1) {
                     if (threadIdx.x == 0) {
-                        uint32_t* const count = arrivals + leader + level;
+                        uint32_t* const count = arrivals + first + meeting_count(from, 1u << apart);
                         const uint32_t before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                         if (before == here - 1) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                         arrived = before;

@@ -539,7 +539,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
     top = top == -INFINITY ? -INFINITY : top * factor;
     uint32_t parts = chunks, mine = item.chunk, apart = 1;      // a part's place is `apart` from the next one's
 #pragma unroll 1
-    for (uint32_t level = 0; parts > 1; ++level, parts = (parts + kTileJoin<DP> - 1) / kTileJoin<DP>, mine /= kTileJoin<DP>, apart *= kTileJoin<DP>) {
+    for (; parts > 1; parts = (parts + kTileJoin<DP> - 1) / kTileJoin<DP>, mine /= kTileJoin<DP>, apart *= kTileJoin<DP>) {
         const uint32_t first = mine - mine % kTileJoin<DP>, together_here = parts - first < kTileJoin<DP> ? parts - first : kTileJoin<DP>;
         if (together_here == 1) continue;
         float* const its = group_parts + static_cast<uint64_t>(first * apart) * SLOT;
@@ -554,8 +554,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (threadIdx.x == 0) {
-            // (two parts or more here: a count for each level)
-            uint32_t* const count = group_arrivals + first * apart + level;
+            uint32_t* const count = group_arrivals + meeting_count(first, apart);
             const uint32_t before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (before == together_here - 1) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             *arrived = before;
