@@ -297,6 +297,12 @@ template <class T> __device__ inline uint32_t finite_only(uint32_t x) {
     return ((x & E) == E ? 0u : x & 0xFFFFu) | (((x >> 16) & E) == E ? 0u : x & 0xFFFF0000u);
 }
 
+// The register's two 16-bit values times 0: NaN where they are infinite or NaN.
+template <class T> __device__ inline uint32_t times_zero(uint32_t x) {
+    constexpr uint32_t E = std::is_same_v<T, f16> ? 0x7C00u : 0x7F80u;
+    return ((x & E) == E ? 0x7FFFu : 0u) | (((x >> 16) & E) == E ? 0x7FFF0000u : 0u);
+}
+
 // fp16 weights are kept 2^8 times as large: those below 2^-22 of the largest lose bits first, not those below 2^-14
 template <class T> constexpr float kWeightShift = std::is_same_v<T, f16> ? 8.0f : 0.0f;
 

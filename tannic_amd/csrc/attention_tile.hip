@@ -184,8 +184,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
     const uint32_t row = item.tile * kTileRows + wave * 32 + col, i_row = p.group_div.div(row), q_head = item.head * p.group + row - i_row * p.group;
     const bool row_lives = i_row < span.count;
     const uint32_t seen = row_lives ? keys_seen(p, span, i_row) : 0;
-    // a negative scale turns the queries round, so that the largest score is that of the largest product; without a scale they are 0
-    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u, keep = p.scale == 0.0f ? 0u : ~0u;
+    // a negative scale turns the queries round, so that the largest score is that of the largest product; a scale of 0 leaves nothing of them but what is infinite or NaN
+    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
     const float factor = (p.scale == 0.0f ? 1.0f : fabsf(p.scale)) * 1.44269504088896340736f;
     uint4a qf[KS];
     {
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP > 128 ? 1 : DP > 64 ? 2 : 3) vo
             const uint32_t e = ks * 16 + half * 8;
             uint4a x = row_lives && e < p.d ? *reinterpret_cast<const uint4a*>(from + e) : uint4a{0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) x[w] = (x[w] ^ flip) & keep;
+            for (int w = 0; w < 4; ++w) x[w] = p.scale == 0.0f ? times_zero<T>(x[w]) : x[w] ^ flip;
             qf[ks] = x;
         }
     }
