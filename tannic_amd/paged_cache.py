@@ -21,10 +21,11 @@ from .tensor import Tensor
 
 
 class Step:
-    """What a step's calls take: ``table``, ``starts`` and ``context`` on the device; ``ids`` and ``new`` say whose tokens its rows are."""
+    """What a step's calls take: ``table``, ``starts`` and ``context`` on the device; ``ids`` and ``new`` say whose tokens its rows are, ``lengths``
+    how many tokens those had when it was planned."""
 
-    def __init__(self, ids, new, whole, table, starts, context):
-        self.ids, self.new, self._whole = ids, new, whole
+    def __init__(self, ids, new, lengths, whole, table, starts, context):
+        self.ids, self.new, self.lengths, self._whole = ids, new, lengths, whole
         self.table, self.starts, self.context = table, starts, context
 
     @property
@@ -150,14 +151,15 @@ class PagedCache:
         for row, (pages, _) in zip(table, sequences):
             row[:min(len(pages), width)] = pages[:width]
         whole[n * width:n * width + n + 1] = np.concatenate([[0], np.cumsum(new)])
-        whole[n * width + n + 1:] = [length for _, length in sequences]
+        lengths = [length for _, length in sequences]
+        whole[n * width + n + 1:] = lengths
         if into is not None:
             into._whole.write_raw(whole)
-            into.ids, into.new = ids, new
+            into.ids, into.new, into.lengths = ids, new, lengths
             return into
         t = Tensor(types.int32, whole.shape).initialize(self.storage.environment)
         t.write_raw(whole)
-        return Step(ids, new, t, t[0:n * width].view(n, width), t[n * width:n * width + n + 1], t[n * width + n + 1:])
+        return Step(ids, new, lengths, t, t[0:n * width].view(n, width), t[n * width:n * width + n + 1], t[n * width + n + 1:])
 
     def _take(self):
         page = self._free.pop()
@@ -165,9 +167,14 @@ class PagedCache:
         return page
 
     def advance(self, step):
-        """The step's tokens have been written, in every layer: they count from now on."""
-        for i, n in zip(step.ids, step.new):
-            self._of(i)[1] += n
+        """The step's tokens have been written, in every layer: they count from now on.  Raises, and changes nothing, if one of its sequences has
+        changed its length or lost a page for them since the step was planned (freed, cut, or advanced already)."""
+        sequences = [self._of(i) for i in step.ids]
+        for i, (pages, length), n, planned in zip(step.ids, sequences, step.new, step.lengths):
+            if length != planned or len(pages) * self.page < length + n:
+                raise TannicError(f"PagedCache: sequence {i} has {length} tokens and {len(pages)} pages, the step was planned for {n} more behind {planned}")
+        for entry, n in zip(sequences, step.new):
+            entry[1] += n
 
     # ---- order --------------------------------------------------------------------------------
     def compact(self):
