@@ -21,6 +21,8 @@ from .tensor import Device
 
 
 class Graph:
+    _open = None      # the recording whose block is running (the backend has one at a time)
+
     def __init__(self, device=None):
         self.device = device if device is not None else Device()
         if not isinstance(self.device, Device):
@@ -38,10 +40,12 @@ class Graph:
         if lib.graph_stream(self.handle).address != self.device.stream().address:
             self.close()
             raise BackendError("Graph: the backend records another stream than the one this device's operators use (a stream popped and not put back?)")
+        Graph._open = self
         return self
 
     def __exit__(self, kind, value, trace):
         lib = library()
+        Graph._open = None
         if kind is not None:
             # the block failed: drop the recording, let the exception through
             self.close()
@@ -52,6 +56,11 @@ class Graph:
             raise BackendError(message)
         self.ready = True
         return False
+
+    @staticmethod
+    def records(environment):
+        """Whether the calls on ``environment`` are being recorded right now."""
+        return Graph._open is not None and Graph._open.device == environment
 
     def launch(self):
         """Queue one replay on the device's stream (asynchronous, like every backend call)."""
@@ -66,6 +75,8 @@ class Graph:
         if self.handle:
             library().graph_destroy(self.handle)
         self.handle, self.ready = None, False
+        if Graph._open is self:
+            Graph._open = None
 
     def __del__(self):
         try:

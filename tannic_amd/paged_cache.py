@@ -16,6 +16,7 @@ sequence.  Nothing here waits for the device but ``plan``, which uploads the tab
 import numpy as np
 
 from . import ops, types
+from .graph import Graph
 from .ops import TannicError
 from .tensor import Tensor
 
@@ -111,7 +112,9 @@ class PagedCache:
         """Gives the sequences ``ids`` pages for ``new[i]`` more tokens each and puts the step's tables on the device: sequence ``i``'s
         tokens are the ``new[i]`` rows behind those of the sequences before.  Shared pages that they will write into are copied first.
         ``columns``: pages a row of the table has room for (else as many as needed); ``into``: an earlier step of as many sequences
-        whose tensors are written again, for a recording that reads them.  Raises, and changes nothing, if there are not enough pages."""
+        whose tensors are written again, for a recording that reads them.  Raises, and changes nothing, if there are not enough pages, and
+        inside a recording."""
+        self._outside_a_recording()
         ids, new = list(ids), [int(n) for n in new]
         if len(ids) != len(new) or len(set(ids)) != len(ids) or any(n < 0 for n in new):
             raise TannicError("PagedCache: every sequence of a step once, with the number of its new tokens")
@@ -161,6 +164,11 @@ class PagedCache:
         t.write_raw(whole)
         return Step(ids, new, lengths, t, t[0:n * width].view(n, width), t[n * width:n * width + n + 1], t[n * width + n + 1:])
 
+    def _outside_a_recording(self):
+        # (the copies of pages would run with every replay, and not now)
+        if Graph.records(self.storage.environment):
+            raise TannicError("PagedCache: pages are planned and moved outside of a recording")
+
     def _take(self):
         page = self._free.pop()
         self._users[page] = 1
@@ -178,7 +186,8 @@ class PagedCache:
 
     # ---- order --------------------------------------------------------------------------------
     def compact(self):
-        """Moves the used pages to the front of the cache (steps planned before name the old places); how many moved."""
+        """Moves the used pages to the front of the cache (steps planned before name the old places); how many moved.  Raises inside a recording."""
+        self._outside_a_recording()
         used = sorted({p for pages, _ in self._sequences.values() for p in pages})
         count = len(used)
         holes = sorted(p for p in self._free if p < count)
