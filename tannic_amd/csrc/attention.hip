@@ -98,6 +98,9 @@ __global__ __launch_bounds__(256) void attention_any_kernel(AttentionProblem p, 
     }
 }
 
+__global__ __launch_bounds__(256) void clear_arrivals_kernel(uint32_t* counts) { counts[blockIdx.x * 256 + threadIdx.x] = 0; }
+static_assert(kAttentionArrivals % 256 == 0);
+
 // The counts of blocks that have left their part of a group: one array per stream, 0 between calls.  It is cleared once, on a stream of its
 // own, so that a first call that is being recorded does not leave the clearing to the replay; kept until the process ends.
 int attention_arrivals(hipStream_t stream, uint32_t*& arrivals) try {
@@ -112,7 +115,10 @@ int attention_arrivals(hipStream_t stream, uint32_t*& arrivals) try {
         hipStream_t own = nullptr;
         hipError_t err = hipMalloc(&counts, kAttentionArrivals * sizeof(uint32_t));
         if (err == hipSuccess) err = hipStreamCreateWithFlags(&own, hipStreamNonBlocking);
-        if (err == hipSuccess) err = hipMemsetAsync(counts, 0, kAttentionArrivals * sizeof(uint32_t), own);
+        if (err == hipSuccess) {
+            hipLaunchKernelGGL(clear_arrivals_kernel, dim3(kAttentionArrivals / 256), dim3(256), 0, own, static_cast<uint32_t*>(counts));
+            err = hipGetLastError();
+        }
         if (err == hipSuccess) err = hipStreamSynchronize(own);
         if (own) (void)hipStreamDestroy(own);
         if (err != hipSuccess) {
