@@ -128,6 +128,8 @@ using LdsVoid = __attribute__((address_space(3))) void*;
 // Loads from memory straight to LDS: the wavefront's 64 lanes' 16 bytes each, one after the other from `to` on.  They are written as assembly because a builtin makes the
 // compiler put a wait for all of them before every transposing read that follows (the two might touch the same bytes, for all it knows), which would leave nothing of a
 // step's head start.  They have no register that anything could read too early; arrive() waits for them.
+// (Scalar registers that a vector instruction has written are not there for a load in the five states behind it, and the compiler, which cannot see these loads, does not wait:
+// it keeps the descriptors in scalar arithmetic, and a test looks its listing over.  Waits in every load instead: 1045 us for 1035, 2048 tokens behind 30720.)
 typedef int int4a __attribute__((ext_vector_type(4)));
 __device__ inline void load_to_lds(int4a from, uint32_t offset, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory", "m0");
