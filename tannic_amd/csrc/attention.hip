@@ -148,6 +148,8 @@ int run_attention(const AttentionProblem& p, const void* q, const void* k, const
 // 16 of the other's tiles, which reads the keys for each (8 tokens of 32 / 8 heads of 128 of 16 sequences behind 8192 173 us there and 109 here, 12 tokens 287 and 111; 4 tokens,
 // one tile for both, 111 and 107, and of 8 sequences' 16 heads of 64 over 2000 states 15 and 20); more than 32 for heads above 128 (12 / 2 heads of 256: 5 tokens of 2 sequences
 // behind 4096 37 and 52, of 16 66 and 66, 8 tokens of 16 83 and 67).
+// The host does not know the lengths, so it is the average that counts: sequences of like lengths are on the right side, a chunk among many single tokens is not (190 tokens behind
+// 8192 with 63 single tokens behind 512 to 8192: 366 us, where the chunk alone takes 74 and the single tokens 139).
 int attention_pieces(int dtype, const AttentionProblem& p, const void* q, const void* k, const void* v, void* out, hipStream_t stream) {
     const int64_t size = static_cast<int64_t>(dtype_size(dtype));
     const int64_t grain = p.d | p.q_batch | p.q_token | p.q_head | p.k_page | p.k_head | p.k_token | p.v_page | p.v_head | p.v_token;

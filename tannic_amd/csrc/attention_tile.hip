@@ -7,7 +7,7 @@
 //           accumulator's order; V is transposed on its way out of LDS (ds_read_b64_tr_b16).
 // The running maximum follows the scores only when one exceeds it by 2^8 (in the weights' power of two): sums in fp32 have the room, and the
 // 64 to 128 sums of a lane are rescaled a few times in a row's life instead of every step.
-// Measured, bf16: 2048 tokens of 32 / 8 heads of 128 behind 30720 1048 us, 1.02 PFLOP/s, the matrix pipe busy 49 % of the time (6.2 vector instructions to a product, two
+// Measured, bf16: 2048 tokens of 32 / 8 heads of 128 behind 30720 1035 us, 1.03 PFLOP/s, the matrix pipe busy 49 % of the time (6.2 vector instructions to a product, two
 // wavefronts on a SIMD); 512 behind 4096 62 us, 10 of them parts written and put together; 700 tokens of 8 sequences' 16 heads of 64 over 500 to 2000 states 52 us, 0.49 PFLOP/s
 // (half the products to a weight).
 #include <algorithm>
