@@ -443,6 +443,35 @@ int tannic_hip_copy_pages(tannic_tensor_t* pool, tannic_stream_t stream, const i
 int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const tannic_tensor_t* v, const tannic_tensor_t* lengths,
                       tannic_tensor_t* dst, tannic_stream_t stream, float scale);
 
+/* ------------------------------------------------------------------ *
+ * Rows in 8-bit integers with a scale each, and their product (no
+ * counterpart in the reference).  values int8 [.., L] with scales float
+ * [..] stand for values * scales: a token's activations, or a channel's
+ * weights (a matrix [out, in] and its transposed view as second operand).
+ *   values = rint(u * (127 / m)), ties to even, scales = m / 127,
+ *   m = max |u| of the row, 2^-119 at least
+ * so that no value is off by more than half a scale.  A row with something
+ * that is not finite has zeros and the scale NaN: all that is computed from
+ * it is NaN.  x: float16, bfloat16 or float, any strides; u is float; the
+ * results are contiguous.
+ * ------------------------------------------------------------------ */
+/* u = x */
+int tannic_hip_quantize(const tannic_tensor_t* x, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream);
+/* u = gate / (1 + exp(-gate)) * up, both of one shape */
+int tannic_hip_swiglu_quantize(const tannic_tensor_t* gate, const tannic_tensor_t* up, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream);
+/* total = x + residual, rounded to x's type; dst = total / sqrt(mean(total^2) + eps) * gain over the last axis, in x's type (float64 too), or with
+ * `scales` in 8 bits (u = total * gain in float, whose integers are the norm's: the root is one number for a row and goes into the scale).
+ * residual and total may both be NULL (x is normed as it is); total may be x or residual itself. */
+int tannic_hip_add_rms_norm(const tannic_tensor_t* x, const tannic_tensor_t* residual, const tannic_tensor_t* gain, tannic_tensor_t* total, tannic_tensor_t* dst,
+                            tannic_tensor_t* scales, tannic_stream_t stream, float eps);
+/* dst = values * scales, rounded once to float16, bfloat16 or float; values with any strides */
+int tannic_hip_dequantize(const tannic_tensor_t* values, const tannic_tensor_t* scales, tannic_tensor_t* dst, tannic_stream_t stream);
+/* dst[m, n] = (sum_k a[m, k] * b[k, n]) * a_scales[m] * b_scales[n]: a int8 [.., M, K], b int8 [.., K, N], a_scales float [.., M], b_scales float
+ * [.., N], batches as tannic_hip_gemm takes them, dst float16, bfloat16 or float.  The sum is exact (K below 2^17) and rounded to float,
+ * the product with the scales is float and rounded once to dst. */
+int tannic_hip_gemm_quantized(const tannic_tensor_t* a, const tannic_tensor_t* a_scales, const tannic_tensor_t* b, const tannic_tensor_t* b_scales, tannic_tensor_t* dst,
+                              tannic_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

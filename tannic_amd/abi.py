@@ -130,6 +130,11 @@ def kernel_signatures(with_stream):
     sig["attend_pages"] = (C.c_int, [TP] * 7 + s + [C.c_float])
     sig["copy_pages"] = (C.c_int, [TP] + s + [I32P, I32P, C.c_size_t])
     sig["attend"] = (C.c_int, [TP] * 5 + s + [C.c_float])    # the fourth operand (lengths) may be NULL
+    sig["add_rms_norm"] = (C.c_int, [TP] * 6 + s + [C.c_float])    # the residual with the sum, and the scales, may be NULL
+    sig["quantize"] = (C.c_int, [TP] * 3 + s)
+    sig["swiglu_quantize"] = (C.c_int, [TP] * 4 + s)
+    sig["dequantize"] = (C.c_int, [TP] * 3 + s)
+    sig["gemm_quantized"] = (C.c_int, [TP] * 5 + s)
     return sig
 
 

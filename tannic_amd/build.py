@@ -43,6 +43,8 @@ UNITS = [
     ("attention_rows.hip", "attention_rows.o", []),
     ("attention_tile.hip", "attention_tile.o", []),
     ("cache.hip", "cache.o", EXACT),
+    ("quantized.hip", "quantized.o", []),
+    ("gemm_quantized.hip", "gemm_quantized.o", []),
     ("gemm.hip", "gemm.o", []),
     ("gemm_mfma.hip", "gemm_mfma.o", []),
     ("gemm_skinny.hip", "gemm_skinny.o", []),

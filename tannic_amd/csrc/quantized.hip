@@ -1,0 +1,217 @@
+// Rows in 8-bit integers with a scale each, what a product of integers takes (gemm_quantized.hip): of any values, of a gated activation, of a
+// root-mean-square norm with the residual's addition before it; that norm in the operands' type; and the way back.
+//   quantize          u = x
+//   swiglu_quantize   u = gate / (1 + exp(-gate)) * up
+//   add_rms_norm      total = round(x + residual),  u = total * gain,  r = 1 / sqrt(mean(total^2) + eps);  u * r in the operands' type, or in 8 bits
+//   values = rint(u * (127 / max|u|)),  scales = max|u| (* r) / 127
+// The norm's r is one number for a row and cancels in the integers, so that these need the row's largest |u| only, which no order of summation changes.
+#include "quantized.hpp"
+
+namespace th {
+
+struct SquaresOp {
+    template <class A> __device__ static inline A combine(A x, A y) { return x + y; }
+};
+
+// One value per block of 256 threads, the same in every thread.
+template <class Op, class A>
+__device__ inline A block_reduce(A v, A* lds) {
+    v = wave_reduce<Op>(v);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    return Op::combine(Op::combine(lds[0], lds[1]), Op::combine(lds[2], lds[3]));
+}
+
+enum class RowSource { plain, gated, norm, sum_norm };
+
+struct RowOperands {
+    const void *x, *second, *gain;      // second: up, or the residual
+    void *total, *dst;                  // dst: the norm in the operands' type, or the integers
+    float* scales;                      // nullptr: in the operands' type
+    RowsMap rows_x, rows_second;
+    uint32_t rows, length;
+    double eps;
+};
+
+__device__ inline float gated(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
+
+// Any row, the rows in turns: a block per row, which is read twice (a sum that was written is read again by the thread that wrote it).
+template <class T, RowSource S, bool INTEGERS>
+__global__ __launch_bounds__(256) void rows_any_kernel(RowOperands p) {
+    using A = std::conditional_t<std::is_same_v<T, double>, double, float>;
+    constexpr bool NORM = S == RowSource::norm || S == RowSource::sum_norm;
+    __shared__ A sums[4];
+    __shared__ uint32_t largest[4];
+    const T* const gain = static_cast<const T*>(p.gain);
+    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* const x = static_cast<const T*>(p.x) + p.rows_x.offset(row);
+        const T* const second = static_cast<const T*>(p.second) + (S == RowSource::gated || S == RowSource::sum_norm ? p.rows_second.offset(row) : 0);
+        const size_t base = static_cast<size_t>(row) * p.length;
+        T* const total = static_cast<T*>(p.total) + base;
+        auto value = [&](uint32_t i, bool first) -> A {
+            if constexpr (S == RowSource::gated) return gated(widen(x[i * p.rows_x.step]), widen(second[i * p.rows_second.step]));
+            if constexpr (S == RowSource::sum_norm) {
+                if (!first) return static_cast<A>(widen(total[i]));
+                const T sum = rounded<T>(static_cast<A>(widen(x[i * p.rows_x.step])) + static_cast<A>(widen(second[i * p.rows_second.step])));
+                total[i] = sum;
+                return static_cast<A>(widen(sum));
+            }
+            return static_cast<A>(widen(x[i * p.rows_x.step]));
+        };
+        A squares = 0;
+        uint32_t most = 0;
+        for (uint32_t i = threadIdx.x; i < p.length; i += 256) {
+            const A v = value(i, true);
+            if constexpr (NORM) squares += v * v;
+            if constexpr (INTEGERS) most = LargestOp::combine(most, magnitude(static_cast<float>(NORM ? v * static_cast<A>(widen(gain[i])) : v)));
+        }
+        A r = 1;
+        if constexpr (NORM) r = A(1) / sqrt(block_reduce<SquaresOp>(squares, sums) / static_cast<A>(p.length) + static_cast<A>(p.eps));
+        if constexpr (INTEGERS) {
+            const RowScale scale(block_reduce<LargestOp>(most, largest));
+            for (uint32_t i = threadIdx.x; i < p.length; i += 256) {
+                const A v = value(i, false);
+                static_cast<int8_t*>(p.dst)[base + i] = scale.integer(static_cast<float>(NORM ? v * static_cast<A>(widen(gain[i])) : v));
+            }
+            if (threadIdx.x == 0) p.scales[row] = scale.scale(static_cast<float>(r));
+        } else {
+            for (uint32_t i = threadIdx.x; i < p.length; i += 256) static_cast<T*>(p.dst)[base + i] = rounded<T>(value(i, false) * r * static_cast<A>(widen(gain[i])));
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void dequantize_any_kernel(const int8_t* values, RowsMap map, const float* scales, T* dst, uint32_t rows, uint32_t length) {
+    for (uint32_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int8_t* const x = values + map.offset(row);
+        const float scale = scales[row];
+        for (uint32_t i = threadIdx.x; i < length; i += 256) dst[static_cast<size_t>(row) * length + i] = rounded<T>(static_cast<float>(x[i * map.step]) * scale);
+    }
+}
+
+constexpr uint32_t kMostRowBlocks = 1u << 20;      // (rows beyond in turns)
+
+template <class T, RowSource S, bool INTEGERS>
+int run_rows(const RowOperands& p, hipStream_t stream) {
+    hipLaunchKernelGGL((rows_any_kernel<T, S, INTEGERS>), dim3(p.rows < kMostRowBlocks ? p.rows : kMostRowBlocks), dim3(256), 0, stream, p);
+    return launch_status("rows_any_kernel");
+}
+
+template <RowSource S, bool INTEGERS>
+int run_rows(int dtype, const RowOperands& p, hipStream_t stream) {
+    switch (dtype) {
+        case TANNIC_FLOAT16: return run_rows<f16, S, INTEGERS>(p, stream);
+        case TANNIC_BFLOAT16: return run_rows<bf16, S, INTEGERS>(p, stream);
+        case TANNIC_FLOAT32: return run_rows<float, S, INTEGERS>(p, stream);
+        case TANNIC_FLOAT64:
+            if constexpr (!INTEGERS) return run_rows<double, S, INTEGERS>(p, stream);
+        default: return TANNIC_UNSUPPORTED_DTYPE;
+    }
+}
+
+// Rows and length of x [.., L]; what is too long for the kernels' 32-bit counts is refused.
+int describe_rows(const tannic_tensor_t* x, RowOperands& p, const char* too_large) {
+    const size_t length = x->shape.sizes[x->rank - 1];
+    size_t rows = 1;
+    for (int d = 0; d < x->rank - 1; ++d) {
+        if (x->shape.sizes[d] >= (1ull << 31)) return refuse(too_large);
+        rows *= x->shape.sizes[d];
+        if (rows >= (1ull << 31)) return refuse(too_large);
+    }
+    if (length >= (1ull << 31)) return refuse(too_large);
+    p.rows = static_cast<uint32_t>(rows);
+    p.length = static_cast<uint32_t>(length);
+    p.x = x->address;
+    p.rows_x = rows_of(x);
+    return TANNIC_SUCCESS;
+}
+
+}  // namespace th
+
+using namespace th;
+
+extern "C" {
+
+int tannic_hip_add_rms_norm(const tannic_tensor_t* x, const tannic_tensor_t* residual, const tannic_tensor_t* gain, tannic_tensor_t* total, tannic_tensor_t* dst,
+                            tannic_tensor_t* scales, tannic_stream_t stream, float eps) {
+    if (!x || !gain || !dst) return refuse("add_rms_norm: a descriptor is missing");
+    if ((residual == nullptr) != (total == nullptr)) return refuse("add_rms_norm: the sum is written where there is a residual, and only there");
+    if (!have_storage(x, residual, gain, total, dst, scales)) return TANNIC_ERROR;
+    if (!(quantizable(x->dtype) || (x->dtype == TANNIC_FLOAT64 && !scales)) || gain->dtype != x->dtype || (residual && (residual->dtype != x->dtype || total->dtype != x->dtype)) ||
+        dst->dtype != (scales ? TANNIC_INT8 : x->dtype) || (scales && scales->dtype != TANNIC_FLOAT32))
+        return TANNIC_UNSUPPORTED_DTYPE;
+    if (x->rank < 1 || !extents_equal(x, dst) || !rows_contiguous(dst) || (residual && (!extents_equal(x, residual) || !extents_equal(x, total) || !rows_contiguous(total))))
+        return refuse("add_rms_norm: x [.., L], the residual, the sum and dst have one shape, the sum and dst are contiguous");
+    if (gain->rank != 1 || gain->shape.sizes[0] != x->shape.sizes[x->rank - 1] || !rows_contiguous(gain)) return refuse("add_rms_norm: gain [L], contiguous");
+    if (scales && !scales_of(scales, dst)) return refuse("add_rms_norm: scales [..] for values [.., L], contiguous");
+    RowOperands p{};
+    if (int status = describe_rows(x, p, "add_rms_norm: 2^31 rows, rows of 2^31 elements or more are not supported")) return status;
+    if (int status = on_device_of("add_rms_norm: the operands live on a device", x, residual, gain, total, dst, scales)) return status;
+    if (p.rows == 0 || (p.length == 0 && !scales)) return TANNIC_SUCCESS;
+    p.gain = gain->address;
+    p.dst = dst->address;
+    p.scales = scales ? static_cast<float*>(scales->address) : nullptr;
+    p.eps = eps;
+    if (residual) {
+        p.second = residual->address;
+        p.rows_second = rows_of(residual);
+        p.total = total->address;
+        return scales ? run_rows<RowSource::sum_norm, true>(x->dtype, p, as_stream(stream)) : run_rows<RowSource::sum_norm, false>(x->dtype, p, as_stream(stream));
+    }
+    return scales ? run_rows<RowSource::norm, true>(x->dtype, p, as_stream(stream)) : run_rows<RowSource::norm, false>(x->dtype, p, as_stream(stream));
+}
+
+int tannic_hip_quantize(const tannic_tensor_t* x, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream) {
+    if (!x || !dst || !scales) return refuse("quantize: a descriptor is missing");
+    if (!have_storage(x, dst, scales)) return TANNIC_ERROR;
+    if (!quantizable(x->dtype) || dst->dtype != TANNIC_INT8 || scales->dtype != TANNIC_FLOAT32) return TANNIC_UNSUPPORTED_DTYPE;
+    if (x->rank < 1 || !extents_equal(x, dst) || !rows_contiguous(dst) || !scales_of(scales, dst)) return refuse("quantize: x and dst [.., L], scales [..], the results contiguous");
+    RowOperands p{};
+    if (int status = describe_rows(x, p, "quantize: 2^31 rows, rows of 2^31 elements or more are not supported")) return status;
+    if (int status = on_device_of("quantize: the operands live on a device", x, dst, scales)) return status;
+    if (p.rows == 0) return TANNIC_SUCCESS;
+    p.dst = dst->address;
+    p.scales = static_cast<float*>(scales->address);
+    return run_rows<RowSource::plain, true>(x->dtype, p, as_stream(stream));
+}
+
+int tannic_hip_swiglu_quantize(const tannic_tensor_t* gate, const tannic_tensor_t* up, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream) {
+    if (!gate || !up || !dst || !scales) return refuse("swiglu_quantize: a descriptor is missing");
+    if (!have_storage(gate, up, dst, scales)) return TANNIC_ERROR;
+    if (!quantizable(gate->dtype) || up->dtype != gate->dtype || dst->dtype != TANNIC_INT8 || scales->dtype != TANNIC_FLOAT32) return TANNIC_UNSUPPORTED_DTYPE;
+    if (gate->rank < 1 || !extents_equal(gate, up) || !extents_equal(gate, dst) || !rows_contiguous(dst) || !scales_of(scales, dst))
+        return refuse("swiglu_quantize: gate, up and dst [.., L], scales [..], the results contiguous");
+    RowOperands p{};
+    if (int status = describe_rows(gate, p, "swiglu_quantize: 2^31 rows, rows of 2^31 elements or more are not supported")) return status;
+    if (int status = on_device_of("swiglu_quantize: the operands live on a device", gate, up, dst, scales)) return status;
+    if (p.rows == 0) return TANNIC_SUCCESS;
+    p.second = up->address;
+    p.rows_second = rows_of(up);
+    p.dst = dst->address;
+    p.scales = static_cast<float*>(scales->address);
+    return run_rows<RowSource::gated, true>(gate->dtype, p, as_stream(stream));
+}
+
+int tannic_hip_dequantize(const tannic_tensor_t* values, const tannic_tensor_t* scales, tannic_tensor_t* dst, tannic_stream_t stream) {
+    if (!values || !scales || !dst) return refuse("dequantize: a descriptor is missing");
+    if (!have_storage(values, scales, dst)) return TANNIC_ERROR;
+    if (values->dtype != TANNIC_INT8 || scales->dtype != TANNIC_FLOAT32 || !quantizable(dst->dtype)) return TANNIC_UNSUPPORTED_DTYPE;
+    if (values->rank < 1 || !extents_equal(values, dst) || !rows_contiguous(dst) || !scales_of(scales, values))
+        return refuse("dequantize: values and dst [.., L], scales [..], dst and scales contiguous");
+    RowOperands p{};
+    if (int status = describe_rows(values, p, "dequantize: 2^31 rows, rows of 2^31 elements or more are not supported")) return status;
+    if (int status = on_device_of("dequantize: the operands live on a device", values, scales, dst)) return status;
+    if (p.rows == 0 || p.length == 0) return TANNIC_SUCCESS;
+    const auto run = [&](auto tag) {
+        using T = typename decltype(tag)::type;
+        hipLaunchKernelGGL((dequantize_any_kernel<T>), dim3(p.rows < kMostRowBlocks ? p.rows : kMostRowBlocks), dim3(256), 0, as_stream(stream),
+                           static_cast<const int8_t*>(values->address), p.rows_x, static_cast<const float*>(scales->address), static_cast<T*>(dst->address), p.rows, p.length);
+        return launch_status("dequantize_any_kernel");
+    };
+    if (dst->dtype == TANNIC_FLOAT16) return run(type_tag<f16>{});
+    if (dst->dtype == TANNIC_BFLOAT16) return run(type_tag<bf16>{});
+    return run(type_tag<float>{});
+}
+
+}  // extern "C"

@@ -643,3 +643,92 @@ def attend(q, k, v, lengths=None, scale=None):
     scale = 1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else scale
     _checked("attend", library().calls["attend"](q.packed(), k.packed(), v.packed(), None if lengths is None else lengths.packed(), dst.packed(), env.stream_number(), scale))
     return dst
+
+
+# ---- rows in 8-bit integers with a scale each, and their product (no twin in the reference) ----
+# ``values`` (int8 ``[.., L]``) with ``scales`` (float32 ``[..]``) stand for ``values * scales``: a token's activations, or a channel's weights
+# (``quantize`` of a matrix ``[out, in]``; its ``transpose()`` is the second operand of a product).  A row's largest value is 127 of its
+# scales; a row with something that is not finite has the scale NaN, and so all that is computed from it is NaN.
+def _in_8_bits(like, env):
+    return Tensor.fresh(types.int8, like.shape, env), Tensor.fresh(types.float32, like.shape[:-1], env)
+
+
+def _some_row(name, x):
+    if x.rank == 0:
+        raise TannicError(f"{name}: operands have rank >= 1")
+
+
+def quantize(x):
+    """``values, scales`` of the rows of ``x [.., L]``."""
+    _some_row("quantize", x)
+    env = _device_of("quantize", x)
+    values, scales = _in_8_bits(x, env)
+    _checked("quantize", library().calls["quantize"](x.packed(), values.packed(), scales.packed(), env.stream_number()))
+    return values, scales
+
+
+def swiglu_quantized(gate, up):
+    """``values, scales`` of the rows of ``gate / (1 + exp(-gate)) * up``, two operands of one shape."""
+    _some_row("swiglu_quantized", gate)
+    env = _device_of("swiglu_quantized", gate, up)
+    values, scales = _in_8_bits(gate, env)
+    _checked("swiglu_quantized", library().calls["swiglu_quantize"](gate.packed(), up.packed(), values.packed(), scales.packed(), env.stream_number()))
+    return values, scales
+
+
+def _add_rms_norm(name, x, residual, gain, eps, integers):
+    _some_row(name, x)
+    env = _device_of(name, x, gain) if residual is None else _device_of(name, x, residual, gain)
+    total = x if residual is None else Tensor.fresh(x.dtype, x.shape, env)
+    normed, scales = _in_8_bits(x, env) if integers else (Tensor.fresh(x.dtype, x.shape, env), None)
+    _checked(name, library().calls["add_rms_norm"](x.packed(), None if residual is None else residual.packed(), gain.packed(), None if residual is None else total.packed(),
+                                                   normed.packed(), scales.packed() if integers else None, env.stream_number(), eps))
+    return normed, scales, total
+
+
+def add_rms_norm(x, residual, gain, eps=1e-5):
+    """``normed, total``: ``total = x + residual`` and ``total / sqrt(mean(total**2, -1) + eps) * gain`` over the last axis (``x`` itself and its norm
+    where ``residual`` is ``None``)."""
+    normed, _, total = _add_rms_norm("add_rms_norm", x, residual, gain, eps, False)
+    return normed, total
+
+
+def add_rms_norm_quantized(x, residual, gain, eps=1e-5):
+    """``values, scales, total``: the same with the norm's rows in 8 bits."""
+    return _add_rms_norm("add_rms_norm_quantized", x, residual, gain, eps, True)
+
+
+def dequantize(values, scales, dtype):
+    """``values * scales`` of every row, in ``dtype``."""
+    env = _device_of("dequantize", values, scales)
+    dst = Tensor.fresh(dtype, values.shape, env)
+    _checked("dequantize", library().calls["dequantize"](values.packed(), scales.packed(), dst.packed(), env.stream_number()))
+    return dst
+
+
+_QUANTIZED_PRODUCTS = {}    # (shape, shape) -> shape of the product
+
+
+def matmul_quantized(a, a_scales, b, b_scales, dtype):
+    """``matmul(a, b) * a_scales[.., :, None] * b_scales[.., None, :]`` in ``dtype``, of ``a [.., M, K]`` with a scale for each row and ``b [.., K, N]`` with
+    one for each column; the whole numbers are summed exactly."""
+    key = (a.shape, b.shape)
+    shape = _QUANTIZED_PRODUCTS.get(key)
+    if shape is None:
+        if a.rank < 2 or b.rank < 2:
+            raise TannicError("Inputs must have rank >= 2")
+        if a.shape[-1] != b.shape[-2]:
+            raise TannicError("Inner dimensions must match for matmul")
+        batch = list(broadcast(a.shape[:-2], b.shape[:-2]))
+        for dims in (a.shape[:-2], b.shape[:-2]):
+            for d, n in enumerate(reversed(dims)):
+                if n == 0:      # (an empty batch over one matrix is empty)
+                    batch[-1 - d] = 0
+        shape = (*batch, a.shape[-2], b.shape[-1])
+        if len(_QUANTIZED_PRODUCTS) > 4096:
+            _QUANTIZED_PRODUCTS.clear()
+        _QUANTIZED_PRODUCTS[key] = shape
+    env = _device_of("matmul_quantized", a, a_scales, b, b_scales)
+    dst = Tensor.fresh(dtype, shape, env)
+    _checked("matmul_quantized", library().calls["gemm_quantized"](a.packed(), a_scales.packed(), b.packed(), b_scales.packed(), dst.packed(), env.stream_number()))
+    return dst
