@@ -448,7 +448,7 @@ int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const 
  * counterpart in the reference).  values int8 [.., L] with scales float
  * [..] stand for values * scales: a token's activations, or a channel's
  * weights (a matrix [out, in] and its transposed view as second operand).
- *   values = rint(u * (127 / m)), ties to even, scales = m / 127,
+ *   values = rint(u * (127 * (1 / m))), ties to even, scales = m / 127,
  *   m = max |u| of the row, 2^-119 at least
  * so that no value is off by more than half a scale.  A row with something
  * that is not finite has zeros and the scale NaN: all that is computed from

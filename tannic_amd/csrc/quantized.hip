@@ -3,7 +3,7 @@
 //   quantize          u = x
 //   swiglu_quantize   u = gate / (1 + exp(-gate)) * up
 //   add_rms_norm      total = round(x + residual),  u = total * gain,  r = 1 / sqrt(mean(total^2) + eps);  u * r in the operands' type, or in 8 bits
-//   values = rint(u * (127 / max|u|)),  scales = max|u| (* r) / 127
+//   values = rint(u * (127 * (1 / max|u|))),  scales = max|u| (* r) / 127
 // The norm's r is one number for a row and cancels in the integers, so that these need the row's largest |u| only, which no order of summation changes.
 #include "quantized.hpp"
 
@@ -34,7 +34,151 @@ struct RowOperands {
     double eps;
 };
 
-__device__ inline float gated(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
+// gate / (1 + exp(-gate)) * up, off by 8 * 2^-24 at most: exp(-gate) is 2^high * (1 + low * ln 2) with high + low = -gate * log2 e (the instruction for powers of two is off by
+// 2 units, and high alone would be by |gate|); the sum with 1 takes both in one rounding, its reciprocal is off by 2 units.  An exponential beyond all floats makes the quotient 0.
+__device__ inline float gated(float gate, float up) {
+    constexpr float log2e = 0x1.715476p+0f, rest = 0x1.4ae0bep-26f, ln2 = 0x1.62e430p-1f;
+    const float high = -gate * log2e, low = fmaf(-gate, rest, fmaf(-gate, log2e, -high));
+    const float sum = fmaf(__builtin_amdgcn_exp2f(high), fmaf(low, ln2, 1.0f), 1.0f);
+    return gate * __builtin_amdgcn_rcpf(sum) * up;
+}
+
+// ---- rows in registers ----------------------------------------------------------------
+// 16 bytes of a row and what its integers take, wherever they start.
+typedef unsigned int uint4any __attribute__((ext_vector_type(4), aligned(1)));
+typedef unsigned int uint2any __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned int uint1any __attribute__((aligned(1)));
+template <class T> constexpr int kPiece = 16 / sizeof(T);
+template <class T> struct Piece {
+    T v[kPiece<T>];
+};
+
+// `live` elements of a piece (the last one of a row may be short), zeros behind them
+template <class T> __device__ inline Piece<T> load_piece(const T* from, uint32_t live) {
+    Piece<T> r;
+    if (live >= kPiece<T>) {
+        const uint4any bits = *reinterpret_cast<const uint4any*>(from);
+        __builtin_memcpy(&r, &bits, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPiece<T>; ++e) r.v[e] = e < static_cast<int>(live) ? from[e] : T{};
+    }
+    return r;
+}
+template <class T> __device__ inline void store_piece(T* to, const Piece<T>& piece, uint32_t live) {
+    if (live >= kPiece<T>) {
+        uint4any bits;
+        __builtin_memcpy(&bits, &piece, 16);
+        *reinterpret_cast<uint4any*>(to) = bits;
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPiece<T>; ++e)
+            if (e < static_cast<int>(live)) to[e] = piece.v[e];
+    }
+}
+template <int N> __device__ inline void store_integers(int8_t* to, const int8_t (&v)[N], uint32_t live) {
+    if (live >= N) {
+        if constexpr (N == 8) {
+            uint2any bits;
+            __builtin_memcpy(&bits, v, 8);
+            *reinterpret_cast<uint2any*>(to) = bits;
+        } else {
+            unsigned int bits;
+            __builtin_memcpy(&bits, v, 4);
+            *reinterpret_cast<uint1any*>(to) = bits;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < static_cast<int>(live)) to[e] = v[e];
+    }
+}
+
+// A group of G threads (a wavefront, or a block) per row, which is read once and kept in registers as u, NCH pieces of 16 bytes of a thread.
+template <class T, RowSource S, bool INTEGERS, int G, int NCH>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void rows_kernel(RowOperands p) {
+    constexpr bool NORM = S == RowSource::norm || S == RowSource::sum_norm;
+    constexpr int VEC = kPiece<T>, BLOCK = G < 256 ? 256 : G, WAVES = BLOCK / 64;
+    __shared__ float sums[WAVES];
+    __shared__ uint32_t largest[WAVES];
+    const uint32_t t = threadIdx.x % G;
+    const T* const gain = static_cast<const T*>(p.gain);
+    for (uint32_t row = blockIdx.x * (BLOCK / G) + threadIdx.x / G; row < p.rows; row += gridDim.x * (BLOCK / G)) {
+        const T* const x = static_cast<const T*>(p.x) + p.rows_x.offset(row);
+        const T* const second = S == RowSource::gated || S == RowSource::sum_norm ? static_cast<const T*>(p.second) + p.rows_second.offset(row) : nullptr;
+        const size_t base = static_cast<size_t>(row) * p.length;
+        Piece<T> a[NCH], b[NCH], g[NCH];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const uint32_t at = (t + i * G) * VEC;
+            if (at < p.length) {
+                a[i] = load_piece(x + at, p.length - at);
+                if constexpr (S == RowSource::gated || S == RowSource::sum_norm) b[i] = load_piece(second + at, p.length - at);
+                if constexpr (NORM) g[i] = load_piece(gain + at, p.length - at);
+            }
+        }
+        float u[NCH][VEC], squares = 0;
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const uint32_t at = (t + i * G) * VEC;
+            if (at < p.length) {
+                if constexpr (S == RowSource::sum_norm) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) a[i].v[e] = rounded<T>(widen(a[i].v[e]) + widen(b[i].v[e]));
+                    store_piece(static_cast<T*>(p.total) + base + at, a[i], p.length - at);
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float v = widen(a[i].v[e]);
+                    if constexpr (NORM) squares += v * v;
+                    if constexpr (S == RowSource::gated) u[i][e] = gated(v, widen(b[i].v[e]));
+                    else if constexpr (NORM && INTEGERS) u[i][e] = v * widen(g[i].v[e]);
+                    else u[i][e] = v;
+                    if constexpr (INTEGERS) most = LargestOp::combine(most, magnitude(u[i][e]));
+                }
+            }
+        }
+        if constexpr (NORM) squares = wave_reduce<SquaresOp>(squares);
+        if constexpr (INTEGERS) most = wave_reduce<LargestOp>(most);
+        if constexpr (G > 64) {
+            __syncthreads();      // (the row before has been read)
+            if (threadIdx.x % 64 == 0) {
+                if constexpr (NORM) sums[threadIdx.x / 64] = squares;
+                if constexpr (INTEGERS) largest[threadIdx.x / 64] = most;
+            }
+            __syncthreads();
+            squares = 0;
+            most = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                if constexpr (NORM) squares += sums[w];
+                if constexpr (INTEGERS) most = LargestOp::combine(most, largest[w]);
+            }
+        }
+        const float r = NORM ? 1.0f / sqrtf(squares / static_cast<float>(p.length) + static_cast<float>(p.eps)) : 1.0f;
+        const RowScale scale(most);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const uint32_t at = (t + i * G) * VEC;
+            if (at < p.length) {
+                if constexpr (INTEGERS) {
+                    int8_t out[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) out[e] = scale.integer(u[i][e]);
+                    store_integers(static_cast<int8_t*>(p.dst) + base + at, out, p.length - at);
+                } else {
+                    Piece<T> out;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) out.v[e] = rounded<T>(u[i][e] * r * widen(g[i].v[e]));
+                    store_piece(static_cast<T*>(p.dst) + base + at, out, p.length - at);
+                }
+            }
+        }
+        if constexpr (INTEGERS)
+            if (t == 0) p.scales[row] = scale.scale(r);
+    }
+}
 
 // Any row, the rows in turns: a block per row, which is read twice (a sum that was written is read again by the thread that wrote it).
 template <class T, RowSource S, bool INTEGERS>
@@ -81,6 +225,35 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowOperands p) {
     }
 }
 
+// Eight elements of a row per thread.
+template <class T>
+__global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* values, RowsMap map, const float* scales, T* dst, uint32_t length, FastDiv per_row, uint32_t items) {
+    const uint32_t item = blockIdx.x * 256 + threadIdx.x;
+    if (item >= items) return;
+    uint32_t row, piece;
+    per_row.divmod(item, row, piece);
+    const uint32_t at = piece * 8, live = length - at;
+    const int8_t* const from = values + map.offset(row) + at;
+    int8_t v[8];
+    if (live >= 8) {
+        const uint2any bits = *reinterpret_cast<const uint2any*>(from);
+        __builtin_memcpy(v, &bits, 8);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < static_cast<int>(live) ? from[e] : int8_t(0);
+    }
+    const float scale = scales[row];
+    T* const to = dst + static_cast<size_t>(row) * length + at;
+    constexpr int VEC = kPiece<T>;
+#pragma unroll
+    for (int i = 0; i < 8; i += VEC) {
+        Piece<T> out;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out.v[e] = rounded<T>(static_cast<float>(v[i + e]) * scale);
+        if (static_cast<int>(live) > i) store_piece(to + i, out, live - i);
+    }
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void dequantize_any_kernel(const int8_t* values, RowsMap map, const float* scales, T* dst, uint32_t rows, uint32_t length) {
     for (uint32_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -92,8 +265,31 @@ __global__ __launch_bounds__(256) void dequantize_any_kernel(const int8_t* value
 
 constexpr uint32_t kMostRowBlocks = 1u << 20;      // (rows beyond in turns)
 
+template <class T, RowSource S, bool INTEGERS, int G, int NCH>
+int launch_rows(const RowOperands& p, hipStream_t stream) {
+    constexpr uint32_t BLOCK = G < 256 ? 256 : G, ROWS = BLOCK / G;
+    const uint32_t blocks = (p.rows + ROWS - 1) / ROWS;
+    hipLaunchKernelGGL((rows_kernel<T, S, INTEGERS, G, NCH>), dim3(blocks < kMostRowBlocks ? blocks : kMostRowBlocks), dim3(BLOCK), 0, stream, p);
+    return launch_status("rows_kernel");
+}
+
 template <class T, RowSource S, bool INTEGERS>
 int run_rows(const RowOperands& p, hipStream_t stream) {
+    if constexpr (!std::is_same_v<T, double>) {
+        // rows whose elements lie one after the other and that the registers of a block hold
+        constexpr bool PAIR = S == RowSource::gated || S == RowSource::sum_norm;
+        const uint32_t pieces = (p.length + kPiece<T> - 1) / kPiece<T>;
+        if (p.length > 0 && (p.length == 1 || (p.rows_x.step == 1 && (!PAIR || p.rows_second.step == 1))) && pieces <= 4096) {
+            if (pieces <= 64) return launch_rows<T, S, INTEGERS, 64, 1>(p, stream);
+            if (pieces <= 128 && p.rows >= 1024) return launch_rows<T, S, INTEGERS, 64, 2>(p, stream);
+            if (pieces <= 256 && p.rows >= 1024) return launch_rows<T, S, INTEGERS, 64, 4>(p, stream);
+            if (pieces <= 256) return launch_rows<T, S, INTEGERS, 256, 1>(p, stream);
+            if (pieces <= 512) return launch_rows<T, S, INTEGERS, 256, 2>(p, stream);
+            if (pieces <= 1024) return launch_rows<T, S, INTEGERS, 256, 4>(p, stream);
+            if (pieces <= 2048) return launch_rows<T, S, INTEGERS, 1024, 2>(p, stream);
+            return launch_rows<T, S, INTEGERS, 1024, 4>(p, stream);
+        }
+    }
     hipLaunchKernelGGL((rows_any_kernel<T, S, INTEGERS>), dim3(p.rows < kMostRowBlocks ? p.rows : kMostRowBlocks), dim3(256), 0, stream, p);
     return launch_status("rows_any_kernel");
 }
@@ -205,6 +401,13 @@ int tannic_hip_dequantize(const tannic_tensor_t* values, const tannic_tensor_t* 
     if (p.rows == 0 || p.length == 0) return TANNIC_SUCCESS;
     const auto run = [&](auto tag) {
         using T = typename decltype(tag)::type;
+        const uint64_t per_row = (static_cast<uint64_t>(p.length) + 7) / 8, items = per_row * p.rows;
+        if ((p.length == 1 || p.rows_x.step == 1) && items < (1ull << 31)) {
+            hipLaunchKernelGGL((dequantize_kernel<T>), dim3(static_cast<uint32_t>((items + 255) / 256)), dim3(256), 0, as_stream(stream), static_cast<const int8_t*>(values->address),
+                               p.rows_x, static_cast<const float*>(scales->address), static_cast<T*>(dst->address), p.length, FastDiv(static_cast<uint32_t>(per_row)),
+                               static_cast<uint32_t>(items));
+            return launch_status("dequantize_kernel");
+        }
         hipLaunchKernelGGL((dequantize_any_kernel<T>), dim3(p.rows < kMostRowBlocks ? p.rows : kMostRowBlocks), dim3(256), 0, as_stream(stream),
                            static_cast<const int8_t*>(values->address), p.rows_x, static_cast<const float*>(scales->address), static_cast<T*>(dst->address), p.rows, p.length);
         return launch_status("dequantize_any_kernel");

@@ -76,10 +76,10 @@ struct LargestOp {
 };
 __device__ inline uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-// A row whose largest value is smaller than this is written as if it were this: 127 divided by it is finite, it divided by 127 no subnormal number.
+// A row whose largest value is smaller than this is written as if it were this: 127 times its reciprocal is finite, it divided by 127 no subnormal number.
 constexpr float kLeastLargest = 0x1p-119f;
 
-// A row's integers are the nearest ones of u * (127 / its largest magnitude), ties to even, and its scale says what a 1 stands for.  A row with something
+// A row's integers are the nearest ones of u * (127 * (1 / its largest magnitude)), each step rounded, ties to even, and its scale says what a 1 stands for.  A row with something
 // that is not finite has the scale NaN and zeros: whatever is computed from it is NaN.
 struct RowScale {
     float factor, largest;
@@ -87,7 +87,7 @@ struct RowScale {
     __device__ explicit RowScale(uint32_t most) {
         finite = most < 0x7F800000u;
         largest = fmaxf(__uint_as_float(most), kLeastLargest);
-        factor = 127.0f / largest;
+        factor = 127.0f * (1.0f / largest);
     }
     __device__ inline int8_t integer(float u) const { return finite ? static_cast<int8_t>(static_cast<int>(rintf(u * factor))) : int8_t(0); }
     // (times `one`: what every element of the row is multiplied by, which cancels in the integers)

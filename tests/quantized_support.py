@@ -20,7 +20,7 @@ def integers_of(u):
     finite = np.isfinite(u).all(-1, keepdims=True)
     largest = np.maximum(np.where(finite, most, 1.0), LEAST).astype(np.float32)
     with np.errstate(invalid="ignore", over="ignore"):
-        values = np.rint(np.where(finite, u, 0.0).astype(np.float32) * (np.float32(127) / largest)).astype(np.int8)
+        values = np.rint(np.where(finite, u, 0.0).astype(np.float32) * (np.float32(127) * (np.float32(1) / largest))).astype(np.int8)
     return values, largest[..., 0], finite[..., 0]
 
 
