@@ -45,6 +45,8 @@ UNITS = [
     ("cache.hip", "cache.o", EXACT),
     ("quantized.hip", "quantized.o", []),
     ("gemm_quantized.hip", "gemm_quantized.o", []),
+    ("gemm_quantized_rows.hip", "gemm_quantized_rows.o", []),
+    ("gemm_quantized_tile.hip", "gemm_quantized_tile.o", []),
     ("gemm.hip", "gemm.o", []),
     ("gemm_mfma.hip", "gemm_mfma.o", []),
     ("gemm_skinny.hip", "gemm_skinny.o", []),

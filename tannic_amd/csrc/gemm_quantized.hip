@@ -2,31 +2,11 @@
 //   dst[m, n] = (sum_k a[m, k] * b[k, n]) * a_scales[m] * b_scales[n]
 // The sum is a whole number and exact in 32 bits (K below 2^17), in any order and in any parts; it is taken to float, multiplied by both scales and rounded once to dst's type.
 // As calls of the operators that were there it is an int32 product, a cast and two broadcasting multiplications.
-#include "gemm_tiles.hpp"
-#include "quantized.hpp"
+#include "gemm_quantized.hpp"
 
 namespace th {
 
 constexpr size_t kMostInner = (1u << 17) - 1;      // 128 * 128 * K is below 2^31
-
-// Where the scales of a product lie: a row's (column's) in a batch.
-struct ScalePlaces {
-    const float *a, *b;
-    int64_t a_step, b_step;
-    int64_t a_bs[6], b_bs[6];
-};
-
-__device__ inline void scale_offsets(const GemmProblem& p, const ScalePlaces& s, uint32_t batch, const float*& a, const float*& b) {
-    int64_t oa = 0, ob = 0;
-    for (int d = p.batch_rank - 1; d >= 0; --d) {
-        const uint32_t idx = batch % p.batch_extent[d];
-        batch /= p.batch_extent[d];
-        oa += static_cast<int64_t>(idx) * s.a_bs[d];
-        ob += static_cast<int64_t>(idx) * s.b_bs[d];
-    }
-    a = s.a + oa;
-    b = s.b + ob;
-}
 
 // Any strides: 64 x 64 results of a block, 4 x 4 of a thread, K in steps of 32 through LDS.
 template <class D>
@@ -80,12 +60,55 @@ __global__ __launch_bounds__(256) void gemm_quantized_any_kernel(const int8_t* a
 }
 
 template <class D>
-int run_quantized(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
+int run_any(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
     const uint64_t tiles_m = (static_cast<uint64_t>(p.M) + 63) / 64, tiles_n = (static_cast<uint64_t>(p.N) + 63) / 64;
     if (tiles_m * tiles_n >= kMostBlocks || p.batches > 65535) return refuse("gemm_quantized: a product of so many tiles or batches is not supported");
     hipLaunchKernelGGL((gemm_quantized_any_kernel<D>), dim3(static_cast<uint32_t>(tiles_m * tiles_n), p.batches), dim3(256), 0, stream, static_cast<const int8_t*>(a),
                        static_cast<const int8_t*>(b), static_cast<D*>(c), p, s, static_cast<uint32_t>(tiles_n));
     return launch_status("gemm_quantized_any_kernel");
+}
+
+// Batches that lie behind each other under one matrix are rows of one product.
+void fold_batches(GemmProblem& p, ScalePlaces& s) {
+    while (p.batch_rank > 0) {
+        const int d = p.batch_rank - 1;
+        const uint64_t extent = p.batch_extent[d], rows = p.M * extent;
+        if (extent != 1) {
+            if (p.b_bs[d] != 0 || s.b_bs[d] != 0 || rows >= (1ull << 31)) return;
+            const int64_t m = p.M;
+            if (m == 1) {      // (a single row's pitch is never used)
+                p.a_rs = p.a_bs[d];
+                s.a_step = s.a_bs[d];
+            } else if (p.a_bs[d] != m * p.a_rs || s.a_bs[d] != m * s.a_step) {
+                return;
+            }
+            p.c_rs = p.N;
+            p.M = static_cast<uint32_t>(rows);
+            p.batches = static_cast<uint32_t>(p.batches / extent);
+        }
+        p.batch_extent[d] = 1;
+        p.a_bs[d] = p.b_bs[d] = p.c_bs[d] = s.a_bs[d] = s.b_bs[d] = 0;
+        --p.batch_rank;
+    }
+}
+
+template <class D>
+int run_quantized(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
+    // operands that do not lie along K, or not in whole pieces, are copied first where that pays
+    GemmProblem q = p;
+    const void *pa = a, *pb = b;
+    void* held[2] = {nullptr, nullptr};
+    if (!quantized_operands_fit(p, a, b)) {
+        const int repacked = gemm_repack(p, 1, a, b, stream, true, q, pa, pb, held);
+        if (repacked == TANNIC_ERROR) return repacked;
+        if (repacked != TANNIC_SUCCESS) q = p;
+    }
+    int status = gemm_quantized_rows<D>(q, s, pa, pb, c, stream);
+    if (status == TANNIC_UNSUPPORTED_DTYPE) status = gemm_quantized_tile<D>(q, s, pa, pb, c, stream);
+    if (status == TANNIC_UNSUPPORTED_DTYPE) status = run_any<D>(p, s, a, b, c, stream);
+    for (void* h : held)
+        if (h) scratch_release(h, stream);
+    return status;
 }
 
 }  // namespace th
@@ -122,6 +145,7 @@ extern "C" int tannic_hip_gemm_quantized(const tannic_tensor_t* a, const tannic_
         s.a_bs[d] = places(a_scales);
         s.b_bs[d] = places(b_scales);
     }
+    fold_batches(p, s);
     switch (dst->dtype) {
         case TANNIC_FLOAT16: return run_quantized<f16>(p, s, a->address, b->address, dst->address, as_stream(stream));
         case TANNIC_BFLOAT16: return run_quantized<bf16>(p, s, a->address, b->address, dst->address, as_stream(stream));

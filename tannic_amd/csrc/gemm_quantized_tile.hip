@@ -1,0 +1,311 @@
+// Products of 8-bit integers with scales for more rows than a few: BM x BN tiles of 2 x 2 wavefronts on v_mfma_i32_16x16x64_i8.
+//
+// Both operands lie along K and come in steps of 128 bytes of a row, straight to LDS (16 bytes of a lane, 1 KB = eight rows of a load; the 16-byte pieces of a row in LDS are
+// turned by the row, on the global side, so that the 16 rows of a fragment are read from different banks).  STAGES steps are in LDS or on their way.  A step multiplies the
+// second half of the step before, whose fragments are in registers, and its own first half; behind the products of a half go the reads of the fragments for the next one, and
+// behind those of the first half the loads of the step that takes the freed stage.  It ends with a wait for the next step's loads and one barrier.
+// The weights are the first operand, so that a lane has four consecutive columns of one row: times the row's and the columns' scales, and to memory by whole rows through LDS (16 bits) or as they are.
+// SPLIT: `splits` blocks share a tile's K and leave whole numbers, which a second kernel adds up and scales.
+#include "gemm_quantized.hpp"
+
+namespace th {
+
+struct SharedK {
+    uint32_t splits, steps;      // blocks per tile; steps of 128 per block
+    int* partials;               // [split][batch][M][pitch]
+    uint32_t pitch;
+};
+
+template <class D, int BM, int BN, int STAGES, int PER_CU, bool SPLIT>
+__global__ __launch_bounds__(256, PER_CU) void gemm_quantized_tile_kernel(const int8_t* A, const int8_t* B, D* C, GemmProblem p, ScalePlaces s, uint32_t tiles_m, uint32_t tiles_n, SharedK shared) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
+    constexpr uint32_t A_TILE = BM * 128, B_TILE = BN * 128, STAGE = A_TILE + B_TILE;      // bytes
+    constexpr int LOADS_A = BM / 32, LOADS_B = BN / 32, LOADS = LOADS_A + LOADS_B;         // of 1 KB, per wavefront and step
+    extern __shared__ __align__(16) unsigned char lds[];
+
+    uint32_t tm, tn;
+    const uint32_t split = SPLIT ? blockIdx.x % shared.splits : 0;
+    tile_of<true>(SPLIT ? blockIdx.x / shared.splits : blockIdx.x, tiles_m, tiles_n, tm, tn);
+    int64_t oa, ob, oc;
+    batch_offsets(p, blockIdx.y, oa, ob, oc);
+    const uint32_t m0 = tm * BM, n0 = tn * BN;
+    const uint32_t all = (p.K + 127) / 128, first = SPLIT ? split * shared.steps : 0;
+    const uint32_t steps = SPLIT ? (all - first < shared.steps ? all - first : shared.steps) : all;
+
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const uint32_t wm = wave / 2 * WM, wn = wave % 2 * WN, frag_row = lane % 16, frag_piece = lane / 16;
+    const uint32_t rows_a = p.M - m0 < BM ? p.M - m0 : BM, rows_b = p.N - n0 < BN ? p.N - n0 : BN;
+    const __amdgpu_buffer_rsrc_t rsrc_a =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(A + oa + static_cast<int64_t>(m0) * p.a_rs), 0, bytes_of_rows(rows_a, p.a_rs, p.K), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsrc_b =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(B + ob + static_cast<int64_t>(n0) * p.b_cs), 0, bytes_of_rows(rows_b, p.b_cs, p.K), 0x00020000);
+    // load j of a wavefront fills 1 KB of a stage (j < LOADS_A: of A's tile): the lane's row and its (turned) piece; rows that are not there are beyond the buffer's range
+    uint32_t voff[LOADS];
+    const uint32_t turned = (lane % 8) ^ ((lane >> 4) & 3u);      // (rows 8 j + lane / 8: (row / 2) % 8 is (lane / 16) % 4 and 4 for odd j)
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+        const bool of_a = j < LOADS_A;
+        const uint32_t block = of_a ? wave * LOADS_A + j : wave * LOADS_B + (j - LOADS_A), row = block * 8 + lane / 8;
+        voff[j] = row < (of_a ? rows_a : rows_b) ? row * static_cast<uint32_t>(of_a ? p.a_rs : p.b_cs) + (turned ^ (block % 2 * 4)) * 16 : kBeyond;
+    }
+    const auto issue = [&](int j, uint32_t stage, uint32_t step) {
+        const bool of_a = j < LOADS_A;
+        const uint32_t block = of_a ? wave * LOADS_A + j : wave * LOADS_B + (j - LOADS_A), k = (first + step) * 128;
+        uint32_t offset = voff[j];
+        // (a step that K ends in: zeros behind it)
+        if (k + 128 > p.K && k + (turned ^ (block % 2 * 4)) * 16 >= p.K) offset = kBeyond;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(of_a ? rsrc_a : rsrc_b, (lds_address)(lds + stage * STAGE + (of_a ? 0 : A_TILE) + block * 1024), 16, offset, k, 0, 0);
+    };
+
+    int4v acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = int4v{0, 0, 0, 0};
+
+    // loads complete in order: with at most AHEAD of them outstanding the next step's are in
+    constexpr int AHEAD = (STAGES - 2) * LOADS;
+    const auto wait_loads = [](bool every) {
+        if (every) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
+    };
+    // own reads of LDS done, then everybody's (a fence would also wait for the loads on their way)
+    const auto meet = [] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) {
+        if (static_cast<uint32_t>(t) < steps) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) issue(j, t, t);
+        }
+    }
+    wait_loads(steps < static_cast<uint32_t>(STAGES - 1));
+    meet();
+
+    constexpr int PRODUCTS = TM * TN;      // of a half
+    constexpr int LOAD_EVERY = PRODUCTS / LOADS > 0 ? PRODUCTS / LOADS : 1;
+    constexpr int READ_EVERY = PRODUCTS / (TM + TN) > 0 ? PRODUCTS / (TM + TN) : 1;
+    uint4v fa[2][TM], fb[2][TN];
+    const auto fragment = [&](const unsigned char* tile, uint32_t row, int half) { return *reinterpret_cast<const uint4v*>(tile + tile_offset<int8_t>(row + frag_row, half * 4 + frag_piece)); };
+    // read n of a half's fragments: the first of A and all of B, which the first products want, then the others
+    const auto read = [&](const unsigned char* stage, int half, int n) {
+        if (n == 0) fa[half][0] = fragment(stage, wm, half);
+        else if (n <= TN) fb[half][n - 1] = fragment(stage + A_TILE, wn + (n - 1) * 16, half);
+        else fa[half][n - TN] = fragment(stage, wm + (n - TN) * 16, half);
+    };
+    const auto step = [&](uint32_t at, uint32_t now, uint32_t fill, auto first_tag, auto fetch_tag) {      // now: the stage of step `at`; fill: the one that is free
+        constexpr bool FIRST = decltype(first_tag)::value, FETCH = decltype(fetch_tag)::value;
+        const unsigned char* const stage = lds + now * STAGE;
+        if constexpr (FIRST) {
+#pragma unroll
+            for (int n = 0; n < TM + TN; ++n) read(stage, 0, n);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<2 * PRODUCTS>([&](auto tag) {
+            constexpr int m = decltype(tag)::value, half = m / PRODUCTS, q = m % PRODUCTS, i = q / TN, j = q % TN;
+            constexpr bool multiplies = !(FIRST && half == 0);
+            if constexpr (multiplies) acc[i][j] = mfma_i8(fb[1 - half][j], fa[1 - half][i], acc[i][j]);
+            // (a half with fewer products than reads has several behind each)
+            if constexpr (multiplies) {
+                constexpr int from = q * (TM + TN) / PRODUCTS, to = (q + 1) * (TM + TN) / PRODUCTS;
+                if constexpr (PRODUCTS >= TM + TN) {
+                    if constexpr (q % READ_EVERY == 0 && q / READ_EVERY < TM + TN) read(stage, half, q / READ_EVERY);
+                } else {
+#pragma unroll
+                    for (int n = from; n < to; ++n) read(stage, half, n);
+                }
+            }
+            constexpr int slot = FIRST ? m - PRODUCTS : m;
+            if constexpr (FETCH && slot >= 0 && slot < PRODUCTS) {
+                if constexpr (PRODUCTS >= LOADS) {
+                    if constexpr (slot % LOAD_EVERY == LOAD_EVERY / 2 && slot / LOAD_EVERY < LOADS) issue(slot / LOAD_EVERY, fill, at + STAGES - 1);
+                } else {
+#pragma unroll
+                    for (int n = slot * LOADS / PRODUCTS; n < (slot + 1) * LOADS / PRODUCTS; ++n) issue(n, fill, at + STAGES - 1);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        wait_loads(!FETCH);
+        meet();
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    const auto next = [](uint32_t stage) { return stage + 1 == STAGES ? 0u : stage + 1; };
+    uint32_t at = 0, now = 0, fill = STAGES - 1;
+    if (steps > STAGES - 1) step(0, now, fill, Yes{}, Yes{});
+    else step(0, now, fill, Yes{}, No{});
+    for (at = 1, now = next(now), fill = next(fill); at + STAGES - 1 < steps; ++at, now = next(now), fill = next(fill)) step(at, now, fill, No{}, Yes{});
+    for (; at < steps; ++at, now = next(now), fill = next(fill)) step(at, now, fill, No{}, No{});
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma_i8(fb[1][j], fa[1][i], acc[i][j]);
+
+    if constexpr (SPLIT) {
+        int* const mine = shared.partials + (static_cast<size_t>(split) * p.batches + blockIdx.y) * p.M * shared.pitch;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const uint32_t row = m0 + wm + i * 16 + lane % 16;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const uint32_t col = n0 + wn + j * 16 + 4 * (lane / 16);
+                if (row < p.M && col < p.N) *reinterpret_cast<int4v*>(mine + static_cast<size_t>(row) * shared.pitch + col) = acc[i][j];
+            }
+        }
+        return;
+    }
+    const float *scale_a, *scale_b;
+    scale_offsets(p, s, blockIdx.y, scale_a, scale_b);
+    float sb[TN][4];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t col = n0 + wn + j * 16 + 4 * (lane / 16) + e;
+            sb[j][e] = scale_b[(col < p.N ? col : p.N - 1) * s.b_step];
+        }
+    D* const c = C + oc;
+    if constexpr (sizeof(D) == 4) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const uint32_t row = m0 + wm + i * 16 + lane % 16;
+            const float sa = scale_a[(row < p.M ? row : p.M - 1) * s.a_step];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const uint32_t col = n0 + wn + j * 16 + 4 * (lane / 16);
+                float out[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[e] = static_cast<float>(acc[i][j][e]) * sa * sb[j][e];
+                if (row < p.M && col < p.N) store_four<D>(c + static_cast<int64_t>(row) * p.c_rs + col, out, p.N - col);
+            }
+        }
+    } else {
+        // a wavefront rounds its part into LDS of its own (no stage is read after the last barrier) and writes it by rows, 16 bytes of a lane
+        constexpr int PITCH = WN + 8;
+        D* const mine = reinterpret_cast<D*>(lds) + wave * (WM * PITCH);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const uint32_t row = m0 + wm + i * 16 + lane % 16;
+            const float sa = scale_a[(row < p.M ? row : p.M - 1) * s.a_step];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                D out[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[e] = rounded<D>(static_cast<float>(acc[i][j][e]) * sa * sb[j][e]);
+                uint2 bits;
+                __builtin_memcpy(&bits, out, 8);
+                *reinterpret_cast<uint2*>(mine + (i * 16 + lane % 16) * PITCH + j * 16 + 4 * (lane / 16)) = bits;
+            }
+        }
+        constexpr int PIECES = WN / 8, LANES = PIECES <= 4 ? 4 : PIECES <= 8 ? 8 : 16, ROWS = 64 / LANES;      // of a row; of a pass
+        const uint32_t piece = lane % LANES, col = n0 + wn + piece * 8;
+        if (piece < PIECES && col < p.N) {
+#pragma unroll
+            for (int r0 = 0; r0 < WM; r0 += ROWS) {
+                const uint32_t r = r0 + lane / LANES, row = m0 + wm + r;
+                if (row < p.M) {
+                    const uint4v bits = *reinterpret_cast<const uint4v*>(mine + r * PITCH + piece * 8);
+                    store_piece_anywhere(c + static_cast<int64_t>(row) * p.c_rs + col, &bits, p.N - col < 8 ? p.N - col : 8);
+                }
+            }
+        }
+    }
+#endif
+}
+
+// The sums of the blocks that shared K, scaled: four columns of a row per thread.
+template <class D>
+__global__ __launch_bounds__(256) void gemm_quantized_join_kernel(D* C, GemmProblem p, ScalePlaces s, SharedK shared, FastDiv per_row, uint32_t items) {
+    const uint32_t item = blockIdx.x * 256 + threadIdx.x;
+    if (item >= items) return;
+    uint32_t row, col;
+    per_row.divmod(item, row, col);
+    col *= 4;
+    int64_t oa, ob, oc;
+    batch_offsets(p, blockIdx.y, oa, ob, oc);
+    const float *scale_a, *scale_b;
+    scale_offsets(p, s, blockIdx.y, scale_a, scale_b);
+    const size_t apart = static_cast<size_t>(p.batches) * p.M * shared.pitch;
+    const int* from = shared.partials + (static_cast<size_t>(blockIdx.y) * p.M + row) * shared.pitch + col;
+    int4v sum = *reinterpret_cast<const int4v*>(from);
+    for (uint32_t i = 1; i < shared.splits; ++i) sum += *reinterpret_cast<const int4v*>(from + i * apart);
+    const float sa = scale_a[row * s.a_step];
+    float out[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = static_cast<float>(sum[e]) * sa * scale_b[(col + e < p.N ? col + e : col) * s.b_step];
+    store_four<D>(C + oc + static_cast<int64_t>(row) * p.c_rs + col, out, p.N - col);
+}
+
+template <class D, int BM, int BN, int STAGES>
+static int launch_tiles(const GemmProblem& p, const ScalePlaces& s, uint32_t splits, const void* a, const void* b, void* c, hipStream_t stream) {
+    const uint32_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, steps = (p.K + 127) / 128;
+    constexpr size_t tile_bytes = static_cast<size_t>(STAGES) * (BM + BN) * 128, out_bytes = sizeof(D) == 2 ? 2 * 4 * (BM / 2) * (BN / 2 + 8) : 0;
+    constexpr size_t lds_bytes = tile_bytes > out_bytes ? tile_bytes : out_bytes;
+    static_assert(lds_bytes <= 160 * 1024);
+    constexpr int PER_CU = lds_bytes <= 80 * 1024 ? 2 : 1;
+    SharedK shared{splits, (steps + splits - 1) / splits, nullptr, (p.N + 3) / 4 * 4};
+    const auto run = [&](auto kernel, std::atomic<uint64_t>& configured) {
+        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(kernel), lds_bytes, configured)) return rc;
+        hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n * shared.splits, p.batches), dim3(256), lds_bytes, stream, static_cast<const int8_t*>(a), static_cast<const int8_t*>(b),
+                           static_cast<D*>(c), p, s, tiles_m, tiles_n, shared);
+        return launch_status("gemm_quantized_tile_kernel");
+    };
+    static std::atomic<uint64_t> configured{0}, configured_split{0};
+    if (splits == 1) return run(gemm_quantized_tile_kernel<D, BM, BN, STAGES, PER_CU, false>, configured);
+    shared.splits = (steps + shared.steps - 1) / shared.steps;      // (none without a step)
+    void* held = nullptr;
+    if (scratch_acquire(&held, static_cast<size_t>(shared.splits) * p.batches * p.M * shared.pitch * sizeof(int), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+    shared.partials = static_cast<int*>(held);
+    int status = run(gemm_quantized_tile_kernel<D, BM, BN, STAGES, PER_CU, true>, configured_split);
+    if (status == TANNIC_SUCCESS) {
+        const uint32_t per_row = shared.pitch / 4, items = p.M * per_row;
+        hipLaunchKernelGGL((gemm_quantized_join_kernel<D>), dim3((items + 255) / 256, p.batches), dim3(256), 0, stream, static_cast<D*>(c), p, s, shared, FastDiv(per_row), items);
+        status = launch_status("gemm_quantized_join_kernel");
+    }
+    scratch_release(held, stream);
+    return status;
+}
+
+#ifdef TH_TILE_PROBE
+#include <cstdlib>
+#endif
+
+template <class D>
+int gemm_quantized_tile(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
+    if (!quantized_operands_fit(p, a, b) || (static_cast<uint64_t>(p.M) + 127) / 128 * ((static_cast<uint64_t>(p.N) + 127) / 128) >= kMostBlocks) return TANNIC_UNSUPPORTED_DTYPE;
+    uint32_t splits = 1;
+    auto tiles = [&](uint64_t bm, uint64_t bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn) * p.batches; };
+    int tile = p.M > 192 && tiles(256, 256) >= 200 ? 0 : p.M > 192 && tiles(256, 128) >= 128 ? 1 : 2;
+#ifdef TH_TILE_PROBE
+    if (const char* e = getenv("TH_TILE")) tile = atoi(e);
+    if (const char* e = getenv("TH_SPLITS")) splits = atoi(e);
+#endif
+    switch (tile) {
+        case 0: return launch_tiles<D, 256, 256, 2>(p, s, splits, a, b, c, stream);
+        case 1: return launch_tiles<D, 256, 128, 3>(p, s, splits, a, b, c, stream);
+        case 2: return launch_tiles<D, 128, 128, 4>(p, s, splits, a, b, c, stream);
+#ifdef TH_TILE_PROBE
+        case 3: return launch_tiles<D, 128, 128, 2>(p, s, splits, a, b, c, stream);
+        case 4: return launch_tiles<D, 128, 96, 5>(p, s, splits, a, b, c, stream);
+        case 5: return launch_tiles<D, 64, 128, 6>(p, s, splits, a, b, c, stream);
+        case 6: return launch_tiles<D, 64, 128, 3>(p, s, splits, a, b, c, stream);
+        case 7: return launch_tiles<D, 64, 64, 8>(p, s, splits, a, b, c, stream);
+        case 8: return launch_tiles<D, 64, 64, 5>(p, s, splits, a, b, c, stream);
+        case 9: return launch_tiles<D, 256, 192, 2>(p, s, splits, a, b, c, stream);
+        case 10: return launch_tiles<D, 32, 128, 6>(p, s, splits, a, b, c, stream);
+        case 11: return launch_tiles<D, 32, 64, 10>(p, s, splits, a, b, c, stream);
+#endif
+    }
+    return TANNIC_UNSUPPORTED_DTYPE;
+}
+
+template int gemm_quantized_tile<f16>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
+template int gemm_quantized_tile<bf16>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
+template int gemm_quantized_tile<float>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
+
+}  // namespace th
