@@ -46,7 +46,9 @@ UNITS = [
     ("quantized.hip", "quantized.o", []),
     ("gemm_quantized.hip", "gemm_quantized.o", []),
     ("gemm_quantized_rows.hip", "gemm_quantized_rows.o", []),
-    ("gemm_quantized_tile.hip", "gemm_quantized_tile.o", []),
+    ("gemm_quantized_tile.hip", "gemm_quantized_tile_f16.o", ["-DTH_TILE_TYPE=f16"]),
+    ("gemm_quantized_tile.hip", "gemm_quantized_tile_bf16.o", ["-DTH_TILE_TYPE=bf16"]),
+    ("gemm_quantized_tile.hip", "gemm_quantized_tile_f32.o", ["-DTH_TILE_TYPE=float"]),
     ("gemm.hip", "gemm.o", []),
     ("gemm_mfma.hip", "gemm_mfma.o", []),
     ("gemm_skinny.hip", "gemm_skinny.o", []),

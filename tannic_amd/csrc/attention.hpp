@@ -325,7 +325,7 @@ __device__ inline void load_through(const float* at, float4a& v) {
     v = float4a{x, y, z, w};
 }
 
-// How many blocks of a group have left their part: counts on a stream, 0 between calls.
+// How many blocks of a group have left their part: counts on a stream, 0 between calls.  (Blocks that share a tile of a product of 8-bit integers count theirs here, too.)
 constexpr uint32_t kAttentionArrivals = 1024;
 int attention_arrivals(hipStream_t stream, uint32_t*& arrivals);
 

@@ -5,20 +5,109 @@
 // second half of the step before, whose fragments are in registers, and its own first half; behind the products of a half go the reads of the fragments for the next one, and
 // behind those of the first half the loads of the step that takes the freed stage.  It ends with a wait for the next step's loads and one barrier.
 // The weights are the first operand, so that a lane has four consecutive columns of one row: times the row's and the columns' scales, and to memory by whole rows through LDS (16 bits) or as they are.
-// SPLIT: `splits` blocks share a tile's K and leave whole numbers, which a second kernel adds up and scales.
+// Blocks that share a tile's K leave whole numbers, which a second kernel adds up and scales, or for small tiles the last of the blocks that gets there.
+#include "attention.hpp"
 #include "gemm_quantized.hpp"
 
 namespace th {
 
 struct SharedK {
     uint32_t splits, steps;      // blocks per tile; steps of 128 per block
-    int* partials;               // [split][batch][M][pitch]
+    int* partials;               // for the second kernel [split][batch][M][pitch], for the last block [batch][tile][split][16 x 16 of a wavefront][thread][4]
     uint32_t pitch;
+    uint32_t* arrivals;          // of a tile's blocks, 0 between calls
 };
+enum class Sharing { none, second_kernel, last_block };
 
-template <class D, int BM, int BN, int STAGES, int PER_CU, bool SPLIT>
+// Sums pass from block to block, and between the L2 caches of the dies, through the memory both see: stores and loads of device scope, which no cache in between keeps.
+__device__ inline void store_through(int* at, const int4v& v) {
+    uint64_t bits[2];
+    __builtin_memcpy(bits, &v, 16);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) __hip_atomic_store(reinterpret_cast<uint64_t*>(at) + i, bits[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline int4v load_through(const int* at) {
+    uint64_t bits[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) bits[i] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    int4v v;
+    __builtin_memcpy(&v, bits, 16);
+    return v;
+}
+
+// A wavefront's TM x TN sums of 16 x 16 from row `row0` and column `col0` on: as they are, into its share of the partial sums.
+template <int TM, int TN>
+__device__ inline void leave_sums(const int4v (&acc)[TM][TN], const GemmProblem& p, const SharedK& shared, uint32_t split, uint32_t row0, uint32_t col0) {
+    const uint32_t lane = threadIdx.x % 64;
+    int* const mine = shared.partials + (static_cast<size_t>(split) * p.batches + blockIdx.y) * p.M * shared.pitch;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const uint32_t row = row0 + i * 16 + lane % 16;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const uint32_t col = col0 + j * 16 + 4 * (lane / 16);
+            if (row < p.M && col < p.N) *reinterpret_cast<int4v*>(mine + static_cast<size_t>(row) * shared.pitch + col) = acc[i][j];
+        }
+    }
+}
+
+// The same scaled and rounded, into the product; `mine`: the wavefront's own part of LDS, in which 16-bit results become whole rows (16 bytes of a lane).
+template <class D, int TM, int TN>
+__device__ inline void write_scaled(const int4v (&acc)[TM][TN], D* mine, D* c, const GemmProblem& p, const ScalePlaces& s, uint32_t row0, uint32_t col0) {
+    const uint32_t lane = threadIdx.x % 64;
+    const float *scale_a, *scale_b;
+    scale_offsets(p, s, blockIdx.y, scale_a, scale_b);
+    float sb[TN][4];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t col = col0 + j * 16 + 4 * (lane / 16) + e;
+            sb[j][e] = scale_b[(col < p.N ? col : p.N - 1) * s.b_step];
+        }
+    constexpr int WM = TM * 16, WN = TN * 16, PITCH = WN + 8;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const uint32_t row = row0 + i * 16 + lane % 16;
+        const float sa = scale_a[(row < p.M ? row : p.M - 1) * s.a_step];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            float out[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] = static_cast<float>(acc[i][j][e]) * sa * sb[j][e];
+            const uint32_t col = col0 + j * 16 + 4 * (lane / 16);
+            if constexpr (sizeof(D) == 4) {
+                if (row < p.M && col < p.N) store_four<D>(c + static_cast<int64_t>(row) * p.c_rs + col, out, p.N - col);
+            } else {
+                D narrow[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) narrow[e] = rounded<D>(out[e]);
+                uint2 bits;
+                __builtin_memcpy(&bits, narrow, 8);
+                *reinterpret_cast<uint2*>(mine + (i * 16 + lane % 16) * PITCH + j * 16 + 4 * (lane / 16)) = bits;
+            }
+        }
+    }
+    if constexpr (sizeof(D) == 2) {
+        constexpr int PIECES = WN / 8, LANES = PIECES <= 2 ? 2 : PIECES <= 4 ? 4 : PIECES <= 8 ? 8 : 16, ROWS = 64 / LANES;      // of a row; of a pass
+        const uint32_t piece = lane % LANES, col = col0 + piece * 8;
+        if (piece < PIECES && col < p.N) {
+#pragma unroll
+            for (int r0 = 0; r0 < WM; r0 += ROWS) {
+                const uint32_t r = r0 + lane / LANES, row = row0 + r;
+                if (r < WM && row < p.M) {
+                    const uint4v bits = *reinterpret_cast<const uint4v*>(mine + r * PITCH + piece * 8);
+                    store_piece_anywhere(c + static_cast<int64_t>(row) * p.c_rs + col, &bits, p.N - col < 8 ? p.N - col : 8);
+                }
+            }
+        }
+    }
+}
+
+template <class D, int BM, int BN, int STAGES, int PER_CU, Sharing SHARING>
 __global__ __launch_bounds__(256, PER_CU) void gemm_quantized_tile_kernel(const int8_t* A, const int8_t* B, D* C, GemmProblem p, ScalePlaces s, uint32_t tiles_m, uint32_t tiles_n, SharedK shared) {
 #if defined(__HIP_DEVICE_COMPILE__)
+    constexpr bool SPLIT = SHARING != Sharing::none;
     constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
     constexpr uint32_t A_TILE = BM * 128, B_TILE = BN * 128, STAGE = A_TILE + B_TILE;      // bytes
     constexpr int LOADS_A = BM / 32, LOADS_B = BN / 32, LOADS = LOADS_A + LOADS_B;         // of 1 KB, per wavefront and step
@@ -146,75 +235,45 @@ __global__ __launch_bounds__(256, PER_CU) void gemm_quantized_tile_kernel(const 
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = mfma_i8(fb[1][j], fa[1][i], acc[i][j]);
 
-    if constexpr (SPLIT) {
-        int* const mine = shared.partials + (static_cast<size_t>(split) * p.batches + blockIdx.y) * p.M * shared.pitch;
+    if constexpr (SHARING == Sharing::last_block) {
+        const uint32_t tile = blockIdx.y * tiles_m * tiles_n + blockIdx.x / shared.splits;
+        int* const parts = shared.partials + (static_cast<size_t>(tile) * shared.splits * (TM * TN) * 256 + threadIdx.x) * 4;
+        const auto of = [&](uint32_t part, int at) { return parts + (static_cast<size_t>(part) * (TM * TN) + at) * 1024; };
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const uint32_t row = m0 + wm + i * 16 + lane % 16;
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                const uint32_t col = n0 + wn + j * 16 + 4 * (lane / 16);
-                if (row < p.M && col < p.N) *reinterpret_cast<int4v*>(mine + static_cast<size_t>(row) * shared.pitch + col) = acc[i][j];
-            }
+            for (int j = 0; j < TN; ++j) store_through(of(split, i * TN + j), acc[i][j]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (they have arrived)
+        __syncthreads();
+        uint32_t* const before = reinterpret_cast<uint32_t*>(lds);
+        if (threadIdx.x == 0) {
+            *before = __hip_atomic_fetch_add(shared.arrivals + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (*before == shared.splits - 1) __hip_atomic_store(shared.arrivals + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        return;
-    }
-    const float *scale_a, *scale_b;
-    scale_offsets(p, s, blockIdx.y, scale_a, scale_b);
-    float sb[TN][4];
+        __syncthreads();
+        if (*before != shared.splits - 1) return;
+        __syncthreads();      // (its place in LDS is used again)
+        // the other parts, four on their way at a time (its own once more, and the last once more than once, where there are not four; times 0)
+        for (uint32_t from = 0; from < shared.splits; from += 4) {
+            int4v got[4][TM][TN];
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+            for (uint32_t n = 0; n < 4; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t col = n0 + wn + j * 16 + 4 * (lane / 16) + e;
-            sb[j][e] = scale_b[(col < p.N ? col : p.N - 1) * s.b_step];
-        }
-    D* const c = C + oc;
-    if constexpr (sizeof(D) == 4) {
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const uint32_t row = m0 + wm + i * 16 + lane % 16;
-            const float sa = scale_a[(row < p.M ? row : p.M - 1) * s.a_step];
+                    for (int j = 0; j < TN; ++j) got[n][i][j] = load_through(of(from + n < shared.splits ? from + n : split, i * TN + j));
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                const uint32_t col = n0 + wn + j * 16 + 4 * (lane / 16);
-                float out[4];
+            for (uint32_t n = 0; n < 4; ++n) {
+                const int counts = from + n < shared.splits && from + n != split;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out[e] = static_cast<float>(acc[i][j][e]) * sa * sb[j][e];
-                if (row < p.M && col < p.N) store_four<D>(c + static_cast<int64_t>(row) * p.c_rs + col, out, p.N - col);
-            }
-        }
-    } else {
-        // a wavefront rounds its part into LDS of its own (no stage is read after the last barrier) and writes it by rows, 16 bytes of a lane
-        constexpr int PITCH = WN + 8;
-        D* const mine = reinterpret_cast<D*>(lds) + wave * (WM * PITCH);
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const uint32_t row = m0 + wm + i * 16 + lane % 16;
-            const float sa = scale_a[(row < p.M ? row : p.M - 1) * s.a_step];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                D out[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) out[e] = rounded<D>(static_cast<float>(acc[i][j][e]) * sa * sb[j][e]);
-                uint2 bits;
-                __builtin_memcpy(&bits, out, 8);
-                *reinterpret_cast<uint2*>(mine + (i * 16 + lane % 16) * PITCH + j * 16 + 4 * (lane / 16)) = bits;
-            }
-        }
-        constexpr int PIECES = WN / 8, LANES = PIECES <= 4 ? 4 : PIECES <= 8 ? 8 : 16, ROWS = 64 / LANES;      // of a row; of a pass
-        const uint32_t piece = lane % LANES, col = n0 + wn + piece * 8;
-        if (piece < PIECES && col < p.N) {
-#pragma unroll
-            for (int r0 = 0; r0 < WM; r0 += ROWS) {
-                const uint32_t r = r0 + lane / LANES, row = m0 + wm + r;
-                if (row < p.M) {
-                    const uint4v bits = *reinterpret_cast<const uint4v*>(mine + r * PITCH + piece * 8);
-                    store_piece_anywhere(c + static_cast<int64_t>(row) * p.c_rs + col, &bits, p.N - col < 8 ? p.N - col : 8);
-                }
+                    for (int j = 0; j < TN; ++j) acc[i][j] += got[n][i][j] * counts;
             }
         }
     }
+    if constexpr (SHARING == Sharing::second_kernel) leave_sums<TM, TN>(acc, p, shared, split, m0 + wm, n0 + wn);
+    else write_scaled<D, TM, TN>(acc, reinterpret_cast<D*>(lds) + wave * (WM * (WN + 8)), C + oc, p, s, m0 + wm, n0 + wn);
 #endif
 }
 
@@ -241,14 +300,15 @@ __global__ __launch_bounds__(256) void gemm_quantized_join_kernel(D* C, GemmProb
     store_four<D>(C + oc + static_cast<int64_t>(row) * p.c_rs + col, out, p.N - col);
 }
 
-template <class D, int BM, int BN, int STAGES>
+template <class D, int BM, int BN, int STAGES, Sharing SHARING = Sharing::second_kernel>
 static int launch_tiles(const GemmProblem& p, const ScalePlaces& s, uint32_t splits, const void* a, const void* b, void* c, hipStream_t stream) {
     const uint32_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, steps = (p.K + 127) / 128;
     constexpr size_t tile_bytes = static_cast<size_t>(STAGES) * (BM + BN) * 128, out_bytes = sizeof(D) == 2 ? 2 * 4 * (BM / 2) * (BN / 2 + 8) : 0;
     constexpr size_t lds_bytes = tile_bytes > out_bytes ? tile_bytes : out_bytes;
     static_assert(lds_bytes <= 160 * 1024);
     constexpr int PER_CU = lds_bytes <= 80 * 1024 ? 2 : 1;
-    SharedK shared{splits, (steps + splits - 1) / splits, nullptr, (p.N + 3) / 4 * 4};
+    SharedK shared{splits, (steps + splits - 1) / splits, nullptr, (p.N + 3) / 4 * 4, nullptr};
+    shared.splits = (steps + shared.steps - 1) / shared.steps;      // (none without a step)
     const auto run = [&](auto kernel, std::atomic<uint64_t>& configured) {
         if (int rc = raise_lds_limit(reinterpret_cast<const void*>(kernel), lds_bytes, configured)) return rc;
         hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n * shared.splits, p.batches), dim3(256), lds_bytes, stream, static_cast<const int8_t*>(a), static_cast<const int8_t*>(b),
@@ -256,13 +316,16 @@ static int launch_tiles(const GemmProblem& p, const ScalePlaces& s, uint32_t spl
         return launch_status("gemm_quantized_tile_kernel");
     };
     static std::atomic<uint64_t> configured{0}, configured_split{0};
-    if (splits == 1) return run(gemm_quantized_tile_kernel<D, BM, BN, STAGES, PER_CU, false>, configured);
-    shared.splits = (steps + shared.steps - 1) / shared.steps;      // (none without a step)
+    if (shared.splits == 1) return run(gemm_quantized_tile_kernel<D, BM, BN, STAGES, PER_CU, Sharing::none>, configured);
+    static_assert(kAttentionArrivals >= 256);
     void* held = nullptr;
-    if (scratch_acquire(&held, static_cast<size_t>(shared.splits) * p.batches * p.M * shared.pitch * sizeof(int), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+    const size_t results = SHARING == Sharing::last_block ? static_cast<size_t>(tiles_m) * tiles_n * BM * BN : static_cast<size_t>(p.M) * shared.pitch;
+    if (SHARING == Sharing::last_block)
+        if (int status = attention_arrivals(stream, shared.arrivals)) return status;
+    if (scratch_acquire(&held, shared.splits * p.batches * results * sizeof(int), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
     shared.partials = static_cast<int*>(held);
-    int status = run(gemm_quantized_tile_kernel<D, BM, BN, STAGES, PER_CU, true>, configured_split);
-    if (status == TANNIC_SUCCESS) {
+    int status = run(gemm_quantized_tile_kernel<D, BM, BN, STAGES, PER_CU, SHARING>, configured_split);
+    if (SHARING == Sharing::second_kernel && status == TANNIC_SUCCESS) {
         const uint32_t per_row = shared.pitch / 4, items = p.M * per_row;
         hipLaunchKernelGGL((gemm_quantized_join_kernel<D>), dim3((items + 255) / 256, p.batches), dim3(256), 0, stream, static_cast<D*>(c), p, s, shared, FastDiv(per_row), items);
         status = launch_status("gemm_quantized_join_kernel");
@@ -271,41 +334,61 @@ static int launch_tiles(const GemmProblem& p, const ScalePlaces& s, uint32_t spl
     return status;
 }
 
-#ifdef TH_TILE_PROBE
-#include <cstdlib>
-#endif
+// The kernel's tiles: rows, columns, us of a step of 128 with the chip full of them, us that a block takes beside its steps, us that the last of
+// the blocks that share a tile takes for each of their parts (0: a second kernel adds them up).  Two blocks of the last three are on a compute unit at a time and share its step times as they share its LDS.  A step is bound by LDS, which takes what is loaded at 64 bytes a clock and gives fragments at 128, and for the largest by the matrix pipe under the chip's
+// power limit (256 x 256 tiles 1.4 us, 3.1 POP/s; MFMAs alone 1.3).  Measured with weights from memory: 31 products of 33 to 8000 rows, each tile and up to 16
+// splits; the fastest of those by what follows is within 7 % of the fastest found for all but a few that one Python call takes longer for than they run.
+struct Tiles8 {
+    int rows, columns;
+    double step, beside, join;
+};
+constexpr Tiles8 kTiles8[] = {{256, 256, 1.40, 15.0, 0}, {256, 192, 1.13, 12.0, 0}, {256, 128, 0.84, 6.0, 0}, {128, 128, 0.50, 4.0, 0},
+                              {128, 96, 0.47, 3.2, 0},   {64, 128, 0.38, 1.1, 0},   {64, 64, 0.235, 0.7, 0.48}, {32, 64, 0.18, 0.6, 0.37}};
+
+// us of a product: the blocks of the busiest compute unit one after another, and the weights from memory, most of the shorter one beside the longer; then the sums of blocks that share K
+static double tiles8_cost(const GemmProblem& p, const Tiles8& t, uint32_t splits) {
+    const uint64_t steps = (p.K + 127) / 128, per_block = (steps + splits - 1) / splits, parts = (steps + per_block - 1) / per_block;
+    const uint64_t tiles = (static_cast<uint64_t>(p.M) + t.rows - 1) / t.rows * ((static_cast<uint64_t>(p.N) + t.columns - 1) / t.columns) * p.batches;
+    const double rounds = static_cast<double>((tiles * parts + 255) / 256), multiplied = 3.0 + rounds * (per_block * t.step + t.beside);
+    const double loaded = 1.5 + static_cast<double>(p.N) * p.K / 5.2e6;
+    const double joined = parts == 1 ? 0.0 : t.join > 0 ? 1.0 + t.join * parts : 2.5 + 8.0 * parts * p.M * p.N * p.batches / 6e6;
+    return multiplied > loaded ? multiplied + 0.3 * loaded + joined : loaded + 0.3 * multiplied + joined;
+}
 
 template <class D>
 int gemm_quantized_tile(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
     if (!quantized_operands_fit(p, a, b) || (static_cast<uint64_t>(p.M) + 127) / 128 * ((static_cast<uint64_t>(p.N) + 127) / 128) >= kMostBlocks) return TANNIC_UNSUPPORTED_DTYPE;
+    int tile = 0;
     uint32_t splits = 1;
-    auto tiles = [&](uint64_t bm, uint64_t bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn) * p.batches; };
-    int tile = p.M > 192 && tiles(256, 256) >= 200 ? 0 : p.M > 192 && tiles(256, 128) >= 128 ? 1 : 2;
-#ifdef TH_TILE_PROBE
-    if (const char* e = getenv("TH_TILE")) tile = atoi(e);
-    if (const char* e = getenv("TH_SPLITS")) splits = atoi(e);
-#endif
+    double least = 0;
+    for (int t = 0; t < 8; ++t)
+        for (uint32_t parts : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u}) {
+            const uint64_t tiles = (static_cast<uint64_t>(p.M) + kTiles8[t].rows - 1) / kTiles8[t].rows * ((static_cast<uint64_t>(p.N) + kTiles8[t].columns - 1) / kTiles8[t].columns) * p.batches;
+            // (parts of four steps and more, of so many blocks that they are all there at once: 512, half as many tiles at most, which there are counts of arrivals for)
+            if (parts > 1 && (p.K / 128 < 4 * parts || tiles * parts > 512)) break;
+            const double cost = tiles8_cost(p, kTiles8[t], parts);
+            if ((t == 0 && parts == 1) || cost < least) {
+                least = cost;
+                tile = t;
+                splits = parts;
+            }
+        }
     switch (tile) {
         case 0: return launch_tiles<D, 256, 256, 2>(p, s, splits, a, b, c, stream);
-        case 1: return launch_tiles<D, 256, 128, 3>(p, s, splits, a, b, c, stream);
-        case 2: return launch_tiles<D, 128, 128, 4>(p, s, splits, a, b, c, stream);
-#ifdef TH_TILE_PROBE
-        case 3: return launch_tiles<D, 128, 128, 2>(p, s, splits, a, b, c, stream);
+        case 1: return launch_tiles<D, 256, 192, 2>(p, s, splits, a, b, c, stream);
+        case 2: return launch_tiles<D, 256, 128, 3>(p, s, splits, a, b, c, stream);
+        case 3: return launch_tiles<D, 128, 128, 4>(p, s, splits, a, b, c, stream);
         case 4: return launch_tiles<D, 128, 96, 5>(p, s, splits, a, b, c, stream);
-        case 5: return launch_tiles<D, 64, 128, 6>(p, s, splits, a, b, c, stream);
-        case 6: return launch_tiles<D, 64, 128, 3>(p, s, splits, a, b, c, stream);
-        case 7: return launch_tiles<D, 64, 64, 8>(p, s, splits, a, b, c, stream);
-        case 8: return launch_tiles<D, 64, 64, 5>(p, s, splits, a, b, c, stream);
-        case 9: return launch_tiles<D, 256, 192, 2>(p, s, splits, a, b, c, stream);
-        case 10: return launch_tiles<D, 32, 128, 6>(p, s, splits, a, b, c, stream);
-        case 11: return launch_tiles<D, 32, 64, 10>(p, s, splits, a, b, c, stream);
-#endif
+        case 5: return launch_tiles<D, 64, 128, 3>(p, s, splits, a, b, c, stream);
+        case 6: return launch_tiles<D, 64, 64, 5, Sharing::last_block>(p, s, splits, a, b, c, stream);
+        default: return launch_tiles<D, 32, 64, 6, Sharing::last_block>(p, s, splits, a, b, c, stream);
     }
-    return TANNIC_UNSUPPORTED_DTYPE;
 }
 
-template int gemm_quantized_tile<f16>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
-template int gemm_quantized_tile<bf16>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
-template int gemm_quantized_tile<float>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
+// This file is compiled once for each type of results (TH_TILE_TYPE).
+#ifndef TH_TILE_TYPE
+#define TH_TILE_TYPE bf16
+#endif
+template int gemm_quantized_tile<TH_TILE_TYPE>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
 
 }  // namespace th

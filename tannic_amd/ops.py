@@ -650,7 +650,7 @@ def attend(q, k, v, lengths=None, scale=None):
 # (``quantize`` of a matrix ``[out, in]``; its ``transpose()`` is the second operand of a product).  A row's largest value is 127 of its
 # scales; a row with something that is not finite has the scale NaN, and so all that is computed from it is NaN.
 def _in_8_bits(like, env):
-    return Tensor.fresh(types.int8, like.shape, env), Tensor.fresh(types.float32, like.shape[:-1], env)
+    return Tensor.fresh_together(env, (types.int8, like.shape), (types.float32, like.shape[:-1]))
 
 
 def _some_row(name, x):
@@ -679,8 +679,18 @@ def swiglu_quantized(gate, up):
 def _add_rms_norm(name, x, residual, gain, eps, integers):
     _some_row(name, x)
     env = _device_of(name, x, gain) if residual is None else _device_of(name, x, residual, gain)
-    total = x if residual is None else Tensor.fresh(x.dtype, x.shape, env)
-    normed, scales = _in_8_bits(x, env) if integers else (Tensor.fresh(x.dtype, x.shape, env), None)
+    scales, total = None, x
+    if residual is None or x.nbytes > 1 << 20:      # (a sum lives longer than its norm: a large one has memory of its own)
+        if residual is not None:
+            total = Tensor.fresh(x.dtype, x.shape, env)
+        if integers:
+            normed, scales = _in_8_bits(x, env)
+        else:
+            normed = Tensor.fresh(x.dtype, x.shape, env)
+    elif integers:
+        normed, scales, total = Tensor.fresh_together(env, (types.int8, x.shape), (types.float32, x.shape[:-1]), (x.dtype, x.shape))
+    else:
+        normed, total = Tensor.fresh_together(env, (x.dtype, x.shape), (x.dtype, x.shape))
     _checked(name, library().calls["add_rms_norm"](x.packed(), None if residual is None else residual.packed(), gain.packed(), None if residual is None else total.packed(),
                                                    normed.packed(), scales.packed() if integers else None, env.stream_number(), eps))
     return normed, scales, total

@@ -119,6 +119,7 @@ assert _TENSOR_T.size == C.sizeof(abi.tensor_t)
 _ADDRESS = struct.Struct("<Q").pack
 _IMAGES = {}      # (shape, strides, dtype, environment) -> packed tensor_t without the address
 _FRESH = {}       # (shape, dtype, environment) -> what a new contiguous tensor is made of: strides, elements, bytes, packed tensor_t behind its address
+_TOGETHER = {}    # ((dtype, shape), ..), environment -> bytes of one buffer for all of them, and every tensor's facts
 _STRIDES = {}     # shape -> (contiguous strides, number of elements); shapes recur, the table stays small
 
 
@@ -192,6 +193,34 @@ class Tensor:
         t.buffer = buffer = Buffer(nbytes, environment)
         t._packed = _ADDRESS(buffer.address) + tail
         return t
+
+    @classmethod
+    def fresh_together(cls, environment, *parts):
+        """New contiguous tensors, a ``(dtype, shape)`` each, in one buffer that lives as long as any of them: what an operator with several small results
+        allocates for them (an allocation is a third of such a call)."""
+        key = (parts, environment.key)
+        known = _TOGETHER.get(key)
+        if known is not None:
+            nbytes, facts = known
+            buffer = Buffer(nbytes, environment)
+            address, tensors = buffer.address, []
+            for dtype, shape, offset, strides, nelements, tail in facts:
+                t = cls.__new__(cls)
+                t.dtype, t.shape, t.offset, t.strides, t.nelements, t.buffer, t._contiguous, t._packed = (
+                    dtype, shape, offset, strides, nelements, buffer, True, _ADDRESS(address + offset) + tail)
+                tensors.append(t)
+            return tensors
+        tensors, at = [], 0
+        for dtype, shape in parts:
+            tensors.append(cls(dtype, shape, offset=at))
+            at += -(-tensors[-1].nbytes // 256) * 256
+        buffer = Buffer(at, environment)
+        for t in tensors:
+            t.buffer = buffer
+        if len(_TOGETHER) > 4096:
+            _TOGETHER.clear()
+        _TOGETHER[key] = at, [(t.dtype, t.shape, t.offset, t.strides, t.nelements, t._image()[8:]) for t in tensors]
+        return tensors
 
     def is_singleton(self):
         return self.nelements == 1
