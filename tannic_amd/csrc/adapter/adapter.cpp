@@ -148,6 +148,17 @@ status copy_pages(tensor_t* pool, stream_t s, const int32_t* sources, const int3
 status attend(const tensor_t* q, const tensor_t* k, const tensor_t* v, const tensor_t* lengths, tensor_t* d, stream_t s, float scale) {
     return code(tannic_hip_attend(in(q), in(k), in(v), in(lengths), out(d), st(s), scale));
 }
+status quantize(const tensor_t* x, tensor_t* values, tensor_t* scales, stream_t s) { return code(tannic_hip_quantize(in(x), out(values), out(scales), st(s))); }
+status swiglu_quantize(const tensor_t* gate, const tensor_t* up, tensor_t* values, tensor_t* scales, stream_t s) {
+    return code(tannic_hip_swiglu_quantize(in(gate), in(up), out(values), out(scales), st(s)));
+}
+status add_rms_norm(const tensor_t* x, const tensor_t* residual, const tensor_t* gain, tensor_t* total, tensor_t* normed, tensor_t* scales, stream_t s, float eps) {
+    return code(tannic_hip_add_rms_norm(in(x), in(residual), in(gain), out(total), out(normed), out(scales), st(s), eps));
+}
+status dequantize(const tensor_t* values, const tensor_t* scales, tensor_t* d, stream_t s) { return code(tannic_hip_dequantize(in(values), in(scales), out(d), st(s))); }
+status gemm_quantized(const tensor_t* a, const tensor_t* a_scales, const tensor_t* b, const tensor_t* b_scales, tensor_t* d, stream_t s) {
+    return code(tannic_hip_gemm_quantized(in(a), in(a_scales), in(b), in(b_scales), out(d), st(s)));
+}
 
 Recording::Recording(int device) {
     tannic_device_t dvc{};

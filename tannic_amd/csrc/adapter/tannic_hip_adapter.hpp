@@ -138,6 +138,12 @@ status attend_pages(const tensor_t* q, const tensor_t* keys, const tensor_t* val
                     float scale);
 status copy_pages(tensor_t* pool, stream_t, const int32_t* sources, const int32_t* targets, size_t count);
 status attend(const tensor_t* q, const tensor_t* k, const tensor_t* v, const tensor_t* lengths_or_null, tensor_t*, stream_t, float scale);
+// rows in 8-bit integers with a scale each, and their product (tannic_hip_quantize, ...)
+status quantize(const tensor_t* x, tensor_t* values, tensor_t* scales, stream_t);
+status swiglu_quantize(const tensor_t* gate, const tensor_t* up, tensor_t* values, tensor_t* scales, stream_t);
+status add_rms_norm(const tensor_t* x, const tensor_t* residual_or_null, const tensor_t* gain, tensor_t* total_or_null, tensor_t* normed, tensor_t* scales_or_null, stream_t, float eps);
+status dequantize(const tensor_t* values, const tensor_t* scales, tensor_t*, stream_t);
+status gemm_quantized(const tensor_t* a, const tensor_t* a_scales, const tensor_t* b, const tensor_t* b_scales, tensor_t*, stream_t);
 
 // A sequence of the front end's evaluations on one device recorded once and replayed as one HIP graph
 // (tannic_hip_graph_begin / end / launch / destroy):

@@ -1,5 +1,5 @@
 // Expression nodes for the operators this backend adds to Tannic's surface: division, dtype conversion, value max / min
-// over an axis, the one-pass row operators (softmax, rms_norm, swiglu, rope), and attention over a cache in pages.  Include it after the front end's headers in
+// over an axis, the one-pass row operators (softmax, rms_norm, swiglu, rope), attention over a cache in pages, and rows in 8-bit integers with their product.  Include it after the front end's headers in
 // a program that links the `cuda::` adapter; the nodes compose with every other expression:
 //
 //     Tensor y = rms_norm(x, gain, 1e-5f) * 2.0f;
@@ -15,6 +15,7 @@
 
 #include <cstdint>
 #include <initializer_list>
+#include <utility>
 #include <variant>
 #include <vector>
 
@@ -177,6 +178,78 @@ struct PagedAttention {      // over the pages of a cache
     }
 };
 
+struct Dequantization {
+    type to;
+    constexpr type result(type) const { return to; }
+    void forward(Tensor const& values, Tensor const& scales, Tensor& target) const {
+        on_device({&values, &scales}, target, "dequantize", [&](stream_t s) { return tannic_hip::dequantize(get_tensor(values.id()), get_tensor(scales.id()), get_tensor(target.id()), s); });
+    }
+};
+
+// (sum_k a b) * a_scales * b_scales of a [.., M, K] and b [.., K, N], whole numbers of 8 bits, with a scale for each row and each column, in the type `dtype`
+struct ScaledProduct {
+    type dtype;
+    void forward(Tensor const& a, Tensor const& a_scales, Tensor const& b, Tensor const& b_scales, Tensor& target) const {
+        on_device({&a, &a_scales, &b, &b_scales}, target, "matmul_quantized", [&](stream_t s) {
+            return tannic_hip::gemm_quantized(get_tensor(a.id()), get_tensor(a_scales.id()), get_tensor(b.id()), get_tensor(b_scales.id()), get_tensor(target.id()), s);
+        });
+    }
+    static Shape shape(Shape const& a, Shape const& b) {
+        if (a.rank() < 2 || b.rank() < 2) throw Exception("Inputs must have rank >= 2");
+        if (a[a.rank() - 1] != b[b.rank() - 2]) throw Exception("Inner dimensions must match for matmul");
+        const auto batches = [](Shape const& of) {
+            Shape out;
+            for (size_t dim = 0; dim + 2 < of.rank(); ++dim) out.expand(of[dim]);
+            return out;
+        };
+        Shape out = b.rank() == 2 ? batches(a) : a.rank() == 2 ? batches(b) : operation::broadcast(batches(a), batches(b));
+        out.expand(a[a.rank() - 2]);
+        out.expand(b[b.rank() - 1]);
+        return out;
+    }
+};
+
+template <Composable... Operands>
+class ScaledMultiplication : public expression::Expression<ScaledProduct, Operands...> {
+public:
+    constexpr ScaledMultiplication(ScaledProduct product, typename Trait<Operands>::Reference... operands)
+    :   expression::Expression<ScaledProduct, Operands...>(product, operands...)
+    ,   shape_(ScaledProduct::shape(std::get<0>(this->operands).shape(), std::get<2>(this->operands).shape()))
+    ,   strides_(shape_) {}
+
+    constexpr type dtype() const { return this->operation.dtype; }
+    constexpr Shape const& shape() const { return shape_; }
+    constexpr Strides const& strides() const { return strides_; }
+    std::ptrdiff_t offset() const { return 0; }
+
+    Tensor forward(Context const& context) const {
+        Tensor target(dtype(), shape_);
+        std::apply([&](auto const&... operand) { this->operation.forward(Tensor(operand.forward(context))..., target); }, this->operands);
+        return target;
+    }
+
+private:
+    Shape shape_;
+    Strides strides_;
+};
+
+// Rows in 8-bit integers, and what a 1 in each stands for: values [.., L], scales [..].
+struct Quantized {
+    Tensor values, scales;
+
+    // for the rows of a tensor of this shape on its device
+    explicit Quantized(Tensor const& like) : values(static_cast<type>(TANNIC_INT8), like.shape()), scales(static_cast<type>(TANNIC_FLOAT32), rows(like.shape())) {
+        values.initialize(like.environment());
+        scales.initialize(like.environment());
+    }
+    static Shape rows(Shape const& shape) {
+        if (shape.rank() == 0) throw Exception("operands have rank >= 1");
+        Shape out;
+        for (size_t dim = 0; dim + 1 < shape.rank(); ++dim) out.expand(shape[dim]);
+        return out;
+    }
+};
+
 }  // namespace tannic::hip
 
 namespace tannic {
@@ -267,6 +340,60 @@ inline Tensor append_pages(Tensor const& k, Tensor const& v, Tensor& keys, Tenso
                                         get_tensor(sines.id()), get_tensor(q.id()), get_tensor(keys.id()), get_tensor(values.id()), get_tensor(turned.id()), s);
     });
     return turned;
+}
+
+// Rows in 8-bit integers with a scale each (include/tannic_hip.h), what has several results evaluated where it is called: the rows of x,
+inline hip::Quantized quantize(Tensor const& x) {
+    hip::Quantized q(x);
+    hip::on_device({&x}, q.values, "quantize", [&](stream_t s) { return tannic_hip::quantize(get_tensor(x.id()), get_tensor(q.values.id()), get_tensor(q.scales.id()), s); });
+    return q;
+}
+// of gate / (1 + exp(-gate)) * up,
+inline hip::Quantized swiglu_quantized(Tensor const& gate, Tensor const& up) {
+    hip::Quantized q(gate);
+    hip::on_device({&gate, &up}, q.values, "swiglu_quantized", [&](stream_t s) {
+        return tannic_hip::swiglu_quantize(get_tensor(gate.id()), get_tensor(up.id()), get_tensor(q.values.id()), get_tensor(q.scales.id()), s);
+    });
+    return q;
+}
+// of x / sqrt(mean(x^2) + epsilon) * gain;
+inline hip::Quantized rms_norm_quantized(Tensor const& x, Tensor const& gain, float epsilon) {
+    hip::Quantized q(x);
+    hip::on_device({&x, &gain}, q.values, "rms_norm_quantized", [&](stream_t s) {
+        return tannic_hip::add_rms_norm(get_tensor(x.id()), nullptr, get_tensor(gain.id()), nullptr, get_tensor(q.values.id()), get_tensor(q.scales.id()), s, epsilon);
+    });
+    return q;
+}
+// the norm of x + residual, and that sum; the same in 8 bits
+inline std::pair<Tensor, Tensor> add_rms_norm(Tensor const& x, Tensor const& residual, Tensor const& gain, float epsilon) {
+    Tensor normed(x.dtype(), x.shape()), total(x.dtype(), x.shape());
+    total.initialize(x.environment());
+    hip::on_device({&x, &residual, &gain}, normed, "add_rms_norm", [&](stream_t s) {
+        return tannic_hip::add_rms_norm(get_tensor(x.id()), get_tensor(residual.id()), get_tensor(gain.id()), get_tensor(total.id()), get_tensor(normed.id()), nullptr, s, epsilon);
+    });
+    return {normed, total};
+}
+inline std::pair<hip::Quantized, Tensor> add_rms_norm_quantized(Tensor const& x, Tensor const& residual, Tensor const& gain, float epsilon) {
+    hip::Quantized q(x);
+    Tensor total(x.dtype(), x.shape());
+    total.initialize(x.environment());
+    hip::on_device({&x, &residual, &gain}, q.values, "add_rms_norm_quantized", [&](stream_t s) {
+        return tannic_hip::add_rms_norm(get_tensor(x.id()), get_tensor(residual.id()), get_tensor(gain.id()), get_tensor(total.id()), get_tensor(q.values.id()), get_tensor(q.scales.id()),
+                                        s, epsilon);
+    });
+    return {q, total};
+}
+
+// values * scales of every row, in another type
+template <Composable Values, Composable Scales>
+constexpr auto dequantize(Values&& values, Scales&& scales, type dtype) {
+    return hip::Rowwise<hip::Dequantization, Values, Scales>{{dtype}, std::forward<Values>(values), std::forward<Scales>(scales)};
+}
+
+// (sum_k a[m, k] b[k, n]) * a_scales[m] * b_scales[n]: tokens in 8 bits times weights in 8 bits (a matrix [out, in] of `quantize`, transposed), in the type `dtype`
+template <Composable A, Composable AScales, Composable B, Composable BScales>
+constexpr auto matmul_quantized(A&& a, AScales&& a_scales, B&& b, BScales&& b_scales, type dtype) {
+    return hip::ScaledMultiplication<A, AScales, B, BScales>{{dtype}, std::forward<A>(a), std::forward<AScales>(a_scales), std::forward<B>(b), std::forward<BScales>(b_scales)};
 }
 
 // page sources[i] of pool [.., pages, kv heads, page, d] over page targets[i], one after another
