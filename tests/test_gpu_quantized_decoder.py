@@ -187,7 +187,7 @@ def test_two_streams_at_once(device):
         for stream in streams:
             assert lib.stream_synchronize(stream) == 0
     finally:
-        for stream in streams:
+        for stream in reversed(streams):      # (the pool hands out the last one: the device's has to be it again)
             lib.put_stream(C.byref(dvc), stream)
     for _, results, want in made:
         for into in results:
