@@ -202,19 +202,22 @@ def test_two_threads(device):
     sw = ta.tensor(np.full(90, 0.01), ta.float32, device)
     d = ta.tensor(x, ta.float32, device)
     want = ops.matmul_quantized(*ops.quantize(d), w, sw, ta.float32).numpy()
-    wrong = []
+    results = [[], []]
 
-    def work():
+    def work(mine):
         for _ in range(30):
-            if not np.array_equal(ops.matmul_quantized(*ops.quantize(d), w, sw, ta.float32).numpy(), want):
-                wrong.append(True)
+            mine.append(ops.matmul_quantized(*ops.quantize(d), w, sw, ta.float32))
 
-    threads = [threading.Thread(target=work) for _ in range(2)]
+    threads = [threading.Thread(target=work, args=(mine,)) for mine in results]
     for t in threads:
         t.start()
     for t in threads:
         t.join()
-    assert not wrong
+    # (read by one thread: copies to the host take streams from the pool, which hands two threads two of them)
+    for mine in results:
+        assert len(mine) == 30
+        for got in mine:
+            np.testing.assert_array_equal(got.numpy(), want)
 
 
 def test_results_that_share_an_allocation(device):
