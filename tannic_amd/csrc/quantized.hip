@@ -54,10 +54,12 @@ template <class T> struct Piece {
 };
 
 // `live` elements of a piece (the last one of a row may be short), zeros behind them
-template <class T> __device__ inline Piece<T> load_piece(const T* from, uint32_t live) {
+template <class T, bool PAST = false> __device__ inline Piece<T> load_piece(const T* from, uint32_t live) {
     Piece<T> r;
     if (live >= kPiece<T>) {
-        const uint4any bits = *reinterpret_cast<const uint4any*>(from);
+        uint4any bits;
+        if constexpr (PAST) bits = __builtin_nontemporal_load(reinterpret_cast<const uint4any*>(from));
+        else bits = *reinterpret_cast<const uint4any*>(from);
         __builtin_memcpy(&r, &bits, 16);
     } else {
 #pragma unroll
@@ -65,28 +67,25 @@ template <class T> __device__ inline Piece<T> load_piece(const T* from, uint32_t
     }
     return r;
 }
-template <class T> __device__ inline void store_piece(T* to, const Piece<T>& piece, uint32_t live) {
+template <class T, bool PAST = false> __device__ inline void store_piece(T* to, const Piece<T>& piece, uint32_t live) {
     if (live >= kPiece<T>) {
         uint4any bits;
         __builtin_memcpy(&bits, &piece, 16);
-        *reinterpret_cast<uint4any*>(to) = bits;
+        if constexpr (PAST) __builtin_nontemporal_store(bits, reinterpret_cast<uint4any*>(to));
+        else *reinterpret_cast<uint4any*>(to) = bits;
     } else {
 #pragma unroll
         for (int e = 0; e < kPiece<T>; ++e)
             if (e < static_cast<int>(live)) to[e] = piece.v[e];
     }
 }
-template <int N> __device__ inline void store_integers(int8_t* to, const int8_t (&v)[N], uint32_t live) {
+template <bool PAST, int N> __device__ inline void store_integers(int8_t* to, const int8_t (&v)[N], uint32_t live) {
     if (live >= N) {
-        if constexpr (N == 8) {
-            uint2any bits;
-            __builtin_memcpy(&bits, v, 8);
-            *reinterpret_cast<uint2any*>(to) = bits;
-        } else {
-            unsigned int bits;
-            __builtin_memcpy(&bits, v, 4);
-            *reinterpret_cast<uint1any*>(to) = bits;
-        }
+        using Any = std::conditional_t<N == 8, uint2any, uint1any>;
+        Any bits;
+        __builtin_memcpy(&bits, v, N);
+        if constexpr (PAST) __builtin_nontemporal_store(bits, reinterpret_cast<Any*>(to));
+        else *reinterpret_cast<Any*>(to) = bits;
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
@@ -94,11 +93,16 @@ template <int N> __device__ inline void store_integers(int8_t* to, const int8_t 
     }
 }
 
-// A group of G threads (a wavefront, or a block) per row, which is read once and kept in registers as u, NCH pieces of 16 bytes of a thread.
-template <class T, RowSource S, bool INTEGERS, int G, int NCH>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void rows_kernel(RowOperands p) {
+// A group of G threads (a wavefront, or a block) per row, which is read once and kept in registers as u, NCH pieces of 16 bytes of a thread.  Bound by memory: 8001 x 5120 fp16
+// with sum and residual 5.6 TB/s, 4096 x 14336 bf16 gated 5.6 TB/s (its arithmetic takes nearly as long), 28672 x 4096 fp16 6.4 TB/s.
+// Wavefronts on a SIMD that the registers have to leave room for: three blocks of 512 on a compute unit where one register too many (81, fp16) would make them two (8001 x 5120 with sum and
+// residual 59 / 50 us).  No such limit for the others: with three or four pieces they would spill.
+template <RowSource S, int G, int NCH> constexpr int kRowWavefronts = (S == RowSource::norm || S == RowSource::sum_norm) && G == 512 && NCH == 2 ? 6 : 1;
+
+template <class T, RowSource S, bool INTEGERS, int G, int NCH, bool PAST>
+__global__ __launch_bounds__(G == 64 ? 256 : G, (kRowWavefronts<S, G, NCH>)) void rows_kernel(RowOperands p) {
     constexpr bool NORM = S == RowSource::norm || S == RowSource::sum_norm;
-    constexpr int VEC = kPiece<T>, BLOCK = G < 256 ? 256 : G, WAVES = BLOCK / 64;
+    constexpr int VEC = kPiece<T>, BLOCK = G == 64 ? 256 : G, WAVES = BLOCK / 64;
     __shared__ float sums[WAVES];
     __shared__ uint32_t largest[WAVES];
     const uint32_t t = threadIdx.x % G;
@@ -112,8 +116,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_kernel(RowOperands p) 
         for (int i = 0; i < NCH; ++i) {
             const uint32_t at = (t + i * G) * VEC;
             if (at < p.length) {
-                a[i] = load_piece(x + at, p.length - at);
-                if constexpr (S == RowSource::gated || S == RowSource::sum_norm) b[i] = load_piece(second + at, p.length - at);
+                a[i] = load_piece<T, PAST>(x + at, p.length - at);
+                if constexpr (S == RowSource::gated || S == RowSource::sum_norm) b[i] = load_piece<T, PAST>(second + at, p.length - at);
                 if constexpr (NORM) g[i] = load_piece(gain + at, p.length - at);
             }
         }
@@ -166,7 +170,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_kernel(RowOperands p) 
                     int8_t out[VEC];
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) out[e] = scale.integer(u[i][e]);
-                    store_integers(static_cast<int8_t*>(p.dst) + base + at, out, p.length - at);
+                    store_integers<PAST>(static_cast<int8_t*>(p.dst) + base + at, out, p.length - at);
                 } else {
                     Piece<T> out;
 #pragma unroll
@@ -226,7 +230,7 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowOperands p) {
 }
 
 // Eight elements of a row per thread.
-template <class T>
+template <class T, bool PAST>
 __global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* values, RowsMap map, const float* scales, T* dst, uint32_t length, FastDiv per_row, uint32_t items) {
     const uint32_t item = blockIdx.x * 256 + threadIdx.x;
     if (item >= items) return;
@@ -250,7 +254,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* values, R
         Piece<T> out;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) out.v[e] = rounded<T>(static_cast<float>(v[i + e]) * scale);
-        if (static_cast<int>(live) > i) store_piece(to + i, out, live - i);
+        if (static_cast<int>(live) > i) store_piece<T, PAST>(to + i, out, live - i);
     }
 }
 
@@ -265,11 +269,22 @@ __global__ __launch_bounds__(256) void dequantize_any_kernel(const int8_t* value
 
 constexpr uint32_t kMostRowBlocks = 1u << 20;      // (rows beyond in turns)
 
+// What does not fit the memory-side cache of 256 MB with its results goes past the caches: a matrix of weights from 128 MB on (28672 x 4096 fp16 with 235 MB 55 us past them, 61 through
+// them; 8000 x 4096 bf16 with its sum and residual 39 and 36, so that the other sources, whose results a product takes next, stay with them).
+constexpr uint64_t kRowsPastCaches = 128ull << 20;
+
 template <class T, RowSource S, bool INTEGERS, int G, int NCH>
 int launch_rows(const RowOperands& p, hipStream_t stream) {
-    constexpr uint32_t BLOCK = G < 256 ? 256 : G, ROWS = BLOCK / G;
+    constexpr uint32_t BLOCK = G == 64 ? 256 : G, ROWS = BLOCK / G;
     const uint32_t blocks = (p.rows + ROWS - 1) / ROWS;
-    hipLaunchKernelGGL((rows_kernel<T, S, INTEGERS, G, NCH>), dim3(blocks < kMostRowBlocks ? blocks : kMostRowBlocks), dim3(BLOCK), 0, stream, p);
+    const dim3 grid(blocks < kMostRowBlocks ? blocks : kMostRowBlocks);
+    if constexpr (S == RowSource::plain) {
+        if (static_cast<uint64_t>(p.rows) * p.length * sizeof(T) > kRowsPastCaches) {
+            hipLaunchKernelGGL((rows_kernel<T, S, INTEGERS, G, NCH, true>), grid, dim3(BLOCK), 0, stream, p);
+            return launch_status("rows_kernel");
+        }
+    }
+    hipLaunchKernelGGL((rows_kernel<T, S, INTEGERS, G, NCH, false>), grid, dim3(BLOCK), 0, stream, p);
     return launch_status("rows_kernel");
 }
 
@@ -277,16 +292,30 @@ template <class T, RowSource S, bool INTEGERS>
 int run_rows(const RowOperands& p, hipStream_t stream) {
     if constexpr (!std::is_same_v<T, double>) {
         // rows whose elements lie one after the other and that the registers of a block hold
-        constexpr bool PAIR = S == RowSource::gated || S == RowSource::sum_norm;
+        constexpr bool PAIR = S == RowSource::gated || S == RowSource::sum_norm, PLAIN = S == RowSource::plain, NORM = S == RowSource::norm || S == RowSource::sum_norm;
         const uint32_t pieces = (p.length + kPiece<T> - 1) / kPiece<T>;
         if (p.length > 0 && (p.length == 1 || (p.rows_x.step == 1 && (!PAIR || p.rows_second.step == 1))) && pieces <= 4096) {
+            // Threads of a row and their pieces, us of a norm with its sum / of values / gated, bf16, operands from memory, in brackets what is nearest: 32768 rows of 128 pieces 64 x 2
+            // 37 / 17 / 27 (128 x 1 36 / 19 / 25); 16384 of 256 256 x 1 36 / - / 26, 128 x 2 - / 17 / - (64 x 4 39 / 17 / 29); 8192 of 512 512 x 1 39 / - / 29, 256 x 2 - / 17 / - (the other
+            // way round 42 / 18 / 31); 8001 of 640 512 x 2 50 / - / -, 256 x 3 - / 21 / 38 (256 x 4 59 / 22 / 40); 4096 of 1024 512 x 2 43 / 18 / 31 (256 x 4 50 / 17 / 34); 4096 of 1536
+            // 512 x 3 67 / 24 / 39 (1024 x 2 74 / 33 / 52); 4096 of 1792 1024 x 2 84 / - / -, 512 x 4 - / 34 / 57 (the other way round 97 / 47 / 68); 2000 of 3584 1024 x 4 94 / 31 / 67.
             if (pieces <= 64) return launch_rows<T, S, INTEGERS, 64, 1>(p, stream);
             if (pieces <= 128 && p.rows >= 1024) return launch_rows<T, S, INTEGERS, 64, 2>(p, stream);
-            if (pieces <= 256 && p.rows >= 1024) return launch_rows<T, S, INTEGERS, 64, 4>(p, stream);
+            if constexpr (PLAIN) {
+                if (pieces > 128 && pieces <= 256 && p.rows >= 1024) return launch_rows<T, S, INTEGERS, 128, 2>(p, stream);
+            }
             if (pieces <= 256) return launch_rows<T, S, INTEGERS, 256, 1>(p, stream);
-            if (pieces <= 512) return launch_rows<T, S, INTEGERS, 256, 2>(p, stream);
-            if (pieces <= 1024) return launch_rows<T, S, INTEGERS, 256, 4>(p, stream);
-            if (pieces <= 2048) return launch_rows<T, S, INTEGERS, 1024, 2>(p, stream);
+            if (pieces <= 512) return launch_rows<T, S, INTEGERS, PLAIN ? 256 : 512, PLAIN ? 2 : 1>(p, stream);
+            if constexpr (!NORM) {
+                if (pieces <= 768) return launch_rows<T, S, INTEGERS, 256, 3>(p, stream);
+            }
+            if (pieces <= 1024) return launch_rows<T, S, INTEGERS, 512, 2>(p, stream);
+            if (pieces <= 1536) return launch_rows<T, S, INTEGERS, 512, 3>(p, stream);
+            if constexpr (NORM) {
+                if (pieces <= 2048) return launch_rows<T, S, INTEGERS, 1024, 2>(p, stream);
+            } else {
+                if (pieces <= 2048) return launch_rows<T, S, INTEGERS, 512, 4>(p, stream);
+            }
             return launch_rows<T, S, INTEGERS, 1024, 4>(p, stream);
         }
     }
@@ -403,9 +432,12 @@ int tannic_hip_dequantize(const tannic_tensor_t* values, const tannic_tensor_t* 
         using T = typename decltype(tag)::type;
         const uint64_t per_row = (static_cast<uint64_t>(p.length) + 7) / 8, items = per_row * p.rows;
         if ((p.length == 1 || p.rows_x.step == 1) && items < (1ull << 31)) {
-            hipLaunchKernelGGL((dequantize_kernel<T>), dim3(static_cast<uint32_t>((items + 255) / 256)), dim3(256), 0, as_stream(stream), static_cast<const int8_t*>(values->address),
-                               p.rows_x, static_cast<const float*>(scales->address), static_cast<T*>(dst->address), p.length, FastDiv(static_cast<uint32_t>(per_row)),
-                               static_cast<uint32_t>(items));
+            const auto launch = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((items + 255) / 256)), dim3(256), 0, as_stream(stream), static_cast<const int8_t*>(values->address), p.rows_x,
+                                   static_cast<const float*>(scales->address), static_cast<T*>(dst->address), p.length, FastDiv(static_cast<uint32_t>(per_row)), static_cast<uint32_t>(items));
+            };
+            if (static_cast<uint64_t>(p.rows) * p.length * sizeof(T) > kRowsPastCaches) launch(dequantize_kernel<T, true>);
+            else launch(dequantize_kernel<T, false>);
             return launch_status("dequantize_kernel");
         }
         hipLaunchKernelGGL((dequantize_any_kernel<T>), dim3(p.rows < kMostRowBlocks ? p.rows : kMostRowBlocks), dim3(256), 0, as_stream(stream),
