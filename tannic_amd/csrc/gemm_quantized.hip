@@ -94,6 +94,10 @@ void fold_batches(GemmProblem& p, ScalePlaces& s) {
 
 template <class D>
 int run_quantized(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
+    if (!quantized_operands_fit(p, a, b)) {
+        const int status = gemm_quantized_bytes<D>(p, s, a, b, c, stream);
+        if (status != TANNIC_UNSUPPORTED_DTYPE) return status;
+    }
     // operands that do not lie along K, or not in whole pieces, are copied first where that pays
     GemmProblem q = p;
     const void *pa = a, *pb = b;

@@ -74,5 +74,7 @@ __device__ inline uint32_t bytes_of_rows(uint32_t rows, int64_t pitch, uint32_t 
 // Up to 32 rows (gemm_quantized_rows.hip) and more (gemm_quantized_tile.hip); TANNIC_UNSUPPORTED_DTYPE: not this kernel's
 template <class D> int gemm_quantized_rows(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream);
 template <class D> int gemm_quantized_tile(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream);
+// rows along K that start anywhere and have any length
+template <class D> int gemm_quantized_bytes(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream);
 
 }  // namespace th

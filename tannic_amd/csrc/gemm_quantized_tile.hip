@@ -35,6 +35,46 @@ __device__ inline int4v load_through(const int* at) {
     return v;
 }
 
+// Leaves a block's sums for the others of its tile; true for the last of them, whose sums are all parts' then.
+template <int TM, int TN>
+__device__ inline bool add_parts(int4v (&acc)[TM][TN], const SharedK& shared, uint32_t split, uint32_t tile, unsigned char* lds) {
+    int* const parts = shared.partials + (static_cast<size_t>(tile) * shared.splits * (TM * TN) * 256 + threadIdx.x) * 4;
+    const auto of = [&](uint32_t part, int at) { return parts + (static_cast<size_t>(part) * (TM * TN) + at) * 1024; };
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) store_through(of(split, i * TN + j), acc[i][j]);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (they have arrived)
+    __syncthreads();
+    uint32_t* const before = reinterpret_cast<uint32_t*>(lds);
+    if (threadIdx.x == 0) {
+        *before = __hip_atomic_fetch_add(shared.arrivals + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (*before == shared.splits - 1) __hip_atomic_store(shared.arrivals + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (*before != shared.splits - 1) return false;
+    __syncthreads();      // (its place in LDS is used again)
+    // the other parts, four on their way at a time (where there are not four, its own in their place, times 0)
+    for (uint32_t from = 0; from < shared.splits; from += 4) {
+        int4v got[4][TM][TN];
+#pragma unroll
+        for (uint32_t n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) got[n][i][j] = load_through(of(from + n < shared.splits ? from + n : split, i * TN + j));
+#pragma unroll
+        for (uint32_t n = 0; n < 4; ++n) {
+            const int counts = from + n < shared.splits && from + n != split;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] += got[n][i][j] * counts;
+        }
+    }
+    return true;
+}
+
 // A wavefront's TM x TN sums of 16 x 16 from row `row0` and column `col0` on: as they are, into its share of the partial sums.
 template <int TM, int TN>
 __device__ inline void leave_sums(const int4v (&acc)[TM][TN], const GemmProblem& p, const SharedK& shared, uint32_t split, uint32_t row0, uint32_t col0) {
@@ -236,45 +276,113 @@ __global__ __launch_bounds__(256, PER_CU) void gemm_quantized_tile_kernel(const 
         for (int j = 0; j < TN; ++j) acc[i][j] = mfma_i8(fb[1][j], fa[1][i], acc[i][j]);
 
     if constexpr (SHARING == Sharing::last_block) {
-        const uint32_t tile = blockIdx.y * tiles_m * tiles_n + blockIdx.x / shared.splits;
-        int* const parts = shared.partials + (static_cast<size_t>(tile) * shared.splits * (TM * TN) * 256 + threadIdx.x) * 4;
-        const auto of = [&](uint32_t part, int at) { return parts + (static_cast<size_t>(part) * (TM * TN) + at) * 1024; };
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) store_through(of(split, i * TN + j), acc[i][j]);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (they have arrived)
-        __syncthreads();
-        uint32_t* const before = reinterpret_cast<uint32_t*>(lds);
-        if (threadIdx.x == 0) {
-            *before = __hip_atomic_fetch_add(shared.arrivals + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (*before == shared.splits - 1) __hip_atomic_store(shared.arrivals + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (*before != shared.splits - 1) return;
-        __syncthreads();      // (its place in LDS is used again)
-        // the other parts, four on their way at a time (its own once more, and the last once more than once, where there are not four; times 0)
-        for (uint32_t from = 0; from < shared.splits; from += 4) {
-            int4v got[4][TM][TN];
-#pragma unroll
-            for (uint32_t n = 0; n < 4; ++n)
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) got[n][i][j] = load_through(of(from + n < shared.splits ? from + n : split, i * TN + j));
-#pragma unroll
-            for (uint32_t n = 0; n < 4; ++n) {
-                const int counts = from + n < shared.splits && from + n != split;
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] += got[n][i][j] * counts;
-            }
-        }
+        if (!add_parts<TM, TN>(acc, shared, split, blockIdx.y * tiles_m * tiles_n + blockIdx.x / shared.splits, lds)) return;
     }
     if constexpr (SHARING == Sharing::second_kernel) leave_sums<TM, TN>(acc, p, shared, split, m0 + wm, n0 + wn);
     else write_scaled<D, TM, TN>(acc, reinterpret_cast<D*>(lds) + wave * (WM * (WN + 8)), C + oc, p, s, m0 + wm, n0 + wn);
 #endif
+}
+
+// Rows along K that start anywhere and have any length from 16 on: tiles of BM x 64 on the same 2 x 2 wavefronts, whose pieces go through registers, up to three steps ahead of the products; LDS
+// holds two steps.  The last piece of a row that is not whole pieces is its last 16 bytes, of which A's have zeros for those that the piece before has: a whole number of
+// products is left out by zeros of one operand, whatever the other holds.  Bound by its loads and writes to LDS, and by the latency of a step where blocks are few; what it saves is copying both
+// operands into aligned rows (us with the copies / so: 77 x 2049 x 1030
+// 11.7 / 7.1, 1 x 28672 x 4095 60.6 / 31.2, 64 x 4096 x 4095 21.5 / 14.0; 2048 x 4096 x 4095 53 / 117, which are copied).
+template <class D, int BM, Sharing SHARING>
+__global__ __launch_bounds__(256, 2) void gemm_quantized_bytes_kernel(const int8_t* A, const int8_t* B, D* C, GemmProblem p, ScalePlaces s, uint32_t tiles_m, uint32_t tiles_n, SharedK shared) {
+    constexpr bool SPLIT = SHARING != Sharing::none;
+    constexpr int BN = 64, WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16, LOADS_A = BM / 32, LOADS = LOADS_A + BN / 32;
+    constexpr uint32_t A_TILE = BM * 128, STAGE = A_TILE + BN * 128, OUT = sizeof(D) == 2 ? 2 * 4 * WM * (WN + 8) : 0;
+    __shared__ __align__(16) unsigned char lds[2 * STAGE > OUT ? 2 * STAGE : OUT];
+    uint32_t tm, tn;
+    const uint32_t split = SPLIT ? blockIdx.x % shared.splits : 0;
+    tile_of<true>(SPLIT ? blockIdx.x / shared.splits : blockIdx.x, tiles_m, tiles_n, tm, tn);
+    int64_t oa, ob, oc;
+    batch_offsets(p, blockIdx.y, oa, ob, oc);
+    const uint32_t m0 = tm * BM, n0 = tn * BN;
+    const uint32_t all = (p.K + 127) / 128, first = SPLIT ? split * shared.steps : 0;
+    const uint32_t steps = SPLIT ? (all - first < shared.steps ? all - first : shared.steps) : all;
+    const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const uint32_t wm = wave / 2 * WM, wn = wave % 2 * WN, frag_row = lane % 16, frag_piece = lane / 16;
+    // load j: piece threadIdx.x % 8 of rows 32 j + threadIdx.x / 8 of A's tile, then of B's
+    const uint32_t piece = threadIdx.x % 8, row = threadIdx.x / 8;
+    const int8_t* from[LOADS];
+    bool there[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+        const uint32_t r = (j < LOADS_A ? m0 + j * 32 : n0 + (j - LOADS_A) * 32) + row;
+        there[j] = r < (j < LOADS_A ? p.M : p.N);
+        from[j] = j < LOADS_A ? A + oa + static_cast<int64_t>(there[j] ? r : 0) * p.a_rs : B + ob + static_cast<int64_t>(there[j] ? r : 0) * p.b_cs;
+    }
+    typedef unsigned int uint4any __attribute__((ext_vector_type(4), aligned(1)));
+    uint4v held[2][LOADS];
+    const auto load = [&](uint32_t step, auto set_tag) {
+        constexpr int set = decltype(set_tag)::value;
+        const uint32_t want = (first + step) * 128 + piece * 16;
+        const uint32_t k = want + 16 <= p.K ? want : p.K - 16, twice = want < p.K ? want - k : 16;      // bytes that the piece before has
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            held[set][j] = uint4v{0, 0, 0, 0};
+            if (there[j] && want < p.K) {
+                const uint4any bits = *reinterpret_cast<const uint4any*>(from[j] + k);
+                held[set][j] = uint4v{bits[0], bits[1], bits[2], bits[3]};
+            }
+            if (j < LOADS_A && twice != 0) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const uint32_t zeros = twice <= 4 * e ? 0u : twice - 4 * e >= 4 ? 4u : twice - 4 * e;      // of the word's bytes
+                    held[set][j][e] = zeros == 4 ? 0u : held[set][j][e] >> (8 * zeros) << (8 * zeros);
+                }
+            }
+        }
+    };
+    const auto keep = [&](auto set_tag) {      // a set's step goes to the stage of its number
+        constexpr int set = decltype(set_tag)::value;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const uint32_t r = (j < LOADS_A ? j : j - LOADS_A) * 32 + row;
+            *reinterpret_cast<uint4v*>(lds + set * STAGE + (j < LOADS_A ? 0 : A_TILE) + tile_offset<int8_t>(r, piece)) = held[set][j];
+        }
+    };
+    int4v acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = int4v{0, 0, 0, 0};
+    using Even = std::integral_constant<int, 0>;
+    using Odd = std::integral_constant<int, 1>;
+    // step `at` from the stage of its number, the next one's operands into the other, those of the third behind it on their way
+    const auto step = [&](uint32_t at, auto here, auto next) {
+        const unsigned char* const stage = lds + decltype(here)::value * STAGE;
+        if (at + 1 < steps) keep(next);
+        if (at + 3 < steps) load(at + 3, next);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            uint4v fa[TM], fb[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const uint4v*>(stage + tile_offset<int8_t>(wm + i * 16 + frag_row, half * 4 + frag_piece));
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const uint4v*>(stage + A_TILE + tile_offset<int8_t>(wn + j * 16 + frag_row, half * 4 + frag_piece));
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = mfma_i8(fb[j], fa[i], acc[i][j]);
+        }
+        __syncthreads();
+    };
+    load(0, Even{});
+    if (steps > 1) load(1, Odd{});
+    keep(Even{});
+    if (steps > 2) load(2, Even{});
+    __syncthreads();
+    for (uint32_t at = 0; at < steps; at += 2) {
+        step(at, Even{}, Odd{});
+        if (at + 1 < steps) step(at + 1, Odd{}, Even{});
+    }
+    if constexpr (SPLIT) {
+        if (!add_parts<TM, TN>(acc, shared, split, blockIdx.y * tiles_m * tiles_n + blockIdx.x / shared.splits, lds)) return;
+    }
+    write_scaled<D, TM, TN>(acc, reinterpret_cast<D*>(lds) + wave * (WM * (WN + 8)), C + oc, p, s, m0 + wm, n0 + wn);
 }
 
 // The sums of the blocks that shared K, scaled: four columns of a row per thread.
@@ -334,55 +442,101 @@ static int launch_tiles(const GemmProblem& p, const ScalePlaces& s, uint32_t spl
     return status;
 }
 
-// The kernel's tiles: rows, columns, us of a step of 128 with the chip full of them, us that a block takes beside its steps, us that the last of
-// the blocks that share a tile takes for each of their parts (0: a second kernel adds them up).  Two blocks of the last three are on a compute unit at a time and share its step times as they share its LDS.  A step is bound by LDS, which takes what is loaded at 64 bytes a clock and gives fragments at 128, and for the largest by the matrix pipe under the chip's
-// power limit (256 x 256 tiles 1.4 us, 3.1 POP/s; MFMAs alone 1.3).  Measured with weights from memory: 31 products of 33 to 8000 rows, each tile and up to 16
-// splits; the fastest of those by what follows is within 7 % of the fastest found for all but a few that one Python call takes longer for than they run.
+// The kernel's tiles: rows, columns, us of a step of 128 with the chip full of them (and of a block that has a compute unit alone, where that is more), us that a block takes beside its
+// steps, us that the last of the blocks that share a tile takes for each of their parts (0: a second kernel adds them up).  Two blocks of the last three are on a compute unit at a time and share
+// its step times as they share its LDS: a step is bound by LDS, which takes 32 KB of what is loaded in 0.24 us and gives 64 KB of fragments in 0.20 (both in 0.35; 128 x 128), at the
+// clock that the products leave, and for the largest by the matrix pipe under the chip's power limit (256 x 256 1.4 us, 3.1 POP/s; MFMAs alone on such values 1.3).  Measured with weights from
+// memory: 31 products of 33 to 8000 rows, each tile and up to 16 splits; what comes out first below is within 7 % of the fastest found.
 struct Tiles8 {
     int rows, columns;
-    double step, beside, join;
+    double step, beside, join, alone;
 };
-constexpr Tiles8 kTiles8[] = {{256, 256, 1.40, 15.0, 0}, {256, 192, 1.13, 12.0, 0}, {256, 128, 0.84, 6.0, 0}, {128, 128, 0.50, 4.0, 0},
-                              {128, 96, 0.47, 3.2, 0},   {64, 128, 0.38, 1.1, 0},   {64, 64, 0.235, 0.7, 0.48}, {32, 64, 0.18, 0.6, 0.37}};
+constexpr Tiles8 kTiles8[] = {{256, 256, 1.40, 15.0, 0, 0}, {256, 192, 1.13, 12.0, 0, 0}, {256, 128, 0.84, 6.0, 0, 0}, {128, 128, 0.50, 4.0, 0, 0},
+                              {128, 96, 0.47, 3.2, 0, 0},   {64, 128, 0.38, 1.1, 0, 0},   {64, 64, 0.235, 0.7, 0.48, 0}, {32, 64, 0.18, 0.6, 0.37, 0}};
 
 // us of a product: the blocks of the busiest compute unit one after another, and the weights from memory, most of the shorter one beside the longer; then the sums of blocks that share K
 static double tiles8_cost(const GemmProblem& p, const Tiles8& t, uint32_t splits) {
     const uint64_t steps = (p.K + 127) / 128, per_block = (steps + splits - 1) / splits, parts = (steps + per_block - 1) / per_block;
     const uint64_t tiles = (static_cast<uint64_t>(p.M) + t.rows - 1) / t.rows * ((static_cast<uint64_t>(p.N) + t.columns - 1) / t.columns) * p.batches;
-    const double rounds = static_cast<double>((tiles * parts + 255) / 256), multiplied = 3.0 + rounds * (per_block * t.step + t.beside);
+    const double rounds = static_cast<double>((tiles * parts + 255) / 256), multiplied = 3.0 + per_block * (rounds * t.step > t.alone ? rounds * t.step : t.alone) + rounds * t.beside;
     const double loaded = 1.5 + static_cast<double>(p.N) * p.K / 5.2e6;
     const double joined = parts == 1 ? 0.0 : t.join > 0 ? 1.0 + t.join * parts : 2.5 + 8.0 * parts * p.M * p.N * p.batches / 6e6;
     return multiplied > loaded ? multiplied + 0.3 * loaded + joined : loaded + 0.3 * multiplied + joined;
 }
 
+struct Choice8 {
+    int tile;
+    uint32_t splits;
+    double cost;
+};
+
+static Choice8 choose_tiles8(const GemmProblem& p, const Tiles8* tiles, int count) {
+    Choice8 best{0, 1, 0};
+    for (int t = 0; t < count; ++t)
+        for (uint32_t parts : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u}) {
+            const uint64_t blocks = (static_cast<uint64_t>(p.M) + tiles[t].rows - 1) / tiles[t].rows * ((static_cast<uint64_t>(p.N) + tiles[t].columns - 1) / tiles[t].columns) * p.batches * parts;
+            // (parts of four steps and more, of so many blocks that they are all there at once: 512, half as many tiles at most, which there are counts of arrivals for)
+            if (parts > 1 && (p.K / 128 < 4 * parts || blocks > 512)) break;
+            const double cost = tiles8_cost(p, tiles[t], parts);
+            if ((t == 0 && parts == 1) || cost < best.cost) best = Choice8{t, parts, cost};
+        }
+    return best;
+}
+
+// (tiles of 128 x 128 and smaller ones are the smallest where there are many: fewer than the blocks that a launch may have)
+static bool few_enough_blocks(const GemmProblem& p, uint64_t bm, uint64_t bn) {
+    return (static_cast<uint64_t>(p.M) + bm - 1) / bm * ((static_cast<uint64_t>(p.N) + bn - 1) / bn) * p.batches < kMostBlocks && p.batches <= 65535;
+}
+
 template <class D>
 int gemm_quantized_tile(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
-    if (!quantized_operands_fit(p, a, b) || (static_cast<uint64_t>(p.M) + 127) / 128 * ((static_cast<uint64_t>(p.N) + 127) / 128) >= kMostBlocks) return TANNIC_UNSUPPORTED_DTYPE;
-    int tile = 0;
-    uint32_t splits = 1;
-    double least = 0;
-    for (int t = 0; t < 8; ++t)
-        for (uint32_t parts : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u}) {
-            const uint64_t tiles = (static_cast<uint64_t>(p.M) + kTiles8[t].rows - 1) / kTiles8[t].rows * ((static_cast<uint64_t>(p.N) + kTiles8[t].columns - 1) / kTiles8[t].columns) * p.batches;
-            // (parts of four steps and more, of so many blocks that they are all there at once: 512, half as many tiles at most, which there are counts of arrivals for)
-            if (parts > 1 && (p.K / 128 < 4 * parts || tiles * parts > 512)) break;
-            const double cost = tiles8_cost(p, kTiles8[t], parts);
-            if ((t == 0 && parts == 1) || cost < least) {
-                least = cost;
-                tile = t;
-                splits = parts;
-            }
-        }
-    switch (tile) {
-        case 0: return launch_tiles<D, 256, 256, 2>(p, s, splits, a, b, c, stream);
-        case 1: return launch_tiles<D, 256, 192, 2>(p, s, splits, a, b, c, stream);
-        case 2: return launch_tiles<D, 256, 128, 3>(p, s, splits, a, b, c, stream);
-        case 3: return launch_tiles<D, 128, 128, 4>(p, s, splits, a, b, c, stream);
-        case 4: return launch_tiles<D, 128, 96, 5>(p, s, splits, a, b, c, stream);
-        case 5: return launch_tiles<D, 64, 128, 3>(p, s, splits, a, b, c, stream);
-        case 6: return launch_tiles<D, 64, 64, 5, Sharing::last_block>(p, s, splits, a, b, c, stream);
-        default: return launch_tiles<D, 32, 64, 6, Sharing::last_block>(p, s, splits, a, b, c, stream);
+    if (!quantized_operands_fit(p, a, b) || !few_enough_blocks(p, 128, 128)) return TANNIC_UNSUPPORTED_DTYPE;
+    const Choice8 choice = choose_tiles8(p, kTiles8, 8);
+    switch (choice.tile) {
+        case 0: return launch_tiles<D, 256, 256, 2>(p, s, choice.splits, a, b, c, stream);
+        case 1: return launch_tiles<D, 256, 192, 2>(p, s, choice.splits, a, b, c, stream);
+        case 2: return launch_tiles<D, 256, 128, 3>(p, s, choice.splits, a, b, c, stream);
+        case 3: return launch_tiles<D, 128, 128, 4>(p, s, choice.splits, a, b, c, stream);
+        case 4: return launch_tiles<D, 128, 96, 5>(p, s, choice.splits, a, b, c, stream);
+        case 5: return launch_tiles<D, 64, 128, 3>(p, s, choice.splits, a, b, c, stream);
+        case 6: return launch_tiles<D, 64, 64, 5, Sharing::last_block>(p, s, choice.splits, a, b, c, stream);
+        default: return launch_tiles<D, 32, 64, 6, Sharing::last_block>(p, s, choice.splits, a, b, c, stream);
     }
+}
+
+template <class D, int BM>
+static int launch_bytes(const GemmProblem& p, const ScalePlaces& s, uint32_t splits, const void* a, const void* b, void* c, hipStream_t stream) {
+    const uint32_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + 63) / 64, steps = (p.K + 127) / 128;
+    SharedK shared{splits, (steps + splits - 1) / splits, nullptr, 0, nullptr};
+    shared.splits = (steps + shared.steps - 1) / shared.steps;
+    void* held = nullptr;
+    if (shared.splits > 1) {
+        if (int status = attention_arrivals(stream, shared.arrivals)) return status;
+        if (scratch_acquire(&held, static_cast<size_t>(shared.splits) * p.batches * tiles_m * tiles_n * BM * 64 * sizeof(int), stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+        shared.partials = static_cast<int*>(held);
+    }
+    const auto run = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n * shared.splits, p.batches), dim3(256), 0, stream, static_cast<const int8_t*>(a), static_cast<const int8_t*>(b), static_cast<D*>(c), p,
+                           s, tiles_m, tiles_n, shared);
+        return launch_status("gemm_quantized_bytes_kernel");
+    };
+    const int status = shared.splits > 1 ? run(gemm_quantized_bytes_kernel<D, BM, Sharing::last_block>) : run(gemm_quantized_bytes_kernel<D, BM, Sharing::none>);
+    if (held) scratch_release(held, stream);
+    return status;
+}
+
+// The tiles for rows that start anywhere, times as above; four blocks and more on a compute unit share its loads, one alone is not faster than `alone`.
+constexpr Tiles8 kBytes8[] = {{64, 64, 0.44, 0.7, 0.48, 0.75}, {32, 64, 0.345, 0.6, 0.37, 0.64}};
+
+template <class D>
+int gemm_quantized_bytes(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
+    if (p.a_cs != 1 || p.b_rs != 1 || p.K < 16 || !few_enough_blocks(p, 32, 64)) return TANNIC_UNSUPPORTED_DTYPE;
+    const Choice8 choice = choose_tiles8(p, kBytes8, 2);
+    // where copies and the tiles of aligned rows are faster those take it: two launches of about 3 us, a read and a write of both operands
+    GemmProblem q = p;
+    q.K = (p.K + 127) / 128 * 128;
+    if (choice.cost > choose_tiles8(q, kTiles8, 8).cost + 6.0 + 2.0 * (static_cast<double>(p.M) + p.N) * p.K * p.batches / 4.5e6) return TANNIC_UNSUPPORTED_DTYPE;
+    return choice.tile == 0 ? launch_bytes<D, 64>(p, s, choice.splits, a, b, c, stream) : launch_bytes<D, 32>(p, s, choice.splits, a, b, c, stream);
 }
 
 // This file is compiled once for each type of results (TH_TILE_TYPE).
@@ -390,5 +544,6 @@ int gemm_quantized_tile(const GemmProblem& p, const ScalePlaces& s, const void* 
 #define TH_TILE_TYPE bf16
 #endif
 template int gemm_quantized_tile<TH_TILE_TYPE>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
+template int gemm_quantized_bytes<TH_TILE_TYPE>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
 
 }  // namespace th
