@@ -475,22 +475,23 @@ static Choice8 choose_tiles8(const GemmProblem& p, const Tiles8* tiles, int coun
     for (int t = 0; t < count; ++t)
         for (uint32_t parts : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u}) {
             const uint64_t blocks = (static_cast<uint64_t>(p.M) + tiles[t].rows - 1) / tiles[t].rows * ((static_cast<uint64_t>(p.N) + tiles[t].columns - 1) / tiles[t].columns) * p.batches * parts;
-            // (parts of four steps and more, of so many blocks that they are all there at once: 512, half as many tiles at most, which there are counts of arrivals for)
-            if (parts > 1 && (p.K / 128 < 4 * parts || blocks > 512)) break;
+            // (fewer blocks than a launch may have; parts of four steps and more, of so many blocks that they are all there at once: 512, half as many tiles at most, which there are
+            // counts of arrivals for)
+            if (blocks >= kMostBlocks || (parts > 1 && (p.K / 128 < 4 * parts || blocks > 512))) break;
             const double cost = tiles8_cost(p, tiles[t], parts);
             if ((t == 0 && parts == 1) || cost < best.cost) best = Choice8{t, parts, cost};
         }
     return best;
 }
 
-// (tiles of 128 x 128 and smaller ones are the smallest where there are many: fewer than the blocks that a launch may have)
+// Fewer blocks of bm x bn results than a launch may have.
 static bool few_enough_blocks(const GemmProblem& p, uint64_t bm, uint64_t bn) {
     return (static_cast<uint64_t>(p.M) + bm - 1) / bm * ((static_cast<uint64_t>(p.N) + bn - 1) / bn) * p.batches < kMostBlocks && p.batches <= 65535;
 }
 
 template <class D>
 int gemm_quantized_tile(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
-    if (!quantized_operands_fit(p, a, b) || !few_enough_blocks(p, 128, 128)) return TANNIC_UNSUPPORTED_DTYPE;
+    if (!quantized_operands_fit(p, a, b) || !few_enough_blocks(p, 256, 256)) return TANNIC_UNSUPPORTED_DTYPE;
     const Choice8 choice = choose_tiles8(p, kTiles8, 8);
     switch (choice.tile) {
         case 0: return launch_tiles<D, 256, 256, 2>(p, s, choice.splits, a, b, c, stream);
@@ -530,7 +531,7 @@ constexpr Tiles8 kBytes8[] = {{64, 64, 0.44, 0.7, 0.48, 0.75}, {32, 64, 0.345, 0
 
 template <class D>
 int gemm_quantized_bytes(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
-    if (p.a_cs != 1 || p.b_rs != 1 || p.K < 16 || !few_enough_blocks(p, 32, 64)) return TANNIC_UNSUPPORTED_DTYPE;
+    if (p.a_cs != 1 || p.b_rs != 1 || p.K < 16 || !few_enough_blocks(p, 64, 64)) return TANNIC_UNSUPPORTED_DTYPE;
     const Choice8 choice = choose_tiles8(p, kBytes8, 2);
     // where copies and the tiles of aligned rows are faster those take it: two launches of about 3 us, a read and a write of both operands
     GemmProblem q = p;
