@@ -6,6 +6,8 @@
 // behind those of the first half the loads of the step that takes the freed stage.  It ends with a wait for the next step's loads and one barrier.
 // The weights are the first operand, so that a lane has four consecutive columns of one row: times the row's and the columns' scales, and to memory by whole rows through LDS (16 bits) or as they are.
 // Blocks that share a tile's K leave whole numbers, which a second kernel adds up and scales, or for small tiles the last of the blocks that gets there.
+#include <algorithm>
+
 #include "attention.hpp"
 #include "gemm_quantized.hpp"
 
@@ -448,21 +450,11 @@ static int launch_tiles(const GemmProblem& p, const ScalePlaces& s, uint32_t spl
 // clock that the products leave, and for the largest by the matrix pipe under the chip's power limit (256 x 256 1.4 us, 3.1 POP/s; MFMAs alone on such values 1.3).  Measured with weights from
 // memory: 31 products of 33 to 8000 rows, each tile and up to 16 splits; what comes out first below is within 7 % of the fastest found.
 struct Tiles8 {
-    int rows, columns;
+    uint32_t rows, columns;
     double step, beside, join, alone;
 };
 constexpr Tiles8 kTiles8[] = {{256, 256, 1.40, 15.0, 0, 0}, {256, 192, 1.13, 12.0, 0, 0}, {256, 128, 0.84, 6.0, 0, 0}, {128, 128, 0.50, 4.0, 0, 0},
                               {128, 96, 0.47, 3.2, 0, 0},   {64, 128, 0.38, 1.1, 0, 0},   {64, 64, 0.235, 0.7, 0.48, 0}, {32, 64, 0.18, 0.6, 0.37, 0}};
-
-// us of a product: the blocks of the busiest compute unit one after another, and the weights from memory, most of the shorter one beside the longer; then the sums of blocks that share K
-static double tiles8_cost(const GemmProblem& p, const Tiles8& t, uint32_t splits) {
-    const uint64_t steps = (p.K + 127) / 128, per_block = (steps + splits - 1) / splits, parts = (steps + per_block - 1) / per_block;
-    const uint64_t tiles = (static_cast<uint64_t>(p.M) + t.rows - 1) / t.rows * ((static_cast<uint64_t>(p.N) + t.columns - 1) / t.columns) * p.batches;
-    const double rounds = static_cast<double>((tiles * parts + 255) / 256), multiplied = 3.0 + per_block * (rounds * t.step > t.alone ? rounds * t.step : t.alone) + rounds * t.beside;
-    const double loaded = 1.5 + static_cast<double>(p.N) * p.K / 5.2e6;
-    const double joined = parts == 1 ? 0.0 : t.join > 0 ? 1.0 + t.join * parts : 2.5 + 8.0 * parts * p.M * p.N * p.batches / 6e6;
-    return multiplied > loaded ? multiplied + 0.3 * loaded + joined : loaded + 0.3 * multiplied + joined;
-}
 
 struct Choice8 {
     int tile;
@@ -470,17 +462,31 @@ struct Choice8 {
     double cost;
 };
 
+template <uint32_t N> using Parts = std::integral_constant<uint32_t, N>;      // (a number that is divided by, known to the compiler)
+
+// The least us of a product by this: the blocks of the busiest compute unit one after another, and the weights from memory, most of the shorter one beside the longer; then the sums of blocks
+// that share K.  (Every product goes through it: 0.2 us of a call.)
 static Choice8 choose_tiles8(const GemmProblem& p, const Tiles8* tiles, int count) {
-    Choice8 best{0, 1, 0};
-    for (int t = 0; t < count; ++t)
-        for (uint32_t parts : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u}) {
-            const uint64_t blocks = (static_cast<uint64_t>(p.M) + tiles[t].rows - 1) / tiles[t].rows * ((static_cast<uint64_t>(p.N) + tiles[t].columns - 1) / tiles[t].columns) * p.batches * parts;
-            // (fewer blocks than a launch may have; parts of four steps and more, of so many blocks that they are all there at once: 512, half as many tiles at most, which there are
-            // counts of arrivals for)
-            if (blocks >= kMostBlocks || (parts > 1 && (p.K / 128 < 4 * parts || blocks > 512))) break;
-            const double cost = tiles8_cost(p, tiles[t], parts);
-            if ((t == 0 && parts == 1) || cost < best.cost) best = Choice8{t, parts, cost};
-        }
+    const uint32_t steps = (p.K + 127) / 128, most_parts = p.K / 512;      // (of four steps and more)
+    const double loaded = 1.5 + static_cast<double>(p.N) * p.K / 5.2e6, results = 8.0 / 6e6 * p.M * p.N * p.batches;
+    Choice8 best{0, 1, -1.0};
+    for (int t = 0; t < count; ++t) {
+        const Tiles8& tile = tiles[t];
+        const uint64_t blocks = static_cast<uint64_t>((p.M - 1) / tile.rows + 1) * ((p.N - 1) / tile.columns + 1) * p.batches;
+        if (blocks >= kMostBlocks) continue;      // (a launch has fewer)
+        const auto of = [&](auto splits) {
+            const double rounds = static_cast<double>(static_cast<int64_t>((blocks * splits + 255) / 256)), of_step = std::max(rounds * tile.step, tile.alone);
+            const double multiplied = 3.0 + static_cast<int>((steps + splits - 1) / splits) * of_step + rounds * tile.beside;
+            const double joined = splits == 1 ? 0.0 : tile.join > 0 ? 1.0 + tile.join * splits : 2.5 + results * splits;
+            const double cost = std::max(multiplied, loaded) + 0.3 * std::min(multiplied, loaded) + joined;
+            if (best.cost < 0 || cost < best.cost) best = Choice8{t, splits, cost};
+        };
+        of(Parts<1>{});
+        // (parts so many that they are all there at once: 512, half as many tiles at most, which there are counts of arrivals for)
+        const uint32_t most = blocks > 256 ? 1 : static_cast<uint32_t>(std::min<uint64_t>(most_parts, 512 / static_cast<uint32_t>(blocks)));
+        const auto each = [&](auto... splits) { ((splits <= most ? of(splits) : void()), ...); };
+        each(Parts<2>{}, Parts<3>{}, Parts<4>{}, Parts<6>{}, Parts<8>{}, Parts<12>{}, Parts<16>{});
+    }
     return best;
 }
 
@@ -533,10 +539,11 @@ template <class D>
 int gemm_quantized_bytes(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
     if (p.a_cs != 1 || p.b_rs != 1 || p.K < 16 || !few_enough_blocks(p, 64, 64)) return TANNIC_UNSUPPORTED_DTYPE;
     const Choice8 choice = choose_tiles8(p, kBytes8, 2);
-    // where copies and the tiles of aligned rows are faster those take it: two launches of about 3 us, a read and a write of both operands
+    // where copies and the tiles of aligned rows are faster those take it: two launches of about 3 us, a read and a write of both operands (and no product is shorter than 4 us)
+    const double copies = 6.0 + 2.0 * (static_cast<double>(p.M) + p.N) * p.K * p.batches / 4.5e6;
     GemmProblem q = p;
     q.K = (p.K + 127) / 128 * 128;
-    if (choice.cost > choose_tiles8(q, kTiles8, 8).cost + 6.0 + 2.0 * (static_cast<double>(p.M) + p.N) * p.K * p.batches / 4.5e6) return TANNIC_UNSUPPORTED_DTYPE;
+    if (choice.cost > copies + 4.0 && choice.cost > copies + choose_tiles8(q, kTiles8, 8).cost) return TANNIC_UNSUPPORTED_DTYPE;
     return choice.tile == 0 ? launch_bytes<D, 64>(p, s, choice.splits, a, b, c, stream) : launch_bytes<D, 32>(p, s, choice.splits, a, b, c, stream);
 }
 
