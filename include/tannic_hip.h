@@ -452,12 +452,13 @@ int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const 
  *   m = max |u| of the row, 2^-119 at least
  * so that no value is off by more than half a scale.  A row with something
  * that is not finite has zeros and the scale NaN: all that is computed from
- * it is NaN.  x: float16, bfloat16 or float, any strides; u is float; the
- * results are contiguous.
+ * it is NaN.  x: float16, bfloat16 or float, any strides; u, and a norm's
+ * mean, are float; the results are contiguous and lie over no operand (but
+ * for a norm's sum).
  * ------------------------------------------------------------------ */
 /* u = x */
 int tannic_hip_quantize(const tannic_tensor_t* x, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream);
-/* u = gate / (1 + exp(-gate)) * up, both of one shape */
+/* u = gate / (1 + exp(-gate)) * up, both of one shape (0 for a gate below -87, whose quotient is less than the smallest normal float) */
 int tannic_hip_swiglu_quantize(const tannic_tensor_t* gate, const tannic_tensor_t* up, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream);
 /* total = x + residual, rounded to x's type; dst = total / sqrt(mean(total^2) + eps) * gain over the last axis, in x's type (float64 too), or with
  * `scales` in 8 bits (u = total * gain in float, whose integers are the norm's: the root is one number for a row and goes into the scale).

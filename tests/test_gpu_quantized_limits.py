@@ -8,7 +8,7 @@ import pytest
 
 import support
 import tannic_amd as ta
-from quantized_support import integers_of, product, rounded
+from quantized_support import assert_stands_for, integers_of, product, rounded
 from tannic_amd import decoder_layer as dl, ops
 from tannic_amd.paged_cache import PagedCache
 
@@ -140,6 +140,20 @@ def test_one_row_and_one_column_seen_as_many(m, n, k, device):
     sa, sb = ta.tensor(rng.uniform(0.001, 0.002, 1), ta.float32, device).expand(m), ta.tensor(rng.uniform(0.01, 0.02, 1), ta.float32, device).expand(n)
     got = ops.matmul_quantized(da.expand(m, k), sa, db.expand(n, k).transpose(), sb, ta.float32).numpy()
     np.testing.assert_array_equal(got, product(np.repeat(a, m, 0), sa.numpy(), np.repeat(b, n, 0).T, sb.numpy()))
+
+
+@pytest.mark.parametrize("length", [40, 41, 5000, 70000])
+@pytest.mark.parametrize("dtype", [ta.bfloat16, ta.float32], ids=str)
+def test_gates_at_the_ends_of_the_type(dtype, length, device):
+    """A gate beyond 2^127 / log2 e is itself, or 0 below 0: a row of nothing else, and beside small ones (the same bounds as everywhere: the steps are the same)."""
+    largest = 3e38
+    rng = np.random.default_rng(30)
+    gate = rounded(np.stack([np.full(length, largest), rng.choice([largest, -largest, 0.5], length), rng.choice([-largest, 1.0], length), rng.choice([-150.0, 150.0, 88.0, -88.0], length)]), dtype)
+    up = rounded(rng.uniform(0.25, 0.75, (4, length)), dtype)
+    values, scales = ops.swiglu_quantized(ta.tensor(gate, dtype, device), ta.tensor(up, dtype, device))
+    wide = gate.astype(np.float64)
+    want = np.where(wide > -700, wide / (1 + np.exp(np.minimum(-wide, 700))), 0) * up
+    assert_stands_for(values.numpy(), scales.numpy(), want, 6 * 2.0 ** -24)
 
 
 SHAPE = dl.LayerShape(hidden=128, heads=4, kv_heads=2, head_dim=32, ffn=320)
