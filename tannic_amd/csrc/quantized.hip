@@ -36,7 +36,7 @@ struct RowOperands {
 
 // gate / (1 + exp(-gate)) * up, off by 8 * 2^-24 at most: exp(-gate) is 2^high * (1 + low * ln 2) with high + low = -gate * log2 e (the instruction for powers of two is off by
 // 2 units, and high alone would be by |gate|); the sum with 1 takes both in one rounding, its reciprocal is off by 2 units.  An exponential beyond all floats makes the quotient 0
-// (and a reciprocal below the normal ones is 0: gates below -87), and the products with log2 e may not be beyond them: the exponential of 200 and more is, that of -200 is nothing beside 1.
+// (a reciprocal below the normal ones may be: gates below -87), and the products with log2 e may not be beyond them: the exponential of 200 and more is, that of -200 is nothing beside 1.
 __device__ inline float gated(float gate, float up) {
     constexpr float log2e = 0x1.715476p+0f, rest = 0x1.4ae0bep-26f, ln2 = 0x1.62e430p-1f;
     const float power = __builtin_amdgcn_fmed3f(-gate, -200.0f, 200.0f), high = power * log2e, low = fmaf(power, rest, fmaf(power, log2e, -high));
