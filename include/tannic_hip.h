@@ -458,7 +458,7 @@ int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const 
  * ------------------------------------------------------------------ */
 /* u = x */
 int tannic_hip_quantize(const tannic_tensor_t* x, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream);
-/* u = gate / (1 + exp(-gate)) * up, both of one shape (for a gate below -87 the quotient, less than the smallest normal float, may be 0) */
+/* u = gate / (1 + exp(-gate)) * up, both of one shape (off by 8 * 2^-24 at most also where the quotient alone is below the floats' range) */
 int tannic_hip_swiglu_quantize(const tannic_tensor_t* gate, const tannic_tensor_t* up, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream);
 /* total = x + residual, rounded to x's type; dst = total / sqrt(mean(total^2) + eps) * gain over the last axis, in x's type (float64 too), or with
  * `scales` in 8 bits (u = total * gain in float, whose integers are the norm's: the root is one number for a row and goes into the scale).

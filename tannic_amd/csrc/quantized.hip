@@ -34,14 +34,26 @@ struct RowOperands {
     double eps;
 };
 
-// gate / (1 + exp(-gate)) * up, off by 8 * 2^-24 at most: exp(-gate) is 2^high * (1 + low * ln 2) with high + low = -gate * log2 e (the instruction for powers of two is off by
-// 2 units, and high alone would be by |gate|); the sum with 1 takes both in one rounding, its reciprocal is off by 2 units.  An exponential beyond all floats makes the quotient 0
-// (a reciprocal below the normal ones may be: gates below -87), and the products with log2 e may not be beyond them: the exponential of 200 and more is, that of -200 is nothing beside 1.
+// gate / (1 + exp(-gate)) * up, off by 8 * 2^-24 at most, for gates from kFarGate on: exp(-gate) is 2^high * (1 + low * ln 2) with high + low = -gate * log2 e (the instruction for
+// powers of two is off by 2 units, and high alone would be by |gate|); the sum with 1 takes both in one rounding, its reciprocal is off by 2 units.  The product with log2 e may not be
+// beyond all floats: the exponential of -200 is nothing beside 1.
+constexpr float kLog2e = 0x1.715476p+0f, kLog2eRest = 0x1.4ae0bep-26f;
 __device__ inline float gated(float gate, float up) {
-    constexpr float log2e = 0x1.715476p+0f, rest = 0x1.4ae0bep-26f, ln2 = 0x1.62e430p-1f;
-    const float power = __builtin_amdgcn_fmed3f(-gate, -200.0f, 200.0f), high = power * log2e, low = fmaf(power, rest, fmaf(power, log2e, -high));
+    constexpr float ln2 = 0x1.62e430p-1f;
+    const float power = __builtin_amdgcn_fmed3f(-gate, -200.0f, 200.0f), high = power * kLog2e, low = fmaf(power, kLog2eRest, fmaf(power, kLog2e, -high));
     const float sum = fmaf(__builtin_amdgcn_exp2f(high), fmaf(low, ln2, 1.0f), 1.0f);
     return gate * __builtin_amdgcn_rcpf(sum) * up;
+}
+
+// Below kFarGate 1 is nothing beside exp(-gate) (2^-92), and gate * exp(gate) * up is it: from -87 on the reciprocal of the sum would be no normal number, from -92 on the quotient, and
+// both come out as 0, while up may make either large.  exp(gate) is 2^whole * 2^part with |part| <= 1/2 (off by 2^-25 before the instruction's 2 units), the powers of two of both factors meet in the last step:
+// off by 5 * 2^-24 at most, or by half of the smallest subnormal number.  exp(-400) is 0 with any factor; a gate that is not finite is what it is in the formula.
+constexpr float kFarGate = -64.0f;
+constexpr uint32_t kFarGateBits = 0xC2800000u;      // (what is below it, as an unsigned number, is above this; so is what is not a number and has a sign)
+__device__ inline float gated_far(float gate, float up) {
+    const float power = fmaxf(gate, -400.0f), whole = rintf(power * kLog2e), part = fmaf(power, kLog2eRest, fmaf(power, kLog2e, -whole));
+    const float near = power * 0x1p-64f * __builtin_amdgcn_exp2f(part) * up;
+    return fmaf(gate, 0.0f, ldexpf(near, static_cast<int>(whole) + 64));
 }
 
 // ---- rows in registers ----------------------------------------------------------------
@@ -123,7 +135,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G, (kRowWavefronts<S, G, NCH>)) voi
             }
         }
         float u[NCH][VEC], squares = 0;
-        uint32_t most = 0;
+        uint32_t most = 0, lowest = 0;      // (the bits of the lowest gate)
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const uint32_t at = (t + i * G) * VEC;
@@ -137,10 +149,28 @@ __global__ __launch_bounds__(G == 64 ? 256 : G, (kRowWavefronts<S, G, NCH>)) voi
                 for (int e = 0; e < VEC; ++e) {
                     const float v = widen(a[i].v[e]);
                     if constexpr (NORM) squares += v * v;
-                    if constexpr (S == RowSource::gated) u[i][e] = gated(v, widen(b[i].v[e]));
+                    if constexpr (S == RowSource::gated) u[i][e] = gated(v, widen(b[i].v[e])), lowest = LargestOp::combine(lowest, __float_as_uint(v));
                     else if constexpr (NORM && INTEGERS) u[i][e] = v * widen(g[i].v[e]);
                     else u[i][e] = v;
                     if constexpr (INTEGERS) most = LargestOp::combine(most, magnitude(u[i][e]));
+                }
+            }
+        }
+        if constexpr (S == RowSource::gated) {
+            // some gate far below zero, hardly ever: the thread's pieces once more, read again so that nothing is kept for it
+            if (lowest > kFarGateBits) {
+                most = 0;
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    const uint32_t at = (t + i * G) * VEC;
+                    if (at < p.length) {
+                        const Piece<T> gate = load_piece<T, PAST>(x + at, p.length - at), up = load_piece<T, PAST>(second + at, p.length - at);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            if (__float_as_uint(widen(gate.v[e])) > kFarGateBits) u[i][e] = gated_far(widen(gate.v[e]), widen(up.v[e]));
+                            most = LargestOp::combine(most, magnitude(u[i][e]));
+                        }
+                    }
                 }
             }
         }
@@ -198,8 +228,17 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowOperands p) {
         const T* const second = static_cast<const T*>(p.second) + (S == RowSource::gated || S == RowSource::sum_norm ? p.rows_second.offset(row) : 0);
         const size_t base = static_cast<size_t>(row) * p.length;
         T* const total = static_cast<T*>(p.total) + base;
-        auto value = [&](uint32_t i, bool first) -> A {
-            if constexpr (S == RowSource::gated) return gated(widen(x[i * p.rows_x.step]), widen(second[i * p.rows_second.step]));
+        uint32_t lowest = 0;      // (the bits of the lowest gate)
+        using Far = std::true_type;      // the row has gates far below zero, hardly ever
+        using Near = std::false_type;
+        auto value = [&](uint32_t i, bool first, auto gates) -> A {
+            if constexpr (S == RowSource::gated) {
+                const float gate = widen(x[i * p.rows_x.step]), up = widen(second[i * p.rows_second.step]);
+                lowest = LargestOp::combine(lowest, __float_as_uint(gate));
+                if constexpr (decltype(gates)::value)
+                    if (__float_as_uint(gate) > kFarGateBits) return gated_far(gate, up);
+                return gated(gate, up);
+            }
             if constexpr (S == RowSource::sum_norm) {
                 if (!first) return static_cast<A>(widen(total[i]));
                 const T sum = rounded<T>(static_cast<A>(widen(x[i * p.rows_x.step])) + static_cast<A>(widen(second[i * p.rows_second.step])));
@@ -210,22 +249,37 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowOperands p) {
         };
         A squares = 0;
         uint32_t most = 0;
-        for (uint32_t i = threadIdx.x; i < p.length; i += 256) {
-            const A v = value(i, true);
-            if constexpr (NORM) squares += v * v;
-            if constexpr (INTEGERS) most = LargestOp::combine(most, magnitude(static_cast<float>(NORM ? v * static_cast<A>(widen(gain[i])) : v)));
+        const auto look = [&](auto gates) {
+            for (uint32_t i = threadIdx.x; i < p.length; i += 256) {
+                const A v = value(i, true, gates);
+                if constexpr (NORM) squares += v * v;
+                if constexpr (INTEGERS) most = LargestOp::combine(most, magnitude(static_cast<float>(NORM ? v * static_cast<A>(widen(gain[i])) : v)));
+            }
+        };
+        look(Near{});
+        bool far = false;
+        if constexpr (S == RowSource::gated) {
+            far = block_reduce<LargestOp>(lowest, largest) > kFarGateBits;
+            if (far) {
+                most = 0;
+                look(Far{});
+            }
         }
         A r = 1;
         if constexpr (NORM) r = A(1) / sqrt(block_reduce<SquaresOp>(squares, sums) / static_cast<A>(p.length) + static_cast<A>(p.eps));
         if constexpr (INTEGERS) {
             const RowScale scale(block_reduce<LargestOp>(most, largest));
-            for (uint32_t i = threadIdx.x; i < p.length; i += 256) {
-                const A v = value(i, false);
-                static_cast<int8_t*>(p.dst)[base + i] = scale.integer(static_cast<float>(NORM ? v * static_cast<A>(widen(gain[i])) : v));
-            }
+            const auto write = [&](auto gates) {
+                for (uint32_t i = threadIdx.x; i < p.length; i += 256) {
+                    const A v = value(i, false, gates);
+                    static_cast<int8_t*>(p.dst)[base + i] = scale.integer(static_cast<float>(NORM ? v * static_cast<A>(widen(gain[i])) : v));
+                }
+            };
+            if (far) write(Far{});
+            else write(Near{});
             if (threadIdx.x == 0) p.scales[row] = scale.scale(static_cast<float>(r));
         } else {
-            for (uint32_t i = threadIdx.x; i < p.length; i += 256) static_cast<T*>(p.dst)[base + i] = rounded<T>(value(i, false) * r * static_cast<A>(widen(gain[i])));
+            for (uint32_t i = threadIdx.x; i < p.length; i += 256) static_cast<T*>(p.dst)[base + i] = rounded<T>(value(i, false, Near{}) * r * static_cast<A>(widen(gain[i])));
         }
     }
 }
