@@ -35,19 +35,15 @@ class Streams {
     }
     hipStream_t pop(int device) {
         std::lock_guard<std::mutex> lock(mutex_);
-        if (device < 0) return nullptr;
-        if (static_cast<size_t>(device) >= pools_.size()) pools_.resize(device + 1);
-        auto& pool = pools_[device];
-        if (!pool.empty()) {
-            hipStream_t s = pool.back();
-            pool.pop_back();
-            return s;
-        }
-        hipStream_t s = nullptr;
-        // default flags: ordered against the legacy stream like the reference's
-        // cudaStreamCreate; default priority
-        if (hipStreamCreate(&s) != hipSuccess) return nullptr;
+        const hipStream_t s = last(device);
+        if (device >= 0 && !pools_[device].empty()) pools_[device].pop_back();
         return s;
+    }
+    // What a pop would hand out, left where it is: what allocations and copies ride on.  (A pop and a put of each of two threads could come back in the other order, and the
+    // stream that one caller keeps would no longer be the one that memory and copies follow.)
+    hipStream_t top(int device) {
+        std::lock_guard<std::mutex> lock(mutex_);
+        return last(device);
     }
     void put(int device, hipStream_t s) {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -57,6 +53,19 @@ class Streams {
     }
 
    private:
+    hipStream_t last(int device) {
+        if (device < 0) return nullptr;
+        if (static_cast<size_t>(device) >= pools_.size()) pools_.resize(device + 1);
+        auto& pool = pools_[device];
+        if (pool.empty()) {
+            hipStream_t s = nullptr;
+            // default flags: ordered against the legacy stream like the reference's
+            // cudaStreamCreate; default priority
+            if (hipStreamCreate(&s) != hipSuccess) return nullptr;
+            pool.push_back(s);
+        }
+        return pool.back();
+    }
     std::mutex mutex_;
     std::vector<std::vector<hipStream_t>> pools_;
 };
@@ -321,9 +330,7 @@ void* tannic_hip_allocate(const tannic_device_t* device, size_t nbytes) {
     count(kCounterMemoryCalls, 1);
     if (!device || tannic_hip_set_device(device->id) != TANNIC_SUCCESS) return nullptr;
     retain_pool_memory(device->id);
-    Streams& streams = Streams::instance();
-    hipStream_t stream = streams.pop(device->id);
-    streams.put(device->id, stream);
+    hipStream_t stream = Streams::instance().top(device->id);
     const size_t size = block_size(nbytes);
     uint64_t recording = 0;
     {
@@ -379,9 +386,7 @@ void* tannic_hip_deallocate(const tannic_device_t* device, void* address) {
     count(kCounterMemoryCalls, 1);
     if (!device || !address) return nullptr;
     if (tannic_hip_set_device(device->id) != TANNIC_SUCCESS) return nullptr;
-    Streams& streams = Streams::instance();
-    hipStream_t stream = streams.pop(device->id);
-    streams.put(device->id, stream);
+    hipStream_t stream = Streams::instance().top(device->id);
     std::vector<FreeBlock> evict;
     bool kept = false;
     FreeBlock released{address, MemBlock{0, stream, device->id}};
@@ -431,17 +436,12 @@ int tannic_hip_copy_from_host(const tannic_device_t* device, const void* host, v
     if (nbytes == 0) return TANNIC_SUCCESS;
     if (!host || !dev) { set_error_text("copy_from_host: null address"); return TANNIC_ERROR; }
     TH_TRY(hipSetDevice(device->id));
-    Streams& streams = Streams::instance();
-    hipStream_t stream = streams.pop(device->id);
-    if (refuses_while_recording(stream, "copy_from_host")) {
-        streams.put(device->id, stream);
-        return TANNIC_ERROR;
-    }
+    hipStream_t stream = Streams::instance().top(device->id);
+    if (refuses_while_recording(stream, "copy_from_host")) return TANNIC_ERROR;
     hipError_t err = hipMemcpyAsync(dev, host, nbytes, hipMemcpyHostToDevice, stream);
     // callers pass temporaries (one element of an initializer list): the source
     // must be consumed before returning
     if (err == hipSuccess) err = hipStreamSynchronize(stream);
-    streams.put(device->id, stream);
     TH_TRY(err);
     return TANNIC_SUCCESS;
 }
@@ -451,15 +451,10 @@ int tannic_hip_copy_device_to_host(const tannic_device_t* device, const void* de
     if (nbytes == 0) return TANNIC_SUCCESS;
     if (!host || !dev) { set_error_text("copy_device_to_host: null address"); return TANNIC_ERROR; }
     TH_TRY(hipSetDevice(device->id));
-    Streams& streams = Streams::instance();
-    hipStream_t stream = streams.pop(device->id);
-    if (refuses_while_recording(stream, "copy_device_to_host")) {
-        streams.put(device->id, stream);
-        return TANNIC_ERROR;
-    }
+    hipStream_t stream = Streams::instance().top(device->id);
+    if (refuses_while_recording(stream, "copy_device_to_host")) return TANNIC_ERROR;
     hipError_t err = hipMemcpyAsync(host, dev, nbytes, hipMemcpyDeviceToHost, stream);
     if (err == hipSuccess) err = hipStreamSynchronize(stream);
-    streams.put(device->id, stream);
     TH_TRY(err);
     return TANNIC_SUCCESS;
 }
@@ -524,9 +519,7 @@ int tannic_hip_device_synchronize(void) {
 
 void* tannic_hip_graph_begin(const tannic_device_t* device) {
     if (!device || tannic_hip_set_device(device->id) != TANNIC_SUCCESS) return nullptr;
-    Streams& streams = Streams::instance();
-    hipStream_t stream = streams.pop(device->id);
-    streams.put(device->id, stream);      // the next backend call pops this same stream
+    hipStream_t stream = Streams::instance().top(device->id);      // the next backend call pops this same stream
     std::scoped_lock lock(g_scratch_mutex, g_mem_mutex);
     if (g_capturing) {
         set_error_text("graph_begin: another recording is open; end it first");

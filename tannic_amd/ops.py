@@ -499,11 +499,7 @@ def allclose(a, b, rtol=1e-5, atol=1e-8):
     env = _resolve(a, b)
     da, db = a.descriptor(), b.descriptor()
     if isinstance(env, Device):
-        lib = library()
-        dvc = env.structure()
-        stream = lib.pop_stream(C.byref(dvc))
-        r = lib.kernels["allclose"](C.byref(da), C.byref(db), stream, rtol, atol)
-        lib.put_stream(C.byref(dvc), stream)
+        r = library().kernels["allclose"](C.byref(da), C.byref(db), env.stream(), rtol, atol)
     else:
         if _host_functions is None:
             raise BackendError("allclose: operands are on the host and tannic_amd holds device kernels only")
@@ -548,10 +544,7 @@ def softmax(x, mask=None, scale=1.0):
     dx, dd = x.descriptor(), dst.descriptor()
     dm = None if mask is None else mask.descriptor()
     lib = library()
-    dvc = env.structure()
-    stream = lib.pop_stream(C.byref(dvc))
-    status = lib.kernels["softmax"](C.byref(dx), None if dm is None else C.byref(dm), C.byref(dd), stream, C.c_float(scale))
-    lib.put_stream(C.byref(dvc), stream)
+    status = lib.kernels["softmax"](C.byref(dx), None if dm is None else C.byref(dm), C.byref(dd), env.stream(), C.c_float(scale))
     if status != abi.SUCCESS:
         detail = lib.error_message() if status == abi.ERROR else ""
         raise TannicError(f"Unsupported dtype (softmax: {abi.STATUS_NAMES[status]}{' ' + detail if detail else ''})")

@@ -10,6 +10,7 @@ layout SINGLETON / CONTIGUOUS / STRIDED.
 import ctypes as C
 import math
 import struct
+import threading
 
 import numpy as np
 
@@ -35,6 +36,7 @@ class Host:
 
 _STREAMS = {}      # device id -> its stream (see Device.stream)
 _STREAM_NUMBERS = {}
+_STREAMS_LOCK = threading.Lock()
 
 
 class Device:
@@ -51,6 +53,7 @@ class Device:
         self.key = (abi.DEVICE, id)
         self._structure = abi.device_t(id)
         self.reference = C.byref(self._structure)    # what every backend call on this device passes
+        self.stream()
 
     def structure(self):
         return self._structure
@@ -58,14 +61,18 @@ class Device:
     def stream(self):
         """The stream this device's backend calls run on.  The reference pops a stream from a per-device LIFO pool
         before every call and puts it back after (``src/bindings.cpp:22-42``, ``src/cuda/streams.cu:23-38``), which hands
-        a host thread the same stream every time; this mirror asks the pool once per device and keeps the answer."""
+        a host thread the same stream every time; this mirror asks the pool once per device, before anything is allocated on
+        it, and keeps the answer, so that the calls, allocations and copies of all threads follow each other."""
         stream = _STREAMS.get(self.id)
         if stream is None:
-            lib = library()
-            stream = lib.pop_stream(self.reference)
-            lib.put_stream(self.reference, stream)
-            _STREAMS[self.id] = stream
-            _STREAM_NUMBERS[self.id] = stream.address
+            with _STREAMS_LOCK:
+                stream = _STREAMS.get(self.id)
+                if stream is None:
+                    lib = library()
+                    stream = lib.pop_stream(self.reference)
+                    lib.put_stream(self.reference, stream)
+                    _STREAM_NUMBERS[self.id] = stream.address
+                    _STREAMS[self.id] = stream
         return stream
 
     def stream_number(self):
@@ -312,11 +319,8 @@ class Tensor:
             C.memmove(out.address, self.address, out.buffer.nbytes)
             return out
         lib = library()
-        dvc = dev.structure()
-        stream = lib.pop_stream(C.byref(dvc))
         src, dst = self.descriptor(), out.descriptor()
-        rc = lib.copy(C.byref(src), C.byref(dst), out.buffer.nbytes, stream)
-        lib.put_stream(C.byref(dvc), stream)
+        rc = lib.copy(C.byref(src), C.byref(dst), out.buffer.nbytes, dev.stream())
         if rc != abi.SUCCESS:
             raise BackendError(lib.error_message())
         return out
