@@ -220,7 +220,7 @@ template <class T, RowSource S, bool INTEGERS>
 __global__ __launch_bounds__(256) void rows_any_kernel(RowOperands p) {
     using A = std::conditional_t<std::is_same_v<T, double>, double, float>;
     constexpr bool NORM = S == RowSource::norm || S == RowSource::sum_norm;
-    __shared__ A sums[4];
+    __shared__ double sums[4];
     __shared__ uint32_t largest[4];
     const T* const gain = static_cast<const T*>(p.gain);
     for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -247,12 +247,12 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowOperands p) {
             }
             return static_cast<A>(widen(x[i * p.rows_x.step]));
         };
-        A squares = 0;
+        double squares = 0;      // (a thread may have millions of them, one after another)
         uint32_t most = 0;
         const auto look = [&](auto gates) {
             for (uint32_t i = threadIdx.x; i < p.length; i += 256) {
                 const A v = value(i, true, gates);
-                if constexpr (NORM) squares += v * v;
+                if constexpr (NORM) squares += static_cast<double>(v) * v;
                 if constexpr (INTEGERS) most = LargestOp::combine(most, magnitude(static_cast<float>(NORM ? v * static_cast<A>(widen(gain[i])) : v)));
             }
         };
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowOperands p) {
             }
         }
         A r = 1;
-        if constexpr (NORM) r = A(1) / sqrt(block_reduce<SquaresOp>(squares, sums) / static_cast<A>(p.length) + static_cast<A>(p.eps));
+        if constexpr (NORM) r = A(1) / sqrt(static_cast<A>(block_reduce<SquaresOp>(squares, sums)) / static_cast<A>(p.length) + static_cast<A>(p.eps));
         if constexpr (INTEGERS) {
             const RowScale scale(block_reduce<LargestOp>(most, largest));
             const auto write = [&](auto gates) {
