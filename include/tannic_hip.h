@@ -232,6 +232,11 @@ int tannic_hip_gemm_rows_batch_lanes(const tannic_tensor_t* a, const tannic_tens
  * rows of the matrix, 5 for up to 64 rows by windows of K through LDS (out[2], out[3] rows and columns of a wavefront; for both out[1] is whether the matrix is loaded
  * past the caches), 0 for any other; 1 to 3 of 16 bits only.  The status is the product's. */
 int tannic_hip_gemm_plan(const tannic_tensor_t* a, const tannic_tensor_t* b, const tannic_tensor_t* dst, uint32_t out[4]);
+/* Which kernel a product of 8-bit integers with scales (tannic_hip_gemm_quantized, the same operands) would run, asked the same way: out[0] is 1 for up to 32
+ * rows, 2 for the tiles with direct loads, 3 for rows along K that start anywhere, 0 for the one for any operands; out[1] whether the operands
+ * are copied into aligned rows first (1 the first, 2 the second, 3 both).  The status is the product's, wherever its operands live. */
+int tannic_hip_gemm_quantized_plan(const tannic_tensor_t* a, const tannic_tensor_t* a_scales, const tannic_tensor_t* b, const tannic_tensor_t* b_scales,
+                                   const tannic_tensor_t* dst, uint32_t out[2]);
 /* The stream a recording captures: a caller that keeps a device's stream to itself checks that it is this one. */
 tannic_stream_t tannic_hip_graph_stream(void* recording);
 

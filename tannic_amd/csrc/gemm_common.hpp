@@ -124,6 +124,8 @@ int gemm_mfma_f32(const GemmProblem& p, const float* a, const float* b, float* c
 // multiply q, a2, b2 instead and release held[0..1] (each may be null) afterwards; UNSUPPORTED: nothing was done.
 int gemm_repack(const GemmProblem& p, size_t esize, const void* a, const void* b, hipStream_t stream, bool may_copy, GemmProblem& q, const void*& a2, const void*& b2,
                 void* held[2]);
+// what it will do, asked beforehand
+int gemm_repack_plan(const GemmProblem& p, size_t esize, const void* a, const void* b, bool may_copy, GemmProblem& q, bool copies[2]);
 // fp32 products of a few hundred rows and columns (32 x 32 tiles whose wavefronts split K; gemm_small.hip)
 int gemm_small_f32(const GemmProblem& p, const float* a, const float* b, float* c, hipStream_t stream);
 // its extents: not when the tiles of the large kernels fill the chip, when K is too short to be worth splitting, or when it is long

@@ -92,41 +92,48 @@ void fold_batches(GemmProblem& p, ScalePlaces& s) {
     }
 }
 
+// Operands that do not lie along K in whole pieces: `q`, the product over copies of them (or over the same, a single row without a pitch), if gemm_repack makes it one that the kernels
+// with direct loads take.  (It copies no batch of several dims and no more than 2 GB, and leaves rows far apart or in reverse order as they are.)
+bool copies_fit(const GemmProblem& p, const void* a, const void* b, GemmProblem& q, bool copies[2]) {
+    return gemm_repack_plan(p, 1, a, b, true, q, copies) == TANNIC_SUCCESS && quantized_operands_fit(q, copies[0] ? nullptr : a, copies[1] ? nullptr : b);
+}
+
 template <class D>
 int run_quantized(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
-    if (!quantized_operands_fit(p, a, b)) {
-        const int status = gemm_quantized_bytes<D>(p, s, a, b, c, stream);
-        if (status != TANNIC_UNSUPPORTED_DTYPE) return status;
-    }
-    // operands that do not lie along K, or not in whole pieces, are copied first where that pays
     GemmProblem q = p;
     const void *pa = a, *pb = b;
     void* held[2] = {nullptr, nullptr};
-    if (!quantized_operands_fit(p, a, b)) {
-        const int repacked = gemm_repack(p, 1, a, b, stream, true, q, pa, pb, held);
-        if (repacked == TANNIC_ERROR) return repacked;
-        if (repacked != TANNIC_SUCCESS) q = p;
+    int status = TANNIC_UNSUPPORTED_DTYPE;
+    bool fit = quantized_operands_fit(p, a, b);
+    if (!fit) {
+        status = gemm_quantized_bytes<D>(p, true, s, a, b, c, stream);
+        if (status != TANNIC_UNSUPPORTED_DTYPE) return status;
+        bool copies[2];
+        if (copies_fit(p, a, b, q, copies)) {
+            status = gemm_repack(p, 1, a, b, stream, true, q, pa, pb, held);
+            if (status != TANNIC_SUCCESS && status != TANNIC_UNSUPPORTED_DTYPE) return status;
+            fit = status == TANNIC_SUCCESS;
+        }
+        if (!fit) status = gemm_quantized_bytes<D>(p, false, s, a, b, c, stream);
     }
-    int status = gemm_quantized_rows<D>(q, s, pa, pb, c, stream);
-    if (status == TANNIC_UNSUPPORTED_DTYPE) status = gemm_quantized_tile<D>(q, s, pa, pb, c, stream);
+    if (fit) {
+        status = gemm_quantized_rows<D>(q, s, pa, pb, c, stream);
+        if (status == TANNIC_UNSUPPORTED_DTYPE) status = gemm_quantized_tile<D>(q, s, pa, pb, c, stream);
+    }
     if (status == TANNIC_UNSUPPORTED_DTYPE) status = run_any<D>(p, s, a, b, c, stream);
     for (void* h : held)
         if (h) scratch_release(h, stream);
     return status;
 }
 
-}  // namespace th
-
-using namespace th;
-
-extern "C" int tannic_hip_gemm_quantized(const tannic_tensor_t* a, const tannic_tensor_t* a_scales, const tannic_tensor_t* b, const tannic_tensor_t* b_scales, tannic_tensor_t* dst,
-                                         tannic_stream_t stream) {
+// The product and where its scales lie, from the descriptors: everything but the device.
+int describe_quantized(const tannic_tensor_t* a, const tannic_tensor_t* a_scales, const tannic_tensor_t* b, const tannic_tensor_t* b_scales, const tannic_tensor_t* dst, GemmProblem& p,
+                       ScalePlaces& s) {
     if (!a || !a_scales || !b || !b_scales || !dst) return refuse("gemm_quantized: a descriptor is missing");
     if (!have_storage(a, a_scales, b, b_scales, dst)) return TANNIC_ERROR;
     if (a->dtype != TANNIC_INT8 || b->dtype != TANNIC_INT8 || a_scales->dtype != TANNIC_FLOAT32 || b_scales->dtype != TANNIC_FLOAT32 ||
         (dst->dtype != TANNIC_FLOAT16 && dst->dtype != TANNIC_BFLOAT16 && dst->dtype != TANNIC_FLOAT32))
         return TANNIC_UNSUPPORTED_DTYPE;
-    GemmProblem p;
     if (int status = describe_gemm(a, b, dst, p)) return status;
     if (!rows_contiguous(dst)) return refuse("gemm_quantized: dst is contiguous");
     if (p.K > kMostInner) return refuse("gemm_quantized: sums over 2^17 elements or more do not fit 32 bits");
@@ -134,9 +141,6 @@ extern "C" int tannic_hip_gemm_quantized(const tannic_tensor_t* a, const tannic_
     for (int d = 0; fit && d < a_scales->rank; ++d) fit = a_scales->shape.sizes[d] == a->shape.sizes[d];
     for (int d = 0; fit && d < b_scales->rank; ++d) fit = b_scales->shape.sizes[d] == b->shape.sizes[d + (d == b_scales->rank - 1)];
     if (!fit) return refuse("gemm_quantized: a scale for each row of a [.., M, K] and each column of b [.., K, N]");
-    if (int status = on_device_of("gemm_quantized: the operands live on a device", a, a_scales, b, b_scales, dst)) return status;
-    if (p.M == 0 || p.N == 0 || p.batches == 0) return TANNIC_SUCCESS;
-    ScalePlaces s{};
     s.a = static_cast<const float*>(a_scales->address);
     s.b = static_cast<const float*>(b_scales->address);
     s.a_step = stride_of(a_scales, a_scales->rank - 1);
@@ -149,10 +153,48 @@ extern "C" int tannic_hip_gemm_quantized(const tannic_tensor_t* a, const tannic_
         s.a_bs[d] = places(a_scales);
         s.b_bs[d] = places(b_scales);
     }
+    return TANNIC_SUCCESS;
+}
+
+}  // namespace th
+
+using namespace th;
+
+extern "C" int tannic_hip_gemm_quantized(const tannic_tensor_t* a, const tannic_tensor_t* a_scales, const tannic_tensor_t* b, const tannic_tensor_t* b_scales, tannic_tensor_t* dst,
+                                         tannic_stream_t stream) {
+    GemmProblem p;
+    ScalePlaces s{};
+    if (int status = describe_quantized(a, a_scales, b, b_scales, dst, p, s)) return status;
+    if (int status = on_device_of("gemm_quantized: the operands live on a device", a, a_scales, b, b_scales, dst)) return status;
+    if (p.M == 0 || p.N == 0 || p.batches == 0) return TANNIC_SUCCESS;
     fold_batches(p, s);
     switch (dst->dtype) {
         case TANNIC_FLOAT16: return run_quantized<f16>(p, s, a->address, b->address, dst->address, as_stream(stream));
         case TANNIC_BFLOAT16: return run_quantized<bf16>(p, s, a->address, b->address, dst->address, as_stream(stream));
         default: return run_quantized<float>(p, s, a->address, b->address, dst->address, as_stream(stream));
     }
+}
+
+extern "C" int tannic_hip_gemm_quantized_plan(const tannic_tensor_t* a, const tannic_tensor_t* a_scales, const tannic_tensor_t* b, const tannic_tensor_t* b_scales, const tannic_tensor_t* dst,
+                                              uint32_t out[2]) {
+    out[0] = out[1] = 0;
+    GemmProblem p;
+    ScalePlaces s{};
+    if (int status = describe_quantized(a, a_scales, b, b_scales, dst, p, s)) return status;
+    if (p.M == 0 || p.N == 0 || p.batches == 0) return TANNIC_SUCCESS;
+    fold_batches(p, s);
+    GemmProblem q = p;
+    bool copies[2] = {false, false};
+    const void *pa = a->address, *pb = b->address;
+    if (!quantized_operands_fit(p, pa, pb)) {
+        if (gemm_quantized_bytes_takes<bf16>(p, true) || !copies_fit(p, pa, pb, q, copies)) {
+            out[0] = gemm_quantized_bytes_takes<bf16>(p, false) ? 3 : 0;
+            return TANNIC_SUCCESS;
+        }
+        if (copies[0]) pa = nullptr;
+        if (copies[1]) pb = nullptr;
+    }
+    out[0] = gemm_quantized_rows_takes(q, pa, pb) ? 1 : gemm_quantized_tile_takes(q, pa, pb) ? 2 : 0;
+    out[1] = (copies[0] ? 1 : 0) + (copies[1] ? 2 : 0);
+    return TANNIC_SUCCESS;
 }

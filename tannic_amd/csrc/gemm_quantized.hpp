@@ -71,10 +71,18 @@ constexpr uint32_t kBeyond = 0x80000000u;
 // The bytes of `rows` rows (256 at most), which end with the last one's K: below kBeyond.
 __device__ inline uint32_t bytes_of_rows(uint32_t rows, int64_t pitch, uint32_t K) { return (rows - 1) * static_cast<uint32_t>(pitch) + K; }
 
+// Fewer blocks of bm x bn results than a launch may have.
+inline bool few_enough_blocks(const GemmProblem& p, uint64_t bm, uint64_t bn) {
+    return (static_cast<uint64_t>(p.M) + bm - 1) / bm * ((static_cast<uint64_t>(p.N) + bn - 1) / bn) * p.batches < kMostBlocks && p.batches <= 65535;
+}
+inline bool gemm_quantized_tile_takes(const GemmProblem& p, const void* a, const void* b) { return quantized_operands_fit(p, a, b) && few_enough_blocks(p, 256, 256); }
+
 // Up to 32 rows (gemm_quantized_rows.hip) and more (gemm_quantized_tile.hip); TANNIC_UNSUPPORTED_DTYPE: not this kernel's
+bool gemm_quantized_rows_takes(const GemmProblem& p, const void* a, const void* b);
 template <class D> int gemm_quantized_rows(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream);
 template <class D> int gemm_quantized_tile(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream);
-// rows along K that start anywhere and have any length
-template <class D> int gemm_quantized_bytes(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream);
+// rows along K that start anywhere and have any length; `or_copies`: not where copying them for the kernels above is faster
+template <class D> int gemm_quantized_bytes(const GemmProblem& p, bool or_copies, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream);
+template <class D> bool gemm_quantized_bytes_takes(const GemmProblem& p, bool or_copies);
 
 }  // namespace th

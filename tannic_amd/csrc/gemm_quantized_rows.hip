@@ -133,15 +133,20 @@ static int launch_rows(const GemmProblem& p, const ScalePlaces& s, const void* a
     return rows_past_caches(p, 1, 40ull << 20) ? launch_rows<D, MB, NB, true>(p, s, a, b, c, stream) : launch_rows<D, MB, NB, false>(p, s, a, b, c, stream);
 }
 
-template <class D>
-int gemm_quantized_rows(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
-    if (p.M > 32 || !quantized_operands_fit(p, a, b)) return TANNIC_UNSUPPORTED_DTYPE;
+static uint64_t blocks_of_16(const GemmProblem& p) { return (static_cast<uint64_t>(p.N) + 15) / 16 * p.batches; }
+
+bool gemm_quantized_rows_takes(const GemmProblem& p, const void* a, const void* b) {
+    if (p.M > 32 || !quantized_operands_fit(p, a, b)) return false;
     // Where the columns fill the chip once, 16 or 32 to a block, and the tiles of 32 x 64 do not do better, whose four wavefronts share x.  us here / there, weights from memory: 1 row of
     // 6144 x 4096 7.3 / 9.5, 4096 x 14336 11.5 / 15.2, 14336 x 4096 13.8 / 13.4, 28672 x 4096 25.5 / 24.5; 32 rows of 4096 x 4096 6.9 / 9.5, 6144 x 4096 8.6 / 10.4, 14336 x 4096 15.8 / 14.1,
     // 28672 x 4096 29.6 / 26.6; more than 16 rows under a long K, which those share between blocks: 4096 x 14336 16.6 / 15.3, 1000 x 14336 13.4 / 10.2 (16 rows 13.2 / 15.2, 10.2 / 10.0).
-    const uint64_t blocks = (static_cast<uint64_t>(p.N) + 15) / 16 * p.batches;
-    if (blocks > 512 || (p.M > 16 && p.K >= 8192)) return TANNIC_UNSUPPORTED_DTYPE;
-    const bool two = blocks > 256;
+    return blocks_of_16(p) <= 512 && !(p.M > 16 && p.K >= 8192);
+}
+
+template <class D>
+int gemm_quantized_rows(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
+    if (!gemm_quantized_rows_takes(p, a, b)) return TANNIC_UNSUPPORTED_DTYPE;
+    const bool two = blocks_of_16(p) > 256;
     if (p.M <= 16) return two ? launch_rows<D, 1, 2>(p, s, a, b, c, stream) : launch_rows<D, 1, 1>(p, s, a, b, c, stream);
     return two ? launch_rows<D, 2, 2>(p, s, a, b, c, stream) : launch_rows<D, 2, 1>(p, s, a, b, c, stream);
 }

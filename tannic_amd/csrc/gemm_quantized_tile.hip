@@ -490,14 +490,9 @@ static Choice8 choose_tiles8(const GemmProblem& p, const Tiles8* tiles, int coun
     return best;
 }
 
-// Fewer blocks of bm x bn results than a launch may have.
-static bool few_enough_blocks(const GemmProblem& p, uint64_t bm, uint64_t bn) {
-    return (static_cast<uint64_t>(p.M) + bm - 1) / bm * ((static_cast<uint64_t>(p.N) + bn - 1) / bn) * p.batches < kMostBlocks && p.batches <= 65535;
-}
-
 template <class D>
 int gemm_quantized_tile(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
-    if (!quantized_operands_fit(p, a, b) || !few_enough_blocks(p, 256, 256)) return TANNIC_UNSUPPORTED_DTYPE;
+    if (!gemm_quantized_tile_takes(p, a, b)) return TANNIC_UNSUPPORTED_DTYPE;
     const Choice8 choice = choose_tiles8(p, kTiles8, 8);
     switch (choice.tile) {
         case 0: return launch_tiles<D, 256, 256, 2>(p, s, choice.splits, a, b, c, stream);
@@ -535,15 +530,26 @@ static int launch_bytes(const GemmProblem& p, const ScalePlaces& s, uint32_t spl
 // The tiles for rows that start anywhere, times as above; four blocks and more on a compute unit share its loads, one alone is not faster than `alone`.
 constexpr Tiles8 kBytes8[] = {{64, 64, 0.44, 0.7, 0.48, 0.75}, {32, 64, 0.345, 0.6, 0.37, 0.64}};
 
-template <class D>
-int gemm_quantized_bytes(const GemmProblem& p, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
-    if (p.a_cs != 1 || p.b_rs != 1 || p.K < 16 || !few_enough_blocks(p, 64, 64)) return TANNIC_UNSUPPORTED_DTYPE;
-    const Choice8 choice = choose_tiles8(p, kBytes8, 2);
+static bool choose_bytes8(const GemmProblem& p, bool or_copies, Choice8& choice) {
+    if (p.a_cs != 1 || p.b_rs != 1 || p.K < 16 || !few_enough_blocks(p, 64, 64)) return false;
+    choice = choose_tiles8(p, kBytes8, 2);
+    if (!or_copies) return true;
     // where copies and the tiles of aligned rows are faster those take it: two launches of about 3 us, a read and a write of both operands (and no product is shorter than 4 us)
     const double copies = 6.0 + 2.0 * (static_cast<double>(p.M) + p.N) * p.K * p.batches / 4.5e6;
     GemmProblem q = p;
     q.K = (p.K + 127) / 128 * 128;
-    if (choice.cost > copies + 4.0 && choice.cost > copies + choose_tiles8(q, kTiles8, 8).cost) return TANNIC_UNSUPPORTED_DTYPE;
+    return !(choice.cost > copies + 4.0 && choice.cost > copies + choose_tiles8(q, kTiles8, 8).cost);
+}
+
+template <class D> bool gemm_quantized_bytes_takes(const GemmProblem& p, bool or_copies) {
+    Choice8 choice;
+    return choose_bytes8(p, or_copies, choice);
+}
+
+template <class D>
+int gemm_quantized_bytes(const GemmProblem& p, bool or_copies, const ScalePlaces& s, const void* a, const void* b, void* c, hipStream_t stream) {
+    Choice8 choice;
+    if (!choose_bytes8(p, or_copies, choice)) return TANNIC_UNSUPPORTED_DTYPE;
     return choice.tile == 0 ? launch_bytes<D, 64>(p, s, choice.splits, a, b, c, stream) : launch_bytes<D, 32>(p, s, choice.splits, a, b, c, stream);
 }
 
@@ -552,6 +558,7 @@ int gemm_quantized_bytes(const GemmProblem& p, const ScalePlaces& s, const void*
 #define TH_TILE_TYPE bf16
 #endif
 template int gemm_quantized_tile<TH_TILE_TYPE>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
-template int gemm_quantized_bytes<TH_TILE_TYPE>(const GemmProblem&, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
+template bool gemm_quantized_bytes_takes<TH_TILE_TYPE>(const GemmProblem&, bool);
+template int gemm_quantized_bytes<TH_TILE_TYPE>(const GemmProblem&, bool, const ScalePlaces&, const void*, const void*, void*, hipStream_t);
 
 }  // namespace th

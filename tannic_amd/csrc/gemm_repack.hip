@@ -92,12 +92,10 @@ static bool lies_well(const void* base, uint32_t rows, uint32_t K, int64_t row_s
     return false;
 }
 
-// Decides, copies, and describes the product over the copies (a single product, or an int8 batch along one dim).  Returns TANNIC_UNSUPPORTED_DTYPE when nothing was done
-// (the caller goes on with the operands as they are); otherwise `q`, `a2`, `b2` are what to multiply and `held[0..1]` what
-// to release after the product has been queued.
-int gemm_repack(const GemmProblem& p, size_t esize, const void* a, const void* b, hipStream_t stream, bool may_copy, GemmProblem& q, const void*& a2, const void*& b2,
-                void* held[2]) {
-    held[0] = held[1] = nullptr;
+// Whether operands are copied, and `q` as the product over the copies.  TANNIC_UNSUPPORTED_DTYPE: the operands are multiplied as they are; TANNIC_SUCCESS without copies: q's single row or
+// column has the pitch of its own length.
+int gemm_repack_plan(const GemmProblem& p, size_t esize, const void* a, const void* b, bool may_copy, GemmProblem& q, bool copies[2]) {
+    copies[0] = copies[1] = false;
     if (p.c_group || p.b_group_stride || p.M == 0 || p.N == 0 || p.K == 0 || p.batches == 0 || p.batches > 65535) return TANNIC_UNSUPPORTED_DTYPE;
     // a batch along one dim: an operand is copied product by product, or once when every product reads the same one
     if (p.batches != 1 && p.batch_rank != 1) return TANNIC_UNSUPPORTED_DTYPE;
@@ -117,15 +115,9 @@ int gemm_repack(const GemmProblem& p, size_t esize, const void* a, const void* b
         a_ok = a_ok && q.a_bs[0] % unit == 0;
         b_ok = b_ok && q.b_bs[0] % unit == 0;
     }
-    a2 = a;
-    b2 = b;
-    if (a_ok && b_ok) {
-        // only the single-row normalisation may have changed something
-        return (q.a_rs != p.a_rs || q.b_cs != p.b_cs) ? TANNIC_SUCCESS : TANNIC_UNSUPPORTED_DTYPE;
-    }
     const bool normalised = q.a_rs != p.a_rs || q.b_cs != p.b_cs;
     const int untouched = normalised ? TANNIC_SUCCESS : TANNIC_UNSUPPORTED_DTYPE;   // (with q = p but for the single row's pitch)
-    if (!may_copy) return untouched;
+    if ((a_ok && b_ok) || !may_copy) return untouched;
     // the copy kernels read along K or along the rows
     if ((!a_ok && q.a_cs != 1 && q.a_rs != 1) || (!b_ok && q.b_rs != 1 && q.b_cs != 1)) return untouched;
     // Worth two more launches: the int8 alternative is the scalar kernel; for the others the kernels for misaligned
@@ -139,33 +131,51 @@ int gemm_repack(const GemmProblem& p, size_t esize, const void* a, const void* b
     const uint32_t copies_a = batched && q.a_bs[0] != 0 ? q.batches : 1, copies_b = batched && q.b_bs[0] != 0 ? q.batches : 1;
     const size_t bytes_a = a_ok ? 0 : static_cast<size_t>(q.M) * Kp * esize * copies_a, bytes_b = b_ok ? 0 : static_cast<size_t>(q.N) * Kp * esize * copies_b;
     if (bytes_a + bytes_b > (2ull << 30)) return untouched;
-    auto copy = [&](const void* src, void* dst, uint32_t rows, int64_t row_stride, int64_t k_stride, uint32_t copies, int64_t batch_stride) {
-        switch (esize) {
-            case 1: return repack_operand<uint8_t>(src, dst, rows, q.K, Kp, row_stride, k_stride, copies, batch_stride, stream);
-            case 2: return repack_operand<uint16_t>(src, dst, rows, q.K, Kp, row_stride, k_stride, copies, batch_stride, stream);
-            default: return repack_operand<uint32_t>(src, dst, rows, q.K, Kp, row_stride, k_stride, copies, batch_stride, stream);
-        }
-    };
-    int status = TANNIC_SUCCESS;
-    if (!a_ok) {
-        if (scratch_acquire(&held[0], bytes_a, stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
-        status = copy(a, held[0], q.M, q.a_rs, q.a_cs, copies_a, q.a_bs[0]);
-        a2 = held[0];
+    copies[0] = !a_ok;
+    copies[1] = !b_ok;
+    if (copies[0]) {
         q.a_rs = Kp;
         q.a_cs = 1;
         if (batched) q.a_bs[0] = copies_a == 1 ? 0 : static_cast<int64_t>(q.M) * Kp;
     }
-    if (status == TANNIC_SUCCESS && !b_ok) {
-        if (scratch_acquire(&held[1], bytes_b, stream) != TANNIC_SUCCESS) status = TANNIC_ERROR;
-        else {
-            status = copy(b, held[1], q.N, q.b_cs, q.b_rs, copies_b, q.b_bs[0]);
-            b2 = held[1];
-            q.b_cs = Kp;
-            q.b_rs = 1;
-            if (batched) q.b_bs[0] = copies_b == 1 ? 0 : static_cast<int64_t>(q.N) * Kp;
-        }
+    if (copies[1]) {
+        q.b_cs = Kp;
+        q.b_rs = 1;
+        if (batched) q.b_bs[0] = copies_b == 1 ? 0 : static_cast<int64_t>(q.N) * Kp;
     }
     q.K = Kp;
+    return TANNIC_SUCCESS;
+}
+
+// Decides, copies, and describes the product over the copies (a single product, or an int8 batch along one dim).  Returns TANNIC_UNSUPPORTED_DTYPE when nothing was done
+// (the caller goes on with the operands as they are); otherwise `q`, `a2`, `b2` are what to multiply and `held[0..1]` what
+// to release after the product has been queued.
+int gemm_repack(const GemmProblem& p, size_t esize, const void* a, const void* b, hipStream_t stream, bool may_copy, GemmProblem& q, const void*& a2, const void*& b2,
+                void* held[2]) {
+    held[0] = held[1] = nullptr;
+    a2 = a;
+    b2 = b;
+    bool copies[2];
+    if (const int planned = gemm_repack_plan(p, esize, a, b, may_copy, q, copies)) return planned;
+    if (!copies[0] && !copies[1]) return TANNIC_SUCCESS;
+    const uint32_t copies_a = p.batches != 1 && p.a_bs[0] != 0 ? p.batches : 1, copies_b = p.batches != 1 && p.b_bs[0] != 0 ? p.batches : 1;
+    auto copy = [&](const void* src, void*& dst, uint32_t rows, int64_t row_stride, int64_t k_stride, uint32_t count, int64_t batch_stride) -> int {
+        if (scratch_acquire(&dst, static_cast<size_t>(rows) * q.K * esize * count, stream) != TANNIC_SUCCESS) return TANNIC_ERROR;
+        switch (esize) {
+            case 1: return repack_operand<uint8_t>(src, dst, rows, p.K, q.K, row_stride, k_stride, count, batch_stride, stream);
+            case 2: return repack_operand<uint16_t>(src, dst, rows, p.K, q.K, row_stride, k_stride, count, batch_stride, stream);
+            default: return repack_operand<uint32_t>(src, dst, rows, p.K, q.K, row_stride, k_stride, count, batch_stride, stream);
+        }
+    };
+    int status = TANNIC_SUCCESS;
+    if (copies[0]) {
+        status = copy(a, held[0], p.M, p.a_rs, p.a_cs, copies_a, p.a_bs[0]);
+        a2 = held[0];
+    }
+    if (status == TANNIC_SUCCESS && copies[1]) {
+        status = copy(b, held[1], p.N, p.b_cs, p.b_rs, copies_b, p.b_bs[0]);
+        b2 = held[1];
+    }
     if (status != TANNIC_SUCCESS) {
         for (int i = 0; i < 2; ++i)
             if (held[i]) scratch_release(held[i], stream);
