@@ -202,7 +202,12 @@ struct ScaledProduct {
             for (size_t dim = 0; dim + 2 < of.rank(); ++dim) out.expand(of[dim]);
             return out;
         };
-        Shape out = b.rank() == 2 ? batches(a) : a.rank() == 2 ? batches(b) : operation::broadcast(batches(a), batches(b));
+        const Shape first = batches(a), second = batches(b), wide = b.rank() == 2 ? first : a.rank() == 2 ? second : operation::broadcast(first, second);
+        Shape out;
+        for (size_t dim = 0; dim < wide.rank(); ++dim) {
+            const auto empty = [&](Shape const& of) { return dim + of.rank() >= wide.rank() && of[dim + of.rank() - wide.rank()] == 0; };
+            out.expand(empty(first) || empty(second) ? 0 : wide[dim]);      // (an empty batch over one matrix is empty)
+        }
         out.expand(a[a.rank() - 2]);
         out.expand(b[b.rank() - 1]);
         return out;
