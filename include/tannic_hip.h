@@ -455,11 +455,14 @@ int tannic_hip_attend(const tannic_tensor_t* q, const tannic_tensor_t* k, const 
  * weights (a matrix [out, in] and its transposed view as second operand).
  *   values = rint(u * (127 * (1 / m))), ties to even, scales = m / 127,
  *   m = max |u| of the row, 2^-119 at least
- * so that no value is off by more than half a scale.  A row with something
- * that is not finite has zeros and the scale NaN: all that is computed from
- * it is NaN.  x: float16, bfloat16 or float, any strides; u, and a norm's
- * mean, are float; the results are contiguous and lie over no operand (but
- * for a norm's sum).
+ * so that no value is off by more than half a scale and 2^-21 of m (the
+ * roundings of the factor, of its product with u and of the scale).  A row
+ * with something that is not finite has zeros and the scale NaN: all that is
+ * computed from it is NaN.  x: float16, bfloat16 or float, any strides; u,
+ * and a norm's mean, are float: where squares of finite values add up to
+ * 2^128 or more (values about 2^64 / sqrt(L)) the norm is 0, as
+ * tannic_hip_rms_norm's is, and in 8 bits its scale is 0.  The results are
+ * contiguous and lie over no operand (but for a norm's sum).
  * ------------------------------------------------------------------ */
 /* u = x */
 int tannic_hip_quantize(const tannic_tensor_t* x, tannic_tensor_t* dst, tannic_tensor_t* scales, tannic_stream_t stream);

@@ -446,8 +446,9 @@ static int launch_tiles(const GemmProblem& p, const ScalePlaces& s, uint32_t spl
 
 // The kernel's tiles: rows, columns, us of a step of 128 with the chip full of them (and of a block that has a compute unit alone, where that is more), us that a block takes beside its
 // steps, us that the last of the blocks that share a tile takes for each of their parts (0: a second kernel adds them up).  Two blocks of the last three are on a compute unit at a time and share
-// its step times as they share its LDS: a step is bound by LDS, which takes 32 KB of what is loaded in 0.24 us and gives 64 KB of fragments in 0.20 (both in 0.35; 128 x 128), at the
-// clock that the products leave, and for the largest by the matrix pipe under the chip's power limit (256 x 256 1.4 us, 3.1 POP/s; MFMAs alone on such values 1.3).  Measured with weights from
+// its step times.  Of the 0.50 us of a 128 x 128 step LDS takes 0.35 (32 KB of what is loaded 0.24, 64 KB of fragments 0.20), and no pipe is busy most of it: a SIMD has one wavefront, which
+// issues 45 % of the time, waits 35 % for loads, fragments and the others and 20 % for a pipe (counted for 128 x 96; the matrix pipe is busy 30 %, LDS with fragments 19 %).  The largest tile is
+// bound by the matrix pipe under the chip's power limit (256 x 256 1.4 us, 3.1 POP/s; MFMAs alone on such values 1.3).  Measured with weights from
 // memory: 31 products of 33 to 8000 rows, each tile and up to 16 splits; what comes out first below is within 7 % of the fastest found.
 struct Tiles8 {
     uint32_t rows, columns;

@@ -107,7 +107,7 @@ template <bool PAST, int N> __device__ inline void store_integers(int8_t* to, co
 }
 
 // A group of G threads (a wavefront, or a block) per row, which is read once and kept in registers as u, NCH pieces of 16 bytes of a thread.  Bound by memory: 8001 x 5120 fp16
-// with sum and residual 5.6 TB/s, 4096 x 14336 bf16 gated 5.6 TB/s (its arithmetic takes nearly as long), 28672 x 4096 fp16 6.4 TB/s.
+// with sum and residual 55.9 us, 5.1 TB/s, 4096 x 14336 bf16 gated 57.2 us, 5.1 TB/s (its arithmetic takes nearly as long), 28672 x 4096 fp16 57.6 us, 6.1 TB/s.
 // Wavefronts on a SIMD that the registers have to leave room for: three blocks of 512 on a compute unit where one register too many (81, fp16) would make them two (8001 x 5120 with sum and
 // residual 59 / 50 us).  No such limit for the others: with three or four pieces they would spill.
 template <RowSource S, int G, int NCH> constexpr int kRowWavefronts = (S == RowSource::norm || S == RowSource::sum_norm) && G == 512 && NCH == 2 ? 6 : 1;

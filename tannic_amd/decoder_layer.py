@@ -168,7 +168,7 @@ def forward_paged(s, w, x, cos, sin, cache, layer, step, trace=None):
 
 def quantize_weights(w):
     """The parameters with every projection (a matrix ``[out, in]``) in 8-bit integers and a scale for each of its channels, under its name with ``_scales`` behind it: half the
-    memory of 16-bit ones for no more than half a scale off each weight (done once, when they are loaded; of ``pack_weights``' the concatenations only)."""
+    memory of 16-bit ones for no more than half a scale (and 2^-21 of the channel's largest) off each weight (done once, when they are loaded; of ``pack_weights``' the concatenations only)."""
     parts = {"wq", "wk", "wv"} if "wqkv" in w else set()
     parts |= {"w1", "w3"} if "w13" in w else set()
     quantized = {}

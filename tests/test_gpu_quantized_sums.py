@@ -54,3 +54,21 @@ def test_a_row_of_millions(dtype, device):
     x = rounded(np.stack([np.full(length, 1.0078125), np.full(length, 0.7)]), dtype)
     gain = rounded(np.resize([0.75, 1.0, 1.5], length), dtype)
     check(ta.tensor(x, dtype, device), None, ta.tensor(gain, dtype, device), x, gain, dtype)
+
+
+@pytest.mark.parametrize("dtype", [ta.bfloat16, ta.float32], ids=str)
+@pytest.mark.parametrize("length", [64, 4096, 16384, 40000])
+def test_squares_beyond_the_floats(length, dtype, device):
+    """A mean of squares that is no float: the norm is 0, as ``rms_norm``'s is, in either form; below that bound it is what it should be."""
+    rng = np.random.default_rng(52)
+    x = rounded(rng.uniform(1, 2, (2, length)) * [[3e19], [2.0 ** 60 / length ** 0.5]], dtype)
+    gain = rounded(np.ones(length), dtype)
+    dx, dg = ta.tensor(x, dtype, device), ta.tensor(gain, dtype, device)
+    normed, _ = ops.add_rms_norm(dx, None, dg, EPS)
+    values, scales, _ = ops.add_rms_norm_quantized(dx, None, dg, EPS)
+    assert not normed.numpy()[0].any() and scales.numpy()[0] == 0
+    assert not ops.rms_norm(dx, dg, EPS).numpy()[0].any()
+    wide = x[1].astype(np.float64)
+    want = wide / np.sqrt((wide * wide).mean() + EPS)
+    assert (np.abs(normed.numpy()[1].astype(np.float64) - want) <= (HALF[dtype] * (1 + 2.0 ** -10) + ROOT + 2 * 2.0 ** -24) * np.abs(want)).all()
+    assert_stands_for(values.numpy()[1:], scales.numpy()[1:], want[None], ROOT + 3 * 2.0 ** -24)
