@@ -34,7 +34,7 @@ struct RowOperands {
     double eps;
 };
 
-// gate / (1 + exp(-gate)) * up, off by 8 * 2^-24 at most, for gates from kFarGate on: exp(-gate) is 2^high * (1 + low * ln 2) with high + low = -gate * log2 e (the instruction for
+// gate / (1 + exp(-gate)) * up, off by 8 * 2^-24 at most, for gates from -64 on: exp(-gate) is 2^high * (1 + low * ln 2) with high + low = -gate * log2 e (the instruction for
 // powers of two is off by 2 units, and high alone would be by |gate|); the sum with 1 takes both in one rounding, its reciprocal is off by 2 units.  The product with log2 e may not be
 // beyond all floats: the exponential of -200 is nothing beside 1.
 constexpr float kLog2e = 0x1.715476p+0f, kLog2eRest = 0x1.4ae0bep-26f;
@@ -45,11 +45,10 @@ __device__ inline float gated(float gate, float up) {
     return gate * __builtin_amdgcn_rcpf(sum) * up;
 }
 
-// Below kFarGate 1 is nothing beside exp(-gate) (2^-92), and gate * exp(gate) * up is it: from -87 on the reciprocal of the sum would be no normal number, from -92 on the quotient, and
+// Below -64 1 is nothing beside exp(-gate) (2^-92), and gate * exp(gate) * up is it: from -87 on the reciprocal of the sum would be no normal number, from -92 on the quotient, and
 // both come out as 0, while up may make either large.  exp(gate) is 2^whole * 2^part with |part| <= 1/2 (off by 2^-25 before the instruction's 2 units), the powers of two of both factors meet in the last step:
 // off by 5 * 2^-24 at most, or by half of the smallest subnormal number.  exp(-400) is 0 with any factor; a gate that is not finite is what it is in the formula.
-constexpr float kFarGate = -64.0f;
-constexpr uint32_t kFarGateBits = 0xC2800000u;      // (what is below it, as an unsigned number, is above this; so is what is not a number and has a sign)
+constexpr uint32_t kFarGateBits = 0xC2800000u;      // -64 (what is below it, as an unsigned number, is above this; so is what is not a number and has a sign)
 __device__ inline float gated_far(float gate, float up) {
     const float power = fmaxf(gate, -400.0f), whole = rintf(power * kLog2e), part = fmaf(power, kLog2eRest, fmaf(power, kLog2e, -whole));
     const float near = power * 0x1p-64f * __builtin_amdgcn_exp2f(part) * up;

@@ -59,9 +59,18 @@ class Streams {
         auto& pool = pools_[device];
         if (pool.empty()) {
             hipStream_t s = nullptr;
-            // default flags: ordered against the legacy stream like the reference's
+            // on that device, whichever is the current one; default flags: ordered against the legacy stream like the reference's
             // cudaStreamCreate; default priority
-            if (hipStreamCreate(&s) != hipSuccess) return nullptr;
+            int current = 0;
+            bool created = hipGetDevice(&current) == hipSuccess && hipSetDevice(device) == hipSuccess;
+            if (created) {
+                created = hipStreamCreate(&s) == hipSuccess;
+                (void)hipSetDevice(current);
+            }
+            if (!created) {
+                (void)hipGetLastError();
+                return nullptr;
+            }
             pool.push_back(s);
         }
         return pool.back();

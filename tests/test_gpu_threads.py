@@ -96,6 +96,15 @@ def test_each_thread_reads_its_own(size, device):
         np.testing.assert_array_equal(got.numpy(), want[0])
 
 
+def test_a_stream_is_of_the_device_that_it_is_asked_for(device):
+    """A device that is not there has no streams (the current one's were handed out for it), and asking leaves no error behind."""
+    from tannic_amd import abi
+    lib = ta.library()
+    nowhere = abi.device_t(lib.get_device_count())
+    assert not lib.pop_stream(C.byref(nowhere)).address
+    assert ops.add(ta.tensor(np.ones(5), ta.float32, device), ta.tensor(np.ones(5), ta.float32, device)).numpy().tolist() == [2.0] * 5
+
+
 def test_the_other_calls_of_two_threads(device):
     """Operators that had taken a stream of the pool for themselves: softmax, allclose and copies between tensors."""
     rng = np.random.default_rng(92)
