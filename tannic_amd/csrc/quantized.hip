@@ -163,7 +163,9 @@ __global__ __launch_bounds__(G == 64 ? 256 : G, (kRowWavefronts<S, G, NCH>)) voi
                 for (int i = 0; i < NCH; ++i) {
                     const uint32_t at = (t + i * G) * VEC;
                     if (at < p.length) {
-                        const Piece<T> gate = load_piece<T, PAST>(x + at, p.length - at), up = load_piece<T, PAST>(second + at, p.length - at);
+                        uint32_t again = at;
+                        asm volatile("" : "+v"(again));      // (a number of its own, or the first reading waits piece by piece for what both have in common: 4096 x 14336 fp16 90 us for 88)
+                        const Piece<T> gate = load_piece<T, PAST>(x + again, p.length - again), up = load_piece<T, PAST>(second + again, p.length - again);
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) {
                             if (__float_as_uint(widen(gate.v[e])) > kFarGateBits) u[i][e] = gated_far(widen(gate.v[e]), widen(up.v[e]));
